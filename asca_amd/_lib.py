@@ -84,6 +84,22 @@ SIGNATURES: dict[str, tuple] = {
     "asca_chunk_ws_bytes_f32": (_i, [_i, _i, _i, _i, _i, C.POINTER(_sz)]),
     "asca_chunk_fwd_f32": (_i, [_p] * 7 + [_i] * 5 + [_p]),
     "asca_chunk_bwd_f32": (_i, [_p] * 7 + [_i] * 5 + [_p]),
+    "asca_conv_fwd": (_i, [_p, _l, _p, _p, _p, _p, _p, _l, _p, _i, _i, _i, _i, _i, _i, _p]),
+    "asca_conv_bwd": (_i, [_p, _l, _p, _p, _p, _p, _p, _l, _p, _p, _l, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
+    "asca_conv_step": (_i, [_p, _p, _l, _p, _p, _p, _l, _i, _i, _i, _i, _i, _p]),
+    "asca_ssm_ws_bytes": (_i, [_i, _i, _i, _i, C.POINTER(_sz)]),
+    "asca_ssm_fwd": (_i, [_p, _l, _p, _l, _p, _p, _p, _l, _p, _l, _p, _p, _p, _p, _l, _p, _p, _i, _i, _i, _i, _i, _i, _i,
+              _p]),
+    "asca_ssm_bwd": (_i, [_p, _l, _p, _l, _p, _p, _p, _l, _p, _l, _p, _p, _p, _l, _p, _p, _p, _l, _p, _l, _p, _p, _p, _l, _p,
+              _l, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p]),
+    "asca_ssm_step": (_i, [_p, _p, _l, _p, _l, _p, _p, _p, _l, _p, _l, _p, _p, _l, _i, _i, _i, _i, _i, _i, _p]),
+    "asca_block_norm_fwd": (_i, [_p, _l, _p, _l, _p, _l, _p, _p, _p, _p, _l, _p, _l, _l, _i, _f, _i, _p]),
+    "asca_block_norm_bwd": (_i, [_p, _l, _p, _l, _p, _l, _p, _p, _p, _p, _l, _p, _l, _p, _l, _p, _l, _p, _l, _p, _p, _p, _l, _i, _f,
+              _i, _p]),
+    "asca_grads_create": (_i, [C.POINTER(_p), C.POINTER(_p), _u64p, _i, _i, C.POINTER(_p)]),
+    "asca_grads_destroy": (_i, [_p]),
+    "asca_grads_norm": (_i, [_p, _p, _p]),
+    "asca_grads_clip": (_i, [_p, _f, _p, _p]),
     "asca_model_create": (_i, [_i] * 6 + [C.POINTER(_p)]),
     "asca_model_destroy": (_i, [_p]),
     "asca_model_num_tensors": (_i, [_p, C.POINTER(_i)]),

@@ -30,7 +30,8 @@ from ._lib import AscaError
 ARCH = "gfx950"
 KERNELS = ("delta_fwd", "delta_bwd", "delta_states", "delta_decode", "rmsnorm", "rmsnorm_bwd", "adamw",
            "hash_route", "gather_rows", "scatter_rows", "colsum", "cross_entropy", "gemm", "moe_fwd", "moe_bwd",
-           "chunk_fwd", "chunk_bwd", "model_train_step")
+           "chunk_fwd", "chunk_bwd", "model_train_step", "conv_fwd", "conv_bwd", "conv_step", "ssm_fwd", "ssm_bwd",
+           "ssm_step", "block_norm_fwd", "block_norm_bwd", "grads_norm", "grads_clip")
 DEFAULT_MIN_FLOPS = 4_000_000
 
 _f32 = np.float32
@@ -258,6 +259,110 @@ def to_bf16(x: np.ndarray) -> np.ndarray:
 def from_bf16(x: np.ndarray) -> np.ndarray:
     """bf16 bit patterns (uint16) -> float32 (exact)."""
     return (np.ascontiguousarray(x, dtype=np.uint16).astype(np.uint32) << 16).view(_f32)
+
+
+F32, BF16 = 0, 1   # ASCA_F32, ASCA_BF16: element types of activation rows
+
+
+def _acts(shape_of: dict, **arrays) -> int:
+    """Check activation matrices (float32, or uint16 bf16 bit patterns, all of one
+    type) against their shapes; the element type."""
+    types = {a.dtype for a in arrays.values() if a is not None}
+    if len(types) != 1 or next(iter(types)) not in (np.dtype(_f32), np.dtype(np.uint16)):
+        raise ValueError(f"activations must be all float32 or all uint16 (bf16 bits), got {sorted(map(str, types))}")
+    for name, a in arrays.items():
+        if a is not None and a.shape != tuple(shape_of[name]):
+            raise ValueError(f"{name} has shape {a.shape}, expected {tuple(shape_of[name])}")
+    return BF16 if next(iter(types)) == np.uint16 else F32
+
+
+class _Bufs:
+    """The device buffers of one call, freed together."""
+
+    def __init__(self):
+        self.all: list[DevBuf] = []
+
+    def up(self, a, name="array", shape=None) -> DevBuf | None:
+        """Upload (None stays None); parameters and states as float32."""
+        if a is None:
+            return None
+        b = DevBuf.from_array(a if shape is None else _mat(a, name, shape))
+        self.all.append(b)
+        return b
+
+    def lens(self, lens, batch: int) -> DevBuf | None:
+        if lens is None:
+            return None
+        a = np.ascontiguousarray(lens, dtype=np.int32)
+        if a.shape != (batch,):
+            raise ValueError(f"lens has shape {a.shape}, expected {(batch,)}")
+        return self.up(a)
+
+    def new(self, nbytes: int) -> DevBuf:
+        b = DevBuf(nbytes)
+        self.all.append(b)
+        return b
+
+    def free(self) -> None:
+        for b in self.all:
+            b.free()
+        self.all = []
+
+
+class SsmDev:
+    """The forward state of Gpu.ssm_scan on the device for its backward: the
+    inputs and the workspace of kept states."""
+
+    def __init__(self, bufs, ins, dims, softplus, dtype):
+        self.bufs, self.ins, self.dims, self.softplus, self.dtype = bufs, ins, dims, softplus, dtype
+
+    def free(self) -> None:
+        self.bufs.free()
+
+
+class GradList:
+    """Gradient tensors in device memory (pairs of DevBuf or address, and size in
+    elements), for their global norm and their clipping by it; `dst` receives the
+    clipped values (None: in place)."""
+
+    def __init__(self, src, dst=None, dtype: int = F32):
+        src = list(src)
+        n = len(src)
+        addr = lambda t: (C.c_void_p * max(n, 1))(*[_vp(b).value for b in t])  # noqa: E731
+        sizes = (C.c_uint64 * max(n, 1))(*[int(k) for _, k in src])
+        if dst is not None and len(dst) != n:
+            raise ValueError(f"{len(dst)} destinations for {n} tensors")
+        h = C.c_void_p()
+        _lib.call("asca_grads_create", addr([b for b, _ in src]), addr(dst) if dst is not None else None, sizes, n, dtype,
+                  C.byref(h))
+        self._h, self._out, self._keep = h, DevBuf(8), (src, dst)
+
+    def norm(self, stream=None) -> float:
+        """The 2-norm over all the tensors (synchronises)."""
+        _lib.call("asca_grads_norm", self._h, _vp(self._out), stream)
+        _lib.call("asca_stream_sync", stream)
+        return float(self._out.to_host((2,))[0])
+
+    def clip(self, max_norm: float, sync: bool = True, stream=None):
+        """Scale by min(1, max_norm / (norm + 1e-6)); (norm, factor), or None without sync."""
+        _lib.call("asca_grads_clip", self._h, max_norm, _vp(self._out), stream)
+        if not sync:
+            return None
+        _lib.call("asca_stream_sync", stream)
+        n, c = self._out.to_host((2,))
+        return float(n), float(c)
+
+    def close(self) -> None:
+        if self._h:
+            _lib.call("asca_grads_destroy", self._h)
+            self._h = None
+            self._out.free()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class ChunkDev:
@@ -720,6 +825,174 @@ class Gpu:
         finally:
             for b in (bdo, *outs):
                 b.free()
+
+    # -- state space block ----------------------------------------------------
+    def conv(self, x, w, bias=None, *, batch: int, state=None, lens=None, silu: bool = True):
+        """Causal depthwise convolution over (batch*T, D) rows (asca_conv_fwd); w
+        (W, D), state (batch, W-1, D).  Returns (y, the state after the last row)."""
+        rows, D = x.shape
+        T, W = rows // max(batch, 1), w.shape[0]
+        ty = _acts({"x": (batch * T, D)}, x=x)
+        b = _Bufs()
+        try:
+            y, so = b.new(x.nbytes), b.new(batch * (W - 1) * D * 4)
+            _lib.call("asca_conv_fwd", _vp(b.up(x)), D, _vp(b.up(w, "w", (W, D))), _vp(b.up(bias, "bias", (D,))),
+                      _vp(b.up(state, "state", (batch, W - 1, D))), _vp(b.lens(lens, batch)), _vp(y), D, _vp(so), batch, T, D,
+                      W, int(silu), ty, None)
+            _lib.call("asca_sync")
+            return y.to_host(x.shape, x.dtype), so.to_host((batch, W - 1, D))
+        finally:
+            b.free()
+
+    def conv_bwd(self, x, w, bias, dy, *, batch: int, state=None, lens=None, dstate_out=None, silu: bool = True):
+        """Its gradients (dx, dw, dbias, dstate_in) from dy and dstate_out (asca_conv_bwd)."""
+        rows, D = x.shape
+        T, W = rows // max(batch, 1), w.shape[0]
+        ty = _acts({"x": (batch * T, D), "dy": (batch * T, D)}, x=x, dy=dy)
+        b = _Bufs()
+        try:
+            dx, dw, db, ds = b.new(x.nbytes), b.new(W * D * 4), b.new(D * 4), b.new(batch * (W - 1) * D * 4)
+            _lib.call("asca_conv_bwd", _vp(b.up(x)), D, _vp(b.up(w, "w", (W, D))), _vp(b.up(bias, "bias", (D,))),
+                      _vp(b.up(state, "state", (batch, W - 1, D))), _vp(b.lens(lens, batch)), _vp(b.up(dy)), D,
+                      _vp(b.up(dstate_out, "dstate_out", (batch, W - 1, D))), _vp(dx), D, _vp(dw), _vp(db), _vp(ds), batch, T,
+                      D, W, int(silu), ty, None)
+            _lib.call("asca_sync")
+            return (dx.to_host(x.shape, x.dtype), dw.to_host((W, D)), db.to_host((D,)), ds.to_host((batch, W - 1, D)))
+        finally:
+            b.free()
+
+    def conv_step(self, state: DevBuf, x, w, bias=None, silu: bool = True):
+        """One row of n sequences on their device states (n, W-1, D), in place (asca_conv_step)."""
+        n, D = x.shape
+        W = w.shape[0]
+        if state.nbytes < n * (W - 1) * D * 4:
+            raise ValueError(f"state of {state.nbytes} bytes for n={n} W={W} D={D}")
+        ty = _acts({"x": (n, D)}, x=x)
+        b = _Bufs()
+        try:
+            y = b.new(x.nbytes)
+            _lib.call("asca_conv_step", _vp(state), _vp(b.up(x)), D, _vp(b.up(w, "w", (W, D))), _vp(b.up(bias, "bias", (D,))),
+                      _vp(y), D, n, D, W, int(silu), ty, None)
+            _lib.call("asca_sync")
+            return y.to_host(x.shape, x.dtype)
+        finally:
+            b.free()
+
+    def ssm_scan(self, x, dt, A, Bm, Cm, *, batch: int, dt_bias=None, Dk=None, h0=None, lens=None, groups: int = 1,
+                 softplus: bool = True, keep: bool = True):
+        """Selective state space scan over (batch*T, D) rows (asca_ssm_fwd); A (N, D),
+        Bm, Cm (batch*T, groups*N), h0 (batch, N, D).  Returns (y, the state after the
+        last row, the SsmDev for ssm_scan_bwd or None without `keep`)."""
+        rows, D = x.shape
+        T, N = rows // max(batch, 1), A.shape[0]
+        gn = (batch * T, groups * N)
+        ty = _acts({"x": (batch * T, D), "dt": (batch * T, D), "Bm": gn, "Cm": gn}, x=x, dt=dt, Bm=Bm, Cm=Cm)
+        dims = (batch, T, D, N, groups)
+        b, out = _Bufs(), _Bufs()
+        try:
+            ws = None
+            if keep:
+                n = C.c_size_t()
+                _lib.call("asca_ssm_ws_bytes", batch, T, D, N, C.byref(n))
+                ws = b.new(n.value)
+            ins = dict(x=b.up(x), dt=b.up(dt), bias=b.up(dt_bias, "dt_bias", (D,)), A=b.up(A, "A", (N, D)), Bm=b.up(Bm),
+                       Cm=b.up(Cm), Dk=b.up(Dk, "Dk", (D,)), lens=b.lens(lens, batch), ws=ws)
+            y, ho = out.new(x.nbytes), out.new(batch * N * D * 4)
+            _lib.call("asca_ssm_fwd", _vp(ins["x"]), D, _vp(ins["dt"]), D, _vp(ins["bias"]), _vp(ins["A"]), _vp(ins["Bm"]), gn[1],
+                      _vp(ins["Cm"]), gn[1], _vp(ins["Dk"]), _vp(out.up(h0, "h0", (batch, N, D))), _vp(ins["lens"]), _vp(y), D,
+                      _vp(ho), _vp(ws), *dims, int(softplus), ty, None)
+            _lib.call("asca_sync")
+            res = y.to_host(x.shape, x.dtype), ho.to_host((batch, N, D))
+        except BaseException:
+            b.free()
+            raise
+        finally:
+            out.free()
+        if keep:
+            return (*res, SsmDev(b, ins, dims, softplus, ty))
+        b.free()
+        return (*res, None)
+
+    def ssm_scan_bwd(self, dev: SsmDev, dy, dh_out=None) -> dict:
+        """The gradients of ssm_scan (asca_ssm_bwd): dx, ddt, dB, dC in the rows'
+        type, ddt_bias, dA, dDk, dh0 in float32."""
+        batch, T, D, N, groups = dev.dims
+        rows, gn, ins = batch * T, groups * N, dev.ins
+        if _acts({"dy": (rows, D)}, dy=dy) != dev.dtype:
+            raise ValueError("dy must have the forward's element type")
+        b = _Bufs()
+        try:
+            size = dy.itemsize
+            o = dict(dx=((rows, D), size), ddt=((rows, D), size), ddt_bias=((D,), 4), dA=((N, D), 4), dB=((rows, gn), size),
+                     dC=((rows, gn), size), dDk=((D,), 4), dh0=((batch, N, D), 4))
+            g = {k: b.new(int(np.prod(sh)) * sz) for k, (sh, sz) in o.items()}
+            _lib.call("asca_ssm_bwd", _vp(ins["x"]), D, _vp(ins["dt"]), D, _vp(ins["bias"]), _vp(ins["A"]), _vp(ins["Bm"]), gn,
+                      _vp(ins["Cm"]), gn, _vp(ins["Dk"]), _vp(ins["lens"]), _vp(b.up(dy)), D,
+                      _vp(b.up(dh_out, "dh_out", (batch, N, D))), _vp(ins["ws"]), _vp(g["dx"]), D, _vp(g["ddt"]), D,
+                      _vp(g["ddt_bias"]), _vp(g["dA"]), _vp(g["dB"]), gn, _vp(g["dC"]), gn, _vp(g["dDk"]), _vp(g["dh0"]),
+                      *dev.dims, int(dev.softplus), dev.dtype, None)
+            _lib.call("asca_sync")
+            return {k: g[k].to_host(sh, dy.dtype if sz == size and k in ("dx", "ddt", "dB", "dC") else _f32)
+                    for k, (sh, sz) in o.items()}
+        finally:
+            b.free()
+
+    def ssm_step(self, h: DevBuf, x, dt, A, Bm, Cm, *, dt_bias=None, Dk=None, groups: int = 1, softplus: bool = True):
+        """One row of n sequences on their device states (n, N, D), in place (asca_ssm_step)."""
+        n, D = x.shape
+        N = A.shape[0]
+        if h.nbytes < n * N * D * 4:
+            raise ValueError(f"states of {h.nbytes} bytes for n={n} N={N} D={D}")
+        gn = groups * N
+        ty = _acts({"x": (n, D), "dt": (n, D), "Bm": (n, gn), "Cm": (n, gn)}, x=x, dt=dt, Bm=Bm, Cm=Cm)
+        b = _Bufs()
+        try:
+            y = b.new(x.nbytes)
+            _lib.call("asca_ssm_step", _vp(h), _vp(b.up(x)), D, _vp(b.up(dt)), D, _vp(b.up(dt_bias, "dt_bias", (D,))),
+                      _vp(b.up(A, "A", (N, D))), _vp(b.up(Bm)), gn, _vp(b.up(Cm)), gn, _vp(b.up(Dk, "Dk", (D,))), _vp(y), D, n, D,
+                      N, groups, int(softplus), ty, None)
+            _lib.call("asca_sync")
+            return y.to_host(x.shape, x.dtype)
+        finally:
+            b.free()
+
+    def block_norm(self, x, y=None, z=None, *, w_post=None, scale=None, w_pre=None, eps: float = 1e-6):
+        """r = x + scale o (rms(y o silu(z)) o w_post) and n = rms(r) o w_pre of
+        (rows, cols) matrices (asca_block_norm_fwd); returns (r, n)."""
+        a = x if x is not None else y
+        rows, cols = a.shape
+        ty = _acts({k: a.shape for k in "xyz"}, x=x, y=y, z=z)
+        b = _Bufs()
+        try:
+            r, n = b.new(a.nbytes), b.new(a.nbytes)
+            _lib.call("asca_block_norm_fwd", _vp(b.up(x)), cols, _vp(b.up(y)), cols, _vp(b.up(z)), cols,
+                      _vp(b.up(w_post, "w_post", (cols,))), _vp(b.up(scale, "scale", (cols,))),
+                      _vp(b.up(w_pre, "w_pre", (cols,))), _vp(r), cols, _vp(n), cols, rows, cols, eps, ty, None)
+            _lib.call("asca_sync")
+            return r.to_host(a.shape, a.dtype), n.to_host(a.shape, a.dtype)
+        finally:
+            b.free()
+
+    def block_norm_bwd(self, x, y, z, dr, dn, *, w_post=None, scale=None, w_pre=None, eps: float = 1e-6) -> dict:
+        """The gradients dx, dy, dz, dw_post, dscale, dw_pre of block_norm from dr and
+        dn (asca_block_norm_bwd), for the inputs that are given."""
+        a = x if x is not None else y
+        rows, cols = a.shape
+        ty = _acts({k: a.shape for k in ("x", "y", "z", "dr", "dn")}, x=x, y=y, z=z, dr=dr, dn=dn)
+        b = _Bufs()
+        try:
+            g = {"d" + k: b.new(a.nbytes) for k, m in (("x", x), ("y", y), ("z", z)) if m is not None}
+            g.update({"d" + k: b.new(cols * 4) for k, m in (("w_post", w_post), ("scale", scale), ("w_pre", w_pre))
+                      if m is not None})
+            at = lambda k: _vp(g.get(k))  # noqa: E731
+            _lib.call("asca_block_norm_bwd", _vp(b.up(x)), cols, _vp(b.up(y)), cols, _vp(b.up(z)), cols,
+                      _vp(b.up(w_post, "w_post", (cols,))), _vp(b.up(scale, "scale", (cols,))),
+                      _vp(b.up(w_pre, "w_pre", (cols,))), _vp(b.up(dr)), cols, _vp(b.up(dn)), cols, at("dx"), cols, at("dy"),
+                      cols, at("dz"), cols, at("dw_post"), at("dscale"), at("dw_pre"), rows, cols, eps, ty, None)
+            _lib.call("asca_sync")
+            return {k: v.to_host(a.shape, a.dtype) if k in ("dx", "dy", "dz") else v.to_host((cols,)) for k, v in g.items()}
+        finally:
+            b.free()
 
     # -- decode -------------------------------------------------------------
     def new_decode_states(self, n_seq: int, n_heads: int, dh: int) -> DevBuf:

@@ -45,6 +45,12 @@ enum {
                                   after updating some tensors (see there)        */
 };
 
+/* Element types of the activation rows of the state space block's operators. */
+enum {
+    ASCA_F32 = 0,
+    ASCA_BF16 = 1,   /* raw 16-bit patterns */
+};
+
 /* ------------------------------------------------------------ runtime ---- */
 
 /* Message of the calling thread's last error ("" if none). */
@@ -498,6 +504,113 @@ ASCA_API int asca_model_train_step(asca_model* model, const uint32_t* ids, const
 ASCA_API int asca_model_decode_state_floats(const asca_model* model, size_t* per_seq);
 ASCA_API int asca_model_decode_step(asca_model* model, const uint32_t* ids, int n_seq, float* states,
                                    float* logits, void* stream);
+
+/* ------------------------------------------------ state space block -- */
+
+/* The operators of an attention-free block whose state decays per channel and
+ * state by the token (a selective state space scan behind a short causal
+ * convolution), beside the delta block.  The reference has no counterpart.
+ *   - Rows are tokens as everywhere (row b*T + t); activation rows are f32 or
+ *     bf16 (`dtype`, ASCA_F32 / ASCA_BF16, one type a call) of any alignment,
+ *     each matrix with its own row stride `ld*` in elements, so that they can be
+ *     columns of a wider one.  Parameters, states and the gradients of both are
+ *     f32.  All arithmetic is f32; a bf16 result is rounded once, at its store.
+ *   - lens (device int32, one per sequence, NULL = all T): sequence b has
+ *     min(max(lens[b], 0), T) rows.  Its further rows are not read; their
+ *     outputs and gradients are zero.
+ *   - Inputs and outputs must not overlap unless stated.  Results are
+ *     deterministic (no atomics).
+ *   - What a call needs for itself comes from the scratch that the library keeps
+ *     for each stream (see asca_delta_ws_bytes). */
+
+/* Causal depthwise convolution of width W (2..8):
+ *   p_t = bias + sum_j w_j x_{t-W+1+j},  y = silu(p) with `silu`, else p.
+ *   x, y : (B*T, D);  w : (W, D);  bias : (D) or NULL
+ *   state_in : (B, W-1, D), the rows before row 0, oldest first (NULL = zeros)
+ *   state_out: (B, W-1, D) or NULL: the last W-1 rows of each sequence, those of
+ *              state_in among them where it is shorter. */
+ASCA_API int asca_conv_fwd(const void* x, long ldx, const float* w, const float* bias, const float* state_in,
+                           const int32_t* lens, void* y, long ldy, float* state_out, int B, int T, int D, int W,
+                           int silu, int dtype, void* stream);
+/* Its backward from dy and dstate_out (NULL = zeros; may be the gradient of
+ * state_out): dx, dw (W, D), dbias (D, NULL without), dstate_in (NULL = not
+ * wanted).  x, w, bias, state_in and lens are the forward's. */
+ASCA_API int asca_conv_bwd(const void* x, long ldx, const float* w, const float* bias, const float* state_in,
+                           const int32_t* lens, const void* dy, long lddy, const float* dstate_out, void* dx,
+                           long lddx, float* dw, float* dbias, float* dstate_in, int B, int T, int D, int W,
+                           int silu, int dtype, void* stream);
+/* One row for each of n sequences: y from state (n, W-1, D) and x (n, D); the
+ * state drops its oldest row and takes x in, in place. */
+ASCA_API int asca_conv_step(float* state, const void* x, long ldx, const float* w, const float* bias, void* y,
+                            long ldy, int n, int D, int W, int silu, int dtype, void* stream);
+
+/* Bytes of the workspace that asca_ssm_fwd leaves for asca_ssm_bwd: the state
+ * before every K-th row (K = 16 at N <= 16, 8 at N <= 32, else 4), which is
+ * B * ceil(T/K) * 4 ceil(N/4) * D floats. */
+ASCA_API int asca_ssm_ws_bytes(int B, int T, int D, int N, size_t* bytes);
+
+/* Selective state space scan, N states (1..64) for each of D channels:
+ *   v = dt + dt_bias;  e = softplus(v) with `softplus`, else v
+ *   h_tn = exp(e_t A_n) h_{t-1,n} + e_t x_t B_tn;  y_t = sum_n C_tn h_tn + Dk x_t
+ *   x, dt, y : (B*T, D);  A : (N, D);  dt_bias, Dk : (D) or NULL (zeros)
+ *   Bm, Cm   : (B*T, G*N); channels g*D/G .. (g+1)*D/G - 1 use columns
+ *              g*N .. (g+1)*N - 1 (D a multiple of G)
+ *   h0       : (B, N, D) state before row 0 (NULL = zeros)
+ *   h_out    : (B, N, D) state after the sequence's last row, or NULL
+ *   ws       : asca_ssm_ws_bytes bytes for a backward, or NULL without one */
+ASCA_API int asca_ssm_fwd(const void* x, long ldx, const void* dt, long lddt, const float* dt_bias, const float* A,
+                          const void* Bm, long ldb, const void* Cm, long ldc, const float* Dk, const float* h0,
+                          const int32_t* lens, void* y, long ldy, float* h_out, void* ws, int B, int T, int D,
+                          int N, int G, int softplus, int dtype, void* stream);
+/* Its backward from dy and dh_out (gradient of h_out, NULL = zeros), on the
+ * forward's inputs and workspace (read only):
+ *   dx, ddt (B*T, D), dB, dC (B*T, G*N), all of `dtype`; ddt_bias, dDk (D, NULL
+ *   without), dA (N, D), dh0 (B, N, D; NULL = not wanted). */
+ASCA_API int asca_ssm_bwd(const void* x, long ldx, const void* dt, long lddt, const float* dt_bias, const float* A,
+                          const void* Bm, long ldb, const void* Cm, long ldc, const float* Dk, const int32_t* lens,
+                          const void* dy, long lddy, const float* dh_out, const void* ws, void* dx, long lddx,
+                          void* ddt, long ldddt, float* ddt_bias, float* dA, void* dB, long lddb, void* dC,
+                          long lddc, float* dDk, float* dh0, int B, int T, int D, int N, int G, int softplus,
+                          int dtype, void* stream);
+/* One row for each of n sequences on their states h (n, N, D), in place. */
+ASCA_API int asca_ssm_step(float* h, const void* x, long ldx, const void* dt, long lddt, const float* dt_bias,
+                           const float* A, const void* Bm, long ldb, const void* Cm, long ldc, const float* Dk,
+                           void* y, long ldy, int n, int D, int N, int G, int softplus, int dtype, void* stream);
+
+/* The norms around a block, with its gate and residual scale, per row (rms(a) =
+ * a / sqrt(mean(a^2) + eps)):
+ *   u = y o silu(z);  r = x + scale o rms(u) o w_post;  n = rms(r) o w_pre
+ *   x : the residual stream (NULL = zeros); y : the block's output; z : its gate
+ *   (NULL = no gate); w_post, scale, w_pre : (cols), NULL = ones
+ *   y NULL: r = x (the norm before the first block; z, w_post, scale NULL too)
+ *   r, n : outputs, either may be NULL.  n is formed from the unrounded r.
+ *   1 <= cols <= 16384.  r may be x. */
+ASCA_API int asca_block_norm_fwd(const void* x, long ldx, const void* y, long ldy, const void* z, long ldz,
+                                 const float* w_post, const float* scale, const float* w_pre, void* r, long ldr,
+                                 void* n, long ldn, long rows, int cols, float eps, int dtype, void* stream);
+/* Its backward from dr and dn (either may be NULL = zeros) on the forward's
+ * inputs: dx, dy, dz and dw_post, dscale, dw_pre, each NULL where not wanted or
+ * where the forward's input is NULL.  dx may be dr. */
+ASCA_API int asca_block_norm_bwd(const void* x, long ldx, const void* y, long ldy, const void* z, long ldz,
+                                 const float* w_post, const float* scale, const float* w_pre, const void* dr,
+                                 long lddr, const void* dn, long lddn, void* dx, long lddx, void* dy, long lddy,
+                                 void* dz, long lddz, float* dw_post, float* dscale, float* dw_pre, long rows,
+                                 int cols, float eps, int dtype, void* stream);
+
+/* A list of `count` gradient tensors src[i] of sizes[i] elements (device
+ * pointers of `dtype` elements in host arrays, which the call copies) for the
+ * calls below, and where they go when clipped (dst[i]; dst NULL = in place).
+ * The list holds device memory of its own until asca_grads_destroy; calls on
+ * one list must not overlap. */
+ASCA_API int asca_grads_create(void** src, void** dst, const uint64_t* sizes, int count, int dtype, void** grads);
+ASCA_API int asca_grads_destroy(void* grads);
+/* out[0] (device) = the 2-norm over all the tensors, its squares summed in 64
+ * bits (no finite gradients overflow it before the norm itself does). */
+ASCA_API int asca_grads_norm(void* grads, float* out, void* stream);
+/* The norm as above into out[0], the factor c = min(1, max_norm / (norm + 1e-6))
+ * into out[1], and dst = c src.  A norm that is not finite gives c = 0 (an
+ * infinite one) or NaN, and what c src then is: the caller sees it in out. */
+ASCA_API int asca_grads_clip(void* grads, float max_norm, float* out, void* stream);
 
 #ifdef __cplusplus
 }

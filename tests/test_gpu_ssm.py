@@ -1,0 +1,518 @@
+"""GPU parity of the state space block's operators (causal convolution, selective
+scan, block norms, gradient clipping) against the float64 oracle, through the
+operator API and the C ABI.
+
+Tolerances (max|d| / max|ref|, as elsewhere): 2e-5 for f32 forwards and 1e-4 for
+f32 gradients; a bf16 result may be half a unit of its 8-bit significand off the
+oracle's (2^-9 of itself) and is allowed twice that, 2^-8, for what f32 arithmetic
+moves it over a rounding boundary."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from oracle import ssm_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+FWD, GRAD, BF = 2e-5, 1e-4, 2.0 ** -8
+
+
+def err(got, ref):
+    got, ref = np.asarray(got, np.float64), np.asarray(ref, np.float64)
+    assert got.shape == ref.shape and np.isfinite(got).all()
+    m = np.abs(ref).max() if ref.size else 0.0
+    d = np.abs(got - ref).max() if ref.size else 0.0
+    return d / m if m else d
+
+
+class Rows:
+    """Random activation rows in a type: what the device gets, and its float64 values."""
+
+    def __init__(self, rng, bf16):
+        from asca_amd import gpu
+
+        self.rng, self.bf16, self.g = rng, bf16, gpu
+
+    def __call__(self, *shape, scale=1.0):
+        a = (self.rng.standard_normal(shape) * scale).astype(np.float32)
+        return self.dev(a)
+
+    def dev(self, a):
+        return self.g.to_bf16(a) if self.bf16 else a
+
+    def val(self, a):
+        return self.g.from_bf16(a) if a is not None and a.dtype == np.uint16 else a
+
+    def tol(self, base):
+        return BF if self.bf16 else base
+
+
+def check(label, pairs):
+    worst = {k: err(a, b) for k, a, b, _ in pairs}
+    print(f"[{label}] " + " ".join(f"{k} {v:.1e}" for k, v in worst.items()), flush=True)
+    for k, _, _, tol in pairs:
+        assert worst[k] <= tol, (k, worst[k], tol)
+
+
+def ragged(B, T):
+    """Lengths from zero and one to all of T, and values outside 0..T."""
+    return [[T, 0, 1, T + 5, -3, T // 2, max(T - 1, 0)][i % 7] for i in range(B)]
+
+
+# ------------------------------------------------------------- convolution
+
+CONV = [(1, 1, 1, 4, False), (2, 3, 5, 4, True), (7, 40, 64, 4, True), (2, 70, 130, 2, True), (3, 65, 33, 3, False),
+        (2, 129, 257, 4, False), (2, 33, 20, 8, True), (1, 10, 7, 5, False), (1, 9, 68, 6, True), (2, 9, 12, 7, True),
+        (1, 1000, 512, 4, False), (4, 2, 16, 4, True)]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("B,T,D,W,rag", CONV)
+def test_conv(g, B, T, D, W, rag, bf16):
+    print(f"[conv] B={B} T={T} D={D} W={W} ragged={rag} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(B * 1000 + T + D + W)
+    r = Rows(rng, bf16)
+    x, dy, w, bias = r(B * T, D), r(B * T, D), rng.standard_normal((W, D)).astype(np.float32), rng.standard_normal(D).astype(np.float32)
+    st, ds = (rng.standard_normal((B, W - 1, D)).astype(np.float32) for _ in range(2))
+    lens = ragged(B, T) if rag else None
+    for silu in (True, False):
+        y, s = g.conv(x, w, bias, batch=B, state=st, lens=lens, silu=silu)
+        ry, rs = so.conv(r.val(x), w, bias, B, st, lens, silu)
+        got = g.conv_bwd(x, w, bias, dy, batch=B, state=st, lens=lens, dstate_out=ds, silu=silu)
+        ref = so.conv_bwd(r.val(x), w, bias, r.val(dy), B, st, lens, ds, silu)
+        check("conv", [("y", r.val(y), ry, r.tol(FWD)), ("state", s, rs, 0.0), ("dx", r.val(got[0]), ref[0], r.tol(GRAD)),
+                       ("dw", got[1], ref[1], GRAD), ("db", got[2], ref[2], GRAD), ("ds", got[3], ref[3], GRAD)])
+
+
+def test_conv_without_bias_and_state(g):
+    rng = np.random.default_rng(1)
+    x, dy, w = (rng.standard_normal(s).astype(np.float32) for s in ((60, 33), (60, 33), (4, 33)))
+    y, s = g.conv(x, w, batch=2)
+    got = g.conv_bwd(x, w, None, dy, batch=2)
+    ref = so.conv_bwd(x, w, None, dy, 2)
+    ry, rs = so.conv(x, w, None, 2)
+    check("conv plain", [("y", y, ry, FWD), ("state", s, rs, 0.0)] + [(k, a, b, GRAD) for k, a, b in zip(("dx", "dw", "db"), got, ref)])
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n,D,W", [(1, 1, 2), (1, 512, 4), (5, 100, 3), (70, 257, 4), (3, 36, 8)])
+def test_conv_step_goes_on_from_a_prompt(g, n, D, W, bf16):
+    rng = np.random.default_rng(n + D)
+    r = Rows(rng, bf16)
+    T = 6
+    x, w, bias = r(n * T, D), rng.standard_normal((W, D)).astype(np.float32), rng.standard_normal(D).astype(np.float32)
+    ref, last = so.conv(r.val(x), w, bias, n)
+    from asca_amd.gpu import DevBuf
+
+    st = DevBuf.from_host(np.zeros((n, W - 1, D), np.float32))
+    for t in range(T):
+        y = g.conv_step(st, np.ascontiguousarray(x.reshape(n, T, D)[:, t]), w, bias)
+        check(f"conv step {t}", [("y", r.val(y), ref.reshape(n, T, D)[:, t], r.tol(FWD))])
+    np.testing.assert_array_equal(st.to_host((n, W - 1, D)), last.astype(np.float32))
+
+
+# -------------------------------------------------------------------- scan
+
+SSM = [(1, 1, 1, 1, 1, False), (2, 5, 3, 4, 1, True), (1, 16, 16, 16, 1, False), (7, 33, 70, 16, 1, True),
+       (2, 100, 130, 12, 2, True), (1, 257, 64, 8, 4, False), (2, 40, 65, 32, 1, True), (1, 37, 20, 64, 2, False),
+       (2, 300, 48, 5, 3, False), (1, 700, 33, 16, 1, False), (2, 64, 256, 16, 1, True), (3, 21, 50, 2, 1, True),
+       (1, 19, 17, 33, 1, False), (2, 1100, 64, 16, 1, True), (1, 2050, 20, 4, 1, False)]
+
+
+def ssm_inputs(r, rng, B, T, D, N, G):
+    """Steps e of about 0.001 to 0.1 and one in twenty around 1; A near -1 .. -N."""
+    e = np.exp(rng.uniform(np.log(1e-3), np.log(1e-1), D))
+    dtv = rng.standard_normal((B * T, D)) + np.where(rng.random((B * T, D)) < 0.05, 4.0, 0.0)
+    return dict(x=r(B * T, D), dt=r.dev(dtv.astype(np.float32)), Bm=r(B * T, G * N), Cm=r(B * T, G * N),
+                A=(-np.arange(1, N + 1)[:, None] * np.exp(0.1 * rng.standard_normal((N, D)))).astype(np.float32),
+                dt_bias=np.log(np.expm1(e)).astype(np.float32), Dk=rng.standard_normal(D).astype(np.float32))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("B,T,D,N,G,rag", SSM)
+def test_ssm(g, B, T, D, N, G, rag, bf16):
+    print(f"[ssm] B={B} T={T} D={D} N={N} G={G} ragged={rag} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(B * 1000 + T + D + N)
+    r = Rows(rng, bf16)
+    i = ssm_inputs(r, rng, B, T, D, N, G)
+    v = {k: r.val(a) for k, a in i.items()}
+    h0, dh = (rng.standard_normal((B, N, D)).astype(np.float32) for _ in range(2))
+    dy, lens = r(B * T, D), ragged(B, T) if rag else None
+    y, h, dev = g.ssm_scan(**i, batch=B, h0=h0, lens=lens, groups=G)
+    ry, rh = so.ssm(**v, B=B, h0=h0, lens=lens, G=G)
+    y2, h2, none = g.ssm_scan(**i, batch=B, h0=h0, lens=lens, groups=G, keep=False)
+    assert none is None
+    np.testing.assert_array_equal(y2, y)
+    np.testing.assert_array_equal(h2, h)
+    got = g.ssm_scan_bwd(dev, dy, dh)
+    again = g.ssm_scan_bwd(dev, dy, dh)
+    ref = so.ssm_bwd(**v, dy=r.val(dy), B=B, h0=h0, lens=lens, G=G, dh_out=dh)
+    dev.free()
+    rows = ("dx", "ddt", "dB", "dC")
+    check("ssm", [("y", r.val(y), ry, r.tol(FWD)), ("h", h, rh, FWD)] +
+          [(k, r.val(got[k]), ref[k], r.tol(GRAD) if k in rows else GRAD) for k in ref])
+    for k in got:
+        np.testing.assert_array_equal(got[k], again[k])
+
+
+def test_ssm_without_softplus_bias_skip_and_states(g):
+    rng = np.random.default_rng(5)
+    B, T, D, N = 2, 37, 40, 16
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    i = dict(x=f(B * T, D), dt=rng.uniform(0.01, 0.3, (B * T, D)).astype(np.float32), A=-rng.uniform(0.5, 8, (N, D)).astype(np.float32),
+             Bm=f(B * T, N), Cm=f(B * T, N))
+    dy = f(B * T, D)
+    y, h, dev = g.ssm_scan(**i, batch=B, softplus=False)
+    ry, rh = so.ssm(**i, B=B, softplus=False)
+    got, ref = g.ssm_scan_bwd(dev, dy), so.ssm_bwd(**i, dy=dy, B=B, softplus=False)
+    check("ssm plain", [("y", y, ry, FWD), ("h", h, rh, FWD)] + [(k, got[k], ref[k], GRAD) for k in ref])
+
+
+def test_ssm_cut_in_two_is_the_sequence(g):
+    rng = np.random.default_rng(6)
+    r = Rows(rng, False)
+    T, D, N, k = 50, 20, 16, 19
+    i = ssm_inputs(r, rng, 1, T, D, N, 1)
+    cut = lambda s: {n: a[s] if n in ("x", "dt", "Bm", "Cm") else a for n, a in i.items()}  # noqa: E731
+    y, h, _ = g.ssm_scan(**i, batch=1, keep=False)
+    y1, h1, _ = g.ssm_scan(**cut(slice(0, k)), batch=1, keep=False)
+    y2, h2, _ = g.ssm_scan(**cut(slice(k, T)), batch=1, h0=h1, keep=False)
+    check("cut", [("y", np.concatenate([y1, y2]), y, FWD), ("h", h2, h, FWD)])
+
+
+@pytest.mark.parametrize("v", [-90.0, -20.0, -5.0, 0.0, 5.0, 25.0, 90.0])
+def test_ssm_softplus_over_its_range(g, v):
+    # one row, one state, B = C = 1: y = e x, whatever the size of e
+    one = np.ones((1, 1), np.float32)
+    y, _, _ = g.ssm_scan(one, one * np.float32(v), -one, one, one, batch=1, keep=False)
+    e = np.logaddexp(np.float64(v), 0)
+    assert abs(y[0, 0] - e) <= 2e-6 * e + 1e-38
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n,D,N,G", [(1, 1, 1, 1), (1, 512, 16, 1), (5, 100, 12, 2), (70, 256, 16, 1), (3, 36, 64, 3), (9, 130, 33, 1)])
+def test_ssm_step_goes_on_from_a_prompt(g, n, D, N, G, bf16):
+    from asca_amd.gpu import DevBuf
+
+    rng = np.random.default_rng(n + D + N)
+    r = Rows(rng, bf16)
+    T = 5
+    i = ssm_inputs(r, rng, n, T, D, N, G)
+    ry, rh = so.ssm(**{k: r.val(a) for k, a in i.items()}, B=n, G=G)
+    cut = lambda a, t: np.ascontiguousarray(a.reshape(n, T, -1)[:, t])  # noqa: E731
+    h = DevBuf.from_host(np.zeros((n, N, D), np.float32))
+    for t in range(T):
+        y = g.ssm_step(h, **{k: cut(i[k], t) for k in ("x", "dt", "Bm", "Cm")}, A=i["A"], dt_bias=i["dt_bias"], Dk=i["Dk"], groups=G)
+        check(f"ssm step {t}", [("y", r.val(y), ry.reshape(n, T, D)[:, t], r.tol(FWD))])
+    check("ssm step", [("h", h.to_host((n, N, D)), rh, FWD)])
+
+
+# -------------------------------------------------------------- block norm
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 64), (9, 256), (130, 260), (33, 512), (7, 1000), (5, 1024), (6, 1025), (3, 2048),
+                                       (2, 4099), (2, 8192), (1, 16383), (1030, 36)])
+def test_block_norm(g, rows, cols, bf16):
+    print(f"[norm] rows={rows} cols={cols} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(rows + cols)
+    r = Rows(rng, bf16)
+    x, y, z, dr, dn = (r(rows, cols) for _ in range(5))
+    p = {k: (rng.standard_normal(cols) * 0.3 + 1).astype(np.float32) for k in ("w_post", "scale", "w_pre")}
+    v = r.val
+    got = g.block_norm(x, y, z, **p)
+    ref = so.block_norm(v(x), v(y), v(z), **p)
+    gb, rb = g.block_norm_bwd(x, y, z, dr, dn, **p), so.block_norm_bwd(v(x), v(y), v(z), v(dr), v(dn), **p)
+    check("norm", [("r", v(got[0]), ref[0], r.tol(FWD)), ("n", v(got[1]), ref[1], r.tol(FWD))] +
+          [(k, v(gb[k]), rb[k], r.tol(GRAD) if k in ("dx", "dy", "dz") else GRAD) for k in gb])
+
+
+@pytest.mark.parametrize("have", ["x y z", "x y", "y z", "y", "x"])
+@pytest.mark.parametrize("gains", [True, False])
+@pytest.mark.parametrize("grads", ["dr dn", "dr", "dn"])
+def test_block_norm_parts(g, have, gains, grads):
+    rng = np.random.default_rng(len(have))
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    a = {k: f(10, 48) if k in have.split() else None for k in "xyz"}
+    d = {k: f(10, 48) if k in grads.split() else None for k in ("dr", "dn")}
+    p = {k: f(48) for k in (("w_post", "scale", "w_pre") if "y" in have else ("w_pre",))} if gains else {}
+    got, ref = g.block_norm(*a.values(), **p), so.block_norm(*a.values(), **p)
+    gb, rb = g.block_norm_bwd(*a.values(), *d.values(), **p), so.block_norm_bwd(*a.values(), *d.values(), **p)
+    check(f"norm {have}", [("r", got[0], ref[0], FWD), ("n", got[1], ref[1], FWD)] + [(k, gb[k], rb[k], GRAD) for k in gb])
+
+
+def test_block_norm_of_zero_rows_is_zero(g):
+    z = np.zeros((3, 40), np.float32)
+    r, n = g.block_norm(z, z, z)
+    assert not r.any() and not n.any()
+    o = g.block_norm_bwd(z, z, z, z + 1, None)
+    assert np.isfinite(o["dy"]).all() and (o["dx"] == 1).all()
+
+
+# ---------------------------------------------------------------- clipping
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("sizes", [[1], [3, 0, 5], [4096, 4097, 1, 12289], [7] * 300, [100003], []])
+@pytest.mark.parametrize("place", ["in", "out"])
+def test_grads_clip(g, sizes, bf16, place):
+    from asca_amd import gpu
+
+    rng = np.random.default_rng(sum(sizes) + len(sizes))
+    r = Rows(rng, bf16)
+    host = [r(k, scale=0.1 * (1 + i % 5)) for i, k in enumerate(sizes)]
+    vals = [r.val(h) for h in host]
+    for max_norm in (0.5, 1e6):
+        src = [gpu.DevBuf.from_array(h) for h in host]
+        dst = [gpu.DevBuf(h.nbytes) for h in host] if place == "out" else None
+        gl = gpu.GradList(list(zip(src, sizes)), dst, dtype=gpu.BF16 if bf16 else gpu.F32)
+        want, c, clipped = so.clip(vals, max_norm)
+        assert abs(gl.norm() - want) <= 1e-6 * want
+        norm, coef = gl.clip(max_norm)
+        assert abs(norm - want) <= 1e-6 * want and abs(coef - c) <= 1e-6 * c
+        for h, s, d, e in zip(host, src, dst or src, clipped):
+            if h.size:
+                got = d.to_host(h.shape, h.dtype)
+                assert err(r.val(got), e) <= r.tol(FWD)
+                if place == "out":
+                    np.testing.assert_array_equal(s.to_host(h.shape, h.dtype), h)
+        gl.close()
+
+
+def test_grads_norm_of_large_small_and_infinite_values(g):
+    from asca_amd import gpu
+
+    for val, n in ((1e30, 1000), (1e-30, 1000), (np.inf, 3), (np.nan, 3)):
+        a = np.full(n, val, np.float32)
+        gl = gpu.GradList([(gpu.DevBuf.from_host(a), n)])
+        want = float(np.float32(np.sqrt((a.astype(np.float64) ** 2).sum())))
+        norm, coef = gl.clip(1.0)
+        assert norm == pytest.approx(want, rel=1e-6, nan_ok=True)
+        assert (np.isnan(coef) if np.isnan(val) else coef == 0.0 if np.isinf(val) else coef == pytest.approx(min(1.0, 1 / want), rel=1e-6))
+        gl.close()
+
+
+def test_grads_clip_repeats_bit_for_bit(g):
+    from asca_amd import gpu
+
+    a = np.random.default_rng(2).standard_normal(1 << 20).astype(np.float32)
+    d, o = gpu.DevBuf.from_host(a), gpu.DevBuf(a.nbytes)
+    gl = gpu.GradList([(d, a.size)], [o])
+    first = gl.clip(1.0)
+    want = o.to_host(a.shape)
+    for _ in range(5):
+        assert gl.clip(1.0) == first
+        np.testing.assert_array_equal(o.to_host(a.shape), want)
+    gl.close()
+
+
+# ------------------------------------- strides, streams, offsets, refusals
+
+
+def _p(buf, off=0):
+    return C.c_void_p(buf.ptr + off)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_columns_of_wider_matrices_and_rows_past_a_length(g, bf16):
+    """Every operand a range of columns of a wider matrix that is NaN elsewhere and past
+    each length, at odd offsets; outputs land in theirs and leave the rest alone."""
+    from asca_amd import _lib, gpu
+
+    rng = np.random.default_rng(8)
+    r = Rows(rng, bf16)
+    B, T, D, N, G, ld, at = 3, 37, 66, 12, 2, 131, 13
+    size, ty = (2, 1) if bf16 else (4, 0)
+    lens = np.array([37, 5, 0], np.int32)
+    i = ssm_inputs(r, rng, B, T, D, N, G)
+    dy = r(B * T, D)
+    past = (np.arange(T)[None] >= lens[:, None]).reshape(-1)
+
+    def wide(a):
+        w = r.dev(np.full((B * T, ld), np.nan, np.float32))
+        w[:, at:at + a.shape[1]] = a
+        w[past] = r.dev(np.full(1, np.nan, np.float32))
+        return gpu.DevBuf.from_array(w)
+
+    ins = {k: wide(i[k]) for k in ("x", "dt", "Bm", "Cm")}
+    bdy, blen = wide(dy), gpu.DevBuf.from_array(lens)
+    par = {k: gpu.DevBuf.from_host(i[k]) for k in ("A", "dt_bias", "Dk")}
+    mark = r.dev(np.full((B * T, ld), 7.0, np.float32))
+    out = {k: gpu.DevBuf.from_array(mark) for k in ("y", "dx", "ddt", "dB", "dC")}
+    f = {k: gpu.DevBuf(n * 4) for k, n in (("h", B * N * D), ("dbias", D), ("dA", N * D), ("dD", D), ("dh0", B * N * D))}
+    n = C.c_size_t()
+    _lib.call("asca_ssm_ws_bytes", B, T, D, N, C.byref(n))
+    ws = gpu.DevBuf(n.value)
+    a = at * size
+    st = C.c_void_p()
+    _lib.call("asca_stream_create", C.byref(st))
+    head = (_p(ins["x"], a), ld, _p(ins["dt"], a), ld, _p(par["dt_bias"]), _p(par["A"]), _p(ins["Bm"], a), ld, _p(ins["Cm"], a), ld,
+            _p(par["Dk"]))
+    _lib.call("asca_ssm_fwd", *head, None, _p(blen), _p(out["y"], a), ld, _p(f["h"]), _p(ws), B, T, D, N, G, 1, ty, st)
+    _lib.call("asca_ssm_bwd", *head, _p(blen), _p(bdy, a), ld, None, _p(ws), _p(out["dx"], a), ld, _p(out["ddt"], a), ld,
+              _p(f["dbias"]), _p(f["dA"]), _p(out["dB"], a), ld, _p(out["dC"], a), ld, _p(f["dD"]), _p(f["dh0"]), B, T, D, N, G, 1,
+              ty, st)
+    w, cb = rng.standard_normal((4, D)).astype(np.float32), gpu.DevBuf.from_array(mark)
+    bw = gpu.DevBuf.from_host(w)
+    _lib.call("asca_conv_fwd", _p(ins["x"], a), ld, _p(bw), None, None, _p(blen), _p(cb, a), ld, None, B, T, D, 4, 1, ty, st)
+    _lib.call("asca_stream_sync", st)
+    _lib.call("asca_stream_destroy", st)
+    v = {k: r.val(m) for k, m in i.items()}
+    ry, rh = so.ssm(**v, B=B, lens=lens, G=G)
+    ref = so.ssm_bwd(**v, dy=r.val(dy), B=B, lens=lens, G=G)
+    ref.update(y=ry, conv=so.conv(v["x"], w, None, B, None, lens)[0])
+    pairs = []
+    for k, b in {**out, "conv": cb}.items():
+        m = b.to_host((B * T, ld), mark.dtype)
+        c = ref[k].shape[1]
+        pairs.append((k, r.val(np.ascontiguousarray(m[:, at:at + c])), ref[k], r.tol(FWD if k in ("y", "conv") else GRAD)))
+        assert (m[:, :at] == mark[0, 0]).all() and (m[:, at + c:] == mark[0, 0]).all(), k
+        assert not r.val(np.ascontiguousarray(m[past, at:at + c])).any(), k
+    pairs += [("h", f["h"].to_host((B, N, D)), rh, FWD), ("dA", f["dA"].to_host((N, D)), ref["dA"], GRAD),
+              ("dD", f["dD"].to_host((D,)), ref["dDk"], GRAD), ("dbias", f["dbias"].to_host((D,)), ref["ddt_bias"], GRAD),
+              ("dh0", f["dh0"].to_host((B, N, D)), ref["dh0"], GRAD)]
+    check("wide", pairs)
+
+
+def test_offsets_past_32_bits(g):
+    """Rows 2^30 elements apart: the last of five begins at element 2^32."""
+    from asca_amd import _lib, gpu
+
+    rng = np.random.default_rng(9)
+    r = Rows(rng, True)
+    T, D, N, ld = 5, 64, 16, 1 << 30
+    i = ssm_inputs(r, rng, 1, T, D, N, 1)
+    v = {k: r.val(m) for k, m in i.items()}
+    big = gpu.DevBuf((4 * ld + 4 * 64) * 2)    # x, dt, y and conv's y side by side
+    small = {k: gpu.DevBuf.from_array(i[k]) for k in ("Bm", "Cm", "A", "dt_bias", "Dk")}
+    put = lambda k, c, t: _lib.call("asca_h2d", _p(big, (t * ld + c) * 2), np.ascontiguousarray(i[k][t]).ctypes.data_as(C.c_void_p), D * 2)  # noqa: E731
+    for t in range(T):
+        put("x", 0, t)
+        put("dt", 64, t)
+    w = rng.standard_normal((4, D)).astype(np.float32)
+    bw = gpu.DevBuf.from_host(w)
+    _lib.call("asca_ssm_fwd", _p(big), ld, _p(big, 128), ld, _p(small["dt_bias"]), _p(small["A"]), _p(small["Bm"]), N, _p(small["Cm"]),
+              N, _p(small["Dk"]), None, None, _p(big, 256), ld, None, None, 1, T, D, N, 1, 1, 1, None)
+    _lib.call("asca_conv_fwd", _p(big), ld, _p(bw), None, None, None, _p(big, 384), ld, None, 1, T, D, 4, 1, 1, None)
+    _lib.call("asca_sync")
+
+    def get(c):
+        rows = np.empty((T, D), np.uint16)
+        for t in range(T):
+            _lib.call("asca_d2h", rows[t].ctypes.data_as(C.c_void_p), _p(big, (t * ld + c) * 2), D * 2)
+        return r.val(rows)
+
+    y, c = get(128), get(192)
+    _lib.call("asca_block_norm_fwd", _p(big), ld, _p(big, 128), ld, None, 0, None, None, None, _p(big, 256), ld, None, 0, T, D, 1e-6, 1, None)
+    _lib.call("asca_sync")
+    n = get(128)
+    big.free()
+    _lib.call("asca_pool_release")
+    check("far", [("y", y, so.ssm(**v, B=1)[0], BF), ("conv", c, so.conv(v["x"], w, None, 1)[0], BF),
+                  ("norm", n, so.block_norm(v["x"], v["dt"])[0], BF)])
+
+
+def test_calls_on_two_streams_at_once(g):
+    """Scans, their backwards and the sums that use a stream's scratch, alternating over
+    two streams without a wait between, against the same calls alone."""
+    from asca_amd import _lib, gpu
+
+    rng = np.random.default_rng(10)
+    r = Rows(rng, False)
+    B, T, D, N = 2, 200, 96, 16
+    st = [C.c_void_p() for _ in range(2)]
+    for s in st:
+        _lib.call("asca_stream_create", C.byref(s))
+    cases = []
+    for _ in range(2):
+        i, dy = ssm_inputs(r, rng, B, T, D, N, 1), r(B * T, D)
+        y, h, dev = g.ssm_scan(**i, batch=B)
+        want = g.ssm_scan_bwd(dev, dy)
+        o = {k: gpu.DevBuf(a.nbytes) for k, a in want.items()}
+        cases.append((dev, gpu.DevBuf.from_host(dy), want, o))
+    for _ in range(4):
+        for (dev, bdy, _, o), s in zip(cases, st):
+            q = dev.ins
+            _lib.call("asca_ssm_bwd", _p(q["x"]), D, _p(q["dt"]), D, _p(q["bias"]), _p(q["A"]), _p(q["Bm"]), N, _p(q["Cm"]), N,
+                      _p(q["Dk"]), None, _p(bdy), D, None, _p(q["ws"]), _p(o["dx"]), D, _p(o["ddt"]), D, _p(o["ddt_bias"]),
+                      _p(o["dA"]), _p(o["dB"]), N, _p(o["dC"]), N, _p(o["dDk"]), _p(o["dh0"]), B, T, D, N, 1, 1, 0, s)
+    for s in st:
+        _lib.call("asca_stream_sync", s)
+        _lib.call("asca_stream_destroy", s)
+    for dev, _, want, o in cases:
+        for k in want:
+            np.testing.assert_array_equal(o[k].to_host(want[k].shape), want[k])
+
+
+def test_empty_calls(g):
+    z = lambda *s: np.zeros(s, np.float32)  # noqa: E731
+    w = z(4, 3) + 1
+    y, s = g.conv(z(0, 3), w, batch=2, state=z(2, 3, 3) + 5)    # no rows: the state goes through
+    assert y.shape == (0, 3) and (s == 5).all()
+    dx, dw, db, ds = g.conv_bwd(z(0, 3), w, z(3), z(0, 3), batch=2, dstate_out=z(2, 3, 3) + 2)
+    assert not dw.any() and not db.any() and (ds == 2).all()
+    y, h, dev = g.ssm_scan(z(0, 3), z(0, 3), z(4, 3) - 1, z(0, 4), z(0, 4), batch=2, h0=z(2, 4, 3) + 5)
+    assert (h == 5).all()
+    o = g.ssm_scan_bwd(dev, z(0, 3), z(2, 4, 3) + 2)
+    assert (o["dh0"] == 2).all() and not o["dA"].any() and not o["ddt_bias"].any()
+
+
+def test_refusals(g):
+    """Bad arguments come back as errors that name the call, and nothing is launched."""
+    from asca_amd import _lib, gpu
+
+    f = C.c_void_p(1 << 12)   # never dereferenced: every call is refused before a launch
+    out = C.c_size_t()
+    conv = lambda D=8, ld=8, W=4, ty=0, x=f, w=f, B=1, so_=None: ("asca_conv_fwd", x, ld, w, None, None, None, f, ld, so_, B, 4, D, W, 1, ty, None)  # noqa: E731
+    ssm = lambda D=8, ld=8, N=4, G=1, ty=0, x=f, A=f, h0=None, ho=None: (  # noqa: E731
+        "asca_ssm_fwd", x, ld, f, 8, None, A, f, 64, f, 64, None, h0, None, f, 8, ho, None, 1, 4, D, N, G, 1, ty, None)
+    norm = lambda cols=8, ld=8, ty=0, x=f, y=f, z=f, r=f, w=None: (  # noqa: E731
+        "asca_block_norm_fwd", x, ld, y, 1 << 15, z, 1 << 15, w, None, None, r, 1 << 15, None, 0, 4, cols, 1e-6, ty, None)
+    h = C.c_void_p()
+    one = (C.c_void_p * 1)(None)
+    bad = [(conv(W=1), 3), (conv(W=9), 3), (conv(ty=2), 3), (conv(ld=7), 1), (conv(x=None), 1), (conv(w=None), 1), (conv(B=-1), 1),
+           (("asca_conv_fwd", f, 8, f, None, f, None, f, 8, f, 1, 4, 8, 4, 1, 0, None), 1),
+           (ssm(N=0), 3), (ssm(N=65), 3), (ssm(G=3), 1), (ssm(G=0), 1), (ssm(ty=-1), 3), (ssm(ld=7), 1), (ssm(x=None), 1), (ssm(A=None), 1),
+           (ssm(h0=f, ho=f), 1), (("asca_ssm_ws_bytes", 1, -1, 8, 4, C.byref(out)), 1), (("asca_ssm_ws_bytes", 1, 1, 8, 4, None), 1),
+           (norm(cols=16385, ld=1 << 15), 3), (norm(ld=7), 1), (norm(y=None), 1), (norm(r=None), 1), (norm(ty=7), 3),
+           (norm(x=None, y=None, z=None), 1),
+           (("asca_grads_create", one, None, (C.c_uint64 * 1)(4), 1, 0, C.byref(h)), 1),
+           (("asca_grads_create", None, None, None, -1, 0, C.byref(h)), 1), (("asca_grads_create", None, None, None, 0, 5, C.byref(h)), 3),
+           (("asca_grads_norm", None, f, None), 1), (("asca_grads_clip", None, 1.0, f, None), 1)]
+    gpu.reset_stats()
+    for (name, *args), code in bad:
+        with pytest.raises(_lib.AscaError) as ei:
+            _lib.call(name, *args)
+        assert ei.value.code == code, (name, args, str(ei.value))
+    gl = gpu.GradList([])
+    for m in (-1.0, float("nan")):
+        with pytest.raises(_lib.AscaError):
+            gl.clip(m)
+    assert gpu.stats()[2] == 0
+    x = np.zeros((4, 8), np.float32)
+    with pytest.raises(ValueError):
+        g.ssm_scan(x, x[:3], np.zeros((4, 8)), x[:, :4], x[:, :4], batch=1)
+    with pytest.raises(ValueError):
+        g.conv(x.astype(np.float64), np.zeros((4, 8)), batch=1)
+
+
+@pytest.mark.parametrize("nth", [0, 1, 2])
+def test_an_injected_failure_is_an_error_and_the_next_call_works(g, nth):
+    from asca_amd import _lib, gpu
+
+    rng = np.random.default_rng(11)
+    r = Rows(rng, False)
+    i, dy = ssm_inputs(r, rng, 1, 20, 8, 4, 1), r(20, 8)
+    _, _, dev = g.ssm_scan(**i, batch=1)
+    want = g.ssm_scan_bwd(dev, dy)
+    gpu.fail_after(nth)
+    try:
+        with pytest.raises(_lib.AscaError) as ei:
+            g.ssm_scan_bwd(dev, dy)
+        assert ei.value.code == 5
+    finally:
+        gpu.fail_after(-1)
+    got = g.ssm_scan_bwd(dev, dy)
+    for k in want:
+        np.testing.assert_array_equal(got[k], want[k])
