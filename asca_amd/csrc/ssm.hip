@@ -11,21 +11,26 @@
 // matrices appears: the work is an exponential (a quarter-rate instruction) and
 // a few multiply-adds for each of them, on the vector unit.
 //
-// A wave holds 16 channels by 4 groups of states: lane (q, c) = 16 q + c has the
-// NS = ceil(N/4) states q NS .. of channel c in registers.  Rows go in blocks of K:
-//   - x, dt (dy) of a quad of rows 4i .. 4i+3 are read with lane group q on row
-//     4i + q, so softplus and its like are computed once per (row, channel); two
-//     kinds of row swap (v_permlane32/16_swap) give every group all four rows.
-//   - B and C of a block lie across the 16 lanes of a group, value v = row NS +
-//     state on lane v % 16 of register v / 16, and reach the arithmetic as a DPP
-//     row broadcast.
-//   - sums over states (y, sum g B, sum A p) end on the group that owns the row:
-//     a transposed pair sum, three swaps for four rows.
-//   - sums over channels (dB, dC) are scattered over the 16 lanes as they are
-//     formed, then added over the block's waves through LDS; the tiles' partial
-//     sums are added by a second kernel in a fixed order.
-// The forward leaves the state before every K-th row; the backward computes a
-// block's states and decays again from it and keeps them in registers.
+// A wave holds 8 channels by 8 groups of states, each lane the NS = ceil(N/8)
+// states of its group in registers; a block has NW waves, 8 NW channels of one
+// sequence, and takes its rows in tiles of K:
+//   - a thread reads x, dt (dy) of one channel at K/8 of the tile's rows, so loads
+//     are whole rows and softplus and its like are computed once per (row,
+//     channel); e and e x go through LDS to the lanes that need them, B and C
+//     beside them.  The next tile's loads are in flight while a tile is scanned.
+//   - sums over states (y, sum g B, sum A p) and over channels (dB, dC) are
+//     scattered over the lanes that they are taken across as they are formed (a
+//     row swap or a DPP move and an add for each value that remains), and the
+//     results go through LDS back to the thread that owns the (row, channel), or
+//     are added over the waves there.
+//   - one barrier a tile: everything in LDS has two copies.
+// The forward leaves the state before every tile; the backward computes a tile's
+// states and decays again from it and keeps them in registers.  Partial sums of dB
+// and dC over a block's channels, and of the parameters' gradients over its rows,
+// are added by further kernels in a fixed order.
+// Where sequences and channels give too few blocks the rows are cut into chunks:
+// a first pass leaves what a chunk makes of a zero state (carry) and its sum of e,
+// from which every chunk works out what enters it, exp(A sum e) being its decay.
 #include <algorithm>
 #include <utility>
 
@@ -34,13 +39,10 @@
 
 namespace asca {
 
-constexpr int SSM_NW = 4;              // waves a block: 64 channels of one group
-constexpr int SSM_CH = 16 * SSM_NW;
 constexpr float LOG2E = 1.44269504088896341f;
 
-// Rows a block of the scan (and between two kept states): with NS states a lane,
-// the backward's registers hold 2 K NS floats of them.
-constexpr int ssm_k(int NS) { return NS <= 4 ? 16 : NS == 8 ? 8 : 4; }
+// Rows a tile (and between two kept states): the backward keeps 2 K NS floats a lane.
+constexpr int ssm_k(int NS) { return NS <= 2 ? 16 : 8; }
 
 struct SsmArgs {
     const void *x, *dt, *Bm, *Cm, *dy;
@@ -50,42 +52,41 @@ struct SsmArgs {
     void *y, *dx, *ddt;
     long ldy, lddx, ldddt;
     float *h_out, *dh0;
-    float* ck;                         // kept states (B, ceil(T/K), 4 NS, D)
-    float* pP;                         // partial dA, dDk, ddt_bias (B, (N + 2) D)
+    float* ck;                         // kept states (B, ceil(T/K), N, D)
+    float* pP;                         // partial dA, dDk, ddt_bias (B nch, (N + 2) D)
     float* pBC;                        // partial dB, dC (tiles, B*T, G, 2, N)
+    float *cs, *ce;                    // per chunk: its own states (B, nch, N, D), sum of e (B, nch, D)
     int T, D, N, G, Dg, tiles, softplus;
+    int B, nch, ctile;                 // chunks a sequence, tiles of K rows a chunk
 };
 
-template <int I>
-ASCA_DEV float row_bcast(float x) {   // lane I of the lane's 16 to all of them
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + I, 0xF, 0xF, true));
+// Halves n values: out[k] = a[k] (lanes with `hi`: a[k + n/2]) of this lane and of
+// the lane that CTRL brings, whose `hi` is the other
+template <int CTRL, int H>
+ASCA_DEV void halve_dpp(const float* a, float* out, bool hi) {
+#pragma unroll
+    for (int k = 0; k < H; ++k) out[k] = (hi ? a[k + H] : a[k]) + dpp<CTRL>(hi ? a[k] : a[k + H]);
 }
 
-// out[q'] = the value that lane group q' holds, in every group
-ASCA_DEV void spread4(float v, float* out) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    const auto a = __builtin_amdgcn_permlane32_swap(r[0], r[0], false, false);
-    const auto b = __builtin_amdgcn_permlane32_swap(r[1], r[1], false, false);
-    out[0] = __uint_as_float(a[0]);
-    out[1] = __uint_as_float(b[0]);
-    out[2] = __uint_as_float(a[1]);
-    out[3] = __uint_as_float(b[1]);
+// Sums over the 8 lanes that differ in bits 3..5 of v[0..8 M): lane l has those of
+// v[M (l >> 3) .. + M)
+template <int M>
+ASCA_DEV void scatter_high(const float* v, int lane, float* out) {
+    float a[4 * M], b[2 * M];
+#pragma unroll
+    for (int k = 0; k < 4 * M; ++k) a[k] = tsum32(v[k], v[k + 4 * M]);
+#pragma unroll
+    for (int k = 0; k < 2 * M; ++k) b[k] = tsum16(a[k], a[k + 2 * M]);
+    halve_dpp<DPP_ROW_ROR8, M>(b, out, lane & 8);
 }
 
-// Sum over the four groups of v[q'], on group q'
-ASCA_DEV float gather4(const float* v) { return tsum16(tsum32(v[0], v[2]), tsum32(v[1], v[3])); }
-
-// Sums over a group's 16 lanes of 16 values: lane i has that of v[i]
-ASCA_DEV float scatter16(const float* v, int c) {
-    float a[8], b[4], d[2];
-    const bool h8 = c & 8, h4 = c & 4, h2 = c & 2, h1 = c & 1;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = (h8 ? v[k + 8] : v[k]) + dpp<DPP_ROW_ROR8>(h8 ? v[k] : v[k + 8]);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) b[k] = (h4 ? a[k + 4] : a[k]) + dpp<DPP_HALF_MIRROR>(h4 ? a[k] : a[k + 4]);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) d[k] = (h2 ? b[k + 2] : b[k]) + dpp<DPP_QUAD_XOR2>(h2 ? b[k] : b[k + 2]);
-    return (h1 ? d[1] : d[0]) + dpp<DPP_QUAD_XOR1>(h1 ? d[0] : d[1]);
+// The same over bits 0..2: lane l has those of v[M (l & 7) .. + M)
+template <int M>
+ASCA_DEV void scatter_low(const float* v, int lane, float* out) {
+    float a[4 * M], b[2 * M];
+    halve_dpp<DPP_HALF_MIRROR, 4 * M>(v, a, lane & 4);
+    halve_dpp<DPP_QUAD_XOR2, 2 * M>(a, b, lane & 2);
+    halve_dpp<DPP_QUAD_XOR1, M>(b, out, lane & 1);
 }
 
 template <typename F, int... I>
@@ -107,215 +108,505 @@ ASCA_DEV float softplus_f(float v) {
     return fmaxf(v, 0.0f) + (m == 0.0f ? t : l);
 }
 
-// What a lane is and reads from
-struct SsmLane {
-    int b, g, tile, lane, q, c, d, w, len;
-    bool live;                         // its channel exists
+// A block's place, and a thread's as the owner of (row, channel) pairs: channel
+// tid % 8 NW of the block, rows tid / 8 NW + 8 r of a tile
+template <int NW>
+struct SsmPlace {
+    int b, ch, g, tile, len, own_c, own_row, own_d;
+    bool own_live;
+    long row0;
+    ASCA_DEV explicit SsmPlace(const SsmArgs& p) {
+        unsigned u = blockIdx.x;
+        tile = u % p.tiles;
+        u /= p.tiles;
+        g = u % p.G;
+        u /= p.G;
+        ch = u % p.nch;
+        b = u / p.nch;
+        own_c = threadIdx.x % (8 * NW);
+        own_row = threadIdx.x / (8 * NW);
+        own_live = tile * 8 * NW + own_c < p.Dg;
+        own_d = g * p.Dg + min(tile * 8 * NW + own_c, p.Dg - 1);
+        len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
+        row0 = (long)b * p.T;
+    }
+    // channel c of wave w
+    ASCA_DEV int chan(const SsmArgs& p, int w, int c, bool* live) const {
+        const int d = tile * 8 * NW + w * 8 + c;
+        *live = d < p.Dg;
+        return g * p.Dg + min(d, p.Dg - 1);
+    }
 };
 
-ASCA_DEV SsmLane ssm_lane(const SsmArgs& p) {
-    SsmLane l;
-    unsigned u = blockIdx.x;
-    l.tile = u % p.tiles;
-    u /= p.tiles;
-    l.g = u % p.G;
-    l.b = u / p.G;
-    l.lane = threadIdx.x & 63;
-    l.w = threadIdx.x >> 6;
-    l.q = l.lane >> 4;
-    l.c = l.lane & 15;
-    const int ch = l.tile * SSM_CH + l.w * 16 + l.c;
-    l.live = ch < p.Dg;
-    l.d = l.g * p.Dg + min(ch, p.Dg - 1);
-    l.len = p.lens ? min(max(p.lens[l.b], 0), p.T) : p.T;
-    return l;
+// A thread's place in an activation matrix: its channel of row own_row of the
+// sequence.  Rows are reached from it by uniform offsets, so a tile's addresses are
+// scalar products.
+template <typename E, int NW>
+ASCA_DEV E* own_ptr(const SsmPlace<NW>& l, const void* m, long ld) {
+    return static_cast<E*>(const_cast<void*>(m)) + (l.row0 + l.own_row) * ld + l.own_d;
 }
 
-// One block's B or C: value v = r 16 + c is row t0 + v / NS, state q NS + v % NS
-template <typename E, int NS, int K>
-ASCA_DEV void load_bc(const SsmArgs& p, const SsmLane& l, const void* m, long ld, int t0, float* out) {
+// A thread's values of the tile at t0, as they are in memory; rows past the
+// sequence's end read its last row again (the reader replaces them).  No load sits
+// under a condition and none is converted here: either would wait for it.
+template <typename E, int NW, int R>
+ASCA_DEV void own_load(const SsmPlace<NW>& l, const E* m, long ld, int t0, E (&out)[R]) {
+    long a[R];
 #pragma unroll
-    for (int r = 0; r < K * NS / 16; ++r) {
-        const int v = r * 16 + l.c, t = t0 + v / NS, n = l.q * NS + v % NS;
-        out[r] = t < l.len && n < p.N
-                     ? act_load(static_cast<const E*>(m) + ((long)l.b * p.T + t) * ld + (long)l.g * p.N + n)
-                     : 0.0f;
+    for (int r = 0; r < R; ++r) a[r] = (t0 + 8 * r) * ld;
+    if (t0 + 8 * R > l.len)
+#pragma unroll
+        for (int r = 0; r < R; ++r) a[r] = (long)(min(t0 + l.own_row + 8 * r, max(l.len - 1, 0)) - l.own_row) * ld;
+#pragma unroll
+    for (int r = 0; r < R; ++r) out[r] = m[a[r]];
+}
+
+// B and C of a tile: value o = thread + 64 NW r is (B or C, row, state), so that a
+// wave's are all of one matrix.
+template <typename E, int NS, int NW, int K>
+struct BcTile {
+    static constexpr int V = K * 8 * NS, R = (2 * V + 64 * NW - 1) / (64 * NW);
+    const E* m[R];
+    long ld[R];
+    E v[R];
+    ASCA_DEV BcTile(const SsmArgs& p, const SsmPlace<NW>& l) {
+        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool C = (w + r * NW) * 64 % (2 * V) >= V;   // a wave past the last value reads again
+            const int o = (threadIdx.x + r * 64 * NW) % V;
+            ld[r] = C ? p.ldc : p.ldb;
+            m[r] = static_cast<const E*>(C ? p.Cm : p.Bm) + (l.row0 + o / (8 * NS)) * ld[r] + (long)l.g * p.N +
+                   min(o % (8 * NS), p.N - 1);
+        }
+    }
+    ASCA_DEV void load(const SsmPlace<NW>& l, int t0) {
+        long a[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) a[r] = t0 * ld[r];
+        if (t0 + K > l.len)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int u = (threadIdx.x + r * 64 * NW) % V / (8 * NS);
+                a[r] = (long)(min(t0 + u, max(l.len - 1, 0)) - u) * ld[r];
+            }
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[r] = m[r][a[r]];
+    }
+    // into [row][group][B's NS, C's NS], zeros for rows and states that do not exist
+    ASCA_DEV void store(const SsmArgs& p, const SsmPlace<NW>& l, int t0, float* lds) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int o = threadIdx.x + r * 64 * NW, u = o % V / (8 * NS), n = o % (8 * NS);
+            const float x = t0 + u < l.len && n < p.N ? act_value(v[r]) : 0.0f;
+            if (2 * V % (64 * NW) == 0 || o < 2 * V) lds[((u * 8 + n / NS) * 2 + o / V) * NS + n % NS] = x;
+        }
+    }
+};
+
+// Waits for a loaded value here: one that a loop uses first would be waited for in
+// every turn of it, together with the loads that the turn itself has in flight.
+ASCA_DEV void settle(float& x) { asm volatile("" : "+v"(x)); }
+
+// Step e of a row from its raw dt (0 past the sequence's end: the state stays)
+ASCA_DEV float ssm_e(const SsmArgs& p, float v, bool in) {
+    const float s = p.softplus ? softplus_f(v) : v;
+    return in ? s : 0.0f;
+}
+
+// The state (or with REV the carry) that enters a chunk: the chunks before (after) it
+// in turn, each as it left its own zero start and by its decay.
+template <int NS, bool REV>
+ASCA_DEV void fold_chunks(const SsmArgs& p, int b, int ch, int q, int d, const float* A2, float* h) {
+    const int n = REV ? p.nch - 1 - ch : ch;
+    for (int k = 0; k < n; ++k) {
+        const long u = (long)b * p.nch + (REV ? p.nch - 1 - k : k);
+        const float e = p.ce[u * p.D + d];
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+            h[j] = fmaf(__builtin_amdgcn_exp2f(e * A2[j]), h[j],
+                        p.cs[(u * p.N + min(q * NS + j, p.N - 1)) * p.D + d]);
     }
 }
 
-template <typename E, int NS>
-__global__ __launch_bounds__(64 * SSM_NW) void ssm_fwd_k(SsmArgs p) {
-    constexpr int K = ssm_k(NS), NP = 4 * NS;
-    const SsmLane l = ssm_lane(p);
-    const long row0 = (long)l.b * p.T;
-    const int nblk = (p.T + K - 1) / K;
-    float A2[NS], h[NS];
+// The sum of the block's e, one a channel, into ce
+template <int NW>
+ASCA_DEV void store_esum(const SsmArgs& p, const SsmPlace<NW>& l, float esum, float (*lds)[8 * NW]) {
+    __syncthreads();
+    lds[l.own_row][l.own_c] = esum;
+    __syncthreads();
+    if (l.own_row || !l.own_live) return;
+#pragma unroll
+    for (int r = 1; r < 8; ++r) esum += lds[r][l.own_c];
+    p.ce[((long)l.b * p.nch + l.ch) * p.D + l.own_d] = esum;
+}
+
+// OUT: the rows' y from the state that enters the chunk; otherwise what a chunk
+// makes of a zero state, and the sum of its e.  Lane = 8 q + c.
+template <typename E, int NS, int NW, bool OUT>
+__global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
+    constexpr int K = ssm_k(NS), R = K / 8;
+    constexpr int YP = 8 * NW + 4;      // 2 YP = 8 mod 64: the groups' stores of y spread over the banks
+    __shared__ float2 ex[2][K][8 * NW];
+    __shared__ float bc[2][K * 8 * 2 * NS];
+    __shared__ float ys[2][K][YP];
+    const SsmPlace<NW> l(p);
+    if (!OUT && l.ch == p.nch - 1) return;   // no chunk follows
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 3, c = lane & 7;
+    bool live;
+    const int d = l.chan(p, w, c, &live);
+    const int ntile = (p.T + K - 1) / K, k0 = l.ch * p.ctile, k1 = min(k0 + p.ctile, ntile);
+    float A2[NS], h[NS], esum = 0.0f, eown = 0.0f;
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-        const int n = l.q * NS + j;
-        A2[j] = n < p.N ? p.A[(long)n * p.D + l.d] * LOG2E : 0.0f;
-        h[j] = p.h0 && n < p.N ? p.h0[((long)l.b * p.N + n) * p.D + l.d] : 0.0f;
+        const int n = q * NS + j;
+        A2[j] = n < p.N ? p.A[(long)n * p.D + d] * LOG2E : 0.0f;
+        h[j] = OUT && p.h0 && n < p.N ? p.h0[((long)l.b * p.N + n) * p.D + d] : 0.0f;
     }
-    const float bias = p.dt_bias ? p.dt_bias[l.d] : 0.0f, Dk = p.Dk ? p.Dk[l.d] : 0.0f;
-    for (int k = 0; k < nblk; ++k) {
-        const int t0 = k * K;
-        if (p.ck && l.live)
+    if (OUT) fold_chunks<NS, false>(p, l.b, l.ch, q, d, A2, h);
+    float bias = p.dt_bias ? p.dt_bias[l.own_d] : 0.0f, Dk = p.Dk ? p.Dk[l.own_d] : 0.0f;
+    settle(bias);
+    settle(Dk);
 #pragma unroll
-            for (int j = 0; j < NS; ++j) p.ck[(((long)l.b * nblk + k) * NP + l.q * NS + j) * p.D + l.d] = h[j];
-        float Bv[K * NS / 16], Cv[K * NS / 16], x[K / 4], e[K / 4];
-        load_bc<E, NS, K>(p, l, p.Bm, p.ldb, t0, Bv);
-        load_bc<E, NS, K>(p, l, p.Cm, p.ldc, t0, Cv);
+    for (int j = 0; j < NS; ++j) settle(h[j]), settle(A2[j]);
+    const E *px = own_ptr<E>(l, p.x, p.ldx), *pdt = own_ptr<E>(l, p.dt, p.lddt);
+    E* py = own_ptr<E>(l, p.y, p.ldy);
+    BcTile<E, NS, NW, K> bct(p, l);
+    E rx[R], rdt[R];
+    float x[R], xk[R];
+    auto fetch = [&](int k) {
+        own_load(l, px, p.ldx, k * K, rx);
+        own_load(l, pdt, p.lddt, k * K, rdt);
+        bct.load(l, k * K);
+    };
+    auto stage = [&](int k, int buf) {
 #pragma unroll
-        for (int i = 0; i < K / 4; ++i) {
-            const int t = t0 + 4 * i + l.q;
-            const bool in = t < l.len;
-            x[i] = in ? act_load(static_cast<const E*>(p.x) + (row0 + t) * p.ldx + l.d) : 0.0f;
-            e[i] = in ? act_load(static_cast<const E*>(p.dt) + (row0 + t) * p.lddt + l.d) : 0.0f;
+        for (int r = 0; r < R; ++r) {
+            const bool in = k * K + l.own_row + 8 * r < l.len;
+            const float e = ssm_e(p, act_value(rdt[r]) + bias, in);
+            x[r] = in ? act_value(rx[r]) : 0.0f;
+            ex[buf][l.own_row + 8 * r][l.own_c] = make_float2(e, e * x[r]);
+            eown += e;
         }
-        unroll<K / 4>([&](auto I) {
-            constexpr int i = I;
-            const int t = t0 + 4 * i + l.q;
-            // past the sequence's end e = 0: the state stays
-            const float v = e[i] + bias, ei = t < l.len ? (p.softplus ? softplus_f(v) : v) : 0.0f;
-            float es[4], xs[4], ys[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            spread4(ei, es);
-            spread4(ei * x[i], xs);
-            unroll<4 * NS>([&](auto V) {
-                constexpr int tt = V / NS, j = V % NS, at = i * 4 * NS + V;
-                const float a = __builtin_amdgcn_exp2f(es[tt] * A2[j]);
-                h[j] = fmaf(a, h[j], row_bcast<at % 16>(Bv[at / 16]) * xs[tt]);
-                ys[tt] = fmaf(row_bcast<at % 16>(Cv[at / 16]), h[j], ys[tt]);
-            });
-            const float y = gather4(ys) + Dk * x[i];
-            if (l.live && t < p.T) act_store(static_cast<E*>(p.y) + (row0 + t) * p.ldy + l.d, t < l.len ? y : 0.0f);
-        });
+        bct.store(p, l, k * K, bc[buf]);
+    };
+    auto emit = [&](int k) {
+        float v[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            v[r] = k * K + l.own_row + 8 * r < l.len ? fmaf(Dk, xk[r], ys[k & 1][l.own_row + 8 * r][l.own_c]) : 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (l.own_live && k * K + l.own_row + 8 * r < p.T) act_store(py + (k * K + 8 * r) * p.ldy, v[r]);
+    };
+    if (k0 < k1) {
+        fetch(k0);
+        stage(k0, k0 & 1);
     }
-    if (p.h_out && l.live)
+    for (int k = k0; k < k1; ++k) {
+        const int buf = k & 1, next = min(k + 1, k1 - 1);   // the last tile is read twice rather than left out
+        lds_barrier();                       // tile k is staged, tile k - 1's y is summed
+        if (OUT && k > k0) emit(k - 1);
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            const int n = l.q * NS + j;
-            if (n < p.N) p.h_out[((long)l.b * p.N + n) * p.D + l.d] = h[j];
+        for (int r = 0; r < R; ++r) xk[r] = x[r];
+        esum = eown;
+        fetch(next);
+        if (OUT && p.ck && live)
+#pragma unroll
+            for (int j = 0; j < NS; ++j)
+                if (q * NS + j < p.N) p.ck[(((long)l.b * ntile + k) * p.N + q * NS + j) * p.D + d] = h[j];
+        // operands are read PR rows ahead: read as they are needed, each row would wait
+        // for its own (8 x 4096 x 2048 bf16: 570 -> 410 us; 4 or 8 rows ahead: 428, 446)
+        constexpr int PR = 2, MS = OUT ? 2 * NS : NS;
+        float2 ev[2][PR];
+        float m[2][PR][MS], y[K];
+        auto read = [&](int g) {
+#pragma unroll
+            for (int u = 0; u < PR; ++u) {
+                ev[g & 1][u] = ex[buf][g * PR + u][w * 8 + c];
+#pragma unroll
+                for (int j = 0; j < MS; ++j) m[g & 1][u][j] = bc[buf][((g * PR + u) * 8 + q) * 2 * NS + j];
+            }
+        };
+        read(0);
+#pragma unroll
+        for (int g = 0; g < K / PR; ++g) {
+            if (g + 1 < K / PR) read(g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < PR; ++u)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    const float2 e = ev[g & 1][u];
+                    const float* v = m[g & 1][u];
+                    h[j] = fmaf(__builtin_amdgcn_exp2f(e.x * A2[j]), h[j], v[j] * e.y);
+                    if (OUT) y[g * PR + u] = j ? fmaf(v[NS + j], h[j], y[g * PR + u]) : v[NS + j] * h[j];
+                }
         }
+        if (OUT) {
+            float s[R];
+            scatter_high<R>(y, lane, s);
+#pragma unroll
+            for (int r = 0; r < R; ++r) ys[buf][R * q + r][w * 8 + c] = s[r];
+        }
+        stage(next, buf ^ 1);
+    }
+    if (OUT && k0 < k1) {
+        lds_barrier();
+        emit(k1 - 1);
+    }
+    if (!OUT) {
+        if (live)
+#pragma unroll
+            for (int j = 0; j < NS; ++j)
+                if (q * NS + j < p.N) p.cs[(((long)l.b * p.nch + l.ch) * p.N + q * NS + j) * p.D + d] = h[j];
+        store_esum<NW>(p, l, esum, reinterpret_cast<float(*)[8 * NW]>(&ys[0][0][0]));
+    } else if (p.h_out && live && l.ch == p.nch - 1) {
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+            if (q * NS + j < p.N) p.h_out[((long)l.b * p.N + q * NS + j) * p.D + d] = h[j];
+    }
 }
 
-template <typename E, int NS>
-__global__ __launch_bounds__(64 * SSM_NW) void ssm_bwd_k(SsmArgs p) {
-    constexpr int K = ssm_k(NS), NP = 4 * NS, KR = K * NS / 16;
-    __shared__ float red[2][SSM_NW][KR * 64];
-    const SsmLane l = ssm_lane(p);
-    const long row0 = (long)l.b * p.T;
-    const int nblk = (p.T + K - 1) / K;
-    float A2[NS], cy[NS], dA[NS];
+// What a chunk makes of a zero carry, from its end to its start, and the sum of its e.
+// Lane = 8 q + c.
+template <typename E, int NS, int NW>
+__global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
+    constexpr int K = ssm_k(NS), R = K / 8;
+    __shared__ float2 ey[2][K][8 * NW];
+    __shared__ float bc[2][K * 8 * 2 * NS];
+    const SsmPlace<NW> l(p);
+    if (l.ch == 0) return;   // no chunk precedes
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 3, c = lane & 7;
+    bool live;
+    const int d = l.chan(p, w, c, &live);
+    const int ntile = (p.T + K - 1) / K, k0 = l.ch * p.ctile, k1 = min(k0 + p.ctile, ntile);
+    float A2[NS], cy[NS], esum = 0.0f, eown = 0.0f;
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-        const int n = l.q * NS + j;
-        A2[j] = n < p.N ? p.A[(long)n * p.D + l.d] * LOG2E : 0.0f;
-        cy[j] = p.dh_out && n < p.N ? p.dh_out[((long)l.b * p.N + n) * p.D + l.d] : 0.0f;
+        A2[j] = q * NS + j < p.N ? p.A[(long)(q * NS + j) * p.D + d] * LOG2E : 0.0f;
+        cy[j] = 0.0f;
+    }
+    float bias = p.dt_bias ? p.dt_bias[l.own_d] : 0.0f;
+    settle(bias);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) settle(A2[j]);
+    const E *pdy = own_ptr<E>(l, p.dy, p.lddy), *pdt = own_ptr<E>(l, p.dt, p.lddt);
+    BcTile<E, NS, NW, K> bct(p, l);
+    E rdy[R], rdt[R];
+    auto fetch = [&](int k) {
+        own_load(l, pdy, p.lddy, k * K, rdy);
+        own_load(l, pdt, p.lddt, k * K, rdt);
+        bct.load(l, k * K);
+    };
+    auto stage = [&](int k, int buf) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool in = k * K + l.own_row + 8 * r < l.len;
+            const float e = ssm_e(p, act_value(rdt[r]) + bias, in);
+            ey[buf][l.own_row + 8 * r][l.own_c] = make_float2(e, in ? act_value(rdy[r]) : 0.0f);
+            eown += e;
+        }
+        bct.store(p, l, k * K, bc[buf]);
+    };
+    fetch(k1 - 1);
+    stage(k1 - 1, (k1 - 1) & 1);
+    for (int k = k1 - 1; k >= k0; --k) {
+        const int buf = k & 1, next = max(k - 1, k0);
+        lds_barrier();
+        esum = eown;
+        fetch(next);
+#pragma unroll
+        for (int t = K - 1; t >= 0; --t) {
+            const float2 e = ey[buf][t][w * 8 + c];
+            const float* m = bc[buf] + (t * 8 + q) * 2 * NS + NS;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) cy[j] = __builtin_amdgcn_exp2f(e.x * A2[j]) * fmaf(m[j], e.y, cy[j]);
+        }
+        stage(next, buf ^ 1);
+    }
+    if (live)
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+            if (q * NS + j < p.N) p.cs[(((long)l.b * p.nch + l.ch) * p.N + q * NS + j) * p.D + d] = cy[j];
+    store_esum<NW>(p, l, esum, reinterpret_cast<float(*)[8 * NW]>(&ey[0][0][0]));
+}
+
+// Lane = 8 c + q: sums over channels (2 NS a row) by row swaps, over states (2 a row) by DPP.
+template <typename E, int NS, int NW>
+__global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
+    constexpr int K = ssm_k(NS), R = K / 8;
+    constexpr int YP = 8 * NW + 4, RED = K * 8 * 2 * NS;   // RED sums over channels a tile and wave
+    // ... in groups of 8 PG: TG rows' 2 NS, or one row's
+    constexpr int TG = NS < 4 ? 4 / NS : 1, PG = NS < 4 ? 1 : NS / 4;
+    __shared__ float2 ex[2][K][8 * NW];
+    __shared__ float dys[2][K][8 * NW];
+    __shared__ float bc[2][K * 8 * 2 * NS];
+    __shared__ float sums[2][2][K][YP];
+    __shared__ float red[2][NW][RED];
+    const SsmPlace<NW> l(p);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane & 7, c = lane >> 3;
+    bool live;
+    const int d = l.chan(p, w, c, &live);
+    const int ntile = (p.T + K - 1) / K, k0 = l.ch * p.ctile, k1 = min(k0 + p.ctile, ntile);
+    float A2[NS], cy[NS], dA[NS], hn[NS];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+        const int n = q * NS + j;
+        A2[j] = n < p.N ? p.A[(long)n * p.D + d] * LOG2E : 0.0f;
+        cy[j] = p.dh_out && n < p.N ? p.dh_out[((long)l.b * p.N + n) * p.D + d] : 0.0f;
         dA[j] = 0.0f;
     }
-    const float bias = p.dt_bias ? p.dt_bias[l.d] : 0.0f, Dk = p.Dk ? p.Dk[l.d] : 0.0f;
-    float dD = 0.0f, db = 0.0f;
-    for (int k = nblk - 1; k >= 0; --k) {
-        const int t0 = k * K;
-        float Bv[KR], Cv[KR], x[K / 4], e[K / 4], v[K / 4], dy[K / 4], h0[NS], h[K * NS], a[K * NS];
-        load_bc<E, NS, K>(p, l, p.Bm, p.ldb, t0, Bv);
-        load_bc<E, NS, K>(p, l, p.Cm, p.ldc, t0, Cv);
+    fold_chunks<NS, true>(p, l.b, l.ch, q, d, A2, cy);
+    float bias = p.dt_bias ? p.dt_bias[l.own_d] : 0.0f, Dk = p.Dk ? p.Dk[l.own_d] : 0.0f;
+    settle(bias);
+    settle(Dk);
 #pragma unroll
-        for (int i = 0; i < K / 4; ++i) {
-            const int t = t0 + 4 * i + l.q;
-            const bool in = t < l.len;
-            x[i] = in ? act_load(static_cast<const E*>(p.x) + (row0 + t) * p.ldx + l.d) : 0.0f;
-            v[i] = in ? act_load(static_cast<const E*>(p.dt) + (row0 + t) * p.lddt + l.d) : 0.0f;
-            dy[i] = in ? act_load(static_cast<const E*>(p.dy) + (row0 + t) * p.lddy + l.d) : 0.0f;
+    for (int j = 0; j < NS; ++j) settle(cy[j]), settle(A2[j]);
+    E rx[R], rdt[R], rdy[R];
+    float x[R], dt[R], dy[R], e[R], dD = 0.0f, db = 0.0f, xk[R], dtk[R], dyk[R], ek[R];
+    const E *px = own_ptr<E>(l, p.x, p.ldx), *pdt = own_ptr<E>(l, p.dt, p.lddt), *pdy = own_ptr<E>(l, p.dy, p.lddy);
+    E *pdx = own_ptr<E>(l, p.dx, p.lddx), *pddt = own_ptr<E>(l, p.ddt, p.ldddt);
+    BcTile<E, NS, NW, K> bct(p, l);
+    const float* pck = p.ck + (long)l.b * ntile * p.N * p.D + d;
+    auto fetch = [&](int k) {
+        own_load(l, px, p.ldx, k * K, rx);
+        own_load(l, pdt, p.lddt, k * K, rdt);
+        own_load(l, pdy, p.lddy, k * K, rdy);
+        bct.load(l, k * K);
+        // a state that does not exist takes another's: its B and C are zero, so it reaches nothing
+#pragma unroll
+        for (int j = 0; j < NS; ++j) hn[j] = pck[(long)k * p.N * p.D + (long)min(q * NS + j, p.N - 1) * p.D];
+    };
+    auto stage = [&](int k, int buf) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool in = k * K + l.own_row + 8 * r < l.len;
+            dt[r] = act_value(rdt[r]) + bias;
+            e[r] = ssm_e(p, dt[r], in);
+            x[r] = in ? act_value(rx[r]) : 0.0f;
+            dy[r] = in ? act_value(rdy[r]) : 0.0f;
+            // a channel that does not exist adds nothing to dB and dC
+            ex[buf][l.own_row + 8 * r][l.own_c] = make_float2(e[r], l.own_live ? e[r] * x[r] : 0.0f);
+            dys[buf][l.own_row + 8 * r][l.own_c] = l.own_live ? dy[r] : 0.0f;
         }
+        bct.store(p, l, k * K, bc[buf]);
+    };
+    auto emit = [&](int k) {
+        const int buf = k & 1, t0 = k * K;
 #pragma unroll
-        for (int j = 0; j < NS; ++j) h0[j] = p.ck[(((long)l.b * nblk + k) * NP + l.q * NS + j) * p.D + l.d];
-        // the block's states and decays again
-        unroll<K / 4>([&](auto I) {
-            constexpr int i = I;
-            v[i] += bias;
-            e[i] = t0 + 4 * i + l.q < l.len ? (p.softplus ? softplus_f(v[i]) : v[i]) : 0.0f;
-            float es[4], xs[4];
-            spread4(e[i], es);
-            spread4(e[i] * x[i], xs);
-            unroll<4 * NS>([&](auto V) {
-                constexpr int tt = V / NS, j = V % NS, at = i * 4 * NS + V;
-                a[at] = __builtin_amdgcn_exp2f(es[tt] * A2[j]);
-                h[at] = fmaf(a[at], at < NS ? h0[j] : h[at < NS ? 0 : at - NS], row_bcast<at % 16>(Bv[at / 16]) * xs[tt]);
-            });
-        });
-        float vB[K * NS], vC[K * NS], dAk[NS];
-#pragma unroll
-        for (int j = 0; j < NS; ++j) dAk[j] = 0.0f;
-        unroll<K / 4>([&](auto I) {
-            constexpr int i = K / 4 - 1 - I;
-            float es[4], xs[4], dys[4], gB[4] = {0.0f, 0.0f, 0.0f, 0.0f}, pA[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            spread4(e[i], es);
-            spread4(e[i] * x[i], xs);
-            spread4(dy[i], dys);
-            unroll<4 * NS>([&](auto V) {
-                constexpr int tt = 3 - V / NS, j = V % NS, at = (i * 4 + tt) * NS + j;
-                const float g = fmaf(row_bcast<at % 16>(Cv[at / 16]), dys[tt], cy[j]);
-                vC[at] = dys[tt] * h[at];
-                vB[at] = g * xs[tt];
-                gB[tt] = fmaf(row_bcast<at % 16>(Bv[at / 16]), g, gB[tt]);
-                cy[j] = a[at] * g;
-                const float pp = cy[j] * (at < NS ? h0[j] : h[at < NS ? 0 : at - NS]);
-                pA[tt] = fmaf(A2[j], pp, pA[tt]);
-                dAk[j] = fmaf(es[tt], pp, dAk[j]);
-            });
-            const int t = t0 + 4 * i + l.q;
+        for (int r = 0; r < R; ++r) {
+            const int row = l.own_row + 8 * r, t = t0 + row;
             const bool in = t < l.len;
-            const float sB = gather4(gB), sA = gather4(pA) * (1.0f / LOG2E);
-            const float de = fmaf(x[i], sB, sA), ddt = p.softplus ? de * act_sigmoid(v[i]) : de;
-            if (l.live && t < p.T) {
-                act_store(static_cast<E*>(p.dx) + (row0 + t) * p.lddx + l.d, in ? fmaf(e[i], sB, Dk * dy[i]) : 0.0f);
-                act_store(static_cast<E*>(p.ddt) + (row0 + t) * p.ldddt + l.d, in ? ddt : 0.0f);
+            const float sB = sums[buf][0][row][l.own_c], sA = sums[buf][1][row][l.own_c] * (1.0f / LOG2E);
+            const float de = fmaf(xk[r], sB, sA), ddt = in ? (p.softplus ? de * act_sigmoid(dtk[r]) : de) : 0.0f;
+            if (l.own_live && t < p.T) {
+                act_store(pdx + (t0 + 8 * r) * p.lddx, in ? fmaf(ek[r], sB, Dk * dyk[r]) : 0.0f);
+                act_store(pddt + (t0 + 8 * r) * p.ldddt, ddt);
             }
-            dD = fmaf(dy[i], x[i], dD);
-            db += in ? ddt : 0.0f;
-        });
-#pragma unroll
-        for (int j = 0; j < NS; ++j) dA[j] += dAk[j];
-        // dB, dC of the block: over the wave's channels, then the waves'
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < KR; ++r) {
-            // a channel that does not exist adds nothing
-            if (!l.live)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) vB[r * 16 + i] = vC[r * 16 + i] = 0.0f;
-            red[0][l.w][r * 64 + l.lane] = scatter16(vB + r * 16, l.c);
-            red[1][l.w][r * 64 + l.lane] = scatter16(vC + r * 16, l.c);
+            dD = fmaf(dyk[r], xk[r], dD);
+            db += ddt;
         }
-        __syncthreads();
-        for (int o = threadIdx.x; o < 2 * KR * 64; o += 64 * SSM_NW) {
-            const int s = o / (KR * 64), u = o % (KR * 64), vv = u / 64 * 16 + (u & 15);
-            const int t = t0 + vv / NS, n = ((u >> 4) & 3) * NS + vv % NS;
+        for (int o = threadIdx.x; o < RED; o += 64 * NW) {
             float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < SSM_NW; ++w) sum += red[s][w][u];
+            for (int u = 0; u < NW; ++u) sum += red[buf][u][o];
+            // value (o / 64 PG) 8 PG + PG (lane >> 3) + o / 64 % PG of the tile's (row, B or C, state)
+            const int v = o / (64 * PG) * 8 * PG + PG * ((o & 63) >> 3) + o / 64 % PG, t = t0 + v / (2 * NS);
+            const int n = (o & 7) * NS + v % NS;
             if (t < p.T && n < p.N)
-                p.pBC[(((((long)l.tile * (gridDim.x / (p.tiles * p.G)) + l.b) * p.T + t) * p.G + l.g) * 2 + s) * p.N + n] =
+                p.pBC[(((((long)l.tile * p.B + l.b) * p.T + t) * p.G + l.g) * 2 + v / NS % 2) * p.N + n] =
                     t < l.len ? sum : 0.0f;
         }
+    };
+    if (k0 < k1) {
+        fetch(k1 - 1);
+        stage(k1 - 1, (k1 - 1) & 1);
     }
-    dD = add_xor32(add_xor16(dD));
-    db = add_xor32(add_xor16(db));
-    if (l.live) {
-        float* part = p.pP + (long)l.b * (p.N + 2) * p.D + l.d;
+    for (int k = k1 - 1; k >= k0; --k) {
+        const int buf = k & 1, next = max(k - 1, k0);
+        float h0[NS], h[K * NS], a[K * NS];
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            const int n = l.q * NS + j;
-            if (n < p.N) {
-                part[(long)n * p.D] = dA[j];
-                if (p.dh0) p.dh0[((long)l.b * p.N + n) * p.D + l.d] = cy[j];
+        for (int j = 0; j < NS; ++j) h0[j] = hn[j], settle(h0[j]);   // before this turn's stores
+        lds_barrier();                       // tile k is staged, tile k + 1's sums are there
+        if (k + 1 < k1) emit(k + 1);
+#pragma unroll
+        for (int r = 0; r < R; ++r) xk[r] = x[r], dtk[r] = dt[r], dyk[r] = dy[r], ek[r] = e[r];
+        fetch(next);
+        // the tile's states and decays again
+#pragma unroll
+        for (int t = 0; t < K; ++t) {
+            const float2 v = ex[buf][t][w * 8 + c];
+            const float* m = bc[buf] + (t * 8 + q) * 2 * NS;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                a[t * NS + j] = __builtin_amdgcn_exp2f(v.x * A2[j]);
+                h[t * NS + j] = fmaf(a[t * NS + j], t ? h[(t ? t - 1 : 0) * NS + j] : h0[j], m[j] * v.y);
             }
         }
-        if (l.q == 0) {
-            part[(long)p.N * p.D] = dD;
-            part[(long)(p.N + 1) * p.D] = db;
+        float gB[K], pA[K], dAk[NS];
+#pragma unroll
+        for (int j = 0; j < NS; ++j) dAk[j] = 0.0f;
+#pragma unroll
+        for (int tg = K / TG - 1; tg >= 0; --tg) {
+            float part[8 * PG];
+#pragma unroll
+            for (int u = TG - 1; u >= 0; --u) {
+                const int t = tg * TG + u;
+                const float2 v = ex[buf][t][w * 8 + c];
+                const float dyt = dys[buf][t][w * 8 + c];
+                const float* m = bc[buf] + (t * 8 + q) * 2 * NS;
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    const float g = fmaf(m[NS + j], dyt, cy[j]);
+                    part[u * 2 * NS + j] = g * v.y;
+                    part[u * 2 * NS + NS + j] = dyt * h[t * NS + j];
+                    gB[t] = j ? fmaf(m[j], g, gB[t]) : m[j] * g;
+                    cy[j] = a[t * NS + j] * g;
+                    const float pp = cy[j] * (t ? h[(t ? t - 1 : 0) * NS + j] : h0[j]);
+                    pA[t] = j ? fmaf(A2[j], pp, pA[t]) : A2[j] * pp;
+                    dAk[j] = fmaf(v.x, pp, dAk[j]);
+                }
+            }
+            float s[PG];
+            scatter_high<PG>(part, lane, s);
+#pragma unroll
+            for (int u = 0; u < PG; ++u) red[buf][w][(tg * PG + u) * 64 + lane] = s[u];
         }
+#pragma unroll
+        for (int j = 0; j < NS; ++j) dA[j] += dAk[j];
+        float s[R];
+        scatter_low<R>(gB, lane, s);
+#pragma unroll
+        for (int r = 0; r < R; ++r) sums[buf][0][R * q + r][w * 8 + c] = s[r];
+        scatter_low<R>(pA, lane, s);
+#pragma unroll
+        for (int r = 0; r < R; ++r) sums[buf][1][R * q + r][w * 8 + c] = s[r];
+        stage(next, buf ^ 1);
+    }
+    if (k0 < k1) {
+        lds_barrier();
+        emit(k0);
+    }
+    float* part = p.pP + ((long)l.b * p.nch + l.ch) * (p.N + 2) * p.D;
+    if (live)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const int n = q * NS + j;
+            if (n < p.N) {
+                part[(long)n * p.D + d] = dA[j];
+                if (p.dh0 && l.ch == 0) p.dh0[((long)l.b * p.N + n) * p.D + d] = cy[j];
+            }
+        }
+    __syncthreads();
+    sums[0][0][l.own_row][l.own_c] = dD;
+    sums[1][0][l.own_row][l.own_c] = db;
+    __syncthreads();
+    if (l.own_row == 0 && l.own_live) {
+#pragma unroll
+        for (int r = 1; r < 8; ++r) dD += sums[0][0][r][l.own_c], db += sums[1][0][r][l.own_c];
+        part[(long)p.N * p.D + l.own_d] = dD;
+        part[(long)(p.N + 1) * p.D + l.own_d] = db;
     }
 }
 
@@ -363,7 +654,7 @@ __global__ __launch_bounds__(256) void ssm_step_k(float* __restrict__ h, SsmArgs
 
 using namespace asca;
 
-static int ssm_ns(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+static int ssm_ns(int N) { return N <= 8 ? 1 : N <= 16 ? 2 : N <= 32 ? 4 : 8; }
 
 static int ssm_check(const char* fn, int B, int T, int D, int N, int G) {
     if (B < 0 || T < 0 || D < 0) return fail(ASCA_ERR_INVALID, "%s: negative shape B=%d T=%d D=%d", fn, B, T, D);
@@ -376,16 +667,36 @@ static int ssm_ld(const char* fn, const char* what, long ld, long cols) {
     return ld >= cols ? ASCA_OK : fail(ASCA_ERR_INVALID, "%s: row stride %s=%ld below its %ld columns", fn, what, ld, cols);
 }
 
-// Calls f with the element type and the compile-time states a lane
+// The waves a block has (8, or 4 where that alone gives a block to every CU), and the
+// rows' cut into p.nch chunks a sequence: where sequences and channels give fewer
+// than `enough` waves, as many chunks as give `want`.  A cut costs a second pass over
+// the rows, so it pays only for waves that are missing (forward, N = 16: 2 x 2048 x
+// 1024 in 512 waves 157 us, cut to 4096 47 us; 32 x 512 x 512 in 2048 waves 54 us,
+// cut to 4096 78 us; backward: 2 x 2048 x 1024 cut to 1024 142 us, to 2048 100 us).
+static int ssm_split(SsmArgs& p, int N, long enough, long want) {
+    const int K = ssm_k(ssm_ns(N)), ntile = (p.T + K - 1) / K;
+    const int NW = ssm_ns(N) <= 4 && (long)p.B * p.G * ((p.Dg + 63) / 64) >= 256 ? 8 : 4;
+    p.tiles = (p.Dg + 8 * NW - 1) / (8 * NW);
+    const long waves = (long)p.B * p.G * p.tiles * NW;
+    const long nch = waves == 0 || waves >= enough ? 1 : std::max(1L, std::min({want / waves, 64L, (long)ntile / 4}));
+    p.ctile = std::max(1, (int)((ntile + nch - 1) / nch));
+    p.nch = std::max(1, (ntile + p.ctile - 1) / p.ctile);
+    return NW;
+}
+static size_t ssm_chunk_floats(const SsmArgs& p) { return p.nch > 1 ? (size_t)p.B * p.nch * (p.N + 1) * p.D : 0; }
+
+// Calls f with the element type, the states a lane and the waves a block
 template <typename F>
-static int ssm_dispatch(int dtype, int N, F f) {
+static int ssm_dispatch(int dtype, int N, int NW, F f) {
     return act_dispatch(dtype, [&](auto* e) {
+        auto go = [&](auto ns) {
+            return NW == 8 ? f(e, ns, std::integral_constant<int, 8>{}) : f(e, ns, std::integral_constant<int, 4>{});
+        };
         switch (ssm_ns(N)) {
-            case 1: return f(e, std::integral_constant<int, 1>{});
-            case 2: return f(e, std::integral_constant<int, 2>{});
-            case 4: return f(e, std::integral_constant<int, 4>{});
-            case 8: return f(e, std::integral_constant<int, 8>{});
-            default: return f(e, std::integral_constant<int, 16>{});
+            case 1: return go(std::integral_constant<int, 1>{});
+            case 2: return go(std::integral_constant<int, 2>{});
+            case 4: return go(std::integral_constant<int, 4>{});
+            default: return f(e, std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
         }
     });
 }
@@ -396,8 +707,8 @@ int asca_ssm_ws_bytes(int B, int T, int D, int N, size_t* bytes) {
     if (!bytes) return fail(ASCA_ERR_INVALID, "null output pointer");
     int rc = ssm_check("asca_ssm_ws_bytes", B, T, D, N, 1);
     if (rc) return rc;
-    const int ns = ssm_ns(N), K = ssm_k(ns);
-    *bytes = (size_t)B * (((size_t)T + K - 1) / K) * 4 * ns * D * sizeof(float);
+    const int K = ssm_k(ssm_ns(N));
+    *bytes = (size_t)B * (((size_t)T + K - 1) / K) * N * D * sizeof(float);
     return ASCA_OK;
 }
 
@@ -421,14 +732,24 @@ int asca_ssm_fwd(const void* x, long ldx, const void* dt, long lddt, const float
     p.dt_bias = dt_bias, p.A = A, p.Dk = Dk, p.h0 = h0, p.lens = lens, p.y = y, p.ldy = ldy, p.h_out = h_out;
     p.ck = static_cast<float*>(ws);
     p.T = T, p.D = D, p.N = N, p.G = G, p.Dg = D / G, p.softplus = softplus;
-    p.tiles = (p.Dg + SSM_CH - 1) / SSM_CH;
-    const long blocks = (long)B * G * p.tiles;
+    p.B = B;
+    const int NW = ssm_split(p, N, 1024, 4096);
+    const long blocks = (long)B * p.nch * G * p.tiles;
     if (blocks > 0x7fffffffL) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many channels", fn);
-    return ssm_dispatch(dtype, N, [&](auto* e, auto ns) {
+    StreamScratch sc;
+    if ((rc = sc.get(ssm_chunk_floats(p), st))) return rc;
+    p.cs = sc.ws.p, p.ce = p.cs + (size_t)B * p.nch * N * D;
+    return ssm_dispatch(dtype, N, NW, [&](auto* e, auto ns, auto nw) {
         using E = std::remove_pointer_t<decltype(e)>;
-        int r = pre_launch("ssm_fwd");
-        if (r) return r;
-        hipLaunchKernelGGL((ssm_fwd_k<E, decltype(ns)::value>), dim3((unsigned)blocks), dim3(64 * SSM_NW), 0, st, p);
+        constexpr int NS = decltype(ns)::value, W = decltype(nw)::value;
+        int r;
+        if (p.nch > 1) {
+            if ((r = pre_launch("ssm_chunk"))) return r;
+            hipLaunchKernelGGL((ssm_fwd_k<E, NS, W, false>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
+            if ((r = post_launch("ssm_chunk"))) return r;
+        }
+        if ((r = pre_launch("ssm_fwd"))) return r;
+        hipLaunchKernelGGL((ssm_fwd_k<E, NS, W, true>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
         return post_launch("ssm_fwd");
     });
 }
@@ -459,19 +780,27 @@ int asca_ssm_bwd(const void* x, long ldx, const void* dt, long lddt, const float
     p.dx = dx, p.lddx = lddx, p.ddt = ddt, p.ldddt = ldddt, p.dh0 = dh0;
     p.ck = static_cast<float*>(const_cast<void*>(ws));
     p.T = T, p.D = D, p.N = N, p.G = G, p.Dg = D / G, p.softplus = softplus;
-    p.tiles = (p.Dg + SSM_CH - 1) / SSM_CH;
-    const long blocks = (long)B * G * p.tiles, rows = (long)B * T, per = rows * G * 2 * N, nd = (long)N * D;
+    p.B = B;
+    const int NW = ssm_split(p, N, 2048, 2048);
+    const long blocks = (long)B * p.nch * G * p.tiles, rows = (long)B * T, parts = (long)B * p.nch, per = rows * G * 2 * N, nd = (long)N * D;
     if (blocks > 0x7fffffffL || (per + 255) / 256 > 0x7fffffffL)
         return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows or channels", fn);
     StreamScratch sc;
-    if ((rc = sc.get((size_t)B * (nd + 2 * D) + (size_t)p.tiles * per, st))) return rc;
-    p.pP = sc.ws.p, p.pBC = p.pP + B * (nd + 2 * D);
-    return ssm_dispatch(dtype, N, [&](auto* e, auto ns) {
+    if ((rc = sc.get((size_t)parts * (nd + 2 * D) + (size_t)p.tiles * per + ssm_chunk_floats(p), st))) return rc;
+    p.pP = sc.ws.p, p.pBC = p.pP + parts * (nd + 2 * D), p.cs = p.pBC + p.tiles * per;
+    p.ce = p.cs + (size_t)parts * N * D;
+    return ssm_dispatch(dtype, N, NW, [&](auto* e, auto ns, auto nw) {
         using E = std::remove_pointer_t<decltype(e)>;
+        constexpr int NS = decltype(ns)::value, W = decltype(nw)::value;
         int r;
+        if (p.nch > 1) {
+            if ((r = pre_launch("ssm_carry"))) return r;
+            hipLaunchKernelGGL((ssm_carry_k<E, NS, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
+            if ((r = post_launch("ssm_carry"))) return r;
+        }
         if (blocks) {
             if ((r = pre_launch("ssm_bwd"))) return r;
-            hipLaunchKernelGGL((ssm_bwd_k<E, decltype(ns)::value>), dim3((unsigned)blocks), dim3(64 * SSM_NW), 0, st, p);
+            hipLaunchKernelGGL((ssm_bwd_k<E, NS, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
             if ((r = post_launch("ssm_bwd"))) return r;
         }
         if (per) {
@@ -480,7 +809,7 @@ int asca_ssm_bwd(const void* x, long ldx, const void* dt, long lddt, const float
                                G, N, static_cast<E*>(dB), lddb, static_cast<E*>(dC), lddc);
             if ((r = post_launch("ssm_fin_bc"))) return r;
         }
-        return sum_parts_launch(p.pP, B, PartsOut{{dA, dDk, ddt_bias}, {nd, D, D}}, st);
+        return sum_parts_launch(p.pP, parts, PartsOut{{dA, dDk, ddt_bias}, {nd, D, D}}, st);
     });
 }
 

@@ -545,8 +545,7 @@ ASCA_API int asca_conv_step(float* state, const void* x, long ldx, const float* 
                             long ldy, int n, int D, int W, int silu, int dtype, void* stream);
 
 /* Bytes of the workspace that asca_ssm_fwd leaves for asca_ssm_bwd: the state
- * before every K-th row (K = 16 at N <= 16, 8 at N <= 32, else 4), which is
- * B * ceil(T/K) * 4 ceil(N/4) * D floats. */
+ * before every K-th row (K = 16 at N <= 16, else 8), B * ceil(T/K) * N * D floats. */
 ASCA_API int asca_ssm_ws_bytes(int B, int T, int D, int N, size_t* bytes);
 
 /* Selective state space scan, N states (1..64) for each of D channels:
