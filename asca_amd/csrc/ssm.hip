@@ -436,7 +436,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
 template <typename E, int NS, int NW>
 __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
     constexpr int K = ssm_k(NS), R = K / 8;
-    constexpr int YP = 8 * NW + 4, RED = K * 8 * 2 * NS;   // RED sums over channels a tile and wave
+    constexpr int PR = 2, YP = 8 * NW + 4, RED = K * 8 * 2 * NS;   // RED sums over channels a tile and wave
     // ... in groups of 8 PG: TG rows' 2 NS, or one row's
     constexpr int TG = NS < 4 ? 4 / NS : 1, PG = NS < 4 ? 1 : NS / 4;
     __shared__ float2 ex[2][K][8 * NW];
@@ -533,29 +533,60 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
 #pragma unroll
         for (int r = 0; r < R; ++r) xk[r] = x[r], dtk[r] = dt[r], dyk[r] = dy[r], ek[r] = e[r];
         fetch(next);
-        // the tile's states and decays again
+        // the tile's states and decays again, operands read PR rows ahead
+        {
+            float2 v[2][PR];
+            float m[2][PR][NS];
+            auto read = [&](int g) {
 #pragma unroll
-        for (int t = 0; t < K; ++t) {
-            const float2 v = ex[buf][t][w * 8 + c];
-            const float* m = bc[buf] + (t * 8 + q) * 2 * NS;
+                for (int u = 0; u < PR; ++u) {
+                    v[g & 1][u] = ex[buf][g * PR + u][w * 8 + c];
 #pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                a[t * NS + j] = __builtin_amdgcn_exp2f(v.x * A2[j]);
-                h[t * NS + j] = fmaf(a[t * NS + j], t ? h[(t ? t - 1 : 0) * NS + j] : h0[j], m[j] * v.y);
+                    for (int j = 0; j < NS; ++j) m[g & 1][u][j] = bc[buf][((g * PR + u) * 8 + q) * 2 * NS + j];
+                }
+            };
+            read(0);
+#pragma unroll
+            for (int g = 0; g < K / PR; ++g) {
+                if (g + 1 < K / PR) read(g + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < PR; ++u)
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        const int t = g * PR + u, at = t * NS + j;
+                        a[at] = __builtin_amdgcn_exp2f(v[g & 1][u].x * A2[j]);
+                        h[at] = fmaf(a[at], t ? h[(t ? t - 1 : 0) * NS + j] : h0[j], m[g & 1][u][j] * v[g & 1][u].y);
+                    }
             }
         }
         float gB[K], pA[K], dAk[NS];
 #pragma unroll
         for (int j = 0; j < NS; ++j) dAk[j] = 0.0f;
+        float2 v2[2][TG];
+        float dy2[2][TG], m2[2][TG][2 * NS];
+        auto read = [&](int tg) {
+#pragma unroll
+            for (int u = 0; u < TG; ++u) {
+                const int t = tg * TG + u;
+                v2[tg & 1][u] = ex[buf][t][w * 8 + c];
+                dy2[tg & 1][u] = dys[buf][t][w * 8 + c];
+#pragma unroll
+                for (int j = 0; j < 2 * NS; ++j) m2[tg & 1][u][j] = bc[buf][(t * 8 + q) * 2 * NS + j];
+            }
+        };
+        read(K / TG - 1);
 #pragma unroll
         for (int tg = K / TG - 1; tg >= 0; --tg) {
             float part[8 * PG];
+            if (tg) read(tg - 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int u = TG - 1; u >= 0; --u) {
                 const int t = tg * TG + u;
-                const float2 v = ex[buf][t][w * 8 + c];
-                const float dyt = dys[buf][t][w * 8 + c];
-                const float* m = bc[buf] + (t * 8 + q) * 2 * NS;
+                const float2 v = v2[tg & 1][u];
+                const float dyt = dy2[tg & 1][u];
+                const float* m = m2[tg & 1][u];
 #pragma unroll
                 for (int j = 0; j < NS; ++j) {
                     const float g = fmaf(m[NS + j], dyt, cy[j]);
