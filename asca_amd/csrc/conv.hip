@@ -2,16 +2,17 @@
 // sequences.  Per channel, with W taps:
 //   p_t = bias + sum_j w_j x_{t-W+1+j},  y = p or silu(p)
 //   g = dy (silu'(p));  dx_t = sum_j w_j g_{t+W-1-j};  dw_j = sum g_t x_{t-W+1+j}
-// A thread has a channel and a run of rows, and slides a window of W rows over
-// it in registers, so a row is read once (and W - 1 more at a run's edge).
-// Bound by memory.
+// A thread has V neighbouring channels and a run of CV_R rows: all of a run's rows
+// (and the W - 1 beside it, which a neighbour reads too) are loaded at once, then
+// each is used W times from registers.  The backward forms g again for the W - 1
+// rows after its run.  Bound by memory.
 #include "act.h"
 #include "parts.h"
 
 namespace asca {
 
-constexpr int CV_FR = 32;    // rows a run, forward
-constexpr int CV_BR = 64;    // backward: a run leaves W + 1 partial sums a channel
+constexpr int CV_R = 16;    // rows a run
+constexpr int CV_NW = 4;    // runs a block (the backward adds their sums)
 
 struct ConvArgs {
     const void *x, *dy;
@@ -26,103 +27,178 @@ struct ConvArgs {
 
 ASCA_DEV int conv_len(const ConvArgs& p, int b) { return p.lens ? min(max(p.lens[b], 0), p.T) : p.T; }
 
-// x at row t of sequence b: the state's for t < 0, zero from the length on
-template <typename E, int W>
-ASCA_DEV float conv_x(const ConvArgs& p, int b, int t, int len, int d) {
-    if (t < 0) return p.state_in ? p.state_in[((long)b * (W - 1) + (W - 1 + t)) * p.D + d] : 0.0f;
-    return t < len ? act_load(static_cast<const E*>(p.x) + ((long)b * p.T + t) * p.ldx + d) : 0.0f;
+// A wave's run: rows t0 .. t1 of sequence b; the lane's V channels start at d
+struct ConvRun {
+    int b, t0, t1, len, d;
+    bool live, last;     // its channels exist; it is a sequence's last
+};
+template <int V>
+ASCA_DEV ConvRun conv_run(const ConvArgs& p, unsigned block, int w) {
+    const unsigned cb = (p.D + 64 * V - 1) / (64 * V);
+    const long u = (long)(block / cb) * CV_NW + w;
+    ConvRun r;
+    r.d = (block % cb * 64 + (threadIdx.x & 63)) * V;
+    r.live = r.d < p.D && u < (long)p.B * p.runs;
+    r.d = min(r.d, p.D - V);
+    const long v = min(u, (long)p.B * p.runs - 1);
+    r.b = (int)(v / p.runs);
+    r.t0 = (int)(v % p.runs) * CV_R;
+    r.last = r.t0 + CV_R >= p.T;
+    r.t1 = min(r.t0 + CV_R, p.T);
+    r.len = conv_len(p, r.b);
+    return r;
 }
 
-template <typename E, int W>
-__global__ __launch_bounds__(256) void conv_fwd_k(ConvArgs p) {
-    const unsigned cb = (p.D + 63) / 64;
-    const int d = blockIdx.x % cb * 64 + (threadIdx.x & 63);
-    const long u = (long)(blockIdx.x / cb) * 4 + (threadIdx.x >> 6);
-    if (d >= p.D || u >= (long)p.B * p.runs) return;
-    const int b = (int)(u / p.runs), run = (int)(u % p.runs), t0 = run * CV_FR, t1 = min(t0 + CV_FR, p.T);
-    const int len = conv_len(p, b);
-    float w[W], win[W];
+// Rows t .. t + N - 1 of x: the state's before row 0, zeros from the length on
+template <typename E, int W, int V, int N>
+ASCA_DEV void conv_rows(const ConvArgs& p, const ConvRun& r, int t, float (&x)[N][V]) {
+    const E* m = static_cast<const E*>(p.x) + (long)r.b * p.T * p.ldx + r.d;
+    if (t >= 0 && t + N <= r.len) {
+        act_raw<V, E> raw[N];
 #pragma unroll
-    for (int j = 0; j < W; ++j) w[j] = p.w[(long)j * p.D + d];
-    const float bias = p.bias ? p.bias[d] : 0.0f;
+        for (int k = 0; k < N; ++k) raw[k] = act_load_raw<V>(m + (long)(t + k) * p.ldx);
 #pragma unroll
-    for (int j = 1; j < W; ++j) win[j] = conv_x<E, W>(p, b, t0 - W + j, len, d);
-    E* y = static_cast<E*>(p.y) + (long)b * p.T * p.ldy + d;
-    for (int t = t0; t < t1; ++t) {
+        for (int k = 0; k < N; ++k) act_values(raw[k], x[k]);
+    } else {
 #pragma unroll
-        for (int j = 0; j + 1 < W; ++j) win[j] = win[j + 1];
-        win[W - 1] = conv_x<E, W>(p, b, t, len, d);
-        float a = bias;
+        for (int k = 0; k < N; ++k) {
+            const int u = t + k;
+            if (u >= 0 && u < r.len) {
+                act_values(act_load_raw<V>(m + (long)u * p.ldx), x[k]);
+            } else if (u < 0 && p.state_in) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) a = fmaf(w[j], win[j], a);
-        if (p.silu) a *= act_sigmoid(a);
-        act_store(y + (long)t * p.ldy, t < len ? a : 0.0f);
-    }
-    if (p.state_out && run == 0)
+                for (int i = 0; i < V; ++i) x[k][i] = p.state_in[((long)r.b * (W - 1) + (W - 1 + u)) * p.D + r.d + i];
+            } else {
 #pragma unroll
-        for (int j = 0; j + 1 < W; ++j)
-            p.state_out[((long)b * (W - 1) + j) * p.D + d] = conv_x<E, W>(p, b, len - (W - 1) + j, len, d);
-}
-
-template <typename E, int W>
-__global__ __launch_bounds__(256) void conv_bwd_k(ConvArgs p) {
-    const unsigned cb = (p.D + 63) / 64;
-    const int d = blockIdx.x % cb * 64 + (threadIdx.x & 63);
-    const long u = (long)(blockIdx.x / cb) * 4 + (threadIdx.x >> 6);
-    if (d >= p.D || u >= (long)p.B * p.runs) return;
-    const int b = (int)(u / p.runs), run = (int)(u % p.runs), t0 = run * CV_BR, t1 = min(t0 + CV_BR, p.T);
-    const int len = conv_len(p, b);
-    float w[W], win[W], gw[W], dw[W], db = 0.0f;
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-        w[j] = p.w[(long)j * p.D + d];
-        gw[j] = dw[j] = 0.0f;
-    }
-    const float bias = p.bias ? p.bias[d] : 0.0f;
-#pragma unroll
-    for (int j = 1; j < W; ++j) win[j] = conv_x<E, W>(p, b, t0 - W + j, len, d);
-    const E* dy = static_cast<const E*>(p.dy) + (long)b * p.T * p.lddy + d;
-    E* dx = static_cast<E*>(p.dx) + (long)b * p.T * p.lddx + d;
-    // g of rows t0 .. t1 + W - 2; dx of row t - W + 1 once row t's is known
-    for (int t = t0; t < t1 + W - 1; ++t) {
-#pragma unroll
-        for (int j = 0; j + 1 < W; ++j) {
-            win[j] = win[j + 1];
-            gw[j] = gw[j + 1];
-        }
-        win[W - 1] = conv_x<E, W>(p, b, t, len, d);
-        float a = bias, g = 0.0f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) a = fmaf(w[j], win[j], a);
-        if (t < len) {
-            g = act_load(dy + (long)t * p.lddy);
-            if (p.silu) {
-                const float s = act_sigmoid(a);
-                g *= s * fmaf(a, 1.0f - s, 1.0f);
+                for (int i = 0; i < V; ++i) x[k][i] = 0.0f;
             }
         }
-        gw[W - 1] = g;
-        if (t < t1) {
-            db += g;
-#pragma unroll
-            for (int j = 0; j < W; ++j) dw[j] = fmaf(g, win[j], dw[j]);
-        }
-        const int r = t - (W - 1);   // gw[i] is g of row r + i
-        if (r < t0 && !(run == 0 && r < 0)) continue;
-        float v = 0.0f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) v = fmaf(w[j], gw[W - 1 - j], v);
-        const int o = r - (len - (W - 1));
-        if (p.dstate_out && o >= 0 && o < W - 1) v += p.dstate_out[((long)b * (W - 1) + o) * p.D + d];
-        if (r >= 0)
-            act_store(dx + (long)r * p.lddx, r < len ? v : 0.0f);
-        else if (p.dstate_in)
-            p.dstate_in[((long)b * (W - 1) + (W - 1 + r)) * p.D + d] = v;
     }
-    float* part = p.part + u * (W + 1) * p.D + d;
+}
+
+template <int V>
+ASCA_DEV void conv_params(const float* m, int d, float* out) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) part[(long)j * p.D] = dw[j];
-    part[(long)W * p.D] = db;
+    for (int i = 0; i < V; ++i) out[i] = m ? m[d + i] : 0.0f;
+}
+
+template <typename E, int W, int V>
+__global__ __launch_bounds__(64 * CV_NW) void conv_fwd_k(ConvArgs p) {
+    const ConvRun r = conv_run<V>(p, blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    if (!r.live) return;
+    float w[W][V], bias[V], x[CV_R + W - 1][V];
+    conv_rows<E, W, V>(p, r, r.t0 - (W - 1), x);
+#pragma unroll
+    for (int j = 0; j < W; ++j) conv_params<V>(p.w + (long)j * p.D, r.d, w[j]);
+    conv_params<V>(p.bias, r.d, bias);
+    E* y = static_cast<E*>(p.y) + (long)r.b * p.T * p.ldy + r.d;
+#pragma unroll
+    for (int k = 0; k < CV_R; ++k) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float a = bias[i];
+#pragma unroll
+            for (int j = 0; j < W; ++j) a = fmaf(w[j][i], x[k + j][i], a);
+            if (p.silu) a *= act_sigmoid(a);
+            o[i] = r.t0 + k < r.len ? a : 0.0f;
+        }
+        if (r.t0 + k < r.t1) act_store_n<V>(y + (long)(r.t0 + k) * p.ldy, o);
+    }
+    if (p.state_out && r.last) {
+        float s[W - 1][V];
+        conv_rows<E, W, V>(p, r, r.len - (W - 1), s);
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) p.state_out[((long)r.b * (W - 1) + j) * p.D + r.d + i] = s[j][i];
+    }
+}
+
+template <typename E, int W, int V>
+__global__ __launch_bounds__(64 * CV_NW) void conv_bwd_k(ConvArgs p) {
+    constexpr int N = CV_R + W - 1;
+    __shared__ float red[CV_NW][W + 1][64 * V];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const ConvRun r = conv_run<V>(p, blockIdx.x, wave);
+    float w[W][V], bias[V], x[N + W - 1][V], g[N][V], dw[W][V], db[V];
+    // g of rows t0 .. t0 + N - 1, from x of t0 - (W - 1) on
+    conv_rows<E, W, V>(p, r, r.t0 - (W - 1), x);
+    const E* dy = static_cast<const E*>(p.dy) + (long)r.b * p.T * p.lddy + r.d;
+    act_raw<V, E> raw[N] = {};
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if (p.T > 0) raw[k] = act_load_raw<V>(dy + (long)min(r.t0 + k, max(r.len - 1, 0)) * p.lddy);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        conv_params<V>(p.w + (long)j * p.D, r.d, w[j]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) dw[j][i] = 0.0f;
+    }
+    conv_params<V>(p.bias, r.d, bias);
+#pragma unroll
+    for (int i = 0; i < V; ++i) db[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        act_values(raw[k], g[k]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float a = bias[i];
+#pragma unroll
+            for (int j = 0; j < W; ++j) a = fmaf(w[j][i], x[k + j][i], a);
+            if (p.silu) {
+                const float s = act_sigmoid(a);
+                g[k][i] *= s * fmaf(a, 1.0f - s, 1.0f);
+            }
+            if (r.t0 + k >= r.len) g[k][i] = 0.0f;
+            if (k < CV_R) {
+                db[i] += g[k][i];
+#pragma unroll
+                for (int j = 0; j < W; ++j) dw[j][i] = fmaf(g[k][i], x[k + j][i], dw[j][i]);
+            }
+        }
+    }
+    // dx of row t0 + k from g of rows t0 + k .. t0 + k + W - 1; the first run goes back
+    // to row -(W - 1), the state's (g is zero before row 0)
+    E* dx = static_cast<E*>(p.dx) + (long)r.b * p.T * p.lddx + r.d;
+#pragma unroll
+    for (int k = -(W - 1); k < CV_R; ++k) {
+        const int t = r.t0 + k, o = t - (r.len - (W - 1));
+        if (!r.live || t >= r.t1 || (k < 0 && (r.t0 > 0 || !p.dstate_in))) continue;
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (k + W - 1 - j >= 0) v[i] = fmaf(w[j][i], g[k + W - 1 - j < 0 ? 0 : k + W - 1 - j][i], v[i]);
+            if (p.dstate_out && o >= 0 && o < W - 1) v[i] += p.dstate_out[((long)r.b * (W - 1) + o) * p.D + r.d + i];
+            if (k >= 0 && t >= r.len) v[i] = 0.0f;
+        }
+        if (k >= 0)
+            act_store_n<V>(dx + (long)t * p.lddx, v);
+        else
+#pragma unroll
+            for (int i = 0; i < V; ++i) p.dstate_in[((long)r.b * (W - 1) + (W - 1 + k)) * p.D + r.d + i] = v[i];
+    }
+    // the block's runs' dw and db, one row of partial sums
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) red[wave][j][lane * V + i] = r.live ? dw[j][i] : 0.0f;
+        red[wave][W][lane * V + i] = r.live ? db[i] : 0.0f;
+    }
+    __syncthreads();
+    const unsigned cb = (p.D + 64 * V - 1) / (64 * V);
+    float* part = p.part + (long)(blockIdx.x / cb) * (W + 1) * p.D;
+    for (int o = threadIdx.x; o < (W + 1) * 64 * V; o += 64 * CV_NW) {
+        const int j = o / (64 * V), d = blockIdx.x % cb * 64 * V + o % (64 * V);
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < CV_NW; ++k) s += red[k][j][o % (64 * V)];
+        if (d < p.D) part[(long)j * p.D + d] = s;
+    }
 }
 
 template <typename E, int W>
@@ -158,17 +234,21 @@ static int conv_ld(const char* fn, const char* what, long ld, int cols) {
     return ld >= cols ? ASCA_OK : fail(ASCA_ERR_INVALID, "%s: row stride %s=%ld below its %d columns", fn, what, ld, cols);
 }
 
+// Calls f with the element type, the taps and the channels a thread takes
 template <typename F>
-static int conv_dispatch(int dtype, int W, F f) {
+static int conv_dispatch(int dtype, int W, bool vec, F f) {
     return act_dispatch(dtype, [&](auto* e) {
+        auto go = [&](auto taps) {
+            return vec ? f(e, taps, std::integral_constant<int, 4>{}) : f(e, taps, std::integral_constant<int, 1>{});
+        };
         switch (W) {
-            case 2: return f(e, std::integral_constant<int, 2>{});
-            case 3: return f(e, std::integral_constant<int, 3>{});
-            case 4: return f(e, std::integral_constant<int, 4>{});
-            case 5: return f(e, std::integral_constant<int, 5>{});
-            case 6: return f(e, std::integral_constant<int, 6>{});
-            case 7: return f(e, std::integral_constant<int, 7>{});
-            default: return f(e, std::integral_constant<int, 8>{});
+            case 2: return go(std::integral_constant<int, 2>{});
+            case 3: return go(std::integral_constant<int, 3>{});
+            case 4: return go(std::integral_constant<int, 4>{});
+            case 5: return go(std::integral_constant<int, 5>{});
+            case 6: return go(std::integral_constant<int, 6>{});
+            case 7: return go(std::integral_constant<int, 7>{});
+            default: return go(std::integral_constant<int, 8>{});
         }
     });
 }
@@ -195,14 +275,16 @@ int asca_conv_fwd(const void* x, long ldx, const float* w, const float* bias, co
     ConvArgs p{};
     p.x = x, p.ldx = ldx, p.w = w, p.bias = bias, p.state_in = state_in, p.lens = lens;
     p.y = y, p.ldy = ldy, p.state_out = state_out;
-    p.B = B, p.T = T, p.D = D, p.runs = T > 0 ? (T + CV_FR - 1) / CV_FR : 1, p.silu = silu;
+    p.B = B, p.T = T, p.D = D, p.runs = T > 0 ? (T + CV_R - 1) / CV_R : 1, p.silu = silu;
     dim3 grid;
-    if ((rc = conv_grid(fn, ((long)B * p.runs + 3) / 4, D, 64, &grid))) return rc;
-    return conv_dispatch(dtype, W, [&](auto* e, auto taps) {
+    const bool vec = D % 4 == 0 && act_vec_ok(x, ldx, dtype) && act_vec_ok(y, ldy, dtype);
+    if ((rc = conv_grid(fn, ((long)B * p.runs + CV_NW - 1) / CV_NW, D, vec ? 256 : 64, &grid))) return rc;
+    return conv_dispatch(dtype, W, vec, [&](auto* e, auto taps, auto v) {
         using E = std::remove_pointer_t<decltype(e)>;
         int r = pre_launch("conv_fwd");
         if (r) return r;
-        hipLaunchKernelGGL((conv_fwd_k<E, decltype(taps)::value>), grid, dim3(256), 0, as_stream(stream), p);
+        hipLaunchKernelGGL((conv_fwd_k<E, decltype(taps)::value, decltype(v)::value>), grid, dim3(64 * CV_NW), 0,
+                           as_stream(stream), p);
         return post_launch("conv_fwd");
     });
 }
@@ -222,19 +304,20 @@ int asca_conv_bwd(const void* x, long ldx, const float* w, const float* bias, co
     ConvArgs p{};
     p.x = x, p.ldx = ldx, p.w = w, p.bias = bias, p.state_in = state_in, p.lens = lens, p.dy = dy, p.lddy = lddy;
     p.dstate_out = dstate_out, p.dx = dx, p.lddx = lddx, p.dstate_in = dstate_in;
-    p.B = B, p.T = T, p.D = D, p.runs = T > 0 ? (T + CV_BR - 1) / CV_BR : 1, p.silu = silu;
+    p.B = B, p.T = T, p.D = D, p.runs = T > 0 ? (T + CV_R - 1) / CV_R : 1, p.silu = silu;
     dim3 grid;
-    if ((rc = conv_grid(fn, ((long)B * p.runs + 3) / 4, D, 64, &grid))) return rc;
-    const long parts = (long)B * p.runs;
+    const long parts = ((long)B * p.runs + CV_NW - 1) / CV_NW;
+    const bool vec = D % 4 == 0 && act_vec_ok(x, ldx, dtype) && act_vec_ok(dy, lddy, dtype) && act_vec_ok(dx, lddx, dtype);
+    if ((rc = conv_grid(fn, parts, D, vec ? 256 : 64, &grid))) return rc;
     StreamScratch sc;
     if ((rc = sc.get((size_t)parts * (W + 1) * D, st))) return rc;
     p.part = sc.ws.p;
     if (parts)
-        rc = conv_dispatch(dtype, W, [&](auto* e, auto taps) {
+        rc = conv_dispatch(dtype, W, vec, [&](auto* e, auto taps, auto v) {
             using E = std::remove_pointer_t<decltype(e)>;
             int r = pre_launch("conv_bwd");
             if (r) return r;
-            hipLaunchKernelGGL((conv_bwd_k<E, decltype(taps)::value>), grid, dim3(256), 0, st, p);
+            hipLaunchKernelGGL((conv_bwd_k<E, decltype(taps)::value, decltype(v)::value>), grid, dim3(64 * CV_NW), 0, st, p);
             return post_launch("conv_bwd");
         });
     if (rc) return rc;
@@ -253,7 +336,7 @@ int asca_conv_step(float* state, const void* x, long ldx, const float* w, const 
     if ((rc = conv_ld(fn, "ldx", ldx, D)) || (rc = conv_ld(fn, "ldy", ldy, D))) return rc;
     ConvArgs p{};
     p.x = x, p.ldx = ldx, p.w = w, p.bias = bias, p.y = y, p.ldy = ldy, p.D = D, p.silu = silu;
-    return conv_dispatch(dtype, W, [&](auto* e, auto taps) {
+    return conv_dispatch(dtype, W, false, [&](auto* e, auto taps, auto) {
         using E = std::remove_pointer_t<decltype(e)>;
         int r = pre_launch("conv_step");
         if (r) return r;
