@@ -1,9 +1,10 @@
 // The global 2-norm of a list of gradient tensors and their clipping by it:
 //   norm = sqrt(sum g^2);  c = min(1, max_norm / (norm + 1e-6));  dst = c src
 // The list is cut into chunks of one tensor each (a table in device memory,
-// made once); a block has a chunk.  The squares are summed in 64 bits, a
-// chunk's sum is stored, and the block that ends last adds the chunks' sums in
-// their order: one launch for the norm, deterministic.  Bound by memory.
+// made once); a block has a chunk.  The squares are summed in 64 bits; the chunks'
+// sums are added in their order by every block that scales, which costs less than a
+// launch between (and than a last block's: a fence in each block before it took the
+// norm of 143M gradients from 122 to 310 us).  Bound by memory.
 #include <algorithm>
 #include <vector>
 
@@ -17,7 +18,9 @@ struct GradChunk {
     long n;
 };
 
-constexpr long GC_MIN = 4096, GC_BLOCKS = 4096;   // elements a chunk at least; about so many chunks
+constexpr int GC_U = 4;                            // accesses of 4 elements a thread has in flight
+constexpr long GC_IT = 256 * 4 * GC_U;             // elements a block takes at a time
+constexpr long GC_MIN = GC_IT, GC_BLOCKS = 2048;   // elements a chunk at least; about so many chunks
 
 ASCA_DEV double wave_sum_d(double x) {
 #pragma unroll
@@ -33,50 +36,77 @@ ASCA_DEV double block_sum_d(double x, double* lds) {
     return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-// sums[chunk]; the last block writes out[0] (and out[1] with `clip`)
+// sums[chunk] = the sum of its squares
 template <typename E>
-__global__ __launch_bounds__(256) void grads_norm_k(const GradChunk* __restrict__ chunks, double* sums, unsigned* done,
-                                                   int clip, float max_norm, float* __restrict__ out) {
+__global__ __launch_bounds__(256) void grads_sums_k(const GradChunk* __restrict__ chunks, double* __restrict__ sums) {
     __shared__ double lds[4];
-    __shared__ bool last;
     const GradChunk c = chunks[blockIdx.x];
     const E* src = static_cast<const E*>(c.src);
     double s = 0.0;
-    for (long i = threadIdx.x; i < c.n; i += 256) {
-        const double v = act_load(src + i);
+    auto add = [&](float x) {
+        const double v = x;
         s = fma(v, v, s);
-    }
-    s = block_sum_d(s, lds);
-    if (threadIdx.x == 0) {
-        sums[blockIdx.x] = s;
-        __threadfence();
-        last = atomicAdd(done, 1u) == gridDim.x - 1;
-    }
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    s = 0.0;
-    for (unsigned i = threadIdx.x; i < gridDim.x; i += 256) s += __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s = block_sum_d(s, lds);
-    if (threadIdx.x == 0) {
-        const float norm = (float)sqrt(s);
-        out[0] = norm;
-        if (clip) {
-            const float r = max_norm / (norm + 1e-6f);
-            out[1] = r >= 1.0f ? 1.0f : r;   // NaN stays
+    };
+    long i = 0;
+    if (reinterpret_cast<uintptr_t>(src) % (4 * sizeof(E)) == 0)
+        for (; i + GC_IT <= c.n; i += GC_IT) {
+            act_raw<4, E> r[GC_U];
+#pragma unroll
+            for (int u = 0; u < GC_U; ++u) r[u] = act_load_raw<4>(src + i + (u * 256 + threadIdx.x) * 4);
+#pragma unroll
+            for (int u = 0; u < GC_U; ++u) {
+                float v[4];
+                act_values(r[u], v);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) add(v[k]);
+            }
         }
-        *done = 0;
-    }
+    for (i += threadIdx.x; i < c.n; i += 256) add(act_load(src + i));
+    s = block_sum_d(s, lds);
+    if (threadIdx.x == 0) sums[blockIdx.x] = s;
+}
+
+// The norm from the chunks' sums, the same in every block that asks
+ASCA_DEV float grads_total(const double* __restrict__ sums, unsigned n, double* lds) {
+    double s = 0.0;
+    for (unsigned i = threadIdx.x; i < n; i += 256) s += sums[i];
+    return (float)sqrt(block_sum_d(s, lds));
+}
+
+__global__ __launch_bounds__(256) void grads_norm_k(const double* __restrict__ sums, unsigned n, float* __restrict__ out) {
+    __shared__ double lds[4];
+    const float norm = grads_total(sums, n, lds);
+    if (threadIdx.x == 0) out[0] = norm;
 }
 
 template <typename E>
-__global__ __launch_bounds__(256) void grads_scale_k(const GradChunk* __restrict__ chunks, const float* __restrict__ out) {
-    const GradChunk c = chunks[blockIdx.x];
-    const float f = out[1];
-    if (f == 1.0f && c.src == c.dst) return;   // nothing changes
+__global__ __launch_bounds__(256) void grads_scale_k(const GradChunk* __restrict__ chunks, const double* __restrict__ sums,
+                                                    float max_norm, float* __restrict__ out) {
+    __shared__ double lds[4];
+    // the chunks that were read last come first: they may still be in a cache
+    const GradChunk c = chunks[gridDim.x - 1 - blockIdx.x];
+    const float norm = grads_total(sums, gridDim.x, lds), ratio = max_norm / (norm + 1e-6f);
+    const float f = ratio >= 1.0f ? 1.0f : ratio;   // NaN stays
+    if (blockIdx.x == 0 && threadIdx.x == 0) out[0] = norm, out[1] = f;
+    if (f == 1.0f && c.src == c.dst) return;        // nothing changes
     const E* src = static_cast<const E*>(c.src);
     E* dst = static_cast<E*>(c.dst);
-    for (long i = threadIdx.x; i < c.n; i += 256) act_store(dst + i, f * act_load(src + i));
+    long i = 0;
+    if ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) % (4 * sizeof(E)) == 0)
+        for (; i + GC_IT <= c.n; i += GC_IT) {
+            act_raw<4, E> r[GC_U];
+#pragma unroll
+            for (int u = 0; u < GC_U; ++u) r[u] = act_load_raw<4>(src + i + (u * 256 + threadIdx.x) * 4);
+#pragma unroll
+            for (int u = 0; u < GC_U; ++u) {
+                float v[4];
+                act_values(r[u], v);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] *= f;
+                act_store_n<4>(dst + i + (u * 256 + threadIdx.x) * 4, v);
+            }
+        }
+    for (i += threadIdx.x; i < c.n; i += 256) act_store(dst + i, f * act_load(src + i));
 }
 
 __global__ void grads_none_k(float* out, int clip) {
@@ -85,9 +115,8 @@ __global__ void grads_none_k(float* out, int clip) {
 }
 
 struct GradList {
-    GradChunk* chunks = nullptr;   // then the sums and the counter, one allocation
+    GradChunk* chunks = nullptr;   // then the sums, one allocation
     double* sums = nullptr;
-    unsigned* done = nullptr;
     unsigned n = 0;
     int dtype = 0;
 };
@@ -105,14 +134,18 @@ static int grads_run(GradList* g, bool clip, float max_norm, float* out, hipStre
     }
     return act_dispatch(g->dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
-        int r = pre_launch("grads_norm");
+        int r = pre_launch("grads_sums");
         if (r) return r;
-        hipLaunchKernelGGL(grads_norm_k<E>, dim3(g->n), dim3(256), 0, st, g->chunks, g->sums, g->done, (int)clip, max_norm,
-                           out);
-        if ((r = post_launch("grads_norm")) || !clip) return r;
-        if ((r = pre_launch("grads_scale"))) return r;
-        hipLaunchKernelGGL(grads_scale_k<E>, dim3(g->n), dim3(256), 0, st, g->chunks, out);
-        return post_launch("grads_scale");
+        hipLaunchKernelGGL(grads_sums_k<E>, dim3(g->n), dim3(256), 0, st, g->chunks, g->sums);
+        if ((r = post_launch("grads_sums"))) return r;
+        if (clip) {
+            if ((r = pre_launch("grads_scale"))) return r;
+            hipLaunchKernelGGL(grads_scale_k<E>, dim3(g->n), dim3(256), 0, st, g->chunks, g->sums, max_norm, out);
+            return post_launch("grads_scale");
+        }
+        if ((r = pre_launch("grads_norm"))) return r;
+        hipLaunchKernelGGL(grads_norm_k, dim3(1), dim3(256), 0, st, g->sums, g->n, out);
+        return post_launch("grads_norm");
     });
 }
 
@@ -150,16 +183,14 @@ int asca_grads_create(void** src, void** dst, const uint64_t* sizes, int count, 
         if (g->n) {
             const size_t tab = t.size() * sizeof(GradChunk), sum = t.size() * sizeof(double);
             char* m = nullptr;
-            hipError_t e = hipMalloc(reinterpret_cast<void**>(&m), tab + sum + 16);
+            hipError_t e = hipMalloc(reinterpret_cast<void**>(&m), tab + sum);
             if (e != hipSuccess) {
                 delete g;
-                return fail(ASCA_ERR_OOM, "%s: %zu bytes: %s", fn, tab + sum + 16, hipGetErrorString(e));
+                return fail(ASCA_ERR_OOM, "%s: %zu bytes: %s", fn, tab + sum, hipGetErrorString(e));
             }
             g->chunks = reinterpret_cast<GradChunk*>(m);
             g->sums = reinterpret_cast<double*>(m + tab);
-            g->done = reinterpret_cast<unsigned*>(m + tab + sum);
             e = hipMemcpy(m, t.data(), tab, hipMemcpyHostToDevice);
-            if (e == hipSuccess) e = hipMemset(g->done, 0, 4);
             if (e == hipSuccess) e = hipDeviceSynchronize();   // done before any stream uses it
             if (e != hipSuccess) {
                 (void)hipFree(m);
