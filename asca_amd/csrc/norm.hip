@@ -16,8 +16,6 @@
 
 namespace asca {
 
-constexpr int BN_MAX = 16384;   // columns: 16 waves of 16 values a lane
-
 struct NormArgs {
     const void *x, *y, *z, *dr, *dn;
     long ldx, ldy, ldz, lddr, lddn;
@@ -30,40 +28,33 @@ struct NormArgs {
     float eps;
 };
 
-// VEC values at column c of a row (zeros past its end; cols is a multiple of VEC)
-template <int VEC, typename E>
-ASCA_DEV void row_load(const E* row, int c, int cols, float* v) {
-    if (VEC == 1 || c >= cols) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[k] = c < cols ? act_load(row + c + k) : 0.0f;
-    } else if constexpr (sizeof(E) == 4) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(row + c);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[k] = a[k & 3];
-    } else {
-        const uint2 a = *reinterpret_cast<const uint2*>(row + c);
-        v[0] = __uint_as_float(a.x << 16);
-        if constexpr (VEC == 4) {
-            v[1] = __uint_as_float(a.x & 0xffff0000u);
-            v[2] = __uint_as_float(a.y << 16);
-            v[3] = __uint_as_float(a.y & 0xffff0000u);
-        }
+// An operand of the rows, or in the place of one that is not given another's, whose
+// values are replaced by zeros once they are there.  All loads of a row are issued
+// before any is looked at: none sits under a condition or is converted on the way,
+// as either would wait for it (16384 x 2048 bf16 backward 307 -> 177 us).
+template <typename E>
+struct NormOp {
+    const E* m;
+    long ld;
+    bool on;
+    ASCA_DEV NormOp(const void* a, long la, const void* other, long lo)
+        : m(static_cast<const E*>(a ? a : other)), ld(a ? la : lo), on(a != nullptr) {}
+    template <int VEC>
+    ASCA_DEV act_raw<VEC, E> load(long row, int c, int cols) const {
+        return act_load_raw<VEC>(m + row * ld + min(c, cols - VEC));
     }
-}
+    // values at column c (zeros past the row's end)
+    template <int VEC>
+    ASCA_DEV void values(act_raw<VEC, E> r, int c, int cols, float* v) const {
+        act_values(r, v);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = on && c < cols ? v[k] : 0.0f;
+    }
+};
 
 template <int VEC, typename E>
 ASCA_DEV void row_store(E* row, int c, int cols, const float* v) {
-    if (c >= cols) return;
-    if constexpr (VEC == 1) {
-        act_store(row + c, v[0]);
-    } else if constexpr (sizeof(E) == 4) {
-        *reinterpret_cast<f32x4*>(row + c) = f32x4{v[0], v[1], v[2], v[3]};
-    } else {
-        bf16_t b[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) act_store(b + k, v[k]);
-        *reinterpret_cast<uint2*>(row + c) = make_uint2(b[0] | (unsigned)b[1] << 16, b[2] | (unsigned)b[3] << 16);
-    }
+    if (c < cols) act_store_n<VEC>(row + c, v);
 }
 
 // Sum over the threads of a row
@@ -81,192 +72,267 @@ ASCA_DEV float row_sum(float x, float* lds) {
     return x;
 }
 
-// The same in 64 bits
+template <int CTRL>
+ASCA_DEV double dpp_d(double x) {
+    const uint2 u = __builtin_bit_cast(uint2, x);
+    return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_mov_dpp((int)u.x, CTRL, 0xF, 0xF, true),
+                                                 __builtin_amdgcn_mov_dpp((int)u.y, CTRL, 0xF, 0xF, true)));
+}
+
+// Sums over the wave of 8 values, in every lane: scattered over the lanes' low three
+// bits while there are several, added over the others, read back by lane.
+ASCA_DEV void wave_sums8(double (&v)[8]) {
+    const int lane = threadIdx.x & 63;
+    double a[4], b[2], x;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a[k] = (lane & 4 ? v[k + 4] : v[k]) + dpp_d<DPP_HALF_MIRROR>(lane & 4 ? v[k] : v[k + 4]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) b[k] = (lane & 2 ? a[k + 2] : a[k]) + dpp_d<DPP_QUAD_XOR2>(lane & 2 ? a[k] : a[k + 2]);
+    x = (lane & 1 ? b[1] : b[0]) + dpp_d<DPP_QUAD_XOR1>(lane & 1 ? b[0] : b[1]);
+    x += dpp_d<DPP_ROW_ROR8>(x);
+    x += __shfl_xor(x, 16, 64);
+    x += __shfl_xor(x, 32, 64);
+    const uint2 u = __builtin_bit_cast(uint2, x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        v[k] = __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_readlane(u.x, k), __builtin_amdgcn_readlane(u.y, k)));
+}
+
+// The same over the threads of a row; `turn` alternates from call to call
 template <int WPR>
-ASCA_DEV double row_sum(double x, double* lds) {
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) x += __shfl_xor(x, s, 64);
+ASCA_DEV void row_sums8(double (&v)[8], double (*lds)[WPR][8], int turn) {
+    wave_sums8(v);
     if constexpr (WPR > 1) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-        __syncthreads();
-        x = 0.0;
+        if ((threadIdx.x & 63) == 0)
 #pragma unroll
-        for (int w = 0; w < WPR; ++w) x += lds[w];
+            for (int k = 0; k < 8; ++k) lds[turn & 1][threadIdx.x >> 6][k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = lds[turn & 1][0][k];
+#pragma unroll
+            for (int w = 1; w < WPR; ++w) v[k] += lds[turn & 1][w][k];
+        }
     }
-    return x;
 }
 
 template <int WPR>
 constexpr int bn_threads() { return WPR == 1 ? 256 : 64 * WPR; }
 
-// A row: u, r, y, silu(z), z and the two inverse norms.  The backward takes the
-// sums of its rows in 64 bits: k - uh mean(k uh) cancels where k is near a multiple
-// of uh (always in a row of one column), and the products of f32 values are exact there.
-template <typename S, int NE>
-struct BnRow {
-    float u[NE], r[NE], y[NE], sz[NE], z[NE];
-    S i1, i2;
-};
-
-template <typename S, typename E, int VEC, int NV, int WPR>
-ASCA_DEV void bn_row(const NormArgs& p, long row, int tid, bool second, S* lds, BnRow<S, VEC * NV>& o) {
-    constexpr int NE = VEC * NV;
-    S ss = 0;
+// VEC values of a parameter (ones where there is none; past the row's end any that
+// exist: they meet zeros)
+template <int VEC>
+ASCA_DEV void par_load(const float* m, int c, int cols, float* v) {
+    if (m) {
+        act_values(act_load_raw<VEC>(m + min(c, cols - VEC)), v);
+    } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * 64 * WPR + tid) * VEC;
-        if (p.x) row_load<VEC>(static_cast<const E*>(p.x) + row * p.ldx, c, p.cols, o.r + i * VEC);
-        if (p.y) row_load<VEC>(static_cast<const E*>(p.y) + row * p.ldy, c, p.cols, o.y + i * VEC);
-        if (p.z) row_load<VEC>(static_cast<const E*>(p.z) + row * p.ldz, c, p.cols, o.z + i * VEC);
-    }
-    if (!p.x)
-#pragma unroll
-        for (int e = 0; e < NE; ++e) o.r[e] = 0.0f;
-    if (p.y) {
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-            o.sz[e] = p.z ? o.z[e] * act_sigmoid(o.z[e]) : 1.0f;
-            o.u[e] = o.y[e] * o.sz[e];
-            ss += (S)o.u[e] * (S)o.u[e];
-        }
-        o.i1 = 1 / sqrt(row_sum<WPR>(ss, lds) / (S)p.cols + (S)p.eps);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * 64 * WPR + tid) * VEC;
-            float w1[VEC], s[VEC];
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) w1[k] = s[k] = 1.0f;
-            if (p.w1) row_load<VEC>(p.w1, c, p.cols, w1);
-            if (p.s) row_load<VEC>(p.s, c, p.cols, s);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k)
-                o.r[i * VEC + k] = fmaf(s[k], o.u[i * VEC + k] * (float)o.i1 * w1[k], o.r[i * VEC + k]);
-        }
-    }
-    if (second) {
-        ss = 0;
-#pragma unroll
-        for (int e = 0; e < NE; ++e) ss += (S)o.r[e] * (S)o.r[e];
-        o.i2 = 1 / sqrt(row_sum<WPR>(ss, lds) / (S)p.cols + (S)p.eps);
+        for (int k = 0; k < VEC; ++k) v[k] = 1.0f;
     }
 }
 
 template <typename E, int VEC, int NV, int WPR>
 __global__ __launch_bounds__(bn_threads<WPR>()) void block_norm_fwd_k(NormArgs p) {
-    __shared__ float lds[16];
-    constexpr int RPB = bn_threads<WPR>() / (64 * WPR);
+    __shared__ float lds[WPR];
+    constexpr int NE = VEC * NV, RPB = bn_threads<WPR>() / (64 * WPR);
     const long row = (long)blockIdx.x * RPB + threadIdx.x / (64 * WPR);
     const int tid = threadIdx.x % (64 * WPR);
     if (row >= p.rows) return;
-    BnRow<float, VEC * NV> o;
-    bn_row<float, E, VEC, NV, WPR>(p, row, tid, p.n != nullptr, lds, o);
+    const void* any = p.x ? p.x : p.y;
+    const long la = p.x ? p.ldx : p.ldy;
+    const NormOp<E> ox(p.x, p.ldx, any, la), oy(p.y, p.ldy, any, la), oz(p.z, p.ldz, any, la);
+    act_raw<VEC, E> rx[NV], ry[NV], rz[NV];
+    float w1[NE], s[NE], w2[NE], r[NE], u[NE], z[NE], ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * 64 * WPR + tid) * VEC;
-        if (p.r) row_store<VEC>(static_cast<E*>(p.r) + row * p.ldr, c, p.cols, o.r + i * VEC);
-        if (p.n) {
-            float w2[VEC];
+        rx[i] = ox.template load<VEC>(row, c, p.cols);
+        ry[i] = oy.template load<VEC>(row, c, p.cols);
+        rz[i] = oz.template load<VEC>(row, c, p.cols);
+    }
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) w2[k] = 1.0f;
-            if (p.w2) row_load<VEC>(p.w2, c, p.cols, w2);
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 64 * WPR + tid) * VEC;
+        par_load<VEC>(p.w1, c, p.cols, w1 + i * VEC);
+        par_load<VEC>(p.s, c, p.cols, s + i * VEC);
+        par_load<VEC>(p.w2, c, p.cols, w2 + i * VEC);
+    }
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) w2[k] *= o.r[i * VEC + k] * o.i2;
-            row_store<VEC>(static_cast<E*>(p.n) + row * p.ldn, c, p.cols, w2);
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 64 * WPR + tid) * VEC;
+        ox.template values<VEC>(rx[i], c, p.cols, r + i * VEC);
+        oy.template values<VEC>(ry[i], c, p.cols, u + i * VEC);
+        oz.template values<VEC>(rz[i], c, p.cols, z + i * VEC);
+    }
+    if (p.y) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            if (p.z) u[e] *= z[e] * act_sigmoid(z[e]);
+            ss = fmaf(u[e], u[e], ss);
         }
+        const float i1 = 1.0f / sqrtf(row_sum<WPR>(ss, lds) / (float)p.cols + p.eps);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) r[e] = fmaf(s[e], u[e] * i1 * w1[e], r[e]);
+    }
+    if (p.r)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            row_store<VEC>(static_cast<E*>(p.r) + row * p.ldr, (i * 64 * WPR + tid) * VEC, p.cols, r + i * VEC);
+    if (!p.n) return;
+    ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) ss = fmaf(r[e], r[e], ss);
+    const float i2 = 1.0f / sqrtf(row_sum<WPR>(ss, lds) / (float)p.cols + p.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 64 * WPR + tid) * VEC;
+        float v[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = r[i * VEC + k] * i2 * w2[i * VEC + k];
+        row_store<VEC>(static_cast<E*>(p.n) + row * p.ldn, c, p.cols, v);
     }
 }
+
+// All sums that a row needs are sums of products of its inputs: with q = s w1 u,
+// k = w2 dn and r = x + i1 q,
+//   sum r^2 = sum x^2 + 2 i1 sum x q + i1^2 sum q^2,  sum k r = sum k x + i1 sum k q,
+//   sum dR q = sum dr q + i2 (sum k q - m2 (sum x q + i1 sum q^2)),
+// so one pass and one exchange between the threads give seven of them, and nothing
+// waits for a second.  They are taken in 64 bits, as k - r m2 and t - u m1 are:
+// these cancel where the gradient is near a multiple of the row (always in a row of
+// one column), and products of two f32 values are exact there.
+// Adds an element's products to the seven sums: c = s w1, k = w2 dn
+ASCA_DEV void norm_sums(double (&v)[8], float x, float u, float c, float k, float dr) {
+    const double ud = u, q = (double)c * ud, kd = k, xd = x;
+    v[0] = fma(ud, ud, v[0]);
+    v[1] = fma(xd, xd, v[1]);
+    v[2] = fma(xd, q, v[2]);
+    v[3] = fma(q, q, v[3]);
+    v[4] = fma(kd, xd, v[4]);
+    v[5] = fma(kd, q, v[5]);
+    v[6] = fma((double)dr, q, v[6]);
+}
+
+// What a row's sums come to
+struct NormStats {
+    double i1, i2, m1, m2;
+    float i1f, i2f;
+    ASCA_DEV NormStats(const NormArgs& p, const double (&v)[8]) {
+        const double in = 1.0 / p.cols;
+        i1 = 1.0 / sqrt(fma(v[0], in, (double)p.eps));
+        const double rq = fma(i1, v[3], v[2]);
+        i2 = p.dn ? 1.0 / sqrt(fma(fma(i1, v[2] + rq, v[1]), in, (double)p.eps)) : 0.0;
+        m2 = fma(i1, v[5], v[4]) * in * (i2 * i2);
+        m1 = fma(i2, v[5] - m2 * rq, v[6]) * in * (i1 * i1);
+        i1f = (float)i1, i2f = (float)i2;
+    }
+};
+
+// An element's dR, du, dR uh and rms(r)
+struct NormGrad {
+    double dR;
+    float du, ru, rh;
+    ASCA_DEV NormGrad(const NormStats& n, float x, float u, float c, float k, float dr) {
+        const double r = fma(n.i1, (double)c * (double)u, (double)x);
+        dR = fma(n.i2, fma(-r, n.m2, (double)k), (double)dr);
+        du = n.i1f * (float)fma(-(double)u, n.m1, dR * c);
+        ru = (float)dR * (u * n.i1f);
+        rh = (float)r * n.i2f;
+    }
+};
 
 template <typename E, int VEC, int NV, int WPR>
 __global__ __launch_bounds__(bn_threads<WPR>()) void block_norm_bwd_k(NormArgs p) {
     constexpr int NE = VEC * NV, NT = bn_threads<WPR>(), RPB = NT / (64 * WPR);
-    __shared__ double lds[16];
+    __shared__ double lds[2][WPR][8];
     __shared__ float acc[RPB > 1 ? NT * NE : 1];
     const int sub = threadIdx.x / (64 * WPR), tid = threadIdx.x % (64 * WPR);
     float g1[NE], gs[NE], g2[NE];
 #pragma unroll
     for (int e = 0; e < NE; ++e) g1[e] = gs[e] = g2[e] = 0.0f;
-    for (long row = (long)blockIdx.x * RPB + sub; row < p.rows; row += (long)gridDim.x * RPB) {
-        BnRow<double, NE> o;
-        float dr[NE], dn[NE];
+    int turn = 0;
+    const void* any = p.x ? p.x : p.y;
+    const long la = p.x ? p.ldx : p.ldy;
+    const NormOp<E> ox(p.x, p.ldx, any, la), oy(p.y, p.ldy, any, la), oz(p.z, p.ldz, any, la), odr(p.dr, p.lddr, any, la),
+        odn(p.dn, p.lddn, any, la);
+    // the parameters stay; a row's operands are loaded while the row before is worked on
+    float w1[NV][VEC], s[NV][VEC], w2[NV][VEC];
+    act_raw<VEC, E> rx[NV], ry[NV], rz[NV], rdr[NV], rdn[NV];
+    auto load = [&](long row) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * 64 * WPR + tid) * VEC;
-            if (p.dr) row_load<VEC>(static_cast<const E*>(p.dr) + row * p.lddr, c, p.cols, dr + i * VEC);
-            if (p.dn) row_load<VEC>(static_cast<const E*>(p.dn) + row * p.lddn, c, p.cols, dn + i * VEC);
+            rx[i] = ox.template load<VEC>(row, c, p.cols);
+            ry[i] = oy.template load<VEC>(row, c, p.cols);
+            rz[i] = oz.template load<VEC>(row, c, p.cols);
+            rdr[i] = odr.template load<VEC>(row, c, p.cols);
+            rdn[i] = odn.template load<VEC>(row, c, p.cols);
         }
-        if (!p.dr)
+    };
+    load(min((long)blockIdx.x * RPB + sub, p.rows - 1));
 #pragma unroll
-            for (int e = 0; e < NE; ++e) dr[e] = 0.0f;
-        bn_row<double, E, VEC, NV, WPR>(p, row, tid, p.dn != nullptr, lds, o);
-        if (p.dn) {
-            const float i2 = (float)o.i2;
-            double m = 0.0;
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 64 * WPR + tid) * VEC;
+        par_load<VEC>(p.w1, c, p.cols, w1[i]);
+        par_load<VEC>(p.s, c, p.cols, s[i]);
+        par_load<VEC>(p.w2, c, p.cols, w2[i]);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (i * 64 * WPR + tid) * VEC;
-                float w2[VEC];
+        for (int m = 0; m < VEC; ++m) asm volatile("" : "+v"(w1[i][m]), "+v"(s[i][m]), "+v"(w2[i][m]));
+    }
+    for (long row = (long)blockIdx.x * RPB + sub; row < p.rows; row += (long)gridDim.x * RPB, ++turn) {
+        float x[NV][VEC], y[NV][VEC], z[NV][VEC], dr[NV][VEC], dn[NV][VEC], sg[NV][VEC];
+        double v[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+        auto values = [&](int i) {
+            const int c = (i * 64 * WPR + tid) * VEC;
+            ox.template values<VEC>(rx[i], c, p.cols, x[i]);
+            oy.template values<VEC>(ry[i], c, p.cols, y[i]);
+            oz.template values<VEC>(rz[i], c, p.cols, z[i]);
+            odr.template values<VEC>(rdr[i], c, p.cols, dr[i]);
+            odn.template values<VEC>(rdn[i], c, p.cols, dn[i]);
+        };
+        auto gates = [&](int i) {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) w2[k] = 1.0f;
-                if (p.w2) row_load<VEC>(p.w2, c, p.cols, w2);
+            for (int m = 0; m < VEC; ++m) sg[i][m] = p.z ? act_sigmoid(z[i][m]) : 1.0f;
+        };
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const int e = i * VEC + k;
-                    g2[e] = fmaf(dn[e], o.r[e] * i2, g2[e]);
-                    dn[e] *= w2[k];
-                    m = fma((double)dn[e], (double)o.r[e], m);
-                }
+        for (int i = 0; i < NV; ++i) values(i);
+        load(min(row + (long)gridDim.x * RPB, p.rows - 1));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            gates(i);
+#pragma unroll
+            for (int m = 0; m < VEC; ++m) {
+                const float u = p.z ? y[i][m] * (z[i][m] * sg[i][m]) : y[i][m];
+                norm_sums(v, x[i][m], u, s[i][m] * w1[i][m], dn[i][m] * w2[i][m], dr[i][m]);
             }
-            m = row_sum<WPR>(m, lds) / p.cols * (o.i2 * o.i2);
-#pragma unroll
-            for (int e = 0; e < NE; ++e) dr[e] = fmaf(i2, (float)fma(-(double)o.r[e], m, (double)dn[e]), dr[e]);
         }
-        if (p.dx)
+        row_sums8<WPR>(v, lds, turn);
+        // the 64-bit copies are made again below rather than kept over the exchange
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                row_store<VEC>(static_cast<E*>(p.dx) + row * p.lddx, (i * 64 * WPR + tid) * VEC, p.cols, dr + i * VEC);
-        if (p.y) {
-            const float i1 = (float)o.i1;
-            double m = 0.0;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (i * 64 * WPR + tid) * VEC;
-                float w1[VEC], s[VEC];
+            for (int m = 0; m < VEC; ++m)
+                asm volatile("" : "+v"(x[i][m]), "+v"(y[i][m]), "+v"(dr[i][m]), "+v"(dn[i][m]), "+v"(sg[i][m]));
+        const NormStats n(p, v);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) w1[k] = s[k] = 1.0f;
-                if (p.w1) row_load<VEC>(p.w1, c, p.cols, w1);
-                if (p.s) row_load<VEC>(p.s, c, p.cols, s);
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 64 * WPR + tid) * VEC;
+            float vx[VEC], vy[VEC], vz[VEC];
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const int e = i * VEC + k;
-                    const float ru = dr[e] * (o.u[e] * i1);
-                    gs[e] = fmaf(ru, w1[k], gs[e]);
-                    g1[e] = fmaf(ru, s[k], g1[e]);
-                    dr[e] *= s[k] * w1[k];
-                    m = fma((double)dr[e], (double)o.u[e], m);
-                }
+            for (int m = 0; m < VEC; ++m) {
+                const int e = i * VEC + m;
+                const float zz = z[i][m], sz = sg[i][m], gate = p.z ? zz * sz : 1.0f;
+                const NormGrad g(n, x[i][m], y[i][m] * gate, s[i][m] * w1[i][m], dn[i][m] * w2[i][m], dr[i][m]);
+                g2[e] = fmaf(dn[i][m], g.rh, g2[e]);
+                gs[e] = fmaf(g.ru, w1[i][m], gs[e]);
+                g1[e] = fmaf(g.ru, s[i][m], g1[e]);
+                vx[m] = (float)g.dR;
+                vy[m] = g.du * gate;
+                vz[m] = p.z ? g.du * y[i][m] * (sz * fmaf(zz, 1.0f - sz, 1.0f)) : 0.0f;
             }
-            m = row_sum<WPR>(m, lds) / p.cols * (o.i1 * o.i1);
-#pragma unroll
-            for (int e = 0; e < NE; ++e) dr[e] = i1 * (float)fma(-(double)o.u[e], m, (double)dr[e]);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (i * 64 * WPR + tid) * VEC;
-                float v[VEC];
-                if (p.dy) {
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) v[k] = dr[i * VEC + k] * o.sz[i * VEC + k];
-                    row_store<VEC>(static_cast<E*>(p.dy) + row * p.lddy, c, p.cols, v);
-                }
-                if (p.z && p.dz) {
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) {
-                        const float z = o.z[i * VEC + k], sg = act_sigmoid(z);
-                        v[k] = dr[i * VEC + k] * o.y[i * VEC + k] * (sg * fmaf(z, 1.0f - sg, 1.0f));
-                    }
-                    row_store<VEC>(static_cast<E*>(p.dz) + row * p.lddz, c, p.cols, v);
-                }
-            }
+            if (p.dx) row_store<VEC>(static_cast<E*>(p.dx) + row * p.lddx, c, p.cols, vx);
+            if (p.dy) row_store<VEC>(static_cast<E*>(p.dy) + row * p.lddy, c, p.cols, vy);
+            if (p.dz) row_store<VEC>(static_cast<E*>(p.dz) + row * p.lddz, c, p.cols, vz);
         }
     }
     if (!p.part) return;
@@ -299,38 +365,163 @@ __global__ __launch_bounds__(bn_threads<WPR>()) void block_norm_bwd_k(NormArgs p
     put(2, g2);
 }
 
+// Rows of any width: a block of BW_NT threads walks the row and reads it again for
+// each further sum (from a cache), and the backward adds to its own row of partial
+// sums in memory.
+constexpr int BW_NT = 512;
+
+template <typename E, int VEC>
+struct NormWide {
+    const NormArgs& p;
+    long row;
+    NormOp<E> ox, oy, oz;
+    ASCA_DEV NormWide(const NormArgs& a, long r)
+        : p(a), row(r), ox(a.x, a.ldx, a.x ? a.x : a.y, a.x ? a.ldx : a.ldy),
+          oy(a.y, a.ldy, a.x ? a.x : a.y, a.x ? a.ldx : a.ldy), oz(a.z, a.ldz, a.x ? a.x : a.y, a.x ? a.ldx : a.ldy) {}
+    // x, y, z and u = y silu(z) at column c
+    ASCA_DEV void at(int c, float* x, float* y, float* z, float* sg, float* u) const {
+        const auto rx = ox.template load<VEC>(row, c, p.cols), ry = oy.template load<VEC>(row, c, p.cols),
+                   rz = oz.template load<VEC>(row, c, p.cols);
+        ox.template values<VEC>(rx, c, p.cols, x);
+        oy.template values<VEC>(ry, c, p.cols, y);
+        oz.template values<VEC>(rz, c, p.cols, z);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            sg[k] = p.z ? act_sigmoid(z[k]) : 1.0f;
+            u[k] = p.z ? y[k] * (z[k] * sg[k]) : y[k];
+        }
+    }
+};
+
+template <typename E, int VEC>
+__global__ __launch_bounds__(BW_NT) void block_norm_fwd_wide_k(NormArgs p) {
+    __shared__ float lds[BW_NT / 64];
+    const NormWide<E, VEC> w(p, blockIdx.x);
+    float x[VEC], y[VEC], z[VEC], sg[VEC], u[VEC], w1[VEC], s[VEC], i1 = 0.0f;
+    if (p.y) {
+        float ss = 0.0f;
+        for (int c = threadIdx.x * VEC; c < p.cols; c += BW_NT * VEC) {
+            w.at(c, x, y, z, sg, u);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) ss = fmaf(u[k], u[k], ss);
+        }
+        i1 = 1.0f / sqrtf(row_sum<BW_NT / 64>(ss, lds) / (float)p.cols + p.eps);
+    }
+    auto r_at = [&](int c, float* r) {
+        w.at(c, r, y, z, sg, u);
+        par_load<VEC>(p.w1, c, p.cols, w1);
+        par_load<VEC>(p.s, c, p.cols, s);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) r[k] = p.y ? fmaf(s[k], u[k] * i1 * w1[k], r[k]) : r[k];
+    };
+    float ss = 0.0f, i2 = 0.0f;
+    if (p.n) {
+        for (int c = threadIdx.x * VEC; c < p.cols; c += BW_NT * VEC) {
+            r_at(c, x);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) ss = fmaf(x[k], x[k], ss);
+        }
+        i2 = 1.0f / sqrtf(row_sum<BW_NT / 64>(ss, lds) / (float)p.cols + p.eps);
+    }
+    // r may be x: a thread overwrites only columns that it has read
+    for (int c = threadIdx.x * VEC; c < p.cols; c += BW_NT * VEC) {
+        r_at(c, x);
+        if (p.r) row_store<VEC>(static_cast<E*>(p.r) + w.row * p.ldr, c, p.cols, x);
+        if (!p.n) continue;
+        par_load<VEC>(p.w2, c, p.cols, w1);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x[k] *= i2 * w1[k];
+        row_store<VEC>(static_cast<E*>(p.n) + w.row * p.ldn, c, p.cols, x);
+    }
+}
+
+template <typename E, int VEC>
+__global__ __launch_bounds__(BW_NT) void block_norm_bwd_wide_k(NormArgs p) {
+    __shared__ double lds[2][BW_NT / 64][8];
+    int turn = 0;
+    for (long row = blockIdx.x; row < p.rows; row += gridDim.x, ++turn) {
+        const NormWide<E, VEC> w(p, row);
+        const NormOp<E> odr(p.dr, p.lddr, p.x ? p.x : p.y, p.x ? p.ldx : p.ldy),
+            odn(p.dn, p.lddn, p.x ? p.x : p.y, p.x ? p.ldx : p.ldy);
+        float x[VEC], y[VEC], z[VEC], sg[VEC], u[VEC], dr[VEC], dn[VEC], w1[VEC], s[VEC], w2[VEC];
+        auto at = [&](int c) {
+            const auto rdr = odr.template load<VEC>(row, c, p.cols), rdn = odn.template load<VEC>(row, c, p.cols);
+            w.at(c, x, y, z, sg, u);
+            odr.template values<VEC>(rdr, c, p.cols, dr);
+            odn.template values<VEC>(rdn, c, p.cols, dn);
+            par_load<VEC>(p.w1, c, p.cols, w1);
+            par_load<VEC>(p.s, c, p.cols, s);
+            par_load<VEC>(p.w2, c, p.cols, w2);
+        };
+        double v[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+        for (int c = threadIdx.x * VEC; c < p.cols; c += BW_NT * VEC) {
+            at(c);
+#pragma unroll
+            for (int m = 0; m < VEC; ++m) norm_sums(v, x[m], u[m], s[m] * w1[m], dn[m] * w2[m], dr[m]);
+        }
+        row_sums8<BW_NT / 64>(v, lds, turn);
+        const NormStats n(p, v);
+        const bool first = row == blockIdx.x;
+        for (int c = threadIdx.x * VEC; c < p.cols; c += BW_NT * VEC) {
+            at(c);
+            float vx[VEC], vy[VEC], vz[VEC];
+#pragma unroll
+            for (int m = 0; m < VEC; ++m) {
+                const NormGrad g(n, x[m], u[m], s[m] * w1[m], dn[m] * w2[m], dr[m]);
+                vx[m] = (float)g.dR;
+                vy[m] = p.z ? g.du * (z[m] * sg[m]) : g.du;
+                vz[m] = g.du * y[m] * (sg[m] * fmaf(z[m], 1.0f - sg[m], 1.0f));
+                if (p.part && c + m < p.cols) {
+                    float* t = p.part + (long)blockIdx.x * 3 * p.cols + c + m;
+                    const float a[3] = {g.ru * s[m], g.ru * w1[m], dn[m] * g.rh};
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) t[(long)k * p.cols] = first ? a[k] : t[(long)k * p.cols] + a[k];
+                }
+            }
+            if (p.dx) row_store<VEC>(static_cast<E*>(p.dx) + row * p.lddx, c, p.cols, vx);
+            if (p.dy) row_store<VEC>(static_cast<E*>(p.dy) + row * p.lddy, c, p.cols, vy);
+            if (p.dz) row_store<VEC>(static_cast<E*>(p.dz) + row * p.lddz, c, p.cols, vz);
+        }
+    }
+}
+
 }  // namespace asca
 
 using namespace asca;
 
-// Calls f with (element type, VEC, NV, WPR): 16-byte (bf16: 8-byte) access where
-// every row and the parameters allow it, a wave a row up to 1024 columns, 4 up to
-// 4096, else 16.
-template <typename F>
+// Columns of the kernels that hold a row in registers; wider rows are walked.
+static int bn_held(bool bwd) { return bwd ? 2048 : 4096; }
+
+// Calls f with (element type, VEC, NV, WPR), NV = 0 for wide rows: 16-byte (bf16:
+// 8-byte) access where every row and the parameters allow it; a row has as few waves
+// as its values a lane allow, 8, or 16 in the forward's widest.
+template <bool BWD, typename F>
 static int bn_dispatch(int dtype, int cols, bool vec, F f) {
     return act_dispatch(dtype, [&](auto* e) {
-        auto go = [&](auto v, auto nv, auto wpr) { return f(e, v, nv, wpr); };
         using std::integral_constant;
+        auto go = [&](auto ne, auto wpr) {
+            constexpr int NE = decltype(ne)::value;
+            return vec ? f(e, integral_constant<int, 4>{}, integral_constant<int, NE / 4>{}, wpr)
+                       : f(e, integral_constant<int, 1>{}, integral_constant<int, NE>{}, wpr);
+        };
+        const integral_constant<int, 0> n0;
         const integral_constant<int, 1> c1;
         const integral_constant<int, 2> c2;
         const integral_constant<int, 4> c4;
+        const integral_constant<int, 8> c8;
         const integral_constant<int, 16> c16;
-        if (vec) {
-            if (cols <= 256) return go(c4, c1, c1);
-            if (cols <= 512) return go(c4, c2, c1);
-            if (cols <= 1024) return go(c4, c4, c1);
-            if (cols <= 4096) return go(c4, c4, c4);
-            return go(c4, c4, c16);
+        if (cols > bn_held(BWD)) return go(n0, c1);
+        if (cols <= 256) return go(c4, c1);
+        if (cols <= 512) return go(c8, c1);
+        if (cols <= 1024) return go(c8, c2);
+        if constexpr (BWD) {
+            return go(c8, c4);
+        } else {
+            if (cols <= 2048) return go(c8, c4);
+            return go(c16, c4);
         }
-        if (cols <= 256) return go(c1, c4, c1);
-        if (cols <= 1024) return go(c1, c16, c1);
-        if (cols <= 4096) return go(c1, c16, c4);
-        return go(c1, c16, c16);
     });
 }
-
-// Rows a block takes for `cols` columns
-static int bn_rpb(int cols) { return cols <= 1024 ? 4 : 1; }
 
 static int bn_row_check(const char* fn, const char* what, const void* a, long ld, int cols) {
     if (!a || ld >= cols) return ASCA_OK;
@@ -346,7 +537,6 @@ int asca_block_norm_fwd(const void* x, long ldx, const void* y, long ldy, const 
     if (rows < 0 || cols < 0) return fail(ASCA_ERR_INVALID, "%s: negative shape", fn);
     int rc = act_dispatch(dtype, [](auto*) { return (int)ASCA_OK; });
     if (rc) return rc;
-    if (cols > BN_MAX) return fail(ASCA_ERR_UNSUPPORTED, "%s: cols=%d above %d", fn, cols, BN_MAX);
     if (!y && (z || w_post || scale)) return fail(ASCA_ERR_INVALID, "%s: z, w_post or scale without y", fn);
     if (!n && w_pre) return fail(ASCA_ERR_INVALID, "%s: w_pre without n", fn);
     if (rows == 0 || cols == 0) return ASCA_OK;
@@ -355,26 +545,27 @@ int asca_block_norm_fwd(const void* x, long ldx, const void* y, long ldy, const 
         (rc = bn_row_check(fn, "ldz", z, ldz, cols)) || (rc = bn_row_check(fn, "ldr", r, ldr, cols)) ||
         (rc = bn_row_check(fn, "ldn", n, ldn, cols)))
         return rc;
-    const size_t size = dtype == ASCA_F32 ? 4 : 2;
     bool vec = cols % 4 == 0;
-    auto rows_ok = [&](const void* a, long ld) {
-        return !a || (ld % 4 == 0 && reinterpret_cast<uintptr_t>(a) % (4 * size) == 0);
-    };
+    auto rows_ok = [&](const void* a, long ld) { return act_vec_ok(a, ld, dtype); };
     auto par_ok = [&](const float* a) { return reinterpret_cast<uintptr_t>(a) % 16 == 0; };
     vec = vec && rows_ok(x, ldx) && rows_ok(y, ldy) && rows_ok(z, ldz) && rows_ok(r, ldr) && rows_ok(n, ldn) &&
           par_ok(w_post) && par_ok(scale) && par_ok(w_pre);
     NormArgs p{};
     p.x = x, p.y = y, p.z = z, p.ldx = ldx, p.ldy = ldy, p.ldz = ldz, p.w1 = w_post, p.s = scale, p.w2 = w_pre;
     p.r = r, p.n = n, p.ldr = ldr, p.ldn = ldn, p.rows = rows, p.cols = cols, p.eps = eps;
-    const long blocks = (rows + bn_rpb(cols) - 1) / bn_rpb(cols);
+    const int rpb = cols <= 512 ? 4 : 1;
+    const long blocks = (rows + rpb - 1) / rpb;
     if (blocks > 0x7fffffffL) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows", fn);
-    return bn_dispatch(dtype, cols, vec, [&](auto* e, auto v, auto nv, auto wpr) {
+    return bn_dispatch<false>(dtype, cols, vec, [&](auto* e, auto v, auto nv, auto wpr) {
         using E = std::remove_pointer_t<decltype(e)>;
         constexpr int V = decltype(v)::value, NV = decltype(nv)::value, WPR = decltype(wpr)::value;
         int q = pre_launch("block_norm_fwd");
         if (q) return q;
-        hipLaunchKernelGGL((block_norm_fwd_k<E, V, NV, WPR>), dim3((unsigned)blocks), dim3(bn_threads<WPR>()), 0,
-                           as_stream(stream), p);
+        const hipStream_t st = as_stream(stream);
+        if constexpr (NV == 0)
+            hipLaunchKernelGGL((block_norm_fwd_wide_k<E, V>), dim3((unsigned)blocks), dim3(BW_NT), 0, st, p);
+        else
+            hipLaunchKernelGGL((block_norm_fwd_k<E, V, NV, WPR>), dim3((unsigned)blocks), dim3(bn_threads<WPR>()), 0, st, p);
         return post_launch("block_norm_fwd");
     });
 }
@@ -387,7 +578,6 @@ int asca_block_norm_bwd(const void* x, long ldx, const void* y, long ldy, const 
     if (rows < 0 || cols < 0) return fail(ASCA_ERR_INVALID, "%s: negative shape", fn);
     int rc = act_dispatch(dtype, [](auto*) { return (int)ASCA_OK; });
     if (rc) return rc;
-    if (cols > BN_MAX) return fail(ASCA_ERR_UNSUPPORTED, "%s: cols=%d above %d", fn, cols, BN_MAX);
     if (!y && (z || w_post || scale)) return fail(ASCA_ERR_INVALID, "%s: z, w_post or scale without y", fn);
     if ((dx && !x) || (dy && !y) || (dz && !z) || (dw_post && !w_post) || (dscale && !scale) || (dw_pre && !w_pre))
         return fail(ASCA_ERR_INVALID, "%s: a gradient of an input that is NULL", fn);
@@ -398,10 +588,7 @@ int asca_block_norm_bwd(const void* x, long ldx, const void* y, long ldy, const 
         (rc = bn_row_check(fn, "lddn", dn, lddn, cols)) || (rc = bn_row_check(fn, "lddx", dx, lddx, cols)) ||
         (rc = bn_row_check(fn, "lddy", dy, lddy, cols)) || (rc = bn_row_check(fn, "lddz", dz, lddz, cols)))
         return rc;
-    const size_t size = dtype == ASCA_F32 ? 4 : 2;
-    auto rows_ok = [&](const void* a, long ld) {
-        return !a || (ld % 4 == 0 && reinterpret_cast<uintptr_t>(a) % (4 * size) == 0);
-    };
+    auto rows_ok = [&](const void* a, long ld) { return act_vec_ok(a, ld, dtype); };
     auto par_ok = [&](const float* a) { return reinterpret_cast<uintptr_t>(a) % 16 == 0; };
     const bool vec = cols % 4 == 0 && rows_ok(x, ldx) && rows_ok(y, ldy) && rows_ok(z, ldz) && rows_ok(dr, lddr) &&
                      rows_ok(dn, lddn) && rows_ok(dx, lddx) && rows_ok(dy, lddy) && rows_ok(dz, lddz) && par_ok(w_post) &&
@@ -411,19 +598,25 @@ int asca_block_norm_bwd(const void* x, long ldx, const void* y, long ldy, const 
     p.x = x, p.y = y, p.z = z, p.ldx = ldx, p.ldy = ldy, p.ldz = ldz, p.w1 = w_post, p.s = scale, p.w2 = w_pre;
     p.dr = dr, p.dn = dn, p.lddr = lddr, p.lddn = lddn, p.dx = dx, p.dy = dy, p.dz = dz;
     p.lddx = lddx, p.lddy = lddy, p.lddz = lddz, p.rows = rows, p.cols = cols, p.eps = eps;
-    const long blocks = std::min((rows + bn_rpb(cols) - 1) / bn_rpb(cols), 1024L);
+    const int rpb = cols <= 512 ? 4 : 1;
+    // what the CUs hold at once: each block is two waves a SIMD's registers allow
+    const long held = cols > 512 && cols <= 1024 ? 1024 : 512;
+    const long blocks = std::min((rows + rpb - 1) / rpb, held);
     const bool sums = dw_post || dscale || dw_pre;
     StreamScratch sc;
     if (sums && (rc = sc.get((size_t)blocks * 3 * cols, st))) return rc;
     p.part = sc.ws.p;
     if (blocks)
-        rc = bn_dispatch(dtype, cols, vec, [&](auto* e, auto v, auto nv, auto wpr) {
+        rc = bn_dispatch<true>(dtype, cols, vec, [&](auto* e, auto v, auto nv, auto wpr) {
             using E = std::remove_pointer_t<decltype(e)>;
             constexpr int V = decltype(v)::value, NV = decltype(nv)::value, WPR = decltype(wpr)::value;
             int q = pre_launch("block_norm_bwd");
             if (q) return q;
-            hipLaunchKernelGGL((block_norm_bwd_k<E, V, NV, WPR>), dim3((unsigned)blocks), dim3(bn_threads<WPR>()), 0, st,
-                               p);
+            if constexpr (NV == 0)
+                hipLaunchKernelGGL((block_norm_bwd_wide_k<E, V>), dim3((unsigned)blocks), dim3(BW_NT), 0, st, p);
+            else
+                hipLaunchKernelGGL((block_norm_bwd_k<E, V, NV, WPR>), dim3((unsigned)blocks), dim3(bn_threads<WPR>()), 0,
+                                   st, p);
             return post_launch("block_norm_bwd");
         });
     if (rc || !sums) return rc;

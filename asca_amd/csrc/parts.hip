@@ -1,7 +1,7 @@
 // Sums of per-block partial gradients.  A gradient that many blocks add to (a
 // weight's, a bias's) is written by each as a row of partial sums; one wave
-// here adds every fourth row of 64 columns, PU loads in flight, and the block's
-// four waves' sums are added through LDS: a fixed order, no atomics.
+// here adds every PWth row of 64 columns, PU loads in flight, and the block's
+// waves' sums are added through LDS: a fixed order, no atomics.
 #include "parts.h"
 
 #include "common.h"
@@ -9,25 +9,26 @@
 
 namespace asca {
 
-constexpr int PU = 8;
+constexpr int PU = 8, PW = 16;
 
-__global__ __launch_bounds__(256) void sum_parts_k(const float* __restrict__ part, long parts, long row, PartsOut o) {
-    __shared__ float red[4][64];
+__global__ __launch_bounds__(64 * PW) void sum_parts_k(const float* __restrict__ part, long parts, long row, PartsOut o) {
+    __shared__ float red[PW][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const long i = (long)blockIdx.x * 64 + lane;
     float s = 0.0f;
     if (i < row)
-        for (long k = w; k < parts; k += 4 * PU) {
+        for (long k = w; k < parts; k += PW * PU) {
             float v[PU];
 #pragma unroll
-            for (int u = 0; u < PU; ++u) v[u] = k + 4 * u < parts ? part[(k + 4 * u) * row + i] : 0.0f;
+            for (int u = 0; u < PU; ++u) v[u] = k + PW * u < parts ? part[(k + PW * u) * row + i] : 0.0f;
 #pragma unroll
             for (int u = 0; u < PU; ++u) s += v[u];
         }
     red[w][lane] = s;
     __syncthreads();
     if (w || i >= row) return;
-    s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+#pragma unroll
+    for (int k = 1; k < PW; ++k) s += red[k][lane];
     long at = i;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
@@ -41,7 +42,7 @@ int sum_parts_launch(const float* part, long parts, const PartsOut& o, hipStream
     if (row == 0) return ASCA_OK;
     int rc = pre_launch("sum_parts");
     if (rc) return rc;
-    hipLaunchKernelGGL(sum_parts_k, dim3((unsigned)((row + 63) / 64)), dim3(256), 0, st, part, parts, row, o);
+    hipLaunchKernelGGL(sum_parts_k, dim3((unsigned)((row + 63) / 64)), dim3(64 * PW), 0, st, part, parts, row, o);
     return post_launch("sum_parts");
 }
 

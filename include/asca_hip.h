@@ -583,7 +583,7 @@ ASCA_API int asca_ssm_step(float* h, const void* x, long ldx, const void* dt, lo
  *   (NULL = no gate); w_post, scale, w_pre : (cols), NULL = ones
  *   y NULL: r = x (the norm before the first block; z, w_post, scale NULL too)
  *   r, n : outputs, either may be NULL.  n is formed from the unrounded r.
- *   1 <= cols <= 16384.  r may be x. */
+ *   r may be x. */
 ASCA_API int asca_block_norm_fwd(const void* x, long ldx, const void* y, long ldy, const void* z, long ldz,
                                  const float* w_post, const float* scale, const float* w_pre, void* r, long ldr,
                                  void* n, long ldn, long rows, int cols, float eps, int dtype, void* stream);

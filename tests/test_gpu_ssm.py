@@ -213,7 +213,7 @@ def test_ssm_step_goes_on_from_a_prompt(g, n, D, N, G, bf16):
 
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 64), (9, 256), (130, 260), (33, 512), (7, 1000), (5, 1024), (6, 1025), (3, 2048),
-                                       (2, 4099), (2, 8192), (1, 16383), (1030, 36)])
+                                       (2, 4099), (2, 8192), (1, 16383), (3, 20001), (1030, 36)])
 def test_block_norm(g, rows, cols, bf16):
     print(f"[norm] rows={rows} cols={cols} bf16={bf16}", flush=True)
     rng = np.random.default_rng(rows + cols)
@@ -475,7 +475,7 @@ def test_refusals(g):
            (("asca_conv_fwd", f, 8, f, None, f, None, f, 8, f, 1, 4, 8, 4, 1, 0, None), 1),
            (ssm(N=0), 3), (ssm(N=65), 3), (ssm(G=3), 1), (ssm(G=0), 1), (ssm(ty=-1), 3), (ssm(ld=7), 1), (ssm(x=None), 1), (ssm(A=None), 1),
            (ssm(h0=f, ho=f), 1), (("asca_ssm_ws_bytes", 1, -1, 8, 4, C.byref(out)), 1), (("asca_ssm_ws_bytes", 1, 1, 8, 4, None), 1),
-           (norm(cols=16385, ld=1 << 15), 3), (norm(ld=7), 1), (norm(y=None), 1), (norm(r=None), 1), (norm(ty=7), 3),
+           (norm(ld=7), 1), (norm(y=None), 1), (norm(r=None), 1), (norm(ty=7), 3),
            (norm(x=None, y=None, z=None), 1),
            (("asca_grads_create", one, None, (C.c_uint64 * 1)(4), 1, 0, C.byref(h)), 1),
            (("asca_grads_create", None, None, None, -1, 0, C.byref(h)), 1), (("asca_grads_create", None, None, None, 0, 5, C.byref(h)), 3),
