@@ -98,13 +98,14 @@ ASCA_DEV void unroll(F f) {
     unroll_(f, std::make_integer_sequence<int, N>{});
 }
 
-// softplus(v) = max(v, 0) + log(1 + t), t = exp(-|v|).  log(w) t / (w - 1) with
+// softplus(v) and its derivative 1 / (1 + exp(-v)).  softplus(v) = max(v, 0) + log(1 + t), t = exp(-|v|).  log(w) t / (w - 1) with
 // w = 1 + t rounded is log(1 + t) to the last bits also where t is small (w - 1
 // is exact); t where w is 1.
-ASCA_DEV float softplus_f(float v) {
+ASCA_DEV float softplus_f(float v, float* slope) {
     const float t = __builtin_amdgcn_exp2f(-fabsf(v) * LOG2E);
     const float w = 1.0f + t, m = w - 1.0f;
     const float l = __builtin_amdgcn_logf(w) * 0.693147180559945f * t * __builtin_amdgcn_rcpf(m);
+    *slope = (v >= 0.0f ? 1.0f : t) * __builtin_amdgcn_rcpf(w);
     return fmaxf(v, 0.0f) + (m == 0.0f ? t : l);
 }
 
@@ -129,6 +130,20 @@ struct SsmPlace {
         own_d = g * p.Dg + min(tile * 8 * NW + own_c, p.Dg - 1);
         len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
         row0 = (long)b * p.T;
+    }
+    // the tiles of K rows that the block walks: those of its chunk that hold a row of
+    // the sequence
+    template <int K>
+    ASCA_DEV void tiles_of(const SsmArgs& p, int* k0, int* k1) const {
+        *k0 = ch * p.ctile;
+        *k1 = max(*k0, min(*k0 + p.ctile, (len + K - 1) / K));
+    }
+    // zeros in the owned channel of the chunk's rows from tile k on
+    template <int K, typename E>
+    ASCA_DEV void zero_rows(const SsmArgs& p, E* m, long ld, int k) const {
+        if (!own_live) return;
+        const int end = min((ch + 1) * p.ctile * K, p.T);
+        for (int t = k * K + own_row; t < end; t += 8) act_store(m + (long)(t - own_row) * ld, 0.0f);
     }
     // channel c of wave w
     ASCA_DEV int chan(const SsmArgs& p, int w, int c, bool* live) const {
@@ -209,8 +224,10 @@ struct BcTile {
 ASCA_DEV void settle(float& x) { asm volatile("" : "+v"(x)); }
 
 // Step e of a row from its raw dt (0 past the sequence's end: the state stays)
-ASCA_DEV float ssm_e(const SsmArgs& p, float v, bool in) {
-    const float s = p.softplus ? softplus_f(v) : v;
+ASCA_DEV float ssm_e(const SsmArgs& p, float v, bool in, float* slope) {
+    float s = v;
+    *slope = 1.0f;
+    if (p.softplus) s = softplus_f(v, slope);
     return in ? s : 0.0f;
 }
 
@@ -255,7 +272,9 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 3, c = lane & 7;
     bool live;
     const int d = l.chan(p, w, c, &live);
-    const int ntile = (p.T + K - 1) / K, k0 = l.ch * p.ctile, k1 = min(k0 + p.ctile, ntile);
+    const int ntile = (p.T + K - 1) / K;
+    int k0, k1;
+    l.template tiles_of<K>(p, &k0, &k1);
     float A2[NS], h[NS], esum = 0.0f, eown = 0.0f;
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
@@ -283,7 +302,8 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const bool in = k * K + l.own_row + 8 * r < l.len;
-            const float e = ssm_e(p, act_value(rdt[r]) + bias, in);
+            float slope;
+            const float e = ssm_e(p, act_value(rdt[r]) + bias, in, &slope);
             x[r] = in ? act_value(rx[r]) : 0.0f;
             ex[buf][l.own_row + 8 * r][l.own_c] = make_float2(e, e * x[r]);
             eown += e;
@@ -351,9 +371,12 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
         }
         stage(next, buf ^ 1);
     }
-    if (OUT && k0 < k1) {
-        lds_barrier();
-        emit(k1 - 1);
+    if (OUT) {
+        if (k0 < k1) {
+            lds_barrier();
+            emit(k1 - 1);
+        }
+        l.template zero_rows<K>(p, py, p.ldy, k1);
     }
     if (!OUT) {
         if (live)
@@ -380,7 +403,8 @@ __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 3, c = lane & 7;
     bool live;
     const int d = l.chan(p, w, c, &live);
-    const int ntile = (p.T + K - 1) / K, k0 = l.ch * p.ctile, k1 = min(k0 + p.ctile, ntile);
+    int k0, k1;
+    l.template tiles_of<K>(p, &k0, &k1);
     float A2[NS], cy[NS], esum = 0.0f, eown = 0.0f;
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
@@ -403,14 +427,17 @@ __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const bool in = k * K + l.own_row + 8 * r < l.len;
-            const float e = ssm_e(p, act_value(rdt[r]) + bias, in);
+            float slope;
+            const float e = ssm_e(p, act_value(rdt[r]) + bias, in, &slope);
             ey[buf][l.own_row + 8 * r][l.own_c] = make_float2(e, in ? act_value(rdy[r]) : 0.0f);
             eown += e;
         }
         bct.store(p, l, k * K, bc[buf]);
     };
-    fetch(k1 - 1);
-    stage(k1 - 1, (k1 - 1) & 1);
+    if (k0 < k1) {
+        fetch(k1 - 1);
+        stage(k1 - 1, (k1 - 1) & 1);
+    }
     for (int k = k1 - 1; k >= k0; --k) {
         const int buf = k & 1, next = max(k - 1, k0);
         lds_barrier();
@@ -448,7 +475,9 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane & 7, c = lane >> 3;
     bool live;
     const int d = l.chan(p, w, c, &live);
-    const int ntile = (p.T + K - 1) / K, k0 = l.ch * p.ctile, k1 = min(k0 + p.ctile, ntile);
+    const int ntile = (p.T + K - 1) / K;
+    int k0, k1;
+    l.template tiles_of<K>(p, &k0, &k1);
     float A2[NS], cy[NS], dA[NS], hn[NS];
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
@@ -464,7 +493,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
 #pragma unroll
     for (int j = 0; j < NS; ++j) settle(cy[j]), settle(A2[j]);
     E rx[R], rdt[R], rdy[R];
-    float x[R], dt[R], dy[R], e[R], dD = 0.0f, db = 0.0f, xk[R], dtk[R], dyk[R], ek[R];
+    float x[R], sl[R], dy[R], e[R], dD = 0.0f, db = 0.0f, xk[R], slk[R], dyk[R], ek[R];
     const E *px = own_ptr<E>(l, p.x, p.ldx), *pdt = own_ptr<E>(l, p.dt, p.lddt), *pdy = own_ptr<E>(l, p.dy, p.lddy);
     E *pdx = own_ptr<E>(l, p.dx, p.lddx), *pddt = own_ptr<E>(l, p.ddt, p.ldddt);
     BcTile<E, NS, NW, K> bct(p, l);
@@ -482,8 +511,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const bool in = k * K + l.own_row + 8 * r < l.len;
-            dt[r] = act_value(rdt[r]) + bias;
-            e[r] = ssm_e(p, dt[r], in);
+            e[r] = ssm_e(p, act_value(rdt[r]) + bias, in, &sl[r]);
             x[r] = in ? act_value(rx[r]) : 0.0f;
             dy[r] = in ? act_value(rdy[r]) : 0.0f;
             // a channel that does not exist adds nothing to dB and dC
@@ -492,6 +520,18 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
         }
         bct.store(p, l, k * K, bc[buf]);
     };
+    // sums over channels that this thread adds over the waves: value (o / 64 PG) 8 PG +
+    // PG (lane >> 3) + o / 64 % PG of the tile's (row, B or C, state)
+    constexpr int RV = (RED + 64 * NW - 1) / (64 * NW);
+    float* pred[RV];
+    int red_t[RV];
+#pragma unroll
+    for (int i = 0; i < RV; ++i) {
+        const int o = (threadIdx.x + i * 64 * NW) % RED, v = o / (64 * PG) * 8 * PG + PG * ((o & 63) >> 3) + o / 64 % PG;
+        const int t = v / (2 * NS), n = (o & 7) * NS + v % NS;
+        red_t[i] = n < p.N && threadIdx.x + i * 64 * NW < RED ? t : p.T;   // others store nothing
+        pred[i] = p.pBC + ((((l.tile * (long)p.B + l.b) * p.T + t) * p.G + l.g) * 2 + v / NS % 2) * p.N + n;
+    }
     auto emit = [&](int k) {
         const int buf = k & 1, t0 = k * K;
 #pragma unroll
@@ -499,7 +539,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
             const int row = l.own_row + 8 * r, t = t0 + row;
             const bool in = t < l.len;
             const float sB = sums[buf][0][row][l.own_c], sA = sums[buf][1][row][l.own_c] * (1.0f / LOG2E);
-            const float de = fmaf(xk[r], sB, sA), ddt = in ? (p.softplus ? de * act_sigmoid(dtk[r]) : de) : 0.0f;
+            const float de = fmaf(xk[r], sB, sA), ddt = in ? de * slk[r] : 0.0f;
             if (l.own_live && t < p.T) {
                 act_store(pdx + (t0 + 8 * r) * p.lddx, in ? fmaf(ek[r], sB, Dk * dyk[r]) : 0.0f);
                 act_store(pddt + (t0 + 8 * r) * p.ldddt, ddt);
@@ -507,16 +547,13 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
             dD = fmaf(dyk[r], xk[r], dD);
             db += ddt;
         }
-        for (int o = threadIdx.x; o < RED; o += 64 * NW) {
+#pragma unroll
+        for (int i = 0; i < RV; ++i) {
+            const int o = (threadIdx.x + i * 64 * NW) % RED;
             float sum = 0.0f;
 #pragma unroll
             for (int u = 0; u < NW; ++u) sum += red[buf][u][o];
-            // value (o / 64 PG) 8 PG + PG (lane >> 3) + o / 64 % PG of the tile's (row, B or C, state)
-            const int v = o / (64 * PG) * 8 * PG + PG * ((o & 63) >> 3) + o / 64 % PG, t = t0 + v / (2 * NS);
-            const int n = (o & 7) * NS + v % NS;
-            if (t < p.T && n < p.N)
-                p.pBC[(((((long)l.tile * p.B + l.b) * p.T + t) * p.G + l.g) * 2 + v / NS % 2) * p.N + n] =
-                    t < l.len ? sum : 0.0f;
+            if (red_t[i] + t0 < l.len) pred[i][(long)t0 * (2 * p.G * p.N)] = sum;
         }
     };
     if (k0 < k1) {
@@ -531,7 +568,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
         lds_barrier();                       // tile k is staged, tile k + 1's sums are there
         if (k + 1 < k1) emit(k + 1);
 #pragma unroll
-        for (int r = 0; r < R; ++r) xk[r] = x[r], dtk[r] = dt[r], dyk[r] = dy[r], ek[r] = e[r];
+        for (int r = 0; r < R; ++r) xk[r] = x[r], slk[r] = sl[r], dyk[r] = dy[r], ek[r] = e[r];
         fetch(next);
         // the tile's states and decays again, operands read PR rows ahead
         {
@@ -619,6 +656,8 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
         lds_barrier();
         emit(k0);
     }
+    l.template zero_rows<K>(p, pdx, p.lddx, k1);
+    l.template zero_rows<K>(p, pddt, p.ldddt, k1);
     float* part = p.pP + ((long)l.b * p.nch + l.ch) * (p.N + 2) * p.D;
     if (live)
 #pragma unroll
@@ -643,14 +682,15 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
 
 // dB, dC from the tiles' partial sums
 template <typename E>
-__global__ __launch_bounds__(256) void ssm_fin_bc_k(const float* __restrict__ pBC, int tiles, long rows, int G, int N,
-                                                   E* __restrict__ dB, long lddb, E* __restrict__ dC, long lddc) {
+__global__ __launch_bounds__(256) void ssm_fin_bc_k(const float* __restrict__ pBC, int tiles, long rows, int T, int G, int N,
+                                                   const int32_t* __restrict__ lens, E* __restrict__ dB, long lddb, E* __restrict__ dC, long lddc) {
     const long i = (long)blockIdx.x * 256 + threadIdx.x, per = rows * G * 2 * N;
     if (i >= per) return;
-    float s = 0.0f;
-    for (int k = 0; k < tiles; ++k) s += pBC[k * per + i];
     const int n = (int)(i % N), which = (int)(i / N % 2), g = (int)(i / (2 * N) % G);
     const long r = i / ((long)2 * N * G);
+    float s = 0.0f;
+    if (!lens || (int)(r % T) < lens[r / T])   // rows past a sequence's end have no sums
+        for (int k = 0; k < tiles; ++k) s += pBC[k * per + i];
     if (which == 0)
         act_store(dB + r * lddb + (long)g * N + n, s);
     else
@@ -667,7 +707,8 @@ __global__ __launch_bounds__(256) void ssm_step_k(float* __restrict__ h, SsmArgs
     const int g = d / p.Dg;
     const float x = act_load(static_cast<const E*>(p.x) + s * p.ldx + d);
     const float v = act_load(static_cast<const E*>(p.dt) + s * p.lddt + d) + (p.dt_bias ? p.dt_bias[d] : 0.0f);
-    const float e = p.softplus ? softplus_f(v) : v, ex = e * x;
+    float slope;
+    const float e = ssm_e(p, v, true, &slope), ex = e * x;
     const E* Br = static_cast<const E*>(p.Bm) + s * p.ldb + (long)g * p.N;
     const E* Cr = static_cast<const E*>(p.Cm) + s * p.ldc + (long)g * p.N;
     float* hr = h + s * p.N * p.D + d;
@@ -837,7 +878,7 @@ int asca_ssm_bwd(const void* x, long ldx, const void* dt, long lddt, const float
         if (per) {
             if ((r = pre_launch("ssm_fin_bc"))) return r;
             hipLaunchKernelGGL(ssm_fin_bc_k<E>, dim3((unsigned)((per + 255) / 256)), dim3(256), 0, st, p.pBC, p.tiles, rows,
-                               G, N, static_cast<E*>(dB), lddb, static_cast<E*>(dC), lddc);
+                               T, G, N, lens, static_cast<E*>(dB), lddb, static_cast<E*>(dC), lddc);
             if ((r = post_launch("ssm_fin_bc"))) return r;
         }
         return sum_parts_launch(p.pP, parts, PartsOut{{dA, dDk, ddt_bias}, {nd, D, D}}, st);
