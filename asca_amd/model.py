@@ -15,7 +15,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from .gpu import DevBuf, _vp, describe, gpu
+from .gpu import DevBuf, GradList, _vp, describe, gpu
 
 _f32 = np.float32
 
@@ -43,6 +43,7 @@ class DeviceModel:
         self.n_floats = nf.value
         self._ptr = {k: p.value for k, p in zip(("params", "grads", "m", "v"), ptrs)}
         self._bufs: dict = {}
+        self._grad_list: GradList | None = None
 
     def num_params(self) -> int:
         return sum(r * c for _, _, r, c in self.tensors)
@@ -130,6 +131,14 @@ class DeviceModel:
         _lib.call("asca_model_forward_backward", self._h, _vp(ids), _vp(targets), batch, seq, _vp(lb), stream)
         return self._read_loss() if sync else None
 
+    def clip_grads(self, max_norm: float, sync: bool = True, stream=None):
+        """Scale every gradient by min(1, max_norm / (norm + 1e-6)), norm the 2-norm
+        over all of them (asca_grads_clip), between forward_backward and adamw:
+        (norm, factor), or None without sync."""
+        if self._grad_list is None:
+            self._grad_list = GradList([(self._ptr["grads"] + 4 * off, r * c) for _, off, r, c in self.tensors])
+        return self._grad_list.clip(max_norm, sync, stream)
+
     def adamw(self, stream=None) -> None:
         _lib.call("asca_model_adamw", self._h, stream)
 
@@ -183,6 +192,9 @@ class DeviceModel:
             for b in self._bufs.values():
                 b.free()
             self._bufs.clear()
+            if self._grad_list is not None:
+                self._grad_list.close()
+                self._grad_list = None
             _lib.call("asca_model_destroy", self._h)
             self._h = None
 
