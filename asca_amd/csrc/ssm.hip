@@ -32,7 +32,6 @@
 // a first pass leaves what a chunk makes of a zero state (carry) and its sum of e,
 // from which every chunk works out what enters it, exp(A sum e) being its decay.
 #include <algorithm>
-#include <utility>
 
 #include "act.h"
 #include "parts.h"
@@ -43,6 +42,11 @@ constexpr float LOG2E = 1.44269504088896341f;
 
 // Rows a tile (and between two kept states): the backward keeps 2 K NS floats a lane.
 constexpr int ssm_k(int NS) { return NS <= 2 ? 16 : 8; }
+
+// The states of a channel lie on Q lane groups (8 or 16), NS to a lane; a wave has
+// 64 / Q channels and a block of NW waves SSM_CB of them.
+template <int Q, int NW>
+constexpr int SSM_CB = 64 / Q * NW;
 
 struct SsmArgs {
     const void *x, *dt, *Bm, *Cm, *dy;
@@ -68,34 +72,47 @@ ASCA_DEV void halve_dpp(const float* a, float* out, bool hi) {
     for (int k = 0; k < H; ++k) out[k] = (hi ? a[k + H] : a[k]) + dpp<CTRL>(hi ? a[k] : a[k + H]);
 }
 
-// Sums over the 8 lanes that differ in bits 3..5 of v[0..8 M): lane l has those of
-// v[M (l >> 3) .. + M)
-template <int M>
-ASCA_DEV void scatter_high(const float* v, int lane, float* out) {
-    float a[4 * M], b[2 * M];
-#pragma unroll
-    for (int k = 0; k < 4 * M; ++k) a[k] = tsum32(v[k], v[k + 4 * M]);
-#pragma unroll
-    for (int k = 0; k < 2 * M; ++k) b[k] = tsum16(a[k], a[k + 2 * M]);
-    halve_dpp<DPP_ROW_ROR8, M>(b, out, lane & 8);
+// The value of the lane whose bit 2 is the other
+ASCA_DEV float xor4(float x) {
+    const int u = __float_as_int(x), lo = __builtin_amdgcn_update_dpp(u, u, 0x104, 0xF, 0x5, false);   // row_shl:4
+    return __int_as_float(__builtin_amdgcn_update_dpp(lo, u, 0x114, 0xF, 0xA, false));                 // row_shr:4
 }
 
-// The same over bits 0..2: lane l has those of v[M (l & 7) .. + M)
-template <int M>
+// Sums over the B lanes that differ in the lane's highest bits (4, 8 or 16: bits 4..5,
+// 3..5, 2..5) of v[0 .. B M): lane l has those of v[M (l / (64 / B)) .. + M)
+template <int B, int M>
+ASCA_DEV void scatter_high(const float* v, int lane, float* out) {
+    float a[B / 2 * M], b[B / 4 * M];
+#pragma unroll
+    for (int k = 0; k < B / 2 * M; ++k) a[k] = tsum32(v[k], v[k + B / 2 * M]);
+#pragma unroll
+    for (int k = 0; k < B / 4 * M; ++k) b[k] = tsum16(a[k], a[k + B / 4 * M]);
+    if constexpr (B == 4) {
+#pragma unroll
+        for (int k = 0; k < M; ++k) out[k] = b[k];
+    } else if constexpr (B == 8) {
+        halve_dpp<DPP_ROW_ROR8, M>(b, out, lane & 8);
+    } else {
+        float d[2 * M];
+        halve_dpp<DPP_ROW_ROR8, 2 * M>(b, d, lane & 8);
+#pragma unroll
+        for (int k = 0; k < M; ++k) out[k] = (lane & 4 ? d[k + M] : d[k]) + xor4(lane & 4 ? d[k] : d[k + M]);
+    }
+}
+
+// The same over the lowest bits (8 or 16 lanes): lane l has those of v[M (l % B) .. + M)
+template <int B, int M>
 ASCA_DEV void scatter_low(const float* v, int lane, float* out) {
-    float a[4 * M], b[2 * M];
-    halve_dpp<DPP_HALF_MIRROR, 4 * M>(v, a, lane & 4);
+    float h[8 * M], a[4 * M], b[2 * M];
+    if constexpr (B == 16) {
+        halve_dpp<DPP_ROW_ROR8, 8 * M>(v, h, lane & 8);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8 * M; ++k) h[k] = v[k];
+    }
+    halve_dpp<DPP_HALF_MIRROR, 4 * M>(h, a, lane & 4);
     halve_dpp<DPP_QUAD_XOR2, 2 * M>(a, b, lane & 2);
     halve_dpp<DPP_QUAD_XOR1, M>(b, out, lane & 1);
-}
-
-template <typename F, int... I>
-ASCA_DEV void unroll_(F f, std::integer_sequence<int, I...>) {
-    (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-ASCA_DEV void unroll(F f) {
-    unroll_(f, std::make_integer_sequence<int, N>{});
 }
 
 // softplus(v) and its derivative 1 / (1 + exp(-v)).  softplus(v) = max(v, 0) + log(1 + t), t = exp(-|v|).  log(w) t / (w - 1) with
@@ -110,8 +127,8 @@ ASCA_DEV float softplus_f(float v, float* slope) {
 }
 
 // A block's place, and a thread's as the owner of (row, channel) pairs: channel
-// tid % 8 NW of the block, rows tid / 8 NW + 8 r of a tile
-template <int NW>
+// tid % CB of the block's CB, rows tid / CB + Q r of a tile
+template <int Q, int CB>
 struct SsmPlace {
     int b, ch, g, tile, len, own_c, own_row, own_d;
     bool own_live;
@@ -124,10 +141,10 @@ struct SsmPlace {
         u /= p.G;
         ch = u % p.nch;
         b = u / p.nch;
-        own_c = threadIdx.x % (8 * NW);
-        own_row = threadIdx.x / (8 * NW);
-        own_live = tile * 8 * NW + own_c < p.Dg;
-        own_d = g * p.Dg + min(tile * 8 * NW + own_c, p.Dg - 1);
+        own_c = threadIdx.x % CB;
+        own_row = threadIdx.x / CB;
+        own_live = tile * CB + own_c < p.Dg;
+        own_d = g * p.Dg + min(tile * CB + own_c, p.Dg - 1);
         len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
         row0 = (long)b * p.T;
     }
@@ -143,11 +160,11 @@ struct SsmPlace {
     ASCA_DEV void zero_rows(const SsmArgs& p, E* m, long ld, int k) const {
         if (!own_live) return;
         const int end = min((ch + 1) * p.ctile * K, p.T);
-        for (int t = k * K + own_row; t < end; t += 8) act_store(m + (long)(t - own_row) * ld, 0.0f);
+        for (int t = k * K + own_row; t < end; t += Q) act_store(m + (long)(t - own_row) * ld, 0.0f);
     }
     // channel c of wave w
     ASCA_DEV int chan(const SsmArgs& p, int w, int c, bool* live) const {
-        const int d = tile * 8 * NW + w * 8 + c;
+        const int d = tile * CB + w * (64 / Q) + c;
         *live = d < p.Dg;
         return g * p.Dg + min(d, p.Dg - 1);
     }
@@ -156,65 +173,65 @@ struct SsmPlace {
 // A thread's place in an activation matrix: its channel of row own_row of the
 // sequence.  Rows are reached from it by uniform offsets, so a tile's addresses are
 // scalar products.
-template <typename E, int NW>
-ASCA_DEV E* own_ptr(const SsmPlace<NW>& l, const void* m, long ld) {
+template <typename E, int Q, int CB>
+ASCA_DEV E* own_ptr(const SsmPlace<Q, CB>& l, const void* m, long ld) {
     return static_cast<E*>(const_cast<void*>(m)) + (l.row0 + l.own_row) * ld + l.own_d;
 }
 
 // A thread's values of the tile at t0, as they are in memory; rows past the
 // sequence's end read its last row again (the reader replaces them).  No load sits
 // under a condition and none is converted here: either would wait for it.
-template <typename E, int NW, int R>
-ASCA_DEV void own_load(const SsmPlace<NW>& l, const E* m, long ld, int t0, E (&out)[R]) {
+template <typename E, int Q, int CB, int R>
+ASCA_DEV void own_load(const SsmPlace<Q, CB>& l, const E* m, long ld, int t0, E (&out)[R]) {
     long a[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) a[r] = (t0 + 8 * r) * ld;
-    if (t0 + 8 * R > l.len)
+    for (int r = 0; r < R; ++r) a[r] = (t0 + Q * r) * ld;
+    if (t0 + Q * R > l.len)
 #pragma unroll
-        for (int r = 0; r < R; ++r) a[r] = (long)(min(t0 + l.own_row + 8 * r, max(l.len - 1, 0)) - l.own_row) * ld;
+        for (int r = 0; r < R; ++r) a[r] = (long)(min(t0 + l.own_row + Q * r, max(l.len - 1, 0)) - l.own_row) * ld;
 #pragma unroll
     for (int r = 0; r < R; ++r) out[r] = m[a[r]];
 }
 
 // B and C of a tile: value o = thread + 64 NW r is (B or C, row, state), so that a
 // wave's are all of one matrix.
-template <typename E, int NS, int NW, int K>
+template <typename E, int NS, int Q, int NW, int K>
 struct BcTile {
-    static constexpr int V = K * 8 * NS, R = (2 * V + 64 * NW - 1) / (64 * NW);
+    static constexpr int CB = SSM_CB<Q, NW>, V = K * Q * NS, R = (2 * V + 64 * NW - 1) / (64 * NW);
     const E* m[R];
     long ld[R];
     E v[R];
-    ASCA_DEV BcTile(const SsmArgs& p, const SsmPlace<NW>& l) {
+    ASCA_DEV BcTile(const SsmArgs& p, const SsmPlace<Q, CB>& l) {
         const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const bool C = (w + r * NW) * 64 % (2 * V) >= V;   // a wave past the last value reads again
             const int o = (threadIdx.x + r * 64 * NW) % V;
             ld[r] = C ? p.ldc : p.ldb;
-            m[r] = static_cast<const E*>(C ? p.Cm : p.Bm) + (l.row0 + o / (8 * NS)) * ld[r] + (long)l.g * p.N +
-                   min(o % (8 * NS), p.N - 1);
+            m[r] = static_cast<const E*>(C ? p.Cm : p.Bm) + (l.row0 + o / (Q * NS)) * ld[r] + (long)l.g * p.N +
+                   min(o % (Q * NS), p.N - 1);
         }
     }
-    ASCA_DEV void load(const SsmPlace<NW>& l, int t0) {
+    ASCA_DEV void load(const SsmPlace<Q, CB>& l, int t0) {
         long a[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) a[r] = t0 * ld[r];
         if (t0 + K > l.len)
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const int u = (threadIdx.x + r * 64 * NW) % V / (8 * NS);
+                const int u = (threadIdx.x + r * 64 * NW) % V / (Q * NS);
                 a[r] = (long)(min(t0 + u, max(l.len - 1, 0)) - u) * ld[r];
             }
 #pragma unroll
         for (int r = 0; r < R; ++r) v[r] = m[r][a[r]];
     }
     // into [row][group][B's NS, C's NS], zeros for rows and states that do not exist
-    ASCA_DEV void store(const SsmArgs& p, const SsmPlace<NW>& l, int t0, float* lds) const {
+    ASCA_DEV void store(const SsmArgs& p, const SsmPlace<Q, CB>& l, int t0, float* lds) const {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int o = threadIdx.x + r * 64 * NW, u = o % V / (8 * NS), n = o % (8 * NS);
+            const int o = threadIdx.x + r * 64 * NW, u = o % V / (Q * NS), n = o % (Q * NS);
             const float x = t0 + u < l.len && n < p.N ? act_value(v[r]) : 0.0f;
-            if (2 * V % (64 * NW) == 0 || o < 2 * V) lds[((u * 8 + n / NS) * 2 + o / V) * NS + n % NS] = x;
+            if (2 * V % (64 * NW) == 0 || o < 2 * V) lds[((u * Q + n / NS) * 2 + o / V) * NS + n % NS] = x;
         }
     }
 };
@@ -247,29 +264,29 @@ ASCA_DEV void fold_chunks(const SsmArgs& p, int b, int ch, int q, int d, const f
 }
 
 // The sum of the block's e, one a channel, into ce
-template <int NW>
-ASCA_DEV void store_esum(const SsmArgs& p, const SsmPlace<NW>& l, float esum, float (*lds)[8 * NW]) {
+template <int Q, int CB>
+ASCA_DEV void store_esum(const SsmArgs& p, const SsmPlace<Q, CB>& l, float esum, float (*lds)[CB]) {
     __syncthreads();
     lds[l.own_row][l.own_c] = esum;
     __syncthreads();
     if (l.own_row || !l.own_live) return;
 #pragma unroll
-    for (int r = 1; r < 8; ++r) esum += lds[r][l.own_c];
+    for (int r = 1; r < Q; ++r) esum += lds[r][l.own_c];
     p.ce[((long)l.b * p.nch + l.ch) * p.D + l.own_d] = esum;
 }
 
 // OUT: the rows' y from the state that enters the chunk; otherwise what a chunk
-// makes of a zero state, and the sum of its e.  Lane = 8 q + c.
-template <typename E, int NS, int NW, bool OUT>
+// makes of a zero state, and the sum of its e.  Lane = CH q + c.
+template <typename E, int NS, int Q, int NW, bool OUT>
 __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
-    constexpr int K = ssm_k(NS), R = K / 8;
-    constexpr int YP = 8 * NW + 4;      // 2 YP = 8 mod 64: the groups' stores of y spread over the banks
-    __shared__ float2 ex[2][K][8 * NW];
-    __shared__ float bc[2][K * 8 * 2 * NS];
+    constexpr int K = ssm_k(NS), R = K / Q, CB = SSM_CB<Q, NW>, CH = 64 / Q;
+    constexpr int YP = CB + 4;          // R YP is CH mod 2 CH: the groups' stores of y spread over the banks
+    __shared__ float2 ex[2][K][CB];
+    __shared__ float bc[2][K * Q * 2 * NS];
     __shared__ float ys[2][K][YP];
-    const SsmPlace<NW> l(p);
+    const SsmPlace<Q, CB> l(p);
     if (!OUT && l.ch == p.nch - 1) return;   // no chunk follows
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 3, c = lane & 7;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane / CH, c = lane % CH;
     bool live;
     const int d = l.chan(p, w, c, &live);
     const int ntile = (p.T + K - 1) / K;
@@ -290,7 +307,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
     for (int j = 0; j < NS; ++j) settle(h[j]), settle(A2[j]);
     const E *px = own_ptr<E>(l, p.x, p.ldx), *pdt = own_ptr<E>(l, p.dt, p.lddt);
     E* py = own_ptr<E>(l, p.y, p.ldy);
-    BcTile<E, NS, NW, K> bct(p, l);
+    BcTile<E, NS, Q, NW, K> bct(p, l);
     E rx[R], rdt[R];
     float x[R], xk[R];
     auto fetch = [&](int k) {
@@ -301,11 +318,11 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
     auto stage = [&](int k, int buf) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const bool in = k * K + l.own_row + 8 * r < l.len;
+            const bool in = k * K + l.own_row + Q * r < l.len;
             float slope;
             const float e = ssm_e(p, act_value(rdt[r]) + bias, in, &slope);
             x[r] = in ? act_value(rx[r]) : 0.0f;
-            ex[buf][l.own_row + 8 * r][l.own_c] = make_float2(e, e * x[r]);
+            ex[buf][l.own_row + Q * r][l.own_c] = make_float2(e, e * x[r]);
             eown += e;
         }
         bct.store(p, l, k * K, bc[buf]);
@@ -314,10 +331,10 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
         float v[R];
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            v[r] = k * K + l.own_row + 8 * r < l.len ? fmaf(Dk, xk[r], ys[k & 1][l.own_row + 8 * r][l.own_c]) : 0.0f;
+            v[r] = k * K + l.own_row + Q * r < l.len ? fmaf(Dk, xk[r], ys[k & 1][l.own_row + Q * r][l.own_c]) : 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (l.own_live && k * K + l.own_row + 8 * r < p.T) act_store(py + (k * K + 8 * r) * p.ldy, v[r]);
+            if (l.own_live && k * K + l.own_row + Q * r < p.T) act_store(py + (k * K + Q * r) * p.ldy, v[r]);
     };
     if (k0 < k1) {
         fetch(k0);
@@ -343,9 +360,9 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
         auto read = [&](int g) {
 #pragma unroll
             for (int u = 0; u < PR; ++u) {
-                ev[g & 1][u] = ex[buf][g * PR + u][w * 8 + c];
+                ev[g & 1][u] = ex[buf][g * PR + u][w * CH + c];
 #pragma unroll
-                for (int j = 0; j < MS; ++j) m[g & 1][u][j] = bc[buf][((g * PR + u) * 8 + q) * 2 * NS + j];
+                for (int j = 0; j < MS; ++j) m[g & 1][u][j] = bc[buf][((g * PR + u) * Q + q) * 2 * NS + j];
             }
         };
         read(0);
@@ -365,9 +382,9 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
         }
         if (OUT) {
             float s[R];
-            scatter_high<R>(y, lane, s);
+            scatter_high<Q, R>(y, lane, s);
 #pragma unroll
-            for (int r = 0; r < R; ++r) ys[buf][R * q + r][w * 8 + c] = s[r];
+            for (int r = 0; r < R; ++r) ys[buf][R * q + r][w * CH + c] = s[r];
         }
         stage(next, buf ^ 1);
     }
@@ -383,7 +400,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
 #pragma unroll
             for (int j = 0; j < NS; ++j)
                 if (q * NS + j < p.N) p.cs[(((long)l.b * p.nch + l.ch) * p.N + q * NS + j) * p.D + d] = h[j];
-        store_esum<NW>(p, l, esum, reinterpret_cast<float(*)[8 * NW]>(&ys[0][0][0]));
+        store_esum(p, l, esum, reinterpret_cast<float(*)[CB]>(&ys[0][0][0]));
     } else if (p.h_out && live && l.ch == p.nch - 1) {
 #pragma unroll
         for (int j = 0; j < NS; ++j)
@@ -392,15 +409,15 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
 }
 
 // What a chunk makes of a zero carry, from its end to its start, and the sum of its e.
-// Lane = 8 q + c.
-template <typename E, int NS, int NW>
+// Lane = CH q + c.
+template <typename E, int NS, int Q, int NW>
 __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
-    constexpr int K = ssm_k(NS), R = K / 8;
-    __shared__ float2 ey[2][K][8 * NW];
-    __shared__ float bc[2][K * 8 * 2 * NS];
-    const SsmPlace<NW> l(p);
+    constexpr int K = ssm_k(NS), R = K / Q, CB = SSM_CB<Q, NW>, CH = 64 / Q;
+    __shared__ float2 ey[2][K][CB];
+    __shared__ float bc[2][K * Q * 2 * NS];
+    const SsmPlace<Q, CB> l(p);
     if (l.ch == 0) return;   // no chunk precedes
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 3, c = lane & 7;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane / CH, c = lane % CH;
     bool live;
     const int d = l.chan(p, w, c, &live);
     int k0, k1;
@@ -416,7 +433,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
 #pragma unroll
     for (int j = 0; j < NS; ++j) settle(A2[j]);
     const E *pdy = own_ptr<E>(l, p.dy, p.lddy), *pdt = own_ptr<E>(l, p.dt, p.lddt);
-    BcTile<E, NS, NW, K> bct(p, l);
+    BcTile<E, NS, Q, NW, K> bct(p, l);
     E rdy[R], rdt[R];
     auto fetch = [&](int k) {
         own_load(l, pdy, p.lddy, k * K, rdy);
@@ -426,10 +443,10 @@ __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
     auto stage = [&](int k, int buf) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const bool in = k * K + l.own_row + 8 * r < l.len;
+            const bool in = k * K + l.own_row + Q * r < l.len;
             float slope;
             const float e = ssm_e(p, act_value(rdt[r]) + bias, in, &slope);
-            ey[buf][l.own_row + 8 * r][l.own_c] = make_float2(e, in ? act_value(rdy[r]) : 0.0f);
+            ey[buf][l.own_row + Q * r][l.own_c] = make_float2(e, in ? act_value(rdy[r]) : 0.0f);
             eown += e;
         }
         bct.store(p, l, k * K, bc[buf]);
@@ -445,8 +462,8 @@ __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
         fetch(next);
 #pragma unroll
         for (int t = K - 1; t >= 0; --t) {
-            const float2 e = ey[buf][t][w * 8 + c];
-            const float* m = bc[buf] + (t * 8 + q) * 2 * NS + NS;
+            const float2 e = ey[buf][t][w * CH + c];
+            const float* m = bc[buf] + (t * Q + q) * 2 * NS + NS;
 #pragma unroll
             for (int j = 0; j < NS; ++j) cy[j] = __builtin_amdgcn_exp2f(e.x * A2[j]) * fmaf(m[j], e.y, cy[j]);
         }
@@ -456,23 +473,23 @@ __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
 #pragma unroll
         for (int j = 0; j < NS; ++j)
             if (q * NS + j < p.N) p.cs[(((long)l.b * p.nch + l.ch) * p.N + q * NS + j) * p.D + d] = cy[j];
-    store_esum<NW>(p, l, esum, reinterpret_cast<float(*)[8 * NW]>(&ey[0][0][0]));
+    store_esum(p, l, esum, reinterpret_cast<float(*)[CB]>(&ey[0][0][0]));
 }
 
-// Lane = 8 c + q: sums over channels (2 NS a row) by row swaps, over states (2 a row) by DPP.
-template <typename E, int NS, int NW>
+// Lane = Q c + q: sums over channels (2 NS a row) by row swaps, over states (2 a row) by DPP.
+template <typename E, int NS, int Q, int NW>
 __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
-    constexpr int K = ssm_k(NS), R = K / 8;
-    constexpr int PR = 2, YP = 8 * NW + 4, RED = K * 8 * 2 * NS;   // RED sums over channels a tile and wave
-    // ... in groups of 8 PG: TG rows' 2 NS, or one row's
-    constexpr int TG = NS < 4 ? 4 / NS : 1, PG = NS < 4 ? 1 : NS / 4;
-    __shared__ float2 ex[2][K][8 * NW];
-    __shared__ float dys[2][K][8 * NW];
-    __shared__ float bc[2][K * 8 * 2 * NS];
+    constexpr int K = ssm_k(NS), R = K / Q, CB = SSM_CB<Q, NW>, CH = 64 / Q;
+    constexpr int PR = 2, YP = CB + 4, RED = K * Q * 2 * NS;   // RED sums over channels a tile and wave
+    // ... in groups of CH PG: TG rows' 2 NS, or one row's
+    constexpr int TG = 2 * NS < CH ? CH / (2 * NS) : 1, PG = 2 * NS < CH ? 1 : 2 * NS / CH;
+    __shared__ float2 ex[2][K][CB];
+    __shared__ float dys[2][K][CB];
+    __shared__ float bc[2][K * Q * 2 * NS];
     __shared__ float sums[2][2][K][YP];
     __shared__ float red[2][NW][RED];
-    const SsmPlace<NW> l(p);
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane & 7, c = lane >> 3;
+    const SsmPlace<Q, CB> l(p);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane % Q, c = lane / Q;
     bool live;
     const int d = l.chan(p, w, c, &live);
     const int ntile = (p.T + K - 1) / K;
@@ -496,7 +513,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
     float x[R], sl[R], dy[R], e[R], dD = 0.0f, db = 0.0f, xk[R], slk[R], dyk[R], ek[R];
     const E *px = own_ptr<E>(l, p.x, p.ldx), *pdt = own_ptr<E>(l, p.dt, p.lddt), *pdy = own_ptr<E>(l, p.dy, p.lddy);
     E *pdx = own_ptr<E>(l, p.dx, p.lddx), *pddt = own_ptr<E>(l, p.ddt, p.ldddt);
-    BcTile<E, NS, NW, K> bct(p, l);
+    BcTile<E, NS, Q, NW, K> bct(p, l);
     const float* pck = p.ck + (long)l.b * ntile * p.N * p.D + d;
     auto fetch = [&](int k) {
         own_load(l, px, p.ldx, k * K, rx);
@@ -510,25 +527,25 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
     auto stage = [&](int k, int buf) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const bool in = k * K + l.own_row + 8 * r < l.len;
+            const bool in = k * K + l.own_row + Q * r < l.len;
             e[r] = ssm_e(p, act_value(rdt[r]) + bias, in, &sl[r]);
             x[r] = in ? act_value(rx[r]) : 0.0f;
             dy[r] = in ? act_value(rdy[r]) : 0.0f;
             // a channel that does not exist adds nothing to dB and dC
-            ex[buf][l.own_row + 8 * r][l.own_c] = make_float2(e[r], l.own_live ? e[r] * x[r] : 0.0f);
-            dys[buf][l.own_row + 8 * r][l.own_c] = l.own_live ? dy[r] : 0.0f;
+            ex[buf][l.own_row + Q * r][l.own_c] = make_float2(e[r], l.own_live ? e[r] * x[r] : 0.0f);
+            dys[buf][l.own_row + Q * r][l.own_c] = l.own_live ? dy[r] : 0.0f;
         }
         bct.store(p, l, k * K, bc[buf]);
     };
-    // sums over channels that this thread adds over the waves: value (o / 64 PG) 8 PG +
-    // PG (lane >> 3) + o / 64 % PG of the tile's (row, B or C, state)
+    // sums over channels that this thread adds over the waves: value (o / 64 PG) CH PG +
+    // PG c + o / 64 % PG of the tile's (row, B or C, state), c = o % 64 / Q
     constexpr int RV = (RED + 64 * NW - 1) / (64 * NW);
     float* pred[RV];
     int red_t[RV];
 #pragma unroll
     for (int i = 0; i < RV; ++i) {
-        const int o = (threadIdx.x + i * 64 * NW) % RED, v = o / (64 * PG) * 8 * PG + PG * ((o & 63) >> 3) + o / 64 % PG;
-        const int t = v / (2 * NS), n = (o & 7) * NS + v % NS;
+        const int o = (threadIdx.x + i * 64 * NW) % RED, v = o / (64 * PG) * CH * PG + PG * (o % 64 / Q) + o / 64 % PG;
+        const int t = v / (2 * NS), n = o % Q * NS + v % NS;
         red_t[i] = n < p.N && threadIdx.x + i * 64 * NW < RED ? t : p.T;   // others store nothing
         pred[i] = p.pBC + ((((l.tile * (long)p.B + l.b) * p.T + t) * p.G + l.g) * 2 + v / NS % 2) * p.N + n;
     }
@@ -536,13 +553,13 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
         const int buf = k & 1, t0 = k * K;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int row = l.own_row + 8 * r, t = t0 + row;
+            const int row = l.own_row + Q * r, t = t0 + row;
             const bool in = t < l.len;
             const float sB = sums[buf][0][row][l.own_c], sA = sums[buf][1][row][l.own_c] * (1.0f / LOG2E);
             const float de = fmaf(xk[r], sB, sA), ddt = in ? de * slk[r] : 0.0f;
             if (l.own_live && t < p.T) {
-                act_store(pdx + (t0 + 8 * r) * p.lddx, in ? fmaf(ek[r], sB, Dk * dyk[r]) : 0.0f);
-                act_store(pddt + (t0 + 8 * r) * p.ldddt, ddt);
+                act_store(pdx + (t0 + Q * r) * p.lddx, in ? fmaf(ek[r], sB, Dk * dyk[r]) : 0.0f);
+                act_store(pddt + (t0 + Q * r) * p.ldddt, ddt);
             }
             dD = fmaf(dyk[r], xk[r], dD);
             db += ddt;
@@ -577,9 +594,9 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
             auto read = [&](int g) {
 #pragma unroll
                 for (int u = 0; u < PR; ++u) {
-                    v[g & 1][u] = ex[buf][g * PR + u][w * 8 + c];
+                    v[g & 1][u] = ex[buf][g * PR + u][w * CH + c];
 #pragma unroll
-                    for (int j = 0; j < NS; ++j) m[g & 1][u][j] = bc[buf][((g * PR + u) * 8 + q) * 2 * NS + j];
+                    for (int j = 0; j < NS; ++j) m[g & 1][u][j] = bc[buf][((g * PR + u) * Q + q) * 2 * NS + j];
                 }
             };
             read(0);
@@ -606,16 +623,16 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
 #pragma unroll
             for (int u = 0; u < TG; ++u) {
                 const int t = tg * TG + u;
-                v2[tg & 1][u] = ex[buf][t][w * 8 + c];
-                dy2[tg & 1][u] = dys[buf][t][w * 8 + c];
+                v2[tg & 1][u] = ex[buf][t][w * CH + c];
+                dy2[tg & 1][u] = dys[buf][t][w * CH + c];
 #pragma unroll
-                for (int j = 0; j < 2 * NS; ++j) m2[tg & 1][u][j] = bc[buf][(t * 8 + q) * 2 * NS + j];
+                for (int j = 0; j < 2 * NS; ++j) m2[tg & 1][u][j] = bc[buf][(t * Q + q) * 2 * NS + j];
             }
         };
         read(K / TG - 1);
 #pragma unroll
         for (int tg = K / TG - 1; tg >= 0; --tg) {
-            float part[8 * PG];
+            float part[CH * PG];
             if (tg) read(tg - 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -637,19 +654,19 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
                 }
             }
             float s[PG];
-            scatter_high<PG>(part, lane, s);
+            scatter_high<CH, PG>(part, lane, s);
 #pragma unroll
             for (int u = 0; u < PG; ++u) red[buf][w][(tg * PG + u) * 64 + lane] = s[u];
         }
 #pragma unroll
         for (int j = 0; j < NS; ++j) dA[j] += dAk[j];
         float s[R];
-        scatter_low<R>(gB, lane, s);
+        scatter_low<Q, R>(gB, lane, s);
 #pragma unroll
-        for (int r = 0; r < R; ++r) sums[buf][0][R * q + r][w * 8 + c] = s[r];
-        scatter_low<R>(pA, lane, s);
+        for (int r = 0; r < R; ++r) sums[buf][0][R * q + r][w * CH + c] = s[r];
+        scatter_low<Q, R>(pA, lane, s);
 #pragma unroll
-        for (int r = 0; r < R; ++r) sums[buf][1][R * q + r][w * 8 + c] = s[r];
+        for (int r = 0; r < R; ++r) sums[buf][1][R * q + r][w * CH + c] = s[r];
         stage(next, buf ^ 1);
     }
     if (k0 < k1) {
@@ -674,7 +691,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
     __syncthreads();
     if (l.own_row == 0 && l.own_live) {
 #pragma unroll
-        for (int r = 1; r < 8; ++r) dD += sums[0][0][r][l.own_c], db += sums[1][0][r][l.own_c];
+        for (int r = 1; r < Q; ++r) dD += sums[0][0][r][l.own_c], db += sums[1][0][r][l.own_c];
         part[(long)p.N * p.D + l.own_d] = dD;
         part[(long)(p.N + 1) * p.D + l.own_d] = db;
     }
@@ -726,7 +743,7 @@ __global__ __launch_bounds__(256) void ssm_step_k(float* __restrict__ h, SsmArgs
 
 using namespace asca;
 
-static int ssm_ns(int N) { return N <= 8 ? 1 : N <= 16 ? 2 : N <= 32 ? 4 : 8; }
+static int ssm_ns(int N) { return N <= 8 ? 1 : N <= 16 ? 2 : N <= 32 ? 4 : 8; }   // states a lane on 8 groups
 
 static int ssm_check(const char* fn, int B, int T, int D, int N, int G) {
     if (B < 0 || T < 0 || D < 0) return fail(ASCA_ERR_INVALID, "%s: negative shape B=%d T=%d D=%d", fn, B, T, D);
@@ -739,36 +756,50 @@ static int ssm_ld(const char* fn, const char* what, long ld, long cols) {
     return ld >= cols ? ASCA_OK : fail(ASCA_ERR_INVALID, "%s: row stride %s=%ld below its %ld columns", fn, what, ld, cols);
 }
 
-// The waves a block has (8, or 4 where that alone gives a block to every CU), and the
-// rows' cut into p.nch chunks a sequence: where sequences and channels give fewer
-// than `enough` waves, as many chunks as give `want`.  A cut costs a second pass over
-// the rows, so it pays only for waves that are missing (forward, N = 16: 2 x 2048 x
-// 1024 in 512 waves 157 us, cut to 4096 47 us; 32 x 512 x 512 in 2048 waves 54 us,
-// cut to 4096 78 us; backward: 2 x 2048 x 1024 cut to 1024 142 us, to 2048 100 us).
-static int ssm_split(SsmArgs& p, int N, long enough, long want) {
+// How a call runs: Q lane groups, NW waves a block, and the rows' cut into p.nch chunks
+// a sequence.
+//   - 16 groups (N of 9 to 16) give twice the waves for a seventh more instructions:
+//     where 8 groups give fewer than two waves a SIMD but 16 most of them (16 x 1024 x
+//     512: 247 -> 212 us), or where few waves cannot be cut enough (1 x 512 x 512
+//     forward 15.4 -> 13.2 us); not where there are two (8 x 4096 x 2048 1288 -> 1544)
+//     or a cut serves better (forward 4 x 1000 x 1000 44 -> 53 us).
+//   - a cut costs a second pass over the rows, so it pays only for waves that are
+//     missing: below `enough`, as many chunks as give `want` (forward: 2 x 2048 x 1024
+//     in 512 waves 157 us, cut to 4096 47; 32 x 512 x 512 in 2048 waves 54 us, cut to
+//     4096 78; backward: 2 x 2048 x 1024 cut to 1024 142 us, to 2048 100).
+struct SsmForm {
+    int Q, NW;
+};
+static SsmForm ssm_form(SsmArgs& p, int N, int NW16, int NW8, long enough, long want) {
     const int K = ssm_k(ssm_ns(N)), ntile = (p.T + K - 1) / K;
-    const int NW = ssm_ns(N) <= 4 && (long)p.B * p.G * ((p.Dg + 63) / 64) >= 256 ? 8 : 4;
-    p.tiles = (p.Dg + 8 * NW - 1) / (8 * NW);
-    const long waves = (long)p.B * p.G * p.tiles * NW;
-    const long nch = waves == 0 || waves >= enough ? 1 : std::max(1L, std::min({want / waves, 64L, (long)ntile / 4}));
+    const long w8 = (long)p.B * p.G * ((p.Dg + 7) / 8), cuts = std::max(1, std::min(64, ntile / 4));
+    SsmForm f{8, ssm_ns(N) == 8 ? 4 : NW8};
+    if (ssm_ns(N) == 2 && ((w8 >= 768 && w8 < 2048) || w8 * cuts < 1024)) f = {16, NW16};
+    const int CB = 64 / f.Q * f.NW;
+    p.tiles = (p.Dg + CB - 1) / CB;
+    const long waves = (long)p.B * p.G * p.tiles * f.NW;
+    const long nch = waves == 0 || waves >= enough ? 1 : std::max(1L, std::min(want / waves, cuts));
     p.ctile = std::max(1, (int)((ntile + nch - 1) / nch));
     p.nch = std::max(1, (ntile + p.ctile - 1) / p.ctile);
-    return NW;
+    return f;
 }
 static size_t ssm_chunk_floats(const SsmArgs& p) { return p.nch > 1 ? (size_t)p.B * p.nch * (p.N + 1) * p.D : 0; }
 
-// Calls f with the element type, the states a lane and the waves a block
+// Calls f with the element type, the states a lane, the lane groups and the waves a block
 template <typename F>
-static int ssm_dispatch(int dtype, int N, int NW, F f) {
+static int ssm_dispatch(int dtype, int N, SsmForm form, F f) {
     return act_dispatch(dtype, [&](auto* e) {
-        auto go = [&](auto ns) {
-            return NW == 8 ? f(e, ns, std::integral_constant<int, 8>{}) : f(e, ns, std::integral_constant<int, 4>{});
-        };
+        using std::integral_constant;
+        const integral_constant<int, 8> c8;
+        const integral_constant<int, 4> c4;
+        const integral_constant<int, 16> c16;
+        auto go = [&](auto ns, auto q) { return form.NW == 8 ? f(e, ns, q, c8) : f(e, ns, q, c4); };
+        if (form.Q == 16) return go(integral_constant<int, 1>{}, c16);
         switch (ssm_ns(N)) {
-            case 1: return go(std::integral_constant<int, 1>{});
-            case 2: return go(std::integral_constant<int, 2>{});
-            case 4: return go(std::integral_constant<int, 4>{});
-            default: return f(e, std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
+            case 1: return go(integral_constant<int, 1>{}, c8);
+            case 2: return go(integral_constant<int, 2>{}, c8);
+            case 4: return go(c4, c8);
+            default: return f(e, c8, c8, c4);
         }
     });
 }
@@ -805,23 +836,23 @@ int asca_ssm_fwd(const void* x, long ldx, const void* dt, long lddt, const float
     p.ck = static_cast<float*>(ws);
     p.T = T, p.D = D, p.N = N, p.G = G, p.Dg = D / G, p.softplus = softplus;
     p.B = B;
-    const int NW = ssm_split(p, N, 1024, 4096);
+    const SsmForm form = ssm_form(p, N, 4, 4, 1024, 4096);
     const long blocks = (long)B * p.nch * G * p.tiles;
     if (blocks > 0x7fffffffL) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many channels", fn);
     StreamScratch sc;
     if ((rc = sc.get(ssm_chunk_floats(p), st))) return rc;
     p.cs = sc.ws.p, p.ce = p.cs + (size_t)B * p.nch * N * D;
-    return ssm_dispatch(dtype, N, NW, [&](auto* e, auto ns, auto nw) {
+    return ssm_dispatch(dtype, N, form, [&](auto* e, auto ns, auto q, auto nw) {
         using E = std::remove_pointer_t<decltype(e)>;
-        constexpr int NS = decltype(ns)::value, W = decltype(nw)::value;
+        constexpr int NS = decltype(ns)::value, Q = decltype(q)::value, W = decltype(nw)::value;
         int r;
         if (p.nch > 1) {
             if ((r = pre_launch("ssm_chunk"))) return r;
-            hipLaunchKernelGGL((ssm_fwd_k<E, NS, W, false>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
+            hipLaunchKernelGGL((ssm_fwd_k<E, NS, Q, W, false>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
             if ((r = post_launch("ssm_chunk"))) return r;
         }
         if ((r = pre_launch("ssm_fwd"))) return r;
-        hipLaunchKernelGGL((ssm_fwd_k<E, NS, W, true>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
+        hipLaunchKernelGGL((ssm_fwd_k<E, NS, Q, W, true>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
         return post_launch("ssm_fwd");
     });
 }
@@ -853,7 +884,8 @@ int asca_ssm_bwd(const void* x, long ldx, const void* dt, long lddt, const float
     p.ck = static_cast<float*>(const_cast<void*>(ws));
     p.T = T, p.D = D, p.N = N, p.G = G, p.Dg = D / G, p.softplus = softplus;
     p.B = B;
-    const int NW = ssm_split(p, N, 2048, 2048);
+    // 8 waves a block halve the partial sums of dB and dC
+    const SsmForm form = ssm_form(p, N, 8, (long)B * G * ((p.Dg + 63) / 64) >= 256 ? 8 : 4, 2048, 2048);
     const long blocks = (long)B * p.nch * G * p.tiles, rows = (long)B * T, parts = (long)B * p.nch, per = rows * G * 2 * N, nd = (long)N * D;
     if (blocks > 0x7fffffffL || (per + 255) / 256 > 0x7fffffffL)
         return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows or channels", fn);
@@ -861,18 +893,18 @@ int asca_ssm_bwd(const void* x, long ldx, const void* dt, long lddt, const float
     if ((rc = sc.get((size_t)parts * (nd + 2 * D) + (size_t)p.tiles * per + ssm_chunk_floats(p), st))) return rc;
     p.pP = sc.ws.p, p.pBC = p.pP + parts * (nd + 2 * D), p.cs = p.pBC + p.tiles * per;
     p.ce = p.cs + (size_t)parts * N * D;
-    return ssm_dispatch(dtype, N, NW, [&](auto* e, auto ns, auto nw) {
+    return ssm_dispatch(dtype, N, form, [&](auto* e, auto ns, auto q, auto nw) {
         using E = std::remove_pointer_t<decltype(e)>;
-        constexpr int NS = decltype(ns)::value, W = decltype(nw)::value;
+        constexpr int NS = decltype(ns)::value, Q = decltype(q)::value, W = decltype(nw)::value;
         int r;
         if (p.nch > 1) {
             if ((r = pre_launch("ssm_carry"))) return r;
-            hipLaunchKernelGGL((ssm_carry_k<E, NS, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
+            hipLaunchKernelGGL((ssm_carry_k<E, NS, Q, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
             if ((r = post_launch("ssm_carry"))) return r;
         }
         if (blocks) {
             if ((r = pre_launch("ssm_bwd"))) return r;
-            hipLaunchKernelGGL((ssm_bwd_k<E, NS, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
+            hipLaunchKernelGGL((ssm_bwd_k<E, NS, Q, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, p);
             if ((r = post_launch("ssm_bwd"))) return r;
         }
         if (per) {

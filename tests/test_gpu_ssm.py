@@ -117,7 +117,10 @@ def test_conv_step_goes_on_from_a_prompt(g, n, D, W, bf16):
 SSM = [(1, 1, 1, 1, 1, False), (2, 5, 3, 4, 1, True), (1, 16, 16, 16, 1, False), (7, 33, 70, 16, 1, True),
        (2, 100, 130, 12, 2, True), (1, 257, 64, 8, 4, False), (2, 40, 65, 32, 1, True), (1, 37, 20, 64, 2, False),
        (2, 300, 48, 5, 3, False), (1, 700, 33, 16, 1, False), (2, 64, 256, 16, 1, True), (3, 21, 50, 2, 1, True),
-       (1, 19, 17, 33, 1, False), (2, 1100, 64, 16, 1, True), (1, 2050, 20, 4, 1, False)]
+       (1, 19, 17, 33, 1, False), (2, 1100, 64, 16, 1, True), (1, 2050, 20, 4, 1, False),
+       # many channels (each width of the lane groups, 8 waves a block), long rows cut into chunks
+       (8, 20, 2048, 16, 1, True), (8, 20, 2048, 7, 1, True), (8, 12, 2048, 20, 1, True), (4, 40, 2048, 10, 2, False),
+       (1, 1100, 512, 16, 1, True), (1, 1100, 500, 12, 2, False), (1, 1100, 260, 33, 1, False), (2, 700, 300, 24, 3, True)]
 
 
 def ssm_inputs(r, rng, B, T, D, N, G):
