@@ -719,12 +719,13 @@ __global__ __launch_bounds__(256) void ssm_fin_bc_k(const float* __restrict__ pB
 // for memory once so (1 x 512, N = 16: 4.8 us one state after another, 4.7 at SU =
 // 8, 3.8 at 16; 64 x 2048 8.6, 8.1, 6.2 us); many are bound by it, and keep more
 // waves with 8 (512 x 2048 37, 30.6, 32.7 us; the states are 134 MB).
+ASCA_DEV float lane_value(float x, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); }
+
 template <typename E, int SU>
 __global__ __launch_bounds__(256) void ssm_step_k(float* __restrict__ h, SsmArgs p) {
     const unsigned cb = (p.D + 255) / 256;
-    const int d = blockIdx.x % cb * 256 + threadIdx.x;
+    const int ch = blockIdx.x % cb * 256 + threadIdx.x, d = min(ch, p.D - 1), lane = threadIdx.x & 63;
     const long s = blockIdx.x / cb;
-    if (d >= p.D) return;
     const int g = d / p.Dg;
     const E rx = static_cast<const E*>(p.x)[s * p.ldx + d], rdt = static_cast<const E*>(p.dt)[s * p.lddt + d];
     const float bias = p.dt_bias ? p.dt_bias[d] : 0.0f, Dk = p.Dk ? p.Dk[d] : 0.0f;
@@ -732,17 +733,24 @@ __global__ __launch_bounds__(256) void ssm_step_k(float* __restrict__ h, SsmArgs
     const E* Cr = static_cast<const E*>(p.Cm) + s * p.ldc + (long)g * p.N;
     float* hr = h + s * p.N * p.D + d;
     float e = 0.0f, xe = 0.0f, y = 0.0f, slope;
+    // a wave within one group has B and C across its lanes, one load each
+    const bool one = __all(g == __builtin_amdgcn_readfirstlane(g));
+    const E rB = Br[min(lane, p.N - 1)], rC = Cr[min(lane, p.N - 1)];
     for (int n0 = 0; n0 < p.N; n0 += SU) {
         float a[SU], hn[SU];
-        E b[SU], c[SU];
+        E b[SU] = {}, c[SU] = {};
 #pragma unroll
         for (int u = 0; u < SU; ++u) {
             const int n = min(n0 + u, p.N - 1);
             hn[u] = hr[(long)n * p.D];
             a[u] = p.A[(long)n * p.D + d];
-            b[u] = Br[n];
-            c[u] = Cr[n];
         }
+        if (!one)
+#pragma unroll
+            for (int u = 0; u < SU; ++u) {
+                b[u] = Br[min(n0 + u, p.N - 1)];
+                c[u] = Cr[min(n0 + u, p.N - 1)];
+            }
         if (n0 == 0) {
             const float x = act_value(rx);
             e = ssm_e(p, act_value(rdt) + bias, true, &slope);
@@ -752,12 +760,14 @@ __global__ __launch_bounds__(256) void ssm_step_k(float* __restrict__ h, SsmArgs
 #pragma unroll
         for (int u = 0; u < SU; ++u) {
             if (n0 + u >= p.N) break;
-            const float v = fmaf(__builtin_amdgcn_exp2f(e * (a[u] * LOG2E)), hn[u], act_value(b[u]) * xe);
-            y = fmaf(act_value(c[u]), v, y);
-            hr[(long)(n0 + u) * p.D] = v;
+            const float fb = one ? lane_value(act_value(rB), n0 + u) : act_value(b[u]);
+            const float fc = one ? lane_value(act_value(rC), n0 + u) : act_value(c[u]);
+            const float v = fmaf(__builtin_amdgcn_exp2f(e * (a[u] * LOG2E)), hn[u], fb * xe);
+            y = fmaf(fc, v, y);
+            if (ch < p.D) hr[(long)(n0 + u) * p.D] = v;
         }
     }
-    act_store(static_cast<E*>(p.y) + s * p.ldy + d, y);
+    if (ch < p.D) act_store(static_cast<E*>(p.y) + s * p.ldy + d, y);
 }
 
 }  // namespace asca
