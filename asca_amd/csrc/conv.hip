@@ -11,8 +11,10 @@
 
 namespace asca {
 
-constexpr int CV_R = 16;    // rows a run
-constexpr int CV_NW = 4;    // runs a block (the backward adds their sums)
+// Rows a run, and runs a block (the backward adds their sums).  Longer runs read and
+// form less twice but hold more registers: 8 x 4096 x 2048 bf16, forward and backward,
+// 175 us with 8 rows, 192 with 16, 252 with 32 forward and 24 backward.
+constexpr int CV_R = 8, CV_NW = 8;
 
 struct ConvArgs {
     const void *x, *dy;
