@@ -519,3 +519,131 @@ def test_an_injected_failure_is_an_error_and_the_next_call_works(g, nth):
     got = g.ssm_scan_bwd(dev, dy)
     for k in want:
         np.testing.assert_array_equal(got[k], want[k])
+
+
+def _ssm_call(g, i, B, T, D, N, dy, G=1, lens=None):
+    """Device buffers of a scan and its backward, and the two calls on a stream."""
+    from asca_amd import _lib, gpu
+
+    b = {k: gpu.DevBuf.from_array(a) for k, a in dict(i, dy=dy).items()}
+    o = {k: gpu.DevBuf(n * 4) for k, n in (("y", B * T * D), ("h", B * N * D), ("dx", B * T * D), ("ddt", B * T * D), ("db", D), ("dA", N * D),
+                                           ("dB", B * T * G * N), ("dC", B * T * G * N), ("dD", D), ("dh0", B * N * D))}
+    n = C.c_size_t()
+    _lib.call("asca_ssm_ws_bytes", B, T, D, N, C.byref(n))
+    ws = gpu.DevBuf(n.value)
+    head = (_p(b["x"]), D, _p(b["dt"]), D, _p(b["dt_bias"]), _p(b["A"]), _p(b["Bm"]), G * N, _p(b["Cm"]), G * N, _p(b["Dk"]))
+
+    def run(st):
+        _lib.call("asca_ssm_fwd", *head, None, None, _p(o["y"]), D, _p(o["h"]), _p(ws), B, T, D, N, G, 1, 0, st)
+        _lib.call("asca_ssm_bwd", *head, None, _p(b["dy"]), D, None, _p(ws), _p(o["dx"]), D, _p(o["ddt"]), D, _p(o["db"]), _p(o["dA"]),
+                  _p(o["dB"]), G * N, _p(o["dC"]), G * N, _p(o["dD"]), _p(o["dh0"]), B, T, D, N, G, 1, 0, st)
+
+    return run, o, (b, ws)
+
+
+def test_captured_calls_replay_the_eager_results(g):
+    """A scan cut into chunks, a convolution, norms and clipping with their backwards,
+    captured into a graph: each replay gives the eager bits, with the program's own
+    calls between the replays."""
+    from asca_amd import _lib, gpu
+
+    hip = C.CDLL("libamdhip64.so.7")
+
+    def ok(rc):
+        assert rc == 0, rc
+
+    rng = np.random.default_rng(12)
+    r = Rows(rng, False)
+    B, T, D, N = 1, 300, 64, 16
+    i, dy = ssm_inputs(r, rng, B, T, D, N, 1), r(B * T, D)
+    run, o, keep = _ssm_call(g, i, B, T, D, N, dy)
+    w = gpu.DevBuf.from_host(rng.standard_normal((4, D)).astype(np.float32))
+    bias = gpu.DevBuf.from_host(rng.standard_normal(D).astype(np.float32))
+    x, bdy = keep[0]["x"], keep[0]["dy"]
+    o.update({k: gpu.DevBuf(n * 4) for k, n in (("c", T * D), ("dc", T * D), ("dw", 4 * D), ("dcb", D), ("r", T * D), ("n", T * D),
+                                                ("nx", T * D), ("ny", T * D), ("dwp", D), ("clip", D), ("stat", 2))})
+    gl = C.c_void_p()
+    one = lambda b: (C.c_void_p * 1)(b.ptr)  # noqa: E731
+    _lib.call("asca_grads_create", one(o["dwp"]), one(o["clip"]), (C.c_uint64 * 1)(D), 1, 0, C.byref(gl))
+
+    def everything(st):
+        run(st)
+        _lib.call("asca_conv_fwd", _p(x), D, _p(w), _p(bias), None, None, _p(o["c"]), D, None, B, T, D, 4, 1, 0, st)
+        _lib.call("asca_conv_bwd", _p(x), D, _p(w), _p(bias), None, None, _p(bdy), D, None, _p(o["dc"]), D, _p(o["dw"]), _p(o["dcb"]),
+                  None, B, T, D, 4, 1, 0, st)
+        _lib.call("asca_block_norm_fwd", _p(x), D, _p(bdy), D, None, 0, _p(bias), None, None, _p(o["r"]), D, _p(o["n"]), D, T, D, 1e-6, 0, st)
+        _lib.call("asca_block_norm_bwd", _p(x), D, _p(bdy), D, None, 0, _p(bias), None, None, _p(x), D, _p(bdy), D, _p(o["nx"]), D,
+                  _p(o["ny"]), D, None, 0, _p(o["dwp"]), None, None, T, D, 1e-6, 0, st)
+        _lib.call("asca_grads_clip", gl, 0.5, _p(o["stat"]), st)
+
+    get = lambda: {k: b.to_host((b.nbytes // 4,)) for k, b in o.items()}  # noqa: E731
+    everything(None)
+    _lib.call("asca_sync")
+    want = get()
+    sp, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    _lib.call("asca_stream_create", C.byref(sp))
+    ok(hip.hipStreamBeginCapture(sp, 0))
+    everything(sp)
+    ok(hip.hipStreamEndCapture(sp, C.byref(graph)))
+    ok(hip.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)))
+    for k in range(4):
+        for b in o.values():
+            _lib.call("asca_memset32", _p(b), 0, b.nbytes // 4, None)
+        _lib.call("asca_sync")
+        ok(hip.hipGraphLaunch(exe, sp))
+        _lib.call("asca_stream_sync", sp)
+        got = get()
+        for name in want:
+            np.testing.assert_array_equal(got[name], want[name], err_msg=f"replay {k}: {name}")
+        g.conv(i["x"], rng.standard_normal((4, D)).astype(np.float32), batch=1)   # the program's own work between
+    ok(hip.hipGraphExecDestroy(exe))
+    ok(hip.hipGraphDestroy(graph))
+    _lib.call("asca_stream_destroy", sp)
+    _lib.call("asca_grads_destroy", gl)
+
+
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("B,T,D,N", [(1, 70, 40, 16), (1, 70, 40, 6), (8, 40, 2048, 16), (1, 1100, 512, 12)])
+def test_an_infinity_or_nan_stays_with_what_it_reaches(g, bad, B, T, D, N):
+    """One bad x: its channel from its row on, and the sums over channels of those rows;
+    one bad dy: its channel up to its row, and those rows' sums.  Everything else keeps
+    its bits."""
+    rng = np.random.default_rng(13)
+    r = Rows(rng, False)
+    i, dy = ssm_inputs(r, rng, B, T, D, N, 1), r(B * T, D)
+    row, ch = 21, 3
+
+    def run(i, dy):
+        y, h, dev = g.ssm_scan(**i, batch=B)
+        o = g.ssm_scan_bwd(dev, dy)
+        dev.free()
+        return dict(o, y=y, h=h)
+
+    want = run(i, dy)
+    rows = np.arange(B * T)
+    later, first = (rows >= row) & (rows < T), rows < T
+    x2, dy2 = i["x"].copy(), dy.copy()
+    x2[row, ch], dy2[row, ch] = bad, bad
+    got = run({**i, "x": x2}, dy)
+    assert not np.isfinite(got["y"][row, ch])
+    clean = np.ones((B * T, D), bool)
+    clean[later, ch] = False
+    np.testing.assert_array_equal(got["y"][clean], want["y"][clean])
+    np.testing.assert_array_equal(got["dC"][~later], want["dC"][~later])
+    np.testing.assert_array_equal(got["dB"][rows != row], want["dB"][rows != row])
+    assert not np.isfinite(got["dB"][row]).any()
+    other = np.arange(D) != ch
+    for k in ("dA", "dDk", "ddt_bias"):
+        np.testing.assert_array_equal(got[k][..., other], want[k][..., other])
+    for k in ("dx", "ddt"):
+        np.testing.assert_array_equal(got[k][:, other], want[k][:, other])
+    got = run(i, dy2)
+    np.testing.assert_array_equal(got["y"], want["y"])
+    up = first & (rows <= row)
+    clean = np.ones((B * T, D), bool)
+    clean[up, ch] = False
+    assert not np.isfinite(got["dx"][row, ch])
+    for k in ("dx", "ddt"):
+        np.testing.assert_array_equal(got[k][clean], want[k][clean])
+    np.testing.assert_array_equal(got["dC"][rows != row], want["dC"][rows != row])
+    np.testing.assert_array_equal(got["dB"][~up], want["dB"][~up])
