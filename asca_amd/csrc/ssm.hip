@@ -707,7 +707,13 @@ __global__ __launch_bounds__(256) void ssm_fin_bc_k(const float* __restrict__ pB
     const long r = i / ((long)2 * N * G);
     float s = 0.0f;
     if (!lens || (int)(r % T) < lens[r / T])   // rows past a sequence's end have no sums
-        for (int k = 0; k < tiles; ++k) s += pBC[k * per + i];
+        for (int k = 0; k < tiles; k += 8) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = pBC[min(k + u, tiles - 1) * per + i];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += k + u < tiles ? v[u] : 0.0f;
+        }
     if (which == 0)
         act_store(dB + r * lddb + (long)g * N + n, s);
     else
