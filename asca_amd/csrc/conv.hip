@@ -228,6 +228,7 @@ using namespace asca;
 
 static int conv_check(const char* fn, int B, int T, int D, int W) {
     if (B < 0 || T < 0 || D < 0) return fail(ASCA_ERR_INVALID, "%s: negative shape B=%d T=%d D=%d", fn, B, T, D);
+    if (T > 1 << 30) return fail(ASCA_ERR_UNSUPPORTED, "%s: T=%d above 2^30", fn, T);
     if (W < 2 || W > 8) return fail(ASCA_ERR_UNSUPPORTED, "%s: W=%d outside 2..8", fn, W);
     return ASCA_OK;
 }

@@ -478,6 +478,8 @@ def test_refusals(g):
            (("asca_conv_fwd", f, 8, f, None, f, None, f, 8, f, 1, 4, 8, 4, 1, 0, None), 1),
            (ssm(N=0), 3), (ssm(N=65), 3), (ssm(G=3), 1), (ssm(G=0), 1), (ssm(ty=-1), 3), (ssm(ld=7), 1), (ssm(x=None), 1), (ssm(A=None), 1),
            (ssm(h0=f, ho=f), 1), (("asca_ssm_ws_bytes", 1, -1, 8, 4, C.byref(out)), 1), (("asca_ssm_ws_bytes", 1, 1, 8, 4, None), 1),
+           (("asca_ssm_ws_bytes", 1, (1 << 30) + 1, 8, 4, C.byref(out)), 3),
+           (("asca_conv_fwd", f, 8, f, None, None, None, f, 8, None, 1, (1 << 30) + 1, 8, 4, 1, 0, None), 3),
            (norm(ld=7), 1), (norm(y=None), 1), (norm(r=None), 1), (norm(ty=7), 3),
            (norm(x=None, y=None, z=None), 1),
            (("asca_grads_create", one, None, (C.c_uint64 * 1)(4), 1, 0, C.byref(h)), 1),
