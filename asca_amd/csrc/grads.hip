@@ -4,7 +4,9 @@
 // made once); a block has a chunk.  The squares are summed in 64 bits; the chunks'
 // sums are added in their order by every block that scales, which costs less than a
 // launch between (and than a last block's: a fence in each block before it took the
-// norm of 143M gradients from 122 to 310 us).  Bound by memory.
+// norm of 143M gradients from 122 to 310 us).  Bound by memory: 143M f32 gradients
+// are read in 126 us (4.5 TB/s) and read and written in 207 us (5.5 TB/s, the part
+// that the last-level cache still holds coming first).
 #include <algorithm>
 #include <vector>
 
