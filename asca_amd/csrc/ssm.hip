@@ -818,14 +818,17 @@ static int ssm_ld(const char* fn, const char* what, long ld, long cols) {
 //     missing: below `enough`, as many chunks as give `want` (forward: 2 x 2048 x 1024
 //     in 512 waves 157 us, cut to 4096 47; 32 x 512 x 512 in 2048 waves 54 us, cut to
 //     4096 78; backward: 2 x 2048 x 1024 cut to 1024 142 us, to 2048 100).
+//   - the backward has 8 waves a block, which halves its partial sums of dB and dC (8 x
+//     4096 x 2048 904 -> 888 us), where that leaves a block for every CU (2 x 2048 x
+//     1024 without: 89.8 -> 90.8 us).
 struct SsmForm {
     int Q, NW;
 };
-static SsmForm ssm_form(SsmArgs& p, int N, int NW16, int NW8, long enough, long want) {
+static SsmForm ssm_form(SsmArgs& p, int N, bool bwd, long enough, long want) {
     const int K = ssm_k(ssm_ns(N)), ntile = (p.T + K - 1) / K;
     const long w8 = (long)p.B * p.G * ((p.Dg + 7) / 8), cuts = std::max(1, std::min(64, ntile / 4));
-    SsmForm f{8, ssm_ns(N) == 8 ? 4 : NW8};
-    if (ssm_ns(N) == 2 && ((w8 >= 768 && w8 < 2048) || w8 * cuts < 1024)) f = {16, NW16};
+    SsmForm f{8, bwd && ssm_ns(N) < 8 && (long)p.B * p.G * ((p.Dg + 63) / 64) >= 256 ? 8 : 4};
+    if (ssm_ns(N) == 2 && ((w8 >= 768 && w8 < 2048) || w8 * cuts < 1024)) f = {16, bwd ? 8 : 4};
     const int CB = 64 / f.Q * f.NW;
     p.tiles = (p.Dg + CB - 1) / CB;
     const long waves = (long)p.B * p.G * p.tiles * f.NW;
@@ -837,19 +840,22 @@ static SsmForm ssm_form(SsmArgs& p, int N, int NW16, int NW8, long enough, long 
 static size_t ssm_chunk_floats(const SsmArgs& p) { return p.nch > 1 ? (size_t)p.B * p.nch * (p.N + 1) * p.D : 0; }
 
 // Calls f with the element type, the states a lane, the lane groups and the waves a block
-template <typename F>
+template <bool BWD, typename F>
 static int ssm_dispatch(int dtype, int N, SsmForm form, F f) {
     return act_dispatch(dtype, [&](auto* e) {
         using std::integral_constant;
         const integral_constant<int, 8> c8;
         const integral_constant<int, 4> c4;
-        const integral_constant<int, 16> c16;
-        auto go = [&](auto ns, auto q) { return form.NW == 8 ? f(e, ns, q, c8) : f(e, ns, q, c4); };
-        if (form.Q == 16) return go(integral_constant<int, 1>{}, c16);
+        if (form.Q == 16) return f(e, integral_constant<int, 1>{}, integral_constant<int, 16>{}, integral_constant<int, BWD ? 8 : 4>{});
+        auto go = [&](auto ns) {
+            if constexpr (BWD)
+                if (form.NW == 8) return f(e, ns, c8, c8);
+            return f(e, ns, c8, c4);
+        };
         switch (ssm_ns(N)) {
-            case 1: return go(integral_constant<int, 1>{}, c8);
-            case 2: return go(integral_constant<int, 2>{}, c8);
-            case 4: return go(c4, c8);
+            case 1: return go(integral_constant<int, 1>{});
+            case 2: return go(integral_constant<int, 2>{});
+            case 4: return go(c4);
             default: return f(e, c8, c8, c4);
         }
     });
@@ -887,13 +893,13 @@ int asca_ssm_fwd(const void* x, long ldx, const void* dt, long lddt, const float
     p.ck = static_cast<float*>(ws);
     p.T = T, p.D = D, p.N = N, p.G = G, p.Dg = D / G, p.softplus = softplus;
     p.B = B;
-    const SsmForm form = ssm_form(p, N, 4, 4, 1024, 4096);
+    const SsmForm form = ssm_form(p, N, false, 1024, 4096);
     const long blocks = (long)B * p.nch * G * p.tiles;
     if (blocks > 0x7fffffffL) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many channels", fn);
     StreamScratch sc;
     if ((rc = sc.get(ssm_chunk_floats(p), st))) return rc;
     p.cs = sc.ws.p, p.ce = p.cs + (size_t)B * p.nch * N * D;
-    return ssm_dispatch(dtype, N, form, [&](auto* e, auto ns, auto q, auto nw) {
+    return ssm_dispatch<false>(dtype, N, form, [&](auto* e, auto ns, auto q, auto nw) {
         using E = std::remove_pointer_t<decltype(e)>;
         constexpr int NS = decltype(ns)::value, Q = decltype(q)::value, W = decltype(nw)::value;
         int r;
@@ -935,8 +941,7 @@ int asca_ssm_bwd(const void* x, long ldx, const void* dt, long lddt, const float
     p.ck = static_cast<float*>(const_cast<void*>(ws));
     p.T = T, p.D = D, p.N = N, p.G = G, p.Dg = D / G, p.softplus = softplus;
     p.B = B;
-    // 8 waves a block halve the partial sums of dB and dC
-    const SsmForm form = ssm_form(p, N, 8, (long)B * G * ((p.Dg + 63) / 64) >= 256 ? 8 : 4, 2048, 2048);
+    const SsmForm form = ssm_form(p, N, true, 2048, 2048);
     const long blocks = (long)B * p.nch * G * p.tiles, rows = (long)B * T, parts = (long)B * p.nch, per = rows * G * 2 * N, nd = (long)N * D;
     if (blocks > 0x7fffffffL || (per + 255) / 256 > 0x7fffffffL)
         return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows or channels", fn);
@@ -944,7 +949,7 @@ int asca_ssm_bwd(const void* x, long ldx, const void* dt, long lddt, const float
     if ((rc = sc.get((size_t)parts * (nd + 2 * D) + (size_t)p.tiles * per + ssm_chunk_floats(p), st))) return rc;
     p.pP = sc.ws.p, p.pBC = p.pP + parts * (nd + 2 * D), p.cs = p.pBC + p.tiles * per;
     p.ce = p.cs + (size_t)parts * N * D;
-    return ssm_dispatch(dtype, N, form, [&](auto* e, auto ns, auto q, auto nw) {
+    return ssm_dispatch<true>(dtype, N, form, [&](auto* e, auto ns, auto q, auto nw) {
         using E = std::remove_pointer_t<decltype(e)>;
         constexpr int NS = decltype(ns)::value, Q = decltype(q)::value, W = decltype(nw)::value;
         int r;
