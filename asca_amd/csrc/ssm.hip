@@ -263,9 +263,12 @@ ASCA_DEV void fold_chunks(const SsmArgs& p, int b, int ch, int q, int d, const f
         const long u = (long)b * p.nch + (REV ? p.nch - 1 - k : k);
         const float e = p.ce[u * p.D + d];
 #pragma unroll
-        for (int j = 0; j < NS; ++j)
-            h[j] = fmaf(__builtin_amdgcn_exp2f(e * A2[j]), h[j],
-                        p.cs[(u * p.N + min(q * NS + j, p.N - 1)) * p.D + d]);
+        for (int j = 0; j < NS; ++j) {
+            // as two factors, and none for a zero: over a chunk a growing state's alone may
+            // pass f32's range where the state does not
+            const float f = __builtin_amdgcn_exp2f(0.5f * e * A2[j]), c = p.cs[(u * p.N + min(q * NS + j, p.N - 1)) * p.D + d];
+            h[j] = h[j] == 0.0f ? c : fmaf(f * h[j], f, c);
+        }
     }
 }
 

@@ -172,6 +172,23 @@ def test_ssm_without_softplus_bias_skip_and_states(g):
     check("ssm plain", [("y", y, ry, FWD), ("h", h, rh, FWD)] + [(k, got[k], ref[k], GRAD) for k in ref])
 
 
+def test_ssm_growth_past_the_range_of_f32_over_rows_without_a_state(g):
+    """States that grow by 1.5 a row in the exponent: 380 rows' growth is far past f32's
+    range, but there is nothing to grow before row 390 (and no gradient after row 9)."""
+    rng = np.random.default_rng(14)
+    T, D, N = 400, 64, 16
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    i = dict(x=f(T, D), dt=np.full((T, D), 1.5, np.float32), A=np.ones((N, D), np.float32), Bm=f(T, N), Cm=f(T, N))
+    dy = f(T, D)
+    i["x"][:390] = 0
+    dy[10:] = 0
+    y, h, dev = g.ssm_scan(**i, batch=1, softplus=False)
+    ry, rh = so.ssm(**i, B=1, softplus=False)
+    got, ref = g.ssm_scan_bwd(dev, dy), so.ssm_bwd(**i, dy=dy, B=1, softplus=False)
+    dev.free()
+    check("growth", [("y", y, ry, FWD), ("h", h, rh, FWD)] + [(k, got[k], ref[k], GRAD) for k in ref])
+
+
 def test_ssm_cut_in_two_is_the_sequence(g):
     rng = np.random.default_rng(6)
     r = Rows(rng, False)
