@@ -11,8 +11,8 @@
 // matrices appears: the work is an exponential (a quarter-rate instruction) and
 // a few multiply-adds for each of them, on the vector unit.
 //
-// A wave holds 64 / Q channels by Q groups of states (Q = 8; 16 where waves are few,
-// see ssm_form), each lane the NS states of its group in registers; a block has NW
+// A wave holds 64 / Q channels by Q groups of states (Q = 8, or 16 where waves are few:
+// ssm_split and ssm_form), each lane the NS states of its group in registers; a block has NW
 // waves, CB = 64 / Q NW channels of one sequence, and takes its rows in tiles of K:
 //   - a thread reads x, dt (dy) of one channel at K / Q of the tile's rows, so loads
 //     are whole rows and softplus and its like are computed once per (row, channel);
@@ -28,9 +28,10 @@
 // states and decays again from it and keeps them in registers.  Partial sums of dB
 // and dC over a block's channels, and of the parameters' gradients over its rows,
 // are added by further kernels in a fixed order.
-// Where sequences and channels give too few blocks the rows are cut into chunks:
-// a first pass leaves what a chunk makes of a zero state (carry) and its sum of e,
-// from which every chunk works out what enters it, exp(A sum e) being its decay.
+// Where sequences and channels give too few blocks the forward's rows are split over a
+// block's waves (ssm_split_k, N <= 16), or the rows are cut into chunks: a first pass
+// leaves what a chunk makes of a zero state (carry) and its sum of e, from which every
+// chunk works out what enters it, exp(A sum e) being its decay.
 //
 // What bounds it is the vector unit, not memory: f32, 32 x 512 x 512, N = 16, the
 // forward (51 us) issues vector instructions in 73% of its cycles and the backward
@@ -417,6 +418,183 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
         for (int j = 0; j < NS; ++j)
             if (q * NS + j < p.N) p.h_out[((long)l.b * p.N + q * NS + j) * p.D + d] = h[j];
     }
+}
+
+// The forward with a sequence's rows split over a block's waves: 64 / Q channels a
+// block, wave w of it takes tiles w, w + NW, ...  In a tile every row's decay is formed
+// once and kept: first the states that the tile makes of a zero state (hl) and its decay
+// so far (P), then, when the waves have exchanged what they have at their tiles' ends and
+// each has gone through the NW of them, the states P h + hl and y.  A wave owns the rows
+// R q .. of its tile, those that it has y of after the sum over states, so nothing of its
+// own passes through another wave.  A growing P that overflows is held at the largest
+// value: there may be nothing to grow (0 times it is 0, as row by row).  Blocks are laid
+// out so that neighbouring channels, which share lines of x, dt and y, run on one XCD.
+// Bound by the vector unit's issue, and by waiting for the block's other waves where it
+// has a CU to itself: 16 x 1024 x 512 f32, N = 16, 60 us; 1 x 4096 x 2048 bf16 64 us;
+// 1 x 512 x 512 8.5 us, two rounds.
+template <typename E, int NS, int Q, int NW>
+__global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
+    constexpr int CH = 64 / Q, K = ssm_k(NS), R = K / Q, V = K * Q * NS, RB = 2 * V / 64;
+    const float BIG = __int_as_float(0x7f7fffff);
+    __shared__ float2 ex[NW][K][CH];
+    __shared__ float bc[NW][2 * V];
+    __shared__ float2 agg[2][NW][64][NS];
+    const unsigned nb = p.B * p.G * p.tiles, per = (nb + 7) / 8, u = blockIdx.x % 8 * per + blockIdx.x / 8;
+    if (u >= nb) return;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane / CH, c = lane % CH;
+    const int tile = u % p.tiles, g = u / p.tiles % p.G, b = u / p.tiles / p.G;
+    const bool live = tile * CH + c < p.Dg;
+    const int d = g * p.Dg + min(tile * CH + c, p.Dg - 1);
+    const int len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
+    const int ntile = (p.T + K - 1) / K, rounds = ((len + K - 1) / K + NW - 1) / NW;
+    const long row0 = (long)b * p.T;
+    float A2[NS], h[NS];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+        const int n = q * NS + j;
+        A2[j] = n < p.N ? p.A[(long)n * p.D + d] * LOG2E : 0.0f;
+        h[j] = p.h0 && n < p.N ? p.h0[((long)b * p.N + n) * p.D + d] : 0.0f;
+    }
+    float bias = p.dt_bias ? p.dt_bias[d] : 0.0f, Dk = p.Dk ? p.Dk[d] : 0.0f;
+    settle(bias);
+    settle(Dk);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) settle(h[j]), settle(A2[j]);
+    const E* px = static_cast<const E*>(p.x) + (row0 + R * q) * p.ldx + d;
+    const E* pdt = static_cast<const E*>(p.dt) + (row0 + R * q) * p.lddt + d;
+    E* py = static_cast<E*>(p.y) + (row0 + R * q) * p.ldy + d;
+    // B and C of the wave's tile: value lane + 64 i
+    const int bn = min(lane % (Q * NS), p.N - 1), br = lane / (Q * NS);
+    constexpr int BR = 64 / (Q * NS);   // rows a value of i apart
+    const E* pB = static_cast<const E*>(p.Bm) + (row0 + br) * p.ldb + (long)g * p.N + bn;
+    const E* pC = static_cast<const E*>(p.Cm) + (row0 + br) * p.ldc + (long)g * p.N + bn;
+    E rx[R], rdt[R], rb[RB];
+    auto fetch = [&](int k) {
+        const int t0 = k * K;
+        if (t0 + K <= len) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) rx[r] = px[(t0 + r) * p.ldx], rdt[r] = pdt[(t0 + r) * p.lddt];
+#pragma unroll
+            for (int i = 0; i < RB / 2; ++i) rb[i] = pB[(t0 + BR * i) * p.ldb], rb[RB / 2 + i] = pC[(t0 + BR * i) * p.ldc];
+        } else {
+            const int last = max(len - 1, 0);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const long t = min(t0 + R * q + r, last) - R * q;
+                rx[r] = px[t * p.ldx], rdt[r] = pdt[t * p.lddt];
+            }
+#pragma unroll
+            for (int i = 0; i < RB / 2; ++i) {
+                const long t = min(t0 + br + BR * i, last) - br;
+                rb[i] = pB[t * p.ldb], rb[RB / 2 + i] = pC[t * p.ldc];
+            }
+        }
+    };
+    if (rounds) fetch(w);
+    for (int o = 0; o < rounds; ++o) {
+        const int k = o * NW + w, t0 = k * K, buf = o & 1;
+        float x[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool in = t0 + R * q + r < len;
+            float slope;
+            const float e = ssm_e(p, act_value(rdt[r]) + bias, in, &slope);
+            x[r] = in ? act_value(rx[r]) : 0.0f;
+            ex[w][R * q + r][c] = make_float2(e, e * x[r]);
+        }
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+            const int r = br + BR * (i % (RB / 2)), n = lane % (Q * NS);
+            const float v = t0 + r < len && n < p.N ? act_value(rb[i]) : 0.0f;
+            bc[w][((r * Q + n / NS) * 2 + i / (RB / 2)) * NS + n % NS] = v;
+        }
+        fetch(min(k + NW, ntile - 1));
+        // the tile from a zero state, and its decay so far
+        float hl[K * NS], P[K * NS];
+        {
+            constexpr int PR = 2;
+            float2 ev[2][PR];
+            float m[2][PR][NS];
+            auto read = [&](int g) {
+#pragma unroll
+                for (int u = 0; u < PR; ++u) {
+                    ev[g & 1][u] = ex[w][g * PR + u][c];
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) m[g & 1][u][j] = bc[w][((g * PR + u) * Q + q) * 2 * NS + j];
+                }
+            };
+            read(0);
+#pragma unroll
+            for (int g = 0; g < K / PR; ++g) {
+                if (g + 1 < K / PR) read(g + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < PR; ++u)
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        const int t = g * PR + u, at = t * NS + j;
+                        const float a = __builtin_amdgcn_exp2f(ev[g & 1][u].x * A2[j]), in = m[g & 1][u][j] * ev[g & 1][u].y;
+                        P[at] = t ? P[t ? at - NS : 0] * a : a;
+                        hl[at] = t ? fmaf(a, hl[t ? at - NS : 0], in) : in;
+                    }
+            }
+        }
+        bool over = false;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const float e = P[(K - 1) * NS + j];
+            over |= e > BIG;
+            agg[buf][w][lane][j] = make_float2(fminf(e, BIG), hl[(K - 1) * NS + j]);
+        }
+        if (__any(over))
+#pragma unroll
+            for (int i = 0; i < K * NS; ++i) P[i] = fminf(P[i], BIG);
+        lds_barrier();
+        float hin[NS];
+#pragma unroll
+        for (int v0 = 0; v0 < NW; v0 += 4) {   // 4 at a time: registers
+            float2 f[4][NS];
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) f[v][j] = agg[buf][v0 + v][lane][j];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                if (v0 + v == w)
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) hin[j] = h[j];
+#pragma unroll
+                for (int j = 0; j < NS; ++j) h[j] = fmaf(f[v][j].x, h[j], f[v][j].y);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (p.ck && live && k < ntile)
+#pragma unroll
+            for (int j = 0; j < NS; ++j)
+                if (q * NS + j < p.N) p.ck[(((long)b * ntile + k) * p.N + q * NS + j) * p.D + d] = hin[j];
+        float y[K];
+#pragma unroll
+        for (int t = 0; t < K; ++t)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                const float v = fmaf(P[t * NS + j], hin[j], hl[t * NS + j]), C = bc[w][((t * Q + q) * 2 + 1) * NS + j];
+                y[t] = j ? fmaf(C, v, y[t]) : C * v;
+            }
+        float s[R];
+        scatter_high<Q, R>(y, lane, s);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (live && t0 + R * q + r < p.T) act_store(py + (t0 + r) * p.ldy, t0 + R * q + r < len ? fmaf(Dk, x[r], s[r]) : 0.0f);
+    }
+    if (!live) return;
+    for (int t = (rounds * NW + w) * K; t < p.T; t += NW * K)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (t + R * q + r < p.T) act_store(py + (long)(t + r) * p.ldy, 0.0f);
+    if (p.h_out && w == 0)
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+            if (q * NS + j < p.N) p.h_out[((long)b * p.N + q * NS + j) * p.D + d] = h[j];
 }
 
 // What a chunk makes of a zero carry, from its end to its start, and the sum of its e.
@@ -810,28 +988,57 @@ static int ssm_ld(const char* fn, const char* what, long ld, long cols) {
     return ld >= cols ? ASCA_OK : fail(ASCA_ERR_INVALID, "%s: row stride %s=%ld below its %ld columns", fn, what, ld, cols);
 }
 
-// How a call runs: Q lane groups, NW waves a block, and the rows' cut into p.nch chunks
-// a sequence.
-//   - 16 groups (N of 9 to 16) give twice the waves for a seventh more instructions:
-//     where 8 groups give fewer than two waves a SIMD but 16 most of them (16 x 1024 x
-//     512: 247 -> 212 us), or where few waves cannot be cut enough (1 x 512 x 512
-//     forward 15.4 -> 13.2 us); not where there are two (8 x 4096 x 2048 1288 -> 1544)
-//     or a cut serves better (forward 4 x 1000 x 1000 44 -> 53 us).
-//   - a cut costs a second pass over the rows, so it pays only for waves that are
-//     missing: below `enough`, as many chunks as give `want` (forward: 2 x 2048 x 1024
-//     in 512 waves 157 us, cut to 4096 47; 32 x 512 x 512 in 2048 waves 54 us, cut to
-//     4096 78; backward: 2 x 2048 x 1024 cut to 1024 142 us, to 2048 100).
-//   - the backward has 8 waves a block, which halves its partial sums of dB and dC (8 x
-//     4096 x 2048 904 -> 888 us), where that leaves a block for every CU (2 x 2048 x
-//     1024 without: 89.8 -> 90.8 us).
+// How a call runs: Q lane groups, NW waves a block.
 struct SsmForm {
     int Q, NW;
 };
+
+// Whether a forward's rows are split over the waves of a block (ssm_split_k): it costs a
+// third more multiply-adds and the waves wait for each other every NW tiles, but fills
+// the chip with 8 (4) channels a block and reads the rows once.  N <= 16, against
+// ssm_fwd_k:
+//   - not where that has two waves a SIMD by itself (32 x 512 x 512: 51 against 56 us).
+//   - below, 4 waves a block fill it (bf16, N = 16: 1 x 2048 x 12288 163 -> 154 us, x 8192
+//     128 -> 114, 1 x 4096 x 4096 142 -> 126), 8 where that takes a block for every CU (1 x
+//     4096 x 2048 77 -> 64 us; 102 with 4).
+//   - 16 groups of one state, 16 waves a block, where 8 groups leave half of the CUs
+//     without (1 x 2048 x 1024 30 -> 23.6 us, 8 groups 33.5; 1 x 512 x 512 14.5 -> 8.4),
+//     with 8 waves for short sequences (128 rows: 12.5 -> 5.5 us, 6.3 with 16).
+//   - where blocks are few and rows many, rows cut into chunks fill more of the chip (1 x
+//     16384 x 1024 146 us, split 154; 1 x 4096 x 512 36 and 41); at 1 x 2048 x 512 (128
+//     blocks) and 1 x 8192 x 1024 (256) both take the same.
+static bool ssm_split(SsmArgs& p, int N, SsmForm* f) {
+    const long w8 = (long)p.B * p.G * ((p.Dg + 7) / 8);
+    if (N > 16 || w8 >= 2048) return false;
+    if (N <= 8)
+        *f = {8, 8};
+    else if (w8 <= 128)
+        *f = {16, p.T < 512 ? 8 : 16};
+    else
+        *f = {8, w8 <= 256 && p.T >= 128 ? 8 : 4};
+    p.tiles = (p.Dg + 64 / f->Q - 1) / (64 / f->Q);
+    const long blocks = (long)p.B * p.G * p.tiles;
+    return blocks > 256 || p.T < std::max(1536L, blocks * blocks / 8);
+}
+
+// Otherwise p.nch chunks a sequence.
+//   - 16 groups (N of 9 to 16) give the backward twice the waves for a sixth more
+//     instructions: where 8 groups give fewer than a wave a SIMD and 16 a block a CU at
+//     most (16 x 1024 x 512 160 -> 145 us, 12 x 1024 x 512 156 -> 142; 24 x 1024 x 512, in
+//     384 blocks, 225 -> 277), or where few waves cannot be cut enough (1 x 512 x 512 28
+//     -> 26 us).
+//   - a cut costs a second pass over the rows, so it pays only for waves that are
+//     missing: below `enough`, as many chunks as give `want` (forward: 2 x 2048 x 1024, N =
+//     32, in 256 waves 237 us, cut to 4096 74; 32 x 512 x 512 in 2048 waves 46 us, cut to
+//     4096 75; backward: 2 x 2048 x 1024 cut to 1024 142 us, to 2048 100).
+//   - the backward has 8 waves a block, which halves its partial sums of dB and dC (8 x
+//     4096 x 2048 904 -> 888 us), where that leaves a block for every CU (2 x 2048 x
+//     1024 without: 89.8 -> 90.8 us).
 static SsmForm ssm_form(SsmArgs& p, int N, bool bwd, long enough, long want) {
     const int K = ssm_k(ssm_ns(N)), ntile = (p.T + K - 1) / K;
     const long w8 = (long)p.B * p.G * ((p.Dg + 7) / 8), cuts = std::max(1, std::min(64, ntile / 4));
     SsmForm f{8, bwd && ssm_ns(N) < 8 && (long)p.B * p.G * ((p.Dg + 63) / 64) >= 256 ? 8 : 4};
-    if (ssm_ns(N) == 2 && ((w8 >= 768 && w8 < 2048) || w8 * cuts < 1024)) f = {16, bwd ? 8 : 4};
+    if (bwd && ssm_ns(N) == 2 && ((w8 >= 768 && (long)p.B * p.G * ((p.Dg + 31) / 32) <= 256) || w8 * cuts < 1024)) f = {16, 8};
     const int CB = 64 / f.Q * f.NW;
     p.tiles = (p.Dg + CB - 1) / CB;
     const long waves = (long)p.B * p.G * p.tiles * f.NW;
@@ -849,7 +1056,8 @@ static int ssm_dispatch(int dtype, int N, SsmForm form, F f) {
         using std::integral_constant;
         const integral_constant<int, 8> c8;
         const integral_constant<int, 4> c4;
-        if (form.Q == 16) return f(e, integral_constant<int, 1>{}, integral_constant<int, 16>{}, integral_constant<int, BWD ? 8 : 4>{});
+        if constexpr (BWD)
+            if (form.Q == 16) return f(e, integral_constant<int, 1>{}, integral_constant<int, 16>{}, c8);
         auto go = [&](auto ns) {
             if constexpr (BWD)
                 if (form.NW == 8) return f(e, ns, c8, c8);
@@ -896,7 +1104,23 @@ int asca_ssm_fwd(const void* x, long ldx, const void* dt, long lddt, const float
     p.ck = static_cast<float*>(ws);
     p.T = T, p.D = D, p.N = N, p.G = G, p.Dg = D / G, p.softplus = softplus;
     p.B = B;
-    const SsmForm form = ssm_form(p, N, false, 1024, 4096);
+    SsmForm form;
+    if (ssm_split(p, N, &form)) {
+        const dim3 grid((unsigned)(((long)B * G * p.tiles + 7) / 8 * 8));
+        return act_dispatch(dtype, [&](auto* e) {
+            using E = std::remove_pointer_t<decltype(e)>;
+            auto go = [&](auto kernel) {
+                int r = pre_launch("ssm_split");
+                if (r) return r;
+                hipLaunchKernelGGL(kernel, grid, dim3(64 * form.NW), 0, st, p);
+                return post_launch("ssm_split");
+            };
+            if (form.Q == 16) return form.NW == 16 ? go(ssm_split_k<E, 1, 16, 16>) : go(ssm_split_k<E, 1, 16, 8>);
+            if (ssm_ns(N) == 1) return go(ssm_split_k<E, 1, 8, 8>);
+            return form.NW == 8 ? go(ssm_split_k<E, 2, 8, 8>) : go(ssm_split_k<E, 2, 8, 4>);
+        });
+    }
+    form = ssm_form(p, N, false, 1024, 4096);
     const long blocks = (long)B * p.nch * G * p.tiles;
     if (blocks > 0x7fffffffL) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many channels", fn);
     StreamScratch sc;

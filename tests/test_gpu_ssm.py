@@ -120,7 +120,9 @@ SSM = [(1, 1, 1, 1, 1, False), (2, 5, 3, 4, 1, True), (1, 16, 16, 16, 1, False),
        (1, 19, 17, 33, 1, False), (2, 1100, 64, 16, 1, True), (1, 2050, 20, 4, 1, False),
        # many channels (each width of the lane groups, 8 waves a block), long rows cut into chunks
        (8, 20, 2048, 16, 1, True), (8, 20, 2048, 7, 1, True), (8, 12, 2048, 20, 1, True), (4, 40, 2048, 10, 2, False),
-       (1, 1100, 512, 16, 1, True), (1, 1100, 500, 12, 2, False), (1, 1100, 260, 33, 1, False), (2, 700, 300, 24, 3, True)]
+       (1, 1100, 512, 16, 1, True), (1, 1100, 500, 12, 2, False), (1, 1100, 260, 33, 1, False), (2, 700, 300, 24, 3, True),
+       # rows split over a block's waves (4, 8 and 16 of them), and narrow long ones in chunks
+       (9, 70, 256, 16, 1, True), (1, 150, 1100, 16, 1, False), (3, 530, 36, 12, 1, True), (1, 1700, 24, 16, 1, False), (2, 1600, 10, 5, 1, True)]
 
 
 def ssm_inputs(r, rng, B, T, D, N, G):
@@ -172,16 +174,18 @@ def test_ssm_without_softplus_bias_skip_and_states(g):
     check("ssm plain", [("y", y, ry, FWD), ("h", h, rh, FWD)] + [(k, got[k], ref[k], GRAD) for k in ref])
 
 
-def test_ssm_growth_past_the_range_of_f32_over_rows_without_a_state(g):
-    """States that grow by 1.5 a row in the exponent: 380 rows' growth is far past f32's
-    range, but there is nothing to grow before row 390 (and no gradient after row 9)."""
+@pytest.mark.parametrize("T,D,N,e", [(400, 64, 16, 1.5), (400, 64, 16, 9.0), (1700, 64, 16, 1.5), (1700, 40, 5, 1.5), (300, 64, 40, 9.0)])
+def test_ssm_growth_past_the_range_of_f32_over_rows_without_a_state(g, T, D, N, e):
+    """States that grow by e a row in the exponent: many rows' growth (a tile's at 9) is far
+    past f32's range, but nothing is there to grow before the last rows, and there is no
+    gradient after the first."""
     rng = np.random.default_rng(14)
-    T, D, N = 400, 64, 16
+    last = int(60 / e)   # rows from the last x (to the first dy) on
     f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
-    i = dict(x=f(T, D), dt=np.full((T, D), 1.5, np.float32), A=np.ones((N, D), np.float32), Bm=f(T, N), Cm=f(T, N))
+    i = dict(x=f(T, D), dt=np.full((T, D), e, np.float32), A=np.ones((N, D), np.float32), Bm=f(T, N), Cm=f(T, N))
     dy = f(T, D)
-    i["x"][:390] = 0
-    dy[10:] = 0
+    i["x"][:-last] = 0
+    dy[last:] = 0
     y, h, dev = g.ssm_scan(**i, batch=1, softplus=False)
     ry, rh = so.ssm(**i, B=1, softplus=False)
     got, ref = g.ssm_scan_bwd(dev, dy), so.ssm_bwd(**i, dy=dy, B=1, softplus=False)
@@ -622,7 +626,7 @@ def test_captured_calls_replay_the_eager_results(g):
 
 
 @pytest.mark.parametrize("bad", [np.inf, np.nan])
-@pytest.mark.parametrize("B,T,D,N", [(1, 70, 40, 16), (1, 70, 40, 6), (8, 40, 2048, 16), (1, 1100, 512, 12)])
+@pytest.mark.parametrize("B,T,D,N", [(1, 70, 40, 16), (1, 70, 40, 6), (8, 40, 2048, 16), (1, 1100, 512, 12), (1, 1700, 24, 12), (5, 80, 512, 16)])
 def test_an_infinity_or_nan_stays_with_what_it_reaches(g, bad, B, T, D, N):
     """One bad x: its channel from its row on, and the sums over channels of those rows;
     one bad dy: its channel up to its row, and those rows' sums.  Everything else keeps
