@@ -421,17 +421,19 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
 }
 
 // The forward with a sequence's rows split over a block's waves: 64 / Q channels a
-// block, wave w of it takes tiles w, w + NW, ...  In a tile every row's decay is formed
-// once and kept: first the states that the tile makes of a zero state (hl) and its decay
-// so far (P), then, when the waves have exchanged what they have at their tiles' ends and
-// each has gone through the NW of them, the states P h + hl and y.  A wave owns the rows
-// R q .. of its tile, those that it has y of after the sum over states, so nothing of its
-// own passes through another wave.  A growing P that overflows is held at the largest
-// value: there may be nothing to grow (0 times it is 0, as row by row).  Blocks are laid
-// out so that neighbouring channels, which share lines of x, dt and y, run on one XCD.
-// Bound by the vector unit's issue, and by waiting for the block's other waves where it
-// has a CU to itself: 16 x 1024 x 512 f32, N = 16, 60 us; 1 x 4096 x 2048 bf16 64 us;
-// 1 x 512 x 512 8.5 us, two rounds.
+// block, wave w of it takes tiles w, w + NW, ...  In a tile every row's decay and input
+// are formed once and kept in registers: first they give the states that the tile makes
+// of a zero state and its sum of e, which the waves exchange and each goes through, NW of
+// them, for the state that enters its own tile; then the tile's states and y.  (The local
+// states and the decays' products kept instead, and the true state's share added by them:
+// 16 x 1024 x 512 63 us; the inputs read and formed again, 26 registers fewer: 1 x 4096 x
+// 4096 120 -> 131.)  A wave owns the rows R q .. of its tile, those that it has y
+// of after the sum over states, so nothing of its own passes through another wave.  A
+// tile's growth that overflows is held at the largest value: there may be nothing to grow
+// (0 times it is 0, as row by row).  Blocks are laid out so that neighbouring channels,
+// which share lines of x, dt and y, run on one XCD.  Bound by the vector unit's issue, and
+// by waiting for the block's other waves where it has a CU to itself: 16 x 1024 x 512 f32,
+// N = 16, 60 us; 1 x 4096 x 2048 bf16 65 us; 1 x 512 x 512 8.2 us, two rounds.
 template <typename E, int NS, int Q, int NW>
 __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
     constexpr int CH = 64 / Q, K = ssm_k(NS), R = K / Q, V = K * Q * NS, RB = 2 * V / 64;
@@ -509,8 +511,11 @@ __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
             bc[w][((r * Q + n / NS) * 2 + i / (RB / 2)) * NS + n % NS] = v;
         }
         fetch(min(k + NW, ntile - 1));
-        // the tile from a zero state, and its decay so far
-        float hl[K * NS], P[K * NS];
+        // the tile from a zero state and its sum of e; decays and inputs are kept
+        float a[K * NS], in[K * NS];
+        float hl[NS], esum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) hl[j] = 0.0f;
         {
             constexpr int PR = 2;
             float2 ev[2][PR];
@@ -529,26 +534,21 @@ __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
                 if (g + 1 < K / PR) read(g + 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int u = 0; u < PR; ++u)
+                for (int u = 0; u < PR; ++u) {
+                    const int t = g * PR + u;
+                    esum += ev[g & 1][u].x;
 #pragma unroll
                     for (int j = 0; j < NS; ++j) {
-                        const int t = g * PR + u, at = t * NS + j;
-                        const float a = __builtin_amdgcn_exp2f(ev[g & 1][u].x * A2[j]), in = m[g & 1][u][j] * ev[g & 1][u].y;
-                        P[at] = t ? P[t ? at - NS : 0] * a : a;
-                        hl[at] = t ? fmaf(a, hl[t ? at - NS : 0], in) : in;
+                        a[t * NS + j] = __builtin_amdgcn_exp2f(ev[g & 1][u].x * A2[j]);
+                        in[t * NS + j] = m[g & 1][u][j] * ev[g & 1][u].y;
+                        hl[j] = t ? fmaf(a[t * NS + j], hl[j], in[t * NS + j]) : in[t * NS + j];
                     }
+                }
             }
         }
-        bool over = false;
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            const float e = P[(K - 1) * NS + j];
-            over |= e > BIG;
-            agg[buf][w][lane][j] = make_float2(fminf(e, BIG), hl[(K - 1) * NS + j]);
-        }
-        if (__any(over))
-#pragma unroll
-            for (int i = 0; i < K * NS; ++i) P[i] = fminf(P[i], BIG);
+        for (int j = 0; j < NS; ++j)
+            agg[buf][w][lane][j] = make_float2(fminf(__builtin_amdgcn_exp2f(esum * A2[j]), BIG), hl[j]);
         lds_barrier();
         float hin[NS];
 #pragma unroll
@@ -577,8 +577,9 @@ __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
         for (int t = 0; t < K; ++t)
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
-                const float v = fmaf(P[t * NS + j], hin[j], hl[t * NS + j]), C = bc[w][((t * Q + q) * 2 + 1) * NS + j];
-                y[t] = j ? fmaf(C, v, y[t]) : C * v;
+                const float C = bc[w][((t * Q + q) * 2 + 1) * NS + j];
+                hin[j] = fmaf(a[t * NS + j], hin[j], in[t * NS + j]);
+                y[t] = j ? fmaf(C, hin[j], y[t]) : C * hin[j];
             }
         float s[R];
         scatter_high<Q, R>(y, lane, s);
@@ -993,14 +994,15 @@ struct SsmForm {
     int Q, NW;
 };
 
-// Whether a forward's rows are split over the waves of a block (ssm_split_k): it costs a
-// third more multiply-adds and the waves wait for each other every NW tiles, but fills
-// the chip with 8 (4) channels a block and reads the rows once.  N <= 16, against
+// Whether a forward's rows are split over the waves of a block (ssm_split_k): it goes
+// through a tile's states twice and the waves wait for each other every NW tiles, but
+// fills the chip with 8 (4) channels a block and reads the rows once.  N <= 16, against
 // ssm_fwd_k:
-//   - not where that has two waves a SIMD by itself (32 x 512 x 512: 51 against 56 us).
+//   - not where that has two waves a SIMD by itself (32 x 512 x 512: 48 against 54 us,
+//     8 x 2048 x 2048 155 against 203).
 //   - below, 4 waves a block fill it (bf16, N = 16: 1 x 2048 x 12288 163 -> 154 us, x 8192
-//     128 -> 114, 1 x 4096 x 4096 142 -> 126), 8 where that takes a block for every CU (1 x
-//     4096 x 2048 77 -> 64 us; 102 with 4).
+//     128 -> 114, 1 x 4096 x 4096 142 -> 120), 8 where that takes a block for every CU (1 x
+//     4096 x 2048 77 -> 65 us; 102 with 4).
 //   - 16 groups of one state, 16 waves a block, where 8 groups leave half of the CUs
 //     without (1 x 2048 x 1024 30 -> 23.6 us, 8 groups 33.5; 1 x 512 x 512 14.5 -> 8.4),
 //     with 8 waves for short sequences (128 rows: 12.5 -> 5.5 us, 6.3 with 16).
