@@ -29,7 +29,7 @@
 // and dC over a block's channels, and of the parameters' gradients over its rows,
 // are added by further kernels in a fixed order.
 // Where sequences and channels give too few blocks the forward's rows are split over a
-// block's waves (ssm_split_k, N <= 16), or the rows are cut into chunks: a first pass
+// block's waves (ssm_split_k), or the rows are cut into chunks: a first pass
 // leaves what a chunk makes of a zero state (carry) and its sum of e, from which every
 // chunk works out what enters it, exp(A sum e) being its decay.
 //
@@ -996,7 +996,7 @@ struct SsmForm {
 
 // Whether a forward's rows are split over the waves of a block (ssm_split_k): it goes
 // through a tile's states twice and the waves wait for each other every NW tiles, but
-// fills the chip with 8 (4) channels a block and reads the rows once.  N <= 16, against
+// fills the chip with 8 (4) channels a block and reads the rows once.  Against
 // ssm_fwd_k:
 //   - not where that has two waves a SIMD by itself (32 x 512 x 512: 48 against 54 us,
 //     8 x 2048 x 2048 155 against 203).
@@ -1008,19 +1008,24 @@ struct SsmForm {
 //     with 8 waves for short sequences (128 rows: 12.5 -> 5.5 us, 6.3 with 16).
 //   - where blocks are few and rows many, rows cut into chunks fill more of the chip (1 x
 //     16384 x 1024 146 us, split 154; 1 x 4096 x 512 36 and 41); at 1 x 2048 x 512 (128
-//     blocks) and 1 x 8192 x 1024 (256) both take the same.
+//     blocks) and 1 x 8192 x 1024 (256) both take the same.  N of 17 to 32, 4 states a
+//     lane: from a quarter of the rows on (1 x 128 x 512 14 -> 7.8 us, 1 x 2048 x 8192 238
+//     -> 205; 1 x 2048 x 1024 45, split 66).
+//   - N above 32 only for few and short rows: a wave has its SIMD to itself (1 x 64 x 2048,
+//     N = 64: 20 -> 10 us; 1 x 512 x 512 32, split 44).
 static bool ssm_split(SsmArgs& p, int N, SsmForm* f) {
     const long w8 = (long)p.B * p.G * ((p.Dg + 7) / 8);
-    if (N > 16 || w8 >= 2048) return false;
+    if (w8 >= 2048) return false;
     if (N <= 8)
         *f = {8, 8};
-    else if (w8 <= 128)
+    else if (N <= 16 && w8 <= 128)
         *f = {16, p.T < 512 ? 8 : 16};
     else
-        *f = {8, w8 <= 256 && p.T >= 128 ? 8 : 4};
+        *f = {8, N <= 32 && w8 <= 256 && p.T >= 128 ? 8 : 4};
     p.tiles = (p.Dg + 64 / f->Q - 1) / (64 / f->Q);
     const long blocks = (long)p.B * p.G * p.tiles;
-    return blocks > 256 || p.T < std::max(1536L, blocks * blocks / 8);
+    if (N > 32) return blocks <= 256 && p.T <= 256;
+    return blocks > 256 || p.T < std::max(1536L, blocks * blocks / 8) / (N > 16 ? 4 : 1);
 }
 
 // Otherwise p.nch chunks a sequence.
@@ -1118,8 +1123,12 @@ int asca_ssm_fwd(const void* x, long ldx, const void* dt, long lddt, const float
                 return post_launch("ssm_split");
             };
             if (form.Q == 16) return form.NW == 16 ? go(ssm_split_k<E, 1, 16, 16>) : go(ssm_split_k<E, 1, 16, 8>);
-            if (ssm_ns(N) == 1) return go(ssm_split_k<E, 1, 8, 8>);
-            return form.NW == 8 ? go(ssm_split_k<E, 2, 8, 8>) : go(ssm_split_k<E, 2, 8, 4>);
+            switch (ssm_ns(N)) {
+                case 1: return go(ssm_split_k<E, 1, 8, 8>);
+                case 2: return form.NW == 8 ? go(ssm_split_k<E, 2, 8, 8>) : go(ssm_split_k<E, 2, 8, 4>);
+                case 4: return form.NW == 8 ? go(ssm_split_k<E, 4, 8, 8>) : go(ssm_split_k<E, 4, 8, 4>);
+                default: return go(ssm_split_k<E, 8, 8, 4>);
+            }
         });
     }
     form = ssm_form(p, N, false, 1024, 4096);

@@ -122,7 +122,8 @@ SSM = [(1, 1, 1, 1, 1, False), (2, 5, 3, 4, 1, True), (1, 16, 16, 16, 1, False),
        (8, 20, 2048, 16, 1, True), (8, 20, 2048, 7, 1, True), (8, 12, 2048, 20, 1, True), (4, 40, 2048, 10, 2, False),
        (1, 1100, 512, 16, 1, True), (1, 1100, 500, 12, 2, False), (1, 1100, 260, 33, 1, False), (2, 700, 300, 24, 3, True),
        # rows split over a block's waves (4, 8 and 16 of them), and narrow long ones in chunks
-       (9, 70, 256, 16, 1, True), (1, 150, 1100, 16, 1, False), (3, 530, 36, 12, 1, True), (1, 1700, 24, 16, 1, False), (2, 1600, 10, 5, 1, True)]
+       (9, 70, 256, 16, 1, True), (1, 150, 1100, 16, 1, False), (3, 530, 36, 12, 1, True), (1, 1700, 24, 16, 1, False), (2, 1600, 10, 5, 1, True),
+       (1, 200, 72, 30, 2, False), (3, 90, 800, 20, 1, True), (2, 130, 30, 50, 1, True)]
 
 
 def ssm_inputs(r, rng, B, T, D, N, G):
@@ -174,7 +175,7 @@ def test_ssm_without_softplus_bias_skip_and_states(g):
     check("ssm plain", [("y", y, ry, FWD), ("h", h, rh, FWD)] + [(k, got[k], ref[k], GRAD) for k in ref])
 
 
-@pytest.mark.parametrize("T,D,N,e", [(400, 64, 16, 1.5), (400, 64, 16, 9.0), (1700, 64, 16, 1.5), (1700, 40, 5, 1.5), (300, 64, 40, 9.0)])
+@pytest.mark.parametrize("T,D,N,e", [(400, 64, 16, 1.5), (400, 64, 16, 9.0), (1700, 64, 16, 1.5), (1700, 40, 5, 1.5), (300, 64, 40, 9.0), (200, 64, 40, 9.0), (300, 64, 20, 9.0)])
 def test_ssm_growth_past_the_range_of_f32_over_rows_without_a_state(g, T, D, N, e):
     """States that grow by e a row in the exponent: many rows' growth (a tile's at 9) is far
     past f32's range, but nothing is there to grow before the last rows, and there is no
