@@ -247,6 +247,10 @@ struct BcTile {
 // every turn of it, together with the loads that the turn itself has in flight.
 ASCA_DEV void settle(float& x) { asm volatile("" : "+v"(x)); }
 
+// LDS that only one wave writes and reads: its accesses keep their order, which the
+// compiler has to know where a lane reads what another wrote.
+ASCA_DEV void lds_wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // Step e of a row from its raw dt (0 past the sequence's end: the state stays)
 ASCA_DEV float ssm_e(const SsmArgs& p, float v, bool in, float* slope) {
     float s = v;
@@ -510,6 +514,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
             const float v = t0 + r < len && n < p.N ? act_value(rb[i]) : 0.0f;
             bc[w][((r * Q + n / NS) * 2 + i / (RB / 2)) * NS + n % NS] = v;
         }
+        lds_wave_order();
         fetch(min(k + NW, ntile - 1));
         // the tile from a zero state and its sum of e; decays and inputs are kept
         float a[K * NS], in[K * NS];
@@ -581,6 +586,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
                 hin[j] = fmaf(a[t * NS + j], hin[j], in[t * NS + j]);
                 y[t] = j ? fmaf(C, hin[j], y[t]) : C * hin[j];
             }
+        lds_wave_order();
         float s[R];
         scatter_high<Q, R>(y, lane, s);
 #pragma unroll
