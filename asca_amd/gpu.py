@@ -960,6 +960,8 @@ class Gpu:
         """r = x + scale o (rms(y o silu(z)) o w_post) and n = rms(r) o w_pre of
         (rows, cols) matrices (asca_block_norm_fwd); returns (r, n)."""
         a = x if x is not None else y
+        if a is None:
+            raise ValueError("block_norm needs x or y")
         rows, cols = a.shape
         ty = _acts({k: a.shape for k in "xyz"}, x=x, y=y, z=z)
         b = _Bufs()
@@ -977,6 +979,8 @@ class Gpu:
         """The gradients dx, dy, dz, dw_post, dscale, dw_pre of block_norm from dr and
         dn (asca_block_norm_bwd), for the inputs that are given."""
         a = x if x is not None else y
+        if a is None:
+            raise ValueError("block_norm needs x or y")
         rows, cols = a.shape
         ty = _acts({k: a.shape for k in ("x", "y", "z", "dr", "dn")}, x=x, y=y, z=z, dr=dr, dn=dn)
         b = _Bufs()

@@ -522,6 +522,8 @@ def test_refusals(g):
         g.ssm_scan(x, x[:3], np.zeros((4, 8)), x[:, :4], x[:, :4], batch=1)
     with pytest.raises(ValueError):
         g.conv(x.astype(np.float64), np.zeros((4, 8)), batch=1)
+    with pytest.raises(ValueError):
+        g.block_norm(None)
 
 
 @pytest.mark.parametrize("nth", [0, 1, 2])
