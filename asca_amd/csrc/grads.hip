@@ -5,8 +5,10 @@
 // sums are added in their order by every block that scales, which costs less than a
 // launch between (and than a last block's: a fence in each block before it took the
 // norm of 143M gradients from 122 to 310 us).  Bound by memory: 143M f32 gradients
-// are read in 126 us (4.5 TB/s) and read and written in 207 us (5.5 TB/s, the part
-// that the last-level cache still holds coming first).
+// are read in 113 us (5.1 TB/s; 155 just after a kernel that filled the last-level
+// cache with its writes) and read and written in 206 us (5.5 TB/s, the part that the
+// cache still holds coming first).  Stores past the caches leave more of the list there,
+// which the next call on it sees (321 -> 294 us) but not an update between (890 us both).
 #include <algorithm>
 #include <vector>
 
@@ -22,7 +24,7 @@ struct GradChunk {
 
 constexpr int GC_U = 4;                            // accesses of 4 elements a thread has in flight
 constexpr long GC_IT = 256 * 4 * GC_U;             // elements a block takes at a time
-constexpr long GC_MIN = GC_IT, GC_BLOCKS = 2048;   // elements a chunk at least; about so many chunks
+constexpr long GC_MIN = GC_IT, GC_BLOCKS = 4096;   // elements a chunk at least; about so many chunks (2048: 334 us, 4096: 321)
 
 ASCA_DEV double wave_sum_d(double x) {
 #pragma unroll

@@ -305,6 +305,29 @@ def test_grads_clip(g, sizes, bf16, place):
         gl.close()
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+def test_grads_clip_of_a_list_larger_than_the_cache(g, bf16):
+    from asca_amd import gpu
+
+    sizes = [67_108_864 << bf16, 5_000_003, 1]
+    rng = np.random.default_rng(3)
+    r = Rows(rng, bf16)
+    block = r(1 << 20)
+    host = [np.resize(block, k) for k in sizes]
+    src = [gpu.DevBuf.from_array(h) for h in host]
+    gl = gpu.GradList(list(zip(src, sizes)), dtype=gpu.BF16 if bf16 else gpu.F32)
+    want = np.sqrt(sum(float(np.square(r.val(h[i:i + (1 << 22)]).astype(np.float64)).sum()) for h in host for i in range(0, h.size, 1 << 22)))
+    norm, coef = gl.clip(100.0)
+    assert abs(norm - want) <= 1e-6 * want and abs(coef - 100.0 / (want + 1e-6)) <= 1e-6 * coef
+    for h, b in zip(host, src):
+        got = b.to_host(h.shape, h.dtype)
+        for i in range(0, h.size, 1 << 22):
+            assert err(r.val(got[i:i + (1 << 22)]), r.val(h[i:i + (1 << 22)]).astype(np.float64) * 100.0 / (want + 1e-6)) <= r.tol(FWD)
+    gl.close()
+    for b in src:
+        b.free()
+
+
 def test_grads_norm_of_large_small_and_infinite_values(g):
     from asca_amd import gpu
 
