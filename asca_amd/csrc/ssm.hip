@@ -259,6 +259,16 @@ ASCA_DEV float ssm_e(const SsmArgs& p, float v, bool in, float* slope) {
     return in ? s : 0.0f;
 }
 
+// Many rows' decay, exp2(x), is held as its square root and met in two factors: a growing
+// state's alone may pass f32's range where the state does not.  The root is held at the
+// largest value, so that it leaves a zero zero, as row by row, and takes any other normal
+// number past the range, as the growth that it stands for would.  NaN stays.
+ASCA_DEV float decay_root(float x) {
+    const float f = __builtin_amdgcn_exp2f(0.5f * x), BIG = __int_as_float(0x7f7fffff);
+    return f > BIG ? BIG : f;
+}
+ASCA_DEV float decayed(float f, float h, float c) { return fmaf(f * h, f, c); }
+
 // The state (or with REV the carry) that enters a chunk: the chunks before (after) it
 // in turn, each as it left its own zero start and by its decay.
 template <int NS, bool REV>
@@ -268,12 +278,8 @@ ASCA_DEV void fold_chunks(const SsmArgs& p, int b, int ch, int q, int d, const f
         const long u = (long)b * p.nch + (REV ? p.nch - 1 - k : k);
         const float e = p.ce[u * p.D + d];
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            // as two factors, and none for a zero: over a chunk a growing state's alone may
-            // pass f32's range where the state does not
-            const float f = __builtin_amdgcn_exp2f(0.5f * e * A2[j]), c = p.cs[(u * p.N + min(q * NS + j, p.N - 1)) * p.D + d];
-            h[j] = h[j] == 0.0f ? c : fmaf(f * h[j], f, c);
-        }
+        for (int j = 0; j < NS; ++j)
+            h[j] = decayed(decay_root(e * A2[j]), h[j], p.cs[(u * p.N + min(q * NS + j, p.N - 1)) * p.D + d]);
     }
 }
 
@@ -432,16 +438,14 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
 // states and the decays' products kept instead, and the true state's share added by them:
 // 16 x 1024 x 512 63 us; the inputs read and formed again, 26 registers fewer: 1 x 4096 x
 // 4096 120 -> 131.)  A wave owns the rows R q .. of its tile, those that it has y
-// of after the sum over states, so nothing of its own passes through another wave.  A
-// tile's growth that overflows is held at the largest value: there may be nothing to grow
-// (0 times it is 0, as row by row).  Blocks are laid out so that neighbouring channels,
-// which share lines of x, dt and y, run on one XCD.  Bound by the vector unit's issue, and
+// of after the sum over states, so nothing of its own passes through another wave.
+// Blocks are laid out so that neighbouring channels, which share lines of x, dt and y, run
+// on one XCD.  Bound by the vector unit's issue, and
 // by waiting for the block's other waves where it has a CU to itself: 16 x 1024 x 512 f32,
 // N = 16, 60 us; 1 x 4096 x 2048 bf16 65 us; 1 x 512 x 512 8.2 us, two rounds.
 template <typename E, int NS, int Q, int NW>
 __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
     constexpr int CH = 64 / Q, K = ssm_k(NS), R = K / Q, V = K * Q * NS, RB = 2 * V / 64;
-    const float BIG = __int_as_float(0x7f7fffff);
     __shared__ float2 ex[NW][K][CH];
     __shared__ float bc[NW][2 * V];
     __shared__ float2 agg[2][NW][64][NS];
@@ -553,7 +557,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
         }
 #pragma unroll
         for (int j = 0; j < NS; ++j)
-            agg[buf][w][lane][j] = make_float2(fminf(__builtin_amdgcn_exp2f(esum * A2[j]), BIG), hl[j]);
+            agg[buf][w][lane][j] = make_float2(decay_root(esum * A2[j]), hl[j]);
         lds_barrier();
         float hin[NS];
 #pragma unroll
@@ -569,7 +573,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
 #pragma unroll
                     for (int j = 0; j < NS; ++j) hin[j] = h[j];
 #pragma unroll
-                for (int j = 0; j < NS; ++j) h[j] = fmaf(f[v][j].x, h[j], f[v][j].y);
+                for (int j = 0; j < NS; ++j) h[j] = decayed(f[v][j].x, h[j], f[v][j].y);
             }
             __builtin_amdgcn_sched_barrier(0);
         }

@@ -194,6 +194,37 @@ def test_ssm_growth_past_the_range_of_f32_over_rows_without_a_state(g, T, D, N, 
     check("growth", [("y", y, ry, FWD), ("h", h, rh, FWD)] + [(k, got[k], ref[k], GRAD) for k in ref])
 
 
+# every instance of the split forward, rows one after another, and rows cut into chunks
+GROWTH = [(1, 34, 16, 4), (1, 34, 16, 16), (1, 520, 16, 16), (1, 34, 1100, 16), (1, 130, 1100, 16), (1, 34, 16, 20), (1, 130, 16, 20),
+          (1, 34, 16, 40), (8, 34, 2048, 16), (1, 1700, 24, 16), (1, 1700, 24, 20)]
+
+
+@pytest.mark.parametrize("small,e", [(1e-10, 6.0), (1e-35, 10.0)])
+@pytest.mark.parametrize("B,T,D,N", GROWTH)
+def test_ssm_growth_of_small_states_past_the_range_of_f32(g, B, T, D, N, small, e):
+    """The first K rows' growth, exp(K e), is past f32's range and the states that it meets
+    are small: they stay finite until the last K rows take it back.  The gradients pass
+    through the same factors from the other end.  A growth of G in the exponent takes the
+    roundings of A and of each e A with it, 2 G 2^-24; twice that is allowed."""
+    K = 16 if N <= 16 else 8
+    e = e * 16 / K
+    rng = np.random.default_rng(15)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    step = np.zeros((B, T, D), np.float32)
+    step[:, :K], step[:, -K:] = e, -e
+    i = dict(x=f(B * T, D) * np.float32(small), dt=step.reshape(B * T, D), A=np.ones((N, D), np.float32), Bm=f(B * T, N), Cm=f(B * T, N))
+    h0, dh, dy = f(B, N, D) * np.float32(small), f(B, N, D) * np.float32(1e10), f(B * T, D) * np.float32(small)
+    h0[:, ::3] = 0
+    y, h, dev = g.ssm_scan(**i, batch=B, h0=h0, softplus=False)
+    ry, rh = so.ssm(**i, B=B, h0=h0, softplus=False)
+    got, ref = g.ssm_scan_bwd(dev, dy, dh), so.ssm_bwd(**i, dy=dy, B=B, h0=h0, softplus=False, dh_out=dh)
+    dev.free()
+    more = 4 * K * e * 2.0 ** -24
+    if small * small < 1e-45:   # dy x has no f32
+        assert not got.pop("dDk").any() and np.abs(ref.pop("dDk")).max() < 1e-45
+    check("small growth", [("y", y, ry, FWD + more), ("h", h, rh, FWD + more)] + [(k, got[k], ref[k], GRAD + more) for k in ref])
+
+
 def test_ssm_cut_in_two_is_the_sequence(g):
     rng = np.random.default_rng(6)
     r = Rows(rng, False)
