@@ -234,19 +234,30 @@ class SsmModel:
             _lib.call("asca_memset32", _vp(b), 0, b.nbytes // 4, None)
         return st
 
+    def _states(self, states, n: int) -> tuple:
+        """The addresses of states that hold n sequences; a layer's begin at its index
+        times n, so those of another number are refused."""
+        for b, k in zip(states, (self.W - 1, self.N), strict=True):
+            if b.nbytes != self.L * n * k * self.d * 4:
+                raise ValueError(f"states of {b.nbytes} bytes for n={n} sequences ({self.L * n * k * self.d * 4})")
+        return tuple(_vp(b) for b in states)
+
     def prompt(self, ids, states, lens=None) -> np.ndarray:
         """Rows of n_seq prompts, ids (n_seq, T) of which sequence b has lens[b], going on
         from `states` and leaving them after each one's last row; the (n_seq, V) logits of
         that row (of a prompt of length 0: of its first column's id, which it does not take)."""
         ids = np.atleast_2d(np.asarray(ids))
         n, T = ids.shape
+        st = self._states(states, n)
         dl = None
         if lens is None:
             last = np.full(n, T - 1)
         else:
             lens = np.clip(np.asarray(lens, np.int32), 0, T)
+            if lens.shape != (n,):
+                raise ValueError(f"lens has shape {lens.shape}, expected {(n,)}")
             dl, last = self._up("lens", lens, np.int32), np.maximum(lens - 1, 0)
-        nrm = self._forward(ids.reshape(-1), n, False, tuple(_vp(b) for b in states), dl)
+        nrm = self._forward(ids.reshape(-1), n, False, st, dl)
         pick = self._rows("pick", n, self.d)
         _lib.call("asca_gather_rows", nrm, self._up("last", np.arange(n) * T + last, np.int32), n, self.d, pick, None)
         self._head(pick, n)
@@ -256,7 +267,7 @@ class SsmModel:
     def step(self, ids, states) -> np.ndarray:
         """One row for each sequence on its states, in place; (n_seq, V) logits."""
         ids = np.atleast_1d(np.asarray(ids))
-        nrm = self._forward(ids, len(ids), False, tuple(_vp(b) for b in states), one=True)
+        nrm = self._forward(ids, len(ids), False, self._states(states, len(ids)), one=True)
         self._head(nrm, len(ids))
         _lib.call("asca_sync")
         return self._bufs["logits"].to_host((len(ids), self.vocab))
