@@ -119,6 +119,15 @@ class SsmModel:
     def _gemm(ta, tb, m, n, k, a, lda, b, ldb, c, ldc, beta=0.0):
         _lib.call("asca_gemm", ta, tb, m, n, k, 1.0, a, lda, b, ldb, beta, c, ldc, None, None)
 
+    def _ids(self, ids, used=None) -> np.ndarray:
+        """Ids as int32; one outside the table is refused, or 0 where it is not `used`."""
+        ids = np.asarray(ids).astype(np.int64)
+        if used is not None:
+            ids = np.where(used, ids, 0)
+        if ids.size and not 0 <= int(ids.min()) <= int(ids.max()) < self.vocab:
+            raise ValueError(f"ids from {ids.min()} to {ids.max()}, expected 0 .. {self.vocab - 1}")
+        return ids.astype(np.int32)
+
     # -- forward --------------------------------------------------------------------
     def _forward(self, ids, batch: int, keep: bool, states=None, lens=None, one: bool = False) -> C.c_void_p:
         """Normalised rows after the last layer.  `keep`: layer by layer, for the
@@ -179,7 +188,7 @@ class SsmModel:
         if rows % batch or len(targets) != rows:
             raise ValueError("ids/targets must hold batch * seq tokens each")
         T = rows // batch
-        nrm = self._forward(ids, batch, True)
+        nrm = self._forward(self._ids(ids), batch, True)
         logits = self._head(nrm, rows)
         dlog, losses = self._rows("dlog", rows, V), self._rows("losses", rows, 1)
         _lib.call("asca_cross_entropy", logits, self._up("tgt", targets, np.uint32), rows, V, dlog, losses, None)
@@ -245,7 +254,8 @@ class SsmModel:
     def prompt(self, ids, states, lens=None) -> np.ndarray:
         """Rows of n_seq prompts, ids (n_seq, T) of which sequence b has lens[b], going on
         from `states` and leaving them after each one's last row; the (n_seq, V) logits of
-        that row (of a prompt of length 0: of its first column's id, which it does not take)."""
+        that row (of a prompt of length 0: of its first column's id, which it does not take).
+        Ids past a length may be anything."""
         ids = np.atleast_2d(np.asarray(ids))
         n, T = ids.shape
         st = self._states(states, n)
@@ -256,7 +266,10 @@ class SsmModel:
             lens = np.clip(np.asarray(lens, np.int32), 0, T)
             if lens.shape != (n,):
                 raise ValueError(f"lens has shape {lens.shape}, expected {(n,)}")
-            dl, last = self._up("lens", lens, np.int32), np.maximum(lens - 1, 0)
+            last = np.maximum(lens - 1, 0)
+        ids = self._ids(ids, np.arange(T) <= last[:, None])
+        if lens is not None:
+            dl = self._up("lens", lens, np.int32)
         nrm = self._forward(ids.reshape(-1), n, False, st, dl)
         pick = self._rows("pick", n, self.d)
         _lib.call("asca_gather_rows", nrm, self._up("last", np.arange(n) * T + last, np.int32), n, self.d, pick, None)
@@ -266,7 +279,7 @@ class SsmModel:
 
     def step(self, ids, states) -> np.ndarray:
         """One row for each sequence on its states, in place; (n_seq, V) logits."""
-        ids = np.atleast_1d(np.asarray(ids))
+        ids = self._ids(np.atleast_1d(ids))
         nrm = self._forward(ids, len(ids), False, self._states(states, len(ids)), one=True)
         self._head(nrm, len(ids))
         _lib.call("asca_sync")

@@ -82,3 +82,26 @@ def test_lengths_of_another_number_of_sequences(model, lens):
     refused(log, m.prompt, np.zeros((3, 5), int), st, lens)
     m.prompt(np.zeros((3, 5), int), st, [4, 0, 9])
     assert "asca_ssm_fwd" in names(log)
+
+
+def test_ids_outside_the_table(model):
+    m, log = model
+    st = m.new_state(2)
+    for bad in (17, -1, 1 << 31, 1 << 32):
+        refused(log, m.step, np.array([0, bad]), st)
+        refused(log, m.prompt, np.array([[0, 1], [bad, 1]]), st)
+        refused(log, m.prompt, np.array([[0, 1], [1, bad]]), st, [2, 2])
+        refused(log, m.prompt, np.array([[0, 1], [bad, 1]]), st, [2, 0])   # its logits are of this row
+        refused(log, m.forward_backward, np.array([0, 1, 2, bad]), np.zeros(4, int), 2)
+    m.step(np.array([0, 16], np.uint8), st)
+    m.step([0, 16], st)
+
+
+def test_ids_past_a_prompts_length_do_not_matter(model):
+    m, log = model
+    st = m.new_state(3)
+    del log[:]
+    m.prompt(np.array([[1, 2, 99], [3, -1, -1], [4, 99, 99]]), st, [2, 1, 0])
+    up = [a for n, a in log if n == "upload" and a.size == 9]
+    assert len(up) == 1 and up[0].min() >= 0 and up[0].max() < 17
+    np.testing.assert_array_equal(up[0].reshape(3, 3)[[0, 0, 1, 2], [0, 1, 0, 0]], [1, 2, 3, 4])
