@@ -185,7 +185,7 @@ class SsmModel:
     def forward_backward(self, ids, targets, batch: int) -> float:
         """Mean cross-entropy of batch sequences (rows b*T ..), its gradients in grads()."""
         rows, d, V, N, W, R, X, L = len(ids), self.d, self.vocab, self.N, self.W, self.R, self.X, self.L
-        if rows % batch or len(targets) != rows:
+        if batch < 1 or rows < 1 or rows % batch or np.shape(ids) != (rows,) or np.shape(targets) != (rows,):
             raise ValueError("ids/targets must hold batch * seq tokens each")
         T = rows // batch
         nrm = self._forward(self._ids(ids), batch, True)
@@ -258,6 +258,8 @@ class SsmModel:
         Ids past a length may be anything."""
         ids = np.atleast_2d(np.asarray(ids))
         n, T = ids.shape
+        if n == 0 or T == 0:
+            raise ValueError(f"ids of shape {ids.shape} have no row to give logits of")
         st = self._states(states, n)
         dl = None
         if lens is None:
@@ -280,6 +282,8 @@ class SsmModel:
     def step(self, ids, states) -> np.ndarray:
         """One row for each sequence on its states, in place; (n_seq, V) logits."""
         ids = self._ids(np.atleast_1d(ids))
+        if ids.size == 0 or ids.size != len(ids):
+            raise ValueError(f"ids of shape {ids.shape}, expected one for each sequence")
         nrm = self._forward(ids, len(ids), False, self._states(states, len(ids)), one=True)
         self._head(nrm, len(ids))
         _lib.call("asca_sync")

@@ -105,3 +105,25 @@ def test_ids_past_a_prompts_length_do_not_matter(model):
     up = [a for n, a in log if n == "upload" and a.size == 9]
     assert len(up) == 1 and up[0].min() >= 0 and up[0].max() < 17
     np.testing.assert_array_equal(up[0].reshape(3, 3)[[0, 0, 1, 2], [0, 1, 0, 0]], [1, 2, 3, 4])
+
+
+def test_no_rows(model):
+    m, log = model
+    st = m.new_state(2)
+    refused(log, m.prompt, np.zeros((2, 0), int), st)         # there is no row to give logits of
+    refused(log, m.prompt, np.zeros((2, 0), int), st, [0, 0])
+    none = m.new_state(0)
+    refused(log, m.prompt, np.zeros((0, 4), int), none)
+    refused(log, m.step, [], none)
+    refused(log, m.step, np.zeros((2, 2), int), st)           # two ids for a sequence
+    for batch in (2, 0, -1):
+        refused(log, m.forward_backward, [], [], batch)
+    refused(log, m.forward_backward, np.zeros(4, int), np.zeros(4, int), 0)
+    refused(log, m.forward_backward, np.zeros(4, int), np.zeros(4, int), -2)
+
+
+def test_training_rows_lie_one_after_another(model):
+    m, log = model
+    refused(log, m.forward_backward, np.zeros((2, 5), int), np.zeros((2, 5), int), 2)   # two rows, by their length
+    m.forward_backward(np.zeros(10, int), np.zeros(10, int), 2)
+    assert "asca_ssm_bwd" in names(log)
