@@ -221,7 +221,7 @@ struct NormStats {
     float i1f, i2f;
     ASCA_DEV NormStats(const NormArgs& p, const double (&v)[8]) {
         const double in = 1.0 / p.cols;
-        i1 = 1.0 / sqrt(fma(v[0], in, (double)p.eps));
+        i1 = p.y ? 1.0 / sqrt(fma(v[0], in, (double)p.eps)) : 0.0;   // without y not of eps alone, which may be 0
         const double rq = fma(i1, v[3], v[2]);
         i2 = p.dn ? 1.0 / sqrt(fma(fma(i1, v[2] + rq, v[1]), in, (double)p.eps)) : 0.0;
         m2 = fma(i1, v[5], v[4]) * in * (i2 * i2);
@@ -537,6 +537,7 @@ int asca_block_norm_fwd(const void* x, long ldx, const void* y, long ldy, const 
                         int cols, float eps, int dtype, void* stream) {
     const char* fn = "asca_block_norm_fwd";
     if (rows < 0 || cols < 0) return fail(ASCA_ERR_INVALID, "%s: negative shape", fn);
+    if (!(eps >= 0.0f)) return fail(ASCA_ERR_INVALID, "%s: eps=%g", fn, (double)eps);
     int rc = act_dispatch(dtype, [](auto*) { return (int)ASCA_OK; });
     if (rc) return rc;
     if (!y && (z || w_post || scale)) return fail(ASCA_ERR_INVALID, "%s: z, w_post or scale without y", fn);
@@ -578,6 +579,7 @@ int asca_block_norm_bwd(const void* x, long ldx, const void* y, long ldy, const 
                         float* dw_pre, long rows, int cols, float eps, int dtype, void* stream) {
     const char* fn = "asca_block_norm_bwd";
     if (rows < 0 || cols < 0) return fail(ASCA_ERR_INVALID, "%s: negative shape", fn);
+    if (!(eps >= 0.0f)) return fail(ASCA_ERR_INVALID, "%s: eps=%g", fn, (double)eps);
     int rc = act_dispatch(dtype, [](auto*) { return (int)ASCA_OK; });
     if (rc) return rc;
     if (!y && (z || w_post || scale)) return fail(ASCA_ERR_INVALID, "%s: z, w_post or scale without y", fn);

@@ -577,7 +577,7 @@ ASCA_API int asca_ssm_step(float* h, const void* x, long ldx, const void* dt, lo
                            void* y, long ldy, int n, int D, int N, int G, int softplus, int dtype, void* stream);
 
 /* The norms around a block, with its gate and residual scale, per row (rms(a) =
- * a / sqrt(mean(a^2) + eps)):
+ * a / sqrt(mean(a^2) + eps), eps >= 0):
  *   u = y o silu(z);  r = x + scale o rms(u) o w_post;  n = rms(r) o w_pre
  *   x : the residual stream (NULL = zeros); y : the block's output; z : its gate
  *   (NULL = no gate); w_post, scale, w_pre : (cols), NULL = ones

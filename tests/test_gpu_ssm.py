@@ -306,6 +306,36 @@ def test_block_norm_of_zero_rows_is_zero(g):
     assert np.isfinite(o["dy"]).all() and (o["dx"] == 1).all()
 
 
+@pytest.mark.parametrize("rows,cols", [(7, 1), (9, 48), (3, 700), (5, 2048), (2, 2050), (3, 4099)])
+def test_block_norm_without_eps(g, rows, cols):
+    """eps = 0 is defined wherever a row is not all zeros, also where there is no y."""
+    rng = np.random.default_rng(cols)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    x, y, dr, dn, w = f(rows, cols) + 3, f(rows, cols) + 3, f(rows, cols), f(rows, cols), f(cols)
+    for y_, p in ((None, dict(w_pre=w)), (y, dict(w_pre=w, scale=f(cols)))):
+        got, ref = g.block_norm(x, y_, **p, eps=0.0), so.block_norm(x, y_, **p, eps=0.0)
+        gb, rb = g.block_norm_bwd(x, y_, None, dr, dn, **p, eps=0.0), so.block_norm_bwd(x, y_, None, dr, dn, **p, eps=0.0)
+        # a row of one column has no gradient: what is left is rounding of its terms, next to dr
+        size = lambda k: np.abs(dr).max() if cols == 1 and k in ("dx", "dy") else 0.0  # noqa: E731
+        check("norm eps=0", [("r", got[0], ref[0], FWD), ("n", got[1], ref[1], FWD)] +
+              [(k, np.append(gb[k], size(k)), np.append(rb[k], size(k)), GRAD) for k in gb if cols > 1 or k in ("dx", "dw_pre")])
+
+
+def test_block_norm_refuses_an_eps_below_zero(g):
+    from asca_amd import _lib, gpu
+
+    f = C.c_void_p(1 << 12)   # never dereferenced
+    gpu.reset_stats()
+    for eps in (-1e-6, float("-inf"), float("nan")):
+        for call in (("asca_block_norm_fwd", f, 8, f, 8, None, 0, None, None, None, f, 8, None, 0, 4, 8, eps, 0, None),
+                     ("asca_block_norm_bwd", f, 8, f, 8, None, 0, None, None, None, f, 8, None, 0, f, 8, None, 0, None, 0, None, None, None, 4, 8,
+                      eps, 0, None)):
+            with pytest.raises(_lib.AscaError) as ei:
+                _lib.call(*call)
+            assert ei.value.code == 1, str(ei.value)
+    assert gpu.stats()[2] == 0
+
+
 # ---------------------------------------------------------------- clipping
 
 
