@@ -332,6 +332,10 @@ class GradList:
         sizes = (C.c_uint64 * max(n, 1))(*[int(k) for _, k in src])
         if dst is not None and len(dst) != n:
             raise ValueError(f"{len(dst)} destinations for {n} tensors")
+        for i, (_, k) in enumerate(src):
+            for b in (src[i][0],) if dst is None else (src[i][0], dst[i]):
+                if isinstance(b, DevBuf) and b.nbytes < int(k) * (2 if dtype == BF16 else 4):
+                    raise ValueError(f"tensor {i}: {k} elements in a buffer of {b.nbytes} bytes")
         h = C.c_void_p()
         _lib.call("asca_grads_create", addr([b for b, _ in src]), addr(dst) if dst is not None else None, sizes, n, dtype,
                   C.byref(h))

@@ -1,0 +1,34 @@
+"""GradList's checks of its tensors before any device call.  CPU only: the library's
+calls and device buffers are replaced by recorders."""
+import pytest
+
+from asca_amd import gpu, model
+
+
+class Buf(gpu.DevBuf):
+    __slots__ = ()
+
+    def __init__(self, nbytes):
+        self.nbytes, self.ptr = int(nbytes), 1 << 20
+
+    def free(self):
+        pass
+
+
+@pytest.fixture
+def log(monkeypatch):
+    calls: list = []
+    monkeypatch.setattr(gpu, "DevBuf", Buf)
+    monkeypatch.setattr(gpu._lib, "call", lambda name, *a: calls.append(name))
+    return calls
+
+
+@pytest.mark.parametrize("dtype,size", [(gpu.F32, 4), (gpu.BF16, 2)])
+def test_a_buffer_smaller_than_its_tensor(log, dtype, size):
+    small, right = Buf(9 * size), Buf(10 * size)
+    for src, dst in (([(small, 10)], None), ([(right, 10), (small, 10)], None), ([(right, 10)], [small])):
+        with pytest.raises(ValueError):
+            gpu.GradList(src, dst, dtype=dtype)
+    assert not log
+    gpu.GradList([(right, 10), (small, 9), (1 << 20, 10)], [right, small, right], dtype=dtype)
+    assert log == ["asca_grads_create"]
