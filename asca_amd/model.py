@@ -135,6 +135,8 @@ class DeviceModel:
         """Scale every gradient by min(1, max_norm / (norm + 1e-6)), norm the 2-norm
         over all of them (asca_grads_clip), between forward_backward and adamw:
         (norm, factor), or None without sync."""
+        if not self._h:
+            raise RuntimeError("the model is closed")
         if self._grad_list is None:
             self._grad_list = GradList([(self._ptr["grads"] + 4 * off, r * c) for _, off, r, c in self.tensors])
         return self._grad_list.clip(max_norm, sync, stream)

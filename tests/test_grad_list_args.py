@@ -32,3 +32,14 @@ def test_a_buffer_smaller_than_its_tensor(log, dtype, size):
     assert not log
     gpu.GradList([(right, 10), (small, 9), (1 << 20, 10)], [right, small, right], dtype=dtype)
     assert log == ["asca_grads_create"]
+
+
+def test_clipping_a_closed_model(log):
+    m = model.DeviceModel.__new__(model.DeviceModel)
+    m._h, m._grad_list, m._ptr, m.tensors, m._bufs = 1, None, {"grads": 1 << 20}, [("w", 0, 3, 4)], {}
+    m.clip_grads(1.0, sync=False)
+    m.close()
+    del log[:]
+    with pytest.raises(RuntimeError):   # its gradients' memory is freed
+        m.clip_grads(1.0, sync=False)
+    assert not log
