@@ -43,6 +43,9 @@ int fail(int code, const char* fmt, ...) {
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
     t_err = buf;
+    // a HIP call's error that is reported here is taken from HIP's own record, where the
+    // next launch would find it and be blamed for it
+    if (code == ASCA_ERR_OOM || code == ASCA_ERR_HIP) (void)hipGetLastError();
     return code;
 }
 
