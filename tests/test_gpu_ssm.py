@@ -264,6 +264,37 @@ def test_ssm_step_goes_on_from_a_prompt(g, n, D, N, G, bf16):
     check("ssm step", [("h", h.to_host((n, N, D)), rh, FWD)])
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n,D,N,G", [(300, 2048, 12, 2), (260, 2050, 16, 1), (600, 1000, 33, 1), (530, 990, 8, 3), (524288, 1, 20, 1)])
+def test_ssm_step_of_many_sequences(g, n, D, N, G, bf16):
+    """From 2^19 channels on (of all sequences) a channel's states are loaded 8 at a time."""
+    from asca_amd.gpu import DevBuf
+
+    print(f"[ssm step] n={n} D={D} N={N} G={G} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(n + D + N)
+    r = Rows(rng, bf16)
+    i = ssm_inputs(r, rng, n, 1, D, N, G)
+    h0 = rng.standard_normal((n, N, D), dtype=np.float32)
+    v = {k: r.val(a).astype(np.float64) for k, a in i.items()}
+    e = np.logaddexp(v["dt"] + v["dt_bias"], 0)
+    wide = lambda m: np.repeat(m.reshape(n, G, N).transpose(0, 2, 1), D // G, axis=2)  # noqa: E731
+    rh = np.exp(e[:, None] * v["A"]) * h0 + (e * v["x"])[:, None] * wide(v["Bm"])
+    ry = (rh * wide(v["Cm"])).sum(1) + v["Dk"] * v["x"]
+    h = DevBuf.from_host(h0)
+    y = g.ssm_step(h, i["x"], i["dt"], i["A"], i["Bm"], i["Cm"], dt_bias=i["dt_bias"], Dk=i["Dk"], groups=G)
+    check("ssm step", [("y", r.val(y), ry, r.tol(FWD)), ("h", h.to_host((n, N, D)), rh, FWD)])
+
+
+@pytest.mark.parametrize("v", [-85.0, -60.0, -40.0])
+def test_ssm_softplus_of_small_steps(g, v):
+    """As above down to the smallest normal e, by itself: exp2 of v log2(e), whose argument
+    is rounded twice (of at most 123, to 2^-17 together, or 2^-17 ln 2 of e)."""
+    one = np.ones((1, 1), np.float32)
+    y, _, _ = g.ssm_scan(one, one * np.float32(v), -one, one, one, batch=1, keep=False)
+    e = np.logaddexp(np.float64(v), 0)
+    assert abs(y[0, 0] - e) <= 2.0 ** -17 * e
+
+
 # -------------------------------------------------------------- block norm
 
 
