@@ -337,6 +337,54 @@ def test_block_norm_of_zero_rows_is_zero(g):
     assert np.isfinite(o["dy"]).all() and (o["dx"] == 1).all()
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,cols", [(2300, 132), (2101, 301), (2050, 500), (1100, 700), (1030, 1024), (600, 2048), (530, 1500), (520, 2052), (515, 2053),
+                                       (3, 2049), (3, 3000), (2, 4096), (2, 4095)])
+def test_block_norm_of_many_rows_and_of_wide_ones(g, rows, cols, bf16):
+    """Backwards whose blocks go over several rows (the next row's loads, the parameters'
+    sums over rows, wide rows' sums in memory), forwards of 2049 to 4096 columns."""
+    print(f"[norm] rows={rows} cols={cols} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(rows + cols)
+    r = Rows(rng, bf16)
+    x, y, z, dr, dn = (r(rows, cols) for _ in range(5))
+    p = {k: (rng.standard_normal(cols) * 0.3 + 1).astype(np.float32) for k in ("w_post", "scale", "w_pre")}
+    v = r.val
+    got, ref = g.block_norm(x, y, z, **p), so.block_norm(v(x), v(y), v(z), **p)
+    gb, rb = g.block_norm_bwd(x, y, z, dr, dn, **p), so.block_norm_bwd(v(x), v(y), v(z), v(dr), v(dn), **p)
+    check("norm", [("r", v(got[0]), ref[0], r.tol(FWD)), ("n", v(got[1]), ref[1], r.tol(FWD))] +
+          [(k, v(gb[k]), rb[k], r.tol(GRAD) if k in ("dx", "dy", "dz") else GRAD) for k in gb])
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,cols", [(2300, 132), (1100, 700), (600, 1501), (520, 2052), (3, 4100), (2, 4099)])
+def test_block_norm_in_place(g, rows, cols, bf16):
+    """r over x, and dx over dr, give the bits of the calls beside them."""
+    from asca_amd import _lib, gpu
+
+    rng = np.random.default_rng(rows + cols)
+    r = Rows(rng, bf16)
+    ty = int(bf16)
+    x, y, z, dr, dn = (r(rows, cols) for _ in range(5))
+    b = {k: gpu.DevBuf.from_array(a) for k, a in dict(x=x, y=y, z=z, dr=dr, dn=dn).items()}
+    o = {k: gpu.DevBuf(x.nbytes) for k in ("r", "n", "n2", "dx", "dy", "dy2", "dz", "dz2")}
+    w = {k: gpu.DevBuf.from_host((rng.standard_normal(cols) * 0.3 + 1).astype(np.float32)) for k in ("w1", "s", "w2")}
+    dw = {k: gpu.DevBuf(cols * 4) for k in ("w1", "s", "w2", "w1_", "s_", "w2_")}
+    ins = lambda: (_p(b["x"]), cols, _p(b["y"]), cols, _p(b["z"]), cols, _p(w["w1"]), _p(w["s"]), _p(w["w2"]))  # noqa: E731
+    bwd = lambda dx, dy, dz, e: _lib.call("asca_block_norm_bwd", *ins(), _p(b["dr"]), cols, _p(b["dn"]), cols, _p(dx), cols, _p(o[dy]), cols,  # noqa: E731
+                                          _p(o[dz]), cols, _p(dw["w1" + e]), _p(dw["s" + e]), _p(dw["w2" + e]), rows, cols, 1e-6, ty, None)
+    fwd = lambda res, n: _lib.call("asca_block_norm_fwd", *ins(), _p(res), cols, _p(o[n]), cols, rows, cols, 1e-6, ty, None)  # noqa: E731
+    bwd(o["dx"], "dy", "dz", "")
+    bwd(b["dr"], "dy2", "dz2", "_")
+    fwd(o["r"], "n")
+    fwd(b["x"], "n2")
+    _lib.call("asca_sync")
+    get = lambda q, like: q.to_host(like.shape, like.dtype)  # noqa: E731
+    for a, c in ((o["dx"], b["dr"]), (o["dy"], o["dy2"]), (o["dz"], o["dz2"]), (o["r"], b["x"]), (o["n"], o["n2"])):
+        np.testing.assert_array_equal(get(a, x), get(c, x))
+    for k in ("w1", "s", "w2"):
+        np.testing.assert_array_equal(dw[k].to_host((cols,)), dw[k + "_"].to_host((cols,)))
+
+
 @pytest.mark.parametrize("rows,cols", [(7, 1), (9, 48), (3, 700), (5, 2048), (2, 2050), (3, 4099)])
 def test_block_norm_without_eps(g, rows, cols):
     """eps = 0 is defined wherever a row is not all zeros, also where there is no y."""
