@@ -791,6 +791,46 @@ def test_captured_calls_replay_the_eager_results(g):
     _lib.call("asca_grads_destroy", gl)
 
 
+@pytest.mark.parametrize("T,D,N", [(1700, 24, 16), (1700, 24, 20), (4096, 8, 40)])
+def test_a_captured_scan_in_chunks_replays_the_eager_results(g, T, D, N):
+    """Both passes of a forward that is cut into chunks, with the scratch between them, and
+    its backward."""
+    from asca_amd import _lib
+
+    hip = C.CDLL("libamdhip64.so.7")
+
+    def ok(rc):
+        assert rc == 0, rc
+
+    rng = np.random.default_rng(16)
+    r = Rows(rng, False)
+    i, dy = ssm_inputs(r, rng, 1, T, D, N, 1), r(T, D)
+    run, o, keep = _ssm_call(g, i, 1, T, D, N, dy)
+    get = lambda: {k: b.to_host((b.nbytes // 4,)) for k, b in o.items()}  # noqa: E731
+    run(None)
+    _lib.call("asca_sync")
+    want = get()
+    sp, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    _lib.call("asca_stream_create", C.byref(sp))
+    ok(hip.hipStreamBeginCapture(sp, 0))
+    run(sp)
+    ok(hip.hipStreamEndCapture(sp, C.byref(graph)))
+    ok(hip.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)))
+    for k in range(4):
+        for b in o.values():
+            _lib.call("asca_memset32", _p(b), 0, b.nbytes // 4, None)
+        _lib.call("asca_sync")
+        ok(hip.hipGraphLaunch(exe, sp))
+        _lib.call("asca_stream_sync", sp)
+        got = get()
+        for name in want:
+            np.testing.assert_array_equal(got[name], want[name], err_msg=f"replay {k}: {name}")
+        g.ssm_scan(**i, batch=1, keep=False)   # the program's own work between
+    ok(hip.hipGraphExecDestroy(exe))
+    ok(hip.hipGraphDestroy(graph))
+    _lib.call("asca_stream_destroy", sp)
+
+
 @pytest.mark.parametrize("bad", [np.inf, np.nan])
 @pytest.mark.parametrize("B,T,D,N", [(1, 70, 40, 16), (1, 70, 40, 6), (8, 40, 2048, 16), (1, 1100, 512, 12), (1, 1700, 24, 12), (5, 80, 512, 16)])
 def test_an_infinity_or_nan_stays_with_what_it_reaches(g, bad, B, T, D, N):
