@@ -261,10 +261,10 @@ static int conv_dispatch(int dtype, int W, bool vec, F f) {
     });
 }
 
-// One block for `ch` channels of `units` units each
-static int conv_grid(const char* fn, long units, int D, int ch, dim3* grid) {
+// One block of `threads` for `ch` channels of `units` units each
+static int conv_grid(const char* fn, long units, int D, int ch, int threads, dim3* grid) {
     const long n = units * ((D + ch - 1) / ch);
-    if (n > 0x7fffffffL) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows or channels", fn);
+    if (!grid_fits(n, threads)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows or channels", fn);
     *grid = dim3((unsigned)n);
     return ASCA_OK;
 }
@@ -286,7 +286,7 @@ int asca_conv_fwd(const void* x, long ldx, const float* w, const float* bias, co
     p.B = B, p.T = T, p.D = D, p.runs = T > 0 ? (T + CV_R - 1) / CV_R : 1, p.silu = silu;
     dim3 grid;
     const bool vec = D % 4 == 0 && act_vec_ok(x, ldx, dtype) && act_vec_ok(y, ldy, dtype);
-    if ((rc = conv_grid(fn, ((long)B * p.runs + CV_NW - 1) / CV_NW, D, vec ? 256 : 64, &grid))) return rc;
+    if ((rc = conv_grid(fn, ((long)B * p.runs + CV_NW - 1) / CV_NW, D, vec ? 256 : 64, 64 * CV_NW, &grid))) return rc;
     return conv_dispatch(dtype, W, vec, [&](auto* e, auto taps, auto v) {
         using E = std::remove_pointer_t<decltype(e)>;
         int r = pre_launch("conv_fwd");
@@ -316,7 +316,7 @@ int asca_conv_bwd(const void* x, long ldx, const float* w, const float* bias, co
     dim3 grid;
     const long parts = ((long)B * p.runs + CV_NW - 1) / CV_NW;
     const bool vec = D % 4 == 0 && act_vec_ok(x, ldx, dtype) && act_vec_ok(dy, lddy, dtype) && act_vec_ok(dx, lddx, dtype);
-    if ((rc = conv_grid(fn, parts, D, vec ? 256 : 64, &grid))) return rc;
+    if ((rc = conv_grid(fn, parts, D, vec ? 256 : 64, 64 * CV_NW, &grid))) return rc;
     StreamScratch sc;
     if ((rc = sc.get((size_t)parts * (W + 1) * D, st))) return rc;
     p.part = sc.ws.p;
@@ -340,7 +340,7 @@ int asca_conv_step(float* state, const void* x, long ldx, const float* w, const 
     if (n == 0 || D == 0) return ASCA_OK;
     if (!state || !x || !w || !y) return fail(ASCA_ERR_INVALID, "null pointer in %s", fn);
     dim3 grid;
-    if ((rc = conv_grid(fn, n, D, 256, &grid))) return rc;
+    if ((rc = conv_grid(fn, n, D, 256, 256, &grid))) return rc;
     if ((rc = conv_ld(fn, "ldx", ldx, D)) || (rc = conv_ld(fn, "ldy", ldy, D))) return rc;
     ConvArgs p{};
     p.x = x, p.ldx = ldx, p.w = w, p.bias = bias, p.y = y, p.ldy = ldy, p.D = D, p.silu = silu;

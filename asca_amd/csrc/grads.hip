@@ -180,7 +180,7 @@ int asca_grads_create(void** src, void** dst, const uint64_t* sizes, int count, 
                 char* s = static_cast<char*>(src[i]) + o * size;
                 t.push_back({s, dst ? static_cast<char*>(dst[i]) + o * size : s, (long)std::min<uint64_t>(per, sizes[i] - o)});
             }
-        if (t.size() > 0x7fffffffu) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many tensors", fn);
+        if (!grid_fits((long)t.size(), 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many tensors", fn);
         g = new GradList;
         g->n = (unsigned)t.size();
         g->dtype = dtype;

@@ -558,10 +558,10 @@ int asca_block_norm_fwd(const void* x, long ldx, const void* y, long ldy, const 
     p.r = r, p.n = n, p.ldr = ldr, p.ldn = ldn, p.rows = rows, p.cols = cols, p.eps = eps;
     const int rpb = cols <= 512 ? 4 : 1;
     const long blocks = (rows + rpb - 1) / rpb;
-    if (blocks > 0x7fffffffL) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows", fn);
     return bn_dispatch<false>(dtype, cols, vec, [&](auto* e, auto v, auto nv, auto wpr) {
         using E = std::remove_pointer_t<decltype(e)>;
         constexpr int V = decltype(v)::value, NV = decltype(nv)::value, WPR = decltype(wpr)::value;
+        if (!grid_fits(blocks, NV ? bn_threads<WPR>() : BW_NT)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows", fn);
         int q = pre_launch("block_norm_fwd");
         if (q) return q;
         const hipStream_t st = as_stream(stream);

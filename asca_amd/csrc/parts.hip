@@ -41,9 +41,11 @@ __global__ __launch_bounds__(64 * PW) void sum_parts_k(const float* __restrict__
 int sum_parts_launch(const float* part, long parts, const PartsOut& o, hipStream_t st) {
     const long row = o.n[0] + o.n[1] + o.n[2];
     if (row == 0) return ASCA_OK;
+    const long blocks = (row + 63) / 64;
+    if (!grid_fits(blocks, 64 * PW)) return fail(ASCA_ERR_UNSUPPORTED, "sums of %ld values", row);
     int rc = pre_launch("sum_parts");
     if (rc) return rc;
-    hipLaunchKernelGGL(sum_parts_k, dim3((unsigned)((row + 63) / 64)), dim3(64 * PW), 0, st, part, parts, row, o);
+    hipLaunchKernelGGL(sum_parts_k, dim3((unsigned)blocks), dim3(64 * PW), 0, st, part, parts, row, o);
     return post_launch("sum_parts");
 }
 

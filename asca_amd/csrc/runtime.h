@@ -19,6 +19,9 @@ int ensure_device();
 // injection set by asca_fail_after() / ASCA_FAIL_LAUNCH.
 int pre_launch(const char* kernel);
 
+// Whether a launch takes so many blocks (HIP: fewer than 2^32 threads in a dimension).
+inline bool grid_fits(long blocks, long threads) { return blocks < (1L << 32) / threads; }
+
 // Map the HIP status of the launch just made to an error code.
 int post_launch(const char* kernel);
 

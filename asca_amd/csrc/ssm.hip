@@ -1143,7 +1143,7 @@ int asca_ssm_fwd(const void* x, long ldx, const void* dt, long lddt, const float
     }
     form = ssm_form(p, N, false, 1024, 4096);
     const long blocks = (long)B * p.nch * G * p.tiles;
-    if (blocks > 0x7fffffffL) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many channels", fn);
+    if (!grid_fits(blocks, 64 * form.NW)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many channels", fn);
     StreamScratch sc;
     if ((rc = sc.get(ssm_chunk_floats(p), st))) return rc;
     p.cs = sc.ws.p, p.ce = p.cs + (size_t)B * p.nch * N * D;
@@ -1191,7 +1191,7 @@ int asca_ssm_bwd(const void* x, long ldx, const void* dt, long lddt, const float
     p.B = B;
     const SsmForm form = ssm_form(p, N, true, 2048, 2048);
     const long blocks = (long)B * p.nch * G * p.tiles, rows = (long)B * T, parts = (long)B * p.nch, per = rows * G * 2 * N, nd = (long)N * D;
-    if (blocks > 0x7fffffffL || (per + 255) / 256 > 0x7fffffffL)
+    if (!grid_fits(blocks, 64 * form.NW) || !grid_fits((per + 255) / 256, 256))
         return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows or channels", fn);
     StreamScratch sc;
     if ((rc = sc.get((size_t)parts * (nd + 2 * D) + (size_t)p.tiles * per + ssm_chunk_floats(p), st))) return rc;
@@ -1230,7 +1230,7 @@ int asca_ssm_step(float* h, const void* x, long ldx, const void* dt, long lddt, 
     if (n == 0 || D == 0) return ASCA_OK;
     if (!h || !x || !dt || !A || !Bm || !Cm || !y) return fail(ASCA_ERR_INVALID, "null pointer in %s", fn);
     const long blocks = (long)n * ((D + 255) / 256);
-    if (blocks > 0x7fffffffL) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many channels", fn);
+    if (!grid_fits(blocks, 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many channels", fn);
     if ((rc = ssm_ld(fn, "ldx", ldx, D)) || (rc = ssm_ld(fn, "lddt", lddt, D)) || (rc = ssm_ld(fn, "ldy", ldy, D)) ||
         (rc = ssm_ld(fn, "ldb", ldb, (long)G * N)) || (rc = ssm_ld(fn, "ldc", ldc, (long)G * N)))
         return rc;

@@ -515,9 +515,11 @@ ASCA_API int asca_model_decode_step(asca_model* model, const uint32_t* ids, int 
  *     each matrix with its own row stride `ld*` in elements, so that they can be
  *     columns of a wider one.  Parameters, states and the gradients of both are
  *     f32.  All arithmetic is f32; a bf16 result is rounded once, at its store.
- *   - T is at most 2^30.  lens (device int32, one per sequence, NULL = all T):
- *     sequence b has min(max(lens[b], 0), T) rows.  What its further rows hold
- *     does not matter; their outputs and gradients are zero.
+ *   - T is at most 2^30, and a call that would take 2^32 threads or more in one
+ *     launch is refused (ASCA_ERR_UNSUPPORTED).
+ *   - lens (device int32, one per sequence, NULL = all T): sequence b has
+ *     min(max(lens[b], 0), T) rows.  What its further rows hold does not matter;
+ *     their outputs and gradients are zero.
  *   - Inputs and outputs must not overlap unless stated.  Results are
  *     deterministic (no atomics).
  *   - What a call needs for itself comes from the scratch that the library keeps

@@ -689,6 +689,28 @@ def test_refusals(g):
         g.block_norm(None)
 
 
+def test_calls_of_more_threads_than_a_launch_takes_are_refused(g):
+    """HIP takes fewer than 2^32 threads in a launch; nothing is launched of a larger call."""
+    from asca_amd import _lib, gpu
+
+    f, k = C.c_void_p(1 << 12), 1 << 24   # the pointer is never dereferenced
+    bad = [("asca_conv_fwd", f, 4096, f, None, None, None, f, 4096, None, 1, 1 << 30, 4096, 4, 1, 0, None),
+           ("asca_conv_bwd", f, 4096, f, None, None, None, f, 4096, None, f, 4096, f, None, None, 1, 1 << 30, 4096, 4, 1, 0, None),
+           ("asca_conv_step", f, f, 256, f, None, f, 256, k, 256, 4, 1, 0, None),
+           ("asca_ssm_fwd", f, 128, f, 128, None, f, f, 8, f, 8, None, None, None, f, 128, None, None, k, 1, 128, 8, 1, 1, 0, None),
+           ("asca_ssm_bwd", f, 128, f, 128, None, f, f, 8, f, 8, None, None, f, 128, None, f, f, 128, f, 128, None, f, f, 8, f, 8, None, None,
+            k, 1, 128, 8, 1, 1, 0, None),
+           ("asca_ssm_step", f, f, 256, f, 256, None, f, f, 8, f, 8, None, f, 256, k, 256, 8, 1, 1, 0, None)]
+    bad += [("asca_block_norm_fwd", f, c, None, 0, None, 0, None, None, None, None, 0, f, c, rows, c, 1e-6, 0, None)
+            for c, rows in ((8, 4 * k), (520, 2 * k), (1030, k), (5000, k // 2))]
+    gpu.reset_stats()
+    for name, *args in bad:
+        with pytest.raises(_lib.AscaError) as ei:
+            _lib.call(name, *args)
+        assert ei.value.code == 3, (name, str(ei.value))
+    assert gpu.stats()[2] == 0
+
+
 @pytest.mark.parametrize("nth", [0, 1, 2])
 def test_an_injected_failure_is_an_error_and_the_next_call_works(g, nth):
     from asca_amd import _lib, gpu
