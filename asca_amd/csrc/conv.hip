@@ -5,10 +5,12 @@
 // A thread has V neighbouring channels and a run of CV_R rows: all of a run's rows
 // (and the W - 1 beside it, which a neighbour reads too) are loaded at once, then
 // each is used W times from registers.  The backward forms g again for the W - 1
-// rows after its run.  Bound by memory: 16 x 1024 x 512 f32, W = 4, forward 13.5 us
-// (5.0 TB/s), backward 22.8 us (4.4 TB/s); 8 x 4096 x 2048 bf16 53 us (5.1) and 111 us
-// (3.6: two bytes a value, and taps and sigmoid formed 11 times for 8 rows, fill part
-// of the vector unit's time too).
+// rows after its run.  Bound by memory: 16 x 1024 x 512 f32, W = 4, forward 13.1 us
+// (5.1 TB/s), backward 22.1 us (4.6 TB/s); 8 x 4096 x 2048 bf16 53 us (5.1) and 106 us
+// (3.8: two bytes a value, and taps and sigmoid formed 11 times for 8 rows, fill part
+// of the vector unit's time too).  Where four channels cannot be loaded together (a width
+// or stride that is not a multiple of four, an offset) V is 1: 8 x 4096 x 2047 bf16 82 and
+// 219 us, 16 x 1024 x 511 f32 15.8 and 29 (512: 12.9 and 25.5, with the sums' launch).
 #include "act.h"
 #include "parts.h"
 
@@ -206,8 +208,8 @@ __global__ __launch_bounds__(64 * CV_NW) void conv_bwd_k(ConvArgs p) {
     }
 }
 
-// One row for each sequence, a thread a channel of one.  512 x 2048 bf16, W = 4: 6.6 us,
-// its state's 25 MB at 4.5 TB/s with the rows; 1 x 512 is a launch and a load (1.9 us).
+// One row for each sequence, a thread a channel of one.  512 x 2048 bf16, W = 4: 6.3 us,
+// its state's 25 MB at 4.7 TB/s with the rows; 1 x 512 is a launch and a load (1.7 us).
 template <typename E, int W>
 __global__ __launch_bounds__(256) void conv_step_k(float* __restrict__ state, ConvArgs p) {
     const unsigned cb = (p.D + 255) / 256;

@@ -9,6 +9,8 @@
 // cache with its writes) and read and written in 206 us (5.5 TB/s, the part that the
 // cache still holds coming first).  Stores past the caches leave more of the list there,
 // which the next call on it sees (321 -> 294 us) but not an update between (890 us both).
+// The chunks' sums are added by every block, so the time grows with the square of the
+// tensors where these are thousands: 1000 of 256 elements 7 us, 3000 12, 10000 61, 30000 415.
 #include <algorithm>
 #include <vector>
 

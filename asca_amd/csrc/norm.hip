@@ -10,7 +10,9 @@
 // and each result written once, in either direction; what the backward needs of
 // the forward it computes again from x, y and z.  Bound by memory: 16384 x 512 f32
 // forward 26 us, backward 47 us (6.5 and 5.7 TB/s, some of it from the last-level
-// cache), 16384 x 2048 bf16 71 and 125 us (4.7 and 4.3 TB/s).
+// cache), 16384 x 2048 bf16 71 and 116 us (4.7 and 4.6 TB/s).  Rows that cannot be loaded
+// four values at a time are loaded one at a time: 16384 x 2047 bf16 85 and 207 us (2048,
+// with the sums' launch too: 71 and 128), 16384 x 511 f32 28 and 57 (26 and 51).
 #include <algorithm>
 
 #include "act.h"

@@ -297,8 +297,8 @@ ASCA_DEV void store_esum(const SsmArgs& p, const SsmPlace<Q, CB>& l, float esum,
 
 // OUT: the rows' y from the state that enters the chunk; otherwise what a chunk
 // makes of a zero state, and the sum of its e.  Lane = CH q + c.  Bound by the vector
-// unit's issue: 8 x 4096 x 2048 bf16, N = 16, 388 us; 1 x 16384 x 1024 bf16 in 32
-// chunks 69 and 93 us.
+// unit's issue: 8 x 4096 x 2048 bf16, N = 16, 387 us; 1 x 16384 x 1024 bf16 in 32
+// chunks 62 and 84 us.
 template <typename E, int NS, int Q, int NW, bool OUT>
 __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
     constexpr int K = ssm_k(NS), R = K / Q, CB = SSM_CB<Q, NW>, CH = 64 / Q;
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_k(SsmArgs p) {
 // Blocks are laid out so that neighbouring channels, which share lines of x, dt and y, run
 // on one XCD.  Bound by the vector unit's issue, and
 // by waiting for the block's other waves where it has a CU to itself: 16 x 1024 x 512 f32,
-// N = 16, 60 us; 1 x 4096 x 2048 bf16 65 us; 1 x 512 x 512 8.2 us, two rounds.
+// N = 16, 60 us; 1 x 4096 x 2048 bf16 64 us; 1 x 512 x 512 8.5 us, two rounds.
 template <typename E, int NS, int Q, int NW>
 __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
     constexpr int CH = 64 / Q, K = ssm_k(NS), R = K / Q, V = K * Q * NS, RB = 2 * V / 64;
@@ -609,7 +609,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_split_k(SsmArgs p) {
 }
 
 // What a chunk makes of a zero carry, from its end to its start, and the sum of its e.
-// Lane = CH q + c.  2 x 2048 x 1024 bf16, N = 16, in 8 chunks 23 us (and 66 us behind it
+// Lane = CH q + c.  2 x 2048 x 1024 bf16, N = 16, in 8 chunks 22 us (and 60 us behind it
 // in the backward proper).
 template <typename E, int NS, int Q, int NW>
 __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_carry_k(SsmArgs p) {
 
 // Lane = Q c + q: sums over channels (2 NS a row) by row swaps, over states (2 a row) by
 // DPP.  Bound by the vector unit's issue (85% of its cycles): 8 x 4096 x 2048 bf16, N =
-// 16, 855 us.
+// 16, 857 us.
 template <typename E, int NS, int Q, int NW>
 __global__ __launch_bounds__(64 * NW) void ssm_bwd_k(SsmArgs p) {
     constexpr int K = ssm_k(NS), R = K / Q, CB = SSM_CB<Q, NW>, CH = 64 / Q;
@@ -985,7 +985,10 @@ __global__ __launch_bounds__(256) void ssm_step_k(float* __restrict__ h, SsmArgs
 
 using namespace asca;
 
-static int ssm_ns(int N) { return N <= 8 ? 1 : N <= 16 ? 2 : N <= 32 ? 4 : 8; }   // states a lane on 8 groups
+// States a lane on 8 groups.  Those that do not exist are computed with the others: N = 4
+// takes what 8 does, 12 what 16 and 24 what 32 (8 x 1024 x 2048 f32, forward and backward:
+// 253 and 255 us, 325 and 328, 567 and 601).
+static int ssm_ns(int N) { return N <= 8 ? 1 : N <= 16 ? 2 : N <= 32 ? 4 : 8; }
 
 static int ssm_check(const char* fn, int B, int T, int D, int N, int G) {
     if (B < 0 || T < 0 || D < 0) return fail(ASCA_ERR_INVALID, "%s: negative shape B=%d T=%d D=%d", fn, B, T, D);
@@ -1008,21 +1011,24 @@ struct SsmForm {
 // through a tile's states twice and the waves wait for each other every NW tiles, but
 // fills the chip with 8 (4) channels a block and reads the rows once.  Against
 // ssm_fwd_k:
-//   - not where that has two waves a SIMD by itself (32 x 512 x 512: 48 against 54 us,
-//     8 x 2048 x 2048 155 against 203).
-//   - below, 4 waves a block fill it (bf16, N = 16: 1 x 2048 x 12288 163 -> 154 us, x 8192
-//     128 -> 114, 1 x 4096 x 4096 142 -> 120), 8 where that takes a block for every CU (1 x
-//     4096 x 2048 77 -> 65 us; 102 with 4).
+//   - not where that has two waves a SIMD by itself (with states in and out, 32 x 512 x 512
+//     f32: 55 us against 65, 8 x 2048 x 2048 bf16 189 against 211).
+//   - below, 4 waves a block fill it (bf16, N = 16: 1 x 2048 x 12288 189 -> 154 us, x 8192
+//     153 -> 112, 1 x 4096 x 4096 145 -> 122), 8 where that takes a block for every CU (1 x
+//     4096 x 2048 78 -> 64 us; 98 with 4).  Just past that, rows cut into chunks are ahead
+//     where they are many: 1 x 4096 x 2080, in 260 blocks, takes 120 us (with 8 waves 124;
+//     cut 86), x 2560 121 (125; 101), x 3584 122 (125; 130), 1 x 1000 x 2080 33 (36; 32), x
+//     4032 35 (36; 44).
 //   - 16 groups of one state, 16 waves a block, where 8 groups leave half of the CUs
-//     without (1 x 2048 x 1024 30 -> 23.6 us, 8 groups 33.5; 1 x 512 x 512 14.5 -> 8.4),
-//     with 8 waves for short sequences (128 rows: 12.5 -> 5.5 us, 6.3 with 16).
+//     without (1 x 2048 x 1024 30 -> 23.4 us, 8 groups 29.3; 1 x 512 x 512 16 -> 8.5, 8
+//     groups 10.5), with 8 waves for short sequences (128 rows: 14.8 -> 5.8 us, 7.0 with 16).
 //   - where blocks are few and rows many, rows cut into chunks fill more of the chip (1 x
-//     16384 x 1024 146 us, split 154; 1 x 4096 x 512 36 and 41); at 1 x 2048 x 512 (128
-//     blocks) and 1 x 8192 x 1024 (256) both take the same.  N of 17 to 32, 4 states a
-//     lane: from a quarter of the rows on (1 x 128 x 512 14 -> 7.8 us, 1 x 2048 x 8192 238
-//     -> 205; 1 x 2048 x 1024 45, split 66).
+//     16384 x 1024 146 us, split 160; 1 x 4096 x 512 36 and 41); 1 x 2048 x 512 (128
+//     blocks) takes 21 and 23, 1 x 8192 x 1024 (256) 82 and 87.  N of 17 to 32, 4 states a
+//     lane: from a quarter of the rows on (1 x 128 x 512 14.7 -> 7.7 us, 1 x 2048 x 8192 245
+//     -> 208; 1 x 2048 x 1024 43, split 66).
 //   - N above 32 only for few and short rows: a wave has its SIMD to itself (1 x 64 x 2048,
-//     N = 64: 20 -> 10 us; 1 x 512 x 512 32, split 44).
+//     N = 64: 20 -> 10 us; 1 x 512 x 512 35, split 46).
 static bool ssm_split(SsmArgs& p, int N, SsmForm* f) {
     const long w8 = (long)p.B * p.G * ((p.Dg + 7) / 8);
     if (w8 >= 2048) return false;
@@ -1040,14 +1046,15 @@ static bool ssm_split(SsmArgs& p, int N, SsmForm* f) {
 
 // Otherwise p.nch chunks a sequence.
 //   - 16 groups (N of 9 to 16) give the backward twice the waves for a sixth more
-//     instructions: where 8 groups give fewer than a wave a SIMD and 16 a block a CU at
-//     most (16 x 1024 x 512 160 -> 145 us, 12 x 1024 x 512 156 -> 142; 24 x 1024 x 512, in
-//     384 blocks, 225 -> 277), or where few waves cannot be cut enough (1 x 512 x 512 28
-//     -> 26 us).
+//     instructions: where 8 groups give about a wave a SIMD and 16 a block a CU at most
+//     (16 x 1024 x 512 161 -> 146 us, 12 x 1024 x 512 158 -> 144; 24 x 1024 x 512, in 384
+//     blocks, 225 -> 277), or where few waves cannot be cut enough (1 x 512 x 512 28 -> 26
+//     us).  Of fewer waves 8 groups have three chunks or more, which are ahead (10 x 1024 x
+//     512 112 us, 16 groups 143; 6 x 75 and 106; at 11 x, two chunks, 157 and 143).
 //   - a cut costs a second pass over the rows, so it pays only for waves that are
 //     missing: below `enough`, as many chunks as give `want` (forward: 2 x 2048 x 1024, N =
-//     32, in 256 waves 237 us, cut to 4096 74; 32 x 512 x 512 in 2048 waves 46 us, cut to
-//     4096 75; backward: 2 x 2048 x 1024 cut to 1024 142 us, to 2048 100).
+//     32, in 256 waves 244 us, cut to 4096 72; 32 x 512 x 512 in 2048 waves 55 us, cut to
+//     4096 82; backward: 2 x 2048 x 1024 cut to 1024 142 us, to 2048 100).
 //   - the backward has 8 waves a block, which halves its partial sums of dB and dC (8 x
 //     4096 x 2048 904 -> 888 us), where that leaves a block for every CU (2 x 2048 x
 //     1024 without: 89.8 -> 90.8 us).

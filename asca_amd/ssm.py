@@ -6,7 +6,8 @@ A layer, with x the residual stream (rows of d) and nrm its normalised rows:
   o = scan(c, dt, A, B, C) w_o
   x' = x + scale o (rms(o o silu(z)) o w_post);  nrm' = rms(x') o w_pre'
 The residual's update and both norms are one call (asca_block_norm_fwd); u, z and
-r, B, C are columns of one product each.  Everything is f32.
+r, B, C are columns of one product each.  Everything is f32, B and C are one group.
+The embedding stays as it is set: no gradient of it is formed (unlike DeviceModel's).
 
 It trains (forward_backward, clip, adamw), reads prompts of different lengths
 (prompt) and decodes one row for many sequences on their states (step), like

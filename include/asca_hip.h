@@ -522,6 +522,8 @@ ASCA_API int asca_model_decode_step(asca_model* model, const uint32_t* ids, int 
  *     their outputs and gradients are zero.
  *   - Inputs and outputs must not overlap unless stated.  Results are
  *     deterministic (no atomics).
+ *   - An infinity or a NaN makes what the formulas take it to infinite or NaN (not
+ *     always the same of the two) and nothing else.
  *   - What a call needs for itself comes from the scratch that the library keeps
  *     for each stream (see asca_delta_ws_bytes). */
 
@@ -553,7 +555,8 @@ ASCA_API int asca_ssm_ws_bytes(int B, int T, int D, int N, size_t* bytes);
 /* Selective state space scan, N states (1..64) for each of D channels:
  *   v = dt + dt_bias;  e = softplus(v) with `softplus`, else v
  *   h_tn = exp(e_t A_n) h_{t-1,n} + e_t x_t B_tn;  y_t = sum_n C_tn h_tn + Dk x_t
- *   x, dt, y : (B*T, D);  A : (N, D);  dt_bias, Dk : (D) or NULL (zeros)
+ *   x, dt, y : (B*T, D);  A : (N, D), finite, of either sign;  dt_bias, Dk : (D) or
+ *              NULL (zeros)
  *   Bm, Cm   : (B*T, G*N); channels g*D/G .. (g+1)*D/G - 1 use columns
  *              g*N .. (g+1)*N - 1 (D a multiple of G)
  *   h0       : (B, N, D) state before row 0 (NULL = zeros)
@@ -602,7 +605,8 @@ ASCA_API int asca_block_norm_bwd(const void* x, long ldx, const void* y, long ld
  * pointers of `dtype` elements in host arrays, which the call copies) for the
  * calls below, and where they go when clipped (dst[i]; dst NULL = in place).
  * The list holds device memory of its own until asca_grads_destroy; calls on
- * one list must not overlap. */
+ * one list must not overlap.  Meant for up to some thousands of tensors: clipping
+ * adds up their sums in every block. */
 ASCA_API int asca_grads_create(void** src, void** dst, const uint64_t* sizes, int count, int dtype, void** grads);
 ASCA_API int asca_grads_destroy(void* grads);
 /* out[0] (device) = the 2-norm over all the tensors, its squares summed in 64
