@@ -100,6 +100,10 @@ SIGNATURES: dict[str, tuple] = {
     "asca_grads_destroy": (_i, [_p]),
     "asca_grads_norm": (_i, [_p, _p, _p]),
     "asca_grads_clip": (_i, [_p, _f, _p, _p]),
+    "asca_top_logits": (_i, [_p, _l, _l, _i, _i, _f, _p, _p, _p, _i, _p]),
+    "asca_distill": (_i, [_p, _l, _p, _p, _p, _i, _p, _p, _f, _f, _f, _p, _p, _l, _l, _i, _i, _p]),
+    "asca_beam_step": (_i, [_p, _l, _p, _p, _i, _i, _p, _p, _p, _p, _i, _i, _i, _i, _p]),
+    "asca_beam_states": (_i, [C.POINTER(_p), C.POINTER(_p), _u64p, _u64p, _i, _p, _i, _i, _i, _p]),
     "asca_model_create": (_i, [_i] * 6 + [C.POINTER(_p)]),
     "asca_model_destroy": (_i, [_p]),
     "asca_model_num_tensors": (_i, [_p, C.POINTER(_i)]),
@@ -108,6 +112,7 @@ SIGNATURES: dict[str, tuple] = {
     "asca_model_set_adamw": (_i, [_p, _f, _f, _f, _f, _f, C.c_uint32]),
     "asca_model_adamw_step_count": (_i, [_p, C.POINTER(C.c_uint32)]),
     "asca_model_forward_backward": (_i, [_p, _p, _p, _i, _i, _p, _p]),
+    "asca_model_distill": (_i, [_p] * 6 + [_i, _p, _f, _f, _i, _i, _p, _p]),
     "asca_model_adamw": (_i, [_p, _p]),
     "asca_model_train_step": (_i, [_p, _p, _p, _i, _i, _p, _p]),
     "asca_model_decode_state_floats": (_i, [_p, C.POINTER(_sz)]),

@@ -396,7 +396,8 @@ static int d2d(void* dst, const void* src, size_t bytes, hipStream_t st) {
 }
 
 // Forward of the whole model, keeping what the backward needs.
-static int model_forward(asca_model* M, const uint32_t* ids, const uint32_t* targets, hipStream_t st) {
+static int model_forward(asca_model* M, const uint32_t* ids, const uint32_t* targets, hipStream_t st,
+                         const DistillTeacher* teacher = nullptr) {
     const int T = M->batch * M->seq, d = M->d, H = M->H, dh = M->dh, E = M->E, dff = M->dff, V = M->V;
     int rc;
     // routing of this batch (the same ids for every layer) and the id buckets
@@ -472,7 +473,14 @@ static int model_forward(asca_model* M, const uint32_t* ids, const uint32_t* tar
     if ((rc = asca_rmsnorm(x, M->h_final, nullptr, T, d, MODEL_EPS, st))) return rc;
     GemmArgs hd = gemm_plain(M->h_final, d, M->p + M->t[1].off, V, M->logits, V, T, V, d);
     if ((rc = gemm_launch(0, 0, EPI_STORE, hd, T, st, "head"))) return rc;
-    if ((rc = asca_cross_entropy(M->logits, targets, T, V, M->dlogits, M->losses, st))) return rc;
+    if (teacher) {
+        const DistillTeacher& t = *teacher;
+        if ((rc = asca_distill(M->logits, V, t.tval, t.tids, t.tlse, t.K, targets, t.weights, t.temperature, t.alpha,
+                               1.0f / (float)T, M->losses, M->dlogits, V, T, V, ASCA_F32, st)))
+            return rc;
+    } else if ((rc = asca_cross_entropy(M->logits, targets, T, V, M->dlogits, M->losses, st))) {
+        return rc;
+    }
     if ((rc = pre_launch("loss_mean"))) return rc;
     hipLaunchKernelGGL(loss_mean_k, dim3(1), dim3(256), 0, st, M->losses, (long)T, 1.0f / (float)T, M->loss);
     if ((rc = post_launch("loss_mean"))) return rc;
@@ -954,6 +962,21 @@ int asca_model_forward_backward(asca_model* M, const uint32_t* ids, const uint32
     if (rc) return rc;
     const hipStream_t st = as_stream(stream);
     if ((rc = model_forward(M, ids, targets, st))) return rc;
+    if ((rc = model_backward(M, st))) return rc;
+    if (loss) return d2d(loss, M->loss, sizeof(float), st);
+    return ASCA_OK;
+}
+
+int asca_model_distill(asca_model* M, const uint32_t* ids, const uint32_t* targets, const float* tval,
+                       const int32_t* tids, const float* tlse, int K, const float* weights, float temperature,
+                       float alpha, int batch, int seq, float* loss, void* stream) {
+    if (!M || !ids) return fail(ASCA_ERR_INVALID, "null pointer");
+    if (batch < 1 || seq < 1 || (long)batch * seq > 0x7fffffffL) return fail(ASCA_ERR_INVALID, "bad batch/seq");
+    const DistillTeacher t{tval, tids, tlse, K, weights, temperature, alpha};
+    int rc = distill_check("asca_model_distill", t, targets, (long)batch * seq, M->V);
+    if (rc || (rc = ensure_acts(M, batch, seq))) return rc;
+    const hipStream_t st = as_stream(stream);
+    if ((rc = model_forward(M, ids, targets, st, &t))) return rc;
     if ((rc = model_backward(M, st))) return rc;
     if (loss) return d2d(loss, M->loss, sizeof(float), st);
     return ASCA_OK;

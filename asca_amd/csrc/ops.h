@@ -15,4 +15,16 @@ int bucket_launch(bool hash, const uint32_t* ids, int n, int E, int32_t* expert,
 int rmsnorm_bwd_launch(const float* x, const float* dy, const float* res, float* dx, long rows, int cols, float eps,
                        hipStream_t st);
 
+// What asca_distill is given beside the logits, and its checks of it (dlogits of the
+// logits' stride; without launching).
+struct DistillTeacher {
+    const float* tval;
+    const int32_t* tids;
+    const float* tlse;
+    int K;
+    const float* weights;
+    float temperature, alpha;
+};
+int distill_check(const char* fn, const DistillTeacher& t, const uint32_t* targets, long T, int V);
+
 }  // namespace asca

@@ -31,7 +31,8 @@ ARCH = "gfx950"
 KERNELS = ("delta_fwd", "delta_bwd", "delta_states", "delta_decode", "rmsnorm", "rmsnorm_bwd", "adamw",
            "hash_route", "gather_rows", "scatter_rows", "colsum", "cross_entropy", "gemm", "moe_fwd", "moe_bwd",
            "chunk_fwd", "chunk_bwd", "model_train_step", "conv_fwd", "conv_bwd", "conv_step", "ssm_fwd", "ssm_bwd",
-           "ssm_step", "block_norm_fwd", "block_norm_bwd", "grads_norm", "grads_clip")
+           "ssm_step", "block_norm_fwd", "block_norm_bwd", "grads_norm", "grads_clip", "top_logits", "distill", "beam_step",
+           "beam_states")
 DEFAULT_MIN_FLOPS = 4_000_000
 
 _f32 = np.float32
@@ -367,6 +368,37 @@ class GradList:
             self.close()
         except Exception:
             pass
+
+
+class Teacher:
+    """A teacher's largest logits on the device, for the distilled training steps of the
+    models: values (rows, K) float32, ids (rows, K) int32 (an id outside the vocabulary is
+    no entry), and with the whole sum's lse (rows) at `temperature` the rest as a class."""
+
+    def __init__(self, values: DevBuf, ids: DevBuf, lse: DevBuf | None, rows: int, k: int, temperature: float):
+        self.values, self.ids, self.lse = values, ids, lse
+        self.rows, self.k, self.temperature = rows, k, float(temperature)
+
+    @classmethod
+    def upload(cls, values, ids, lse=None, temperature: float = 1.0) -> "Teacher":
+        values = _mat(values, "values")
+        ids = np.asarray(ids)
+        if values.ndim != 2 or ids.shape != values.shape or (lse is not None and np.shape(lse) != values.shape[:1]):
+            raise ValueError(f"values {values.shape}, ids {ids.shape}, lse {np.shape(lse)}")
+        rows, k = values.shape
+        return cls(DevBuf.from_host(values), DevBuf.from_array(ids.astype(np.int32)),
+                   None if lse is None else DevBuf.from_host(np.asarray(lse, _f32)), rows, k, temperature)
+
+    def to_host(self):
+        """(values, ids, lse or None)."""
+        shape = (self.rows, self.k)
+        return (self.values.to_host(shape), self.ids.to_host(shape, np.int32),
+                None if self.lse is None else self.lse.to_host((self.rows,)))
+
+    def free(self) -> None:
+        for b in (self.values, self.ids, self.lse):
+            if b is not None:
+                b.free()
 
 
 class ChunkDev:
@@ -1001,6 +1033,96 @@ class Gpu:
             return {k: v.to_host(a.shape, a.dtype) if k in ("dx", "dy", "dz") else v.to_host((cols,)) for k, v in g.items()}
         finally:
             b.free()
+
+    # -- behind the logits ------------------------------------------------------
+    def top_logits(self, logits, k: int, temperature: float = 1.0):
+        """The k largest logits of each row, descending, ties to the lower id
+        (asca_top_logits): (values, ids, log sum exp(logits / temperature))."""
+        ty = _acts({"logits": logits.shape}, logits=logits)
+        rows, V = logits.shape
+        b = _Bufs()
+        try:
+            v, i, s = b.new(rows * k * 4), b.new(rows * k * 4), b.new(rows * 4)
+            _lib.call("asca_top_logits", _vp(b.up(logits)), V, rows, V, k, temperature, _vp(v), _vp(i), _vp(s), ty, None)
+            _lib.call("asca_sync")
+            return v.to_host((rows, k)), i.to_host((rows, k), np.int32), s.to_host((rows,))
+        finally:
+            b.free()
+
+    def distill(self, logits, tval=None, tids=None, *, tlse=None, targets=None, weights=None, temperature: float = 1.0,
+                alpha: float = 1.0, scale: float = 1.0, grad: bool = True):
+        """Losses of rows of logits against a teacher's largest logits (and targets, for
+        alpha < 1) and scale times their gradient, in the logits' type (asca_distill):
+        (losses, dlogits or None)."""
+        ty = _acts({"logits": logits.shape}, logits=logits)
+        T, V = logits.shape
+        K = 0 if tval is None else np.shape(tval)[1]
+        b = _Bufs()
+        try:
+            if tids is not None and np.shape(tids) != (T, K):
+                raise ValueError(f"tids has shape {np.shape(tids)}, expected {(T, K)}")
+            if targets is not None and np.shape(targets) != (T,):
+                raise ValueError(f"targets has shape {np.shape(targets)}, expected {(T,)}")
+            bl = b.up(logits)
+            dl, ls = b.new(logits.nbytes) if grad else None, b.new(T * 4)
+            _lib.call("asca_distill", _vp(bl), V, _vp(b.up(tval, "tval", (T, K))),
+                      _vp(None if tids is None else b.up(np.asarray(tids, np.int32))), _vp(b.up(tlse, "tlse", (T,))), K,
+                      _vp(None if targets is None else b.up(np.asarray(targets, np.uint32))), _vp(b.up(weights, "weights", (T,))),
+                      temperature, alpha, scale, _vp(ls), _vp(dl), V, T, V, ty, None)
+            _lib.call("asca_sync")
+            return ls.to_host((T,)), dl.to_host(logits.shape, logits.dtype) if grad else None
+        finally:
+            b.free()
+
+    def beam_step(self, logits, scores, *, k: int, ended=None, eos: int = -1, stay: bool = False):
+        """One choice of groups of k beams over rows of logits (asca_beam_step): new scores,
+        tokens, parents and, with `ended`, the new ended flags."""
+        ty = _acts({"logits": logits.shape}, logits=logits)
+        n, V = logits.shape
+        if k < 1 or n % k:
+            raise ValueError(f"{n} rows are no groups of {k} beams")
+        if ended is not None and np.shape(ended) != (n,):
+            raise ValueError(f"ended has shape {np.shape(ended)}, expected {(n,)}")
+        b = _Bufs()
+        try:
+            s, t, p = b.new(n * 4), b.new(n * 4), b.new(n * 4)
+            e = None if ended is None else b.up(np.asarray(ended, np.int32))
+            _lib.call("asca_beam_step", _vp(b.up(logits)), V, _vp(b.up(scores, "scores", (n,))), _vp(e), eos, int(stay), _vp(s),
+                      _vp(e), _vp(t), _vp(p), n // k, k, V, ty, None)
+            _lib.call("asca_sync")
+            out = s.to_host((n,)), t.to_host((n,), np.uint32), p.to_host((n,), np.int32)
+            return out if ended is None else (*out, e.to_host((n,), np.int32))
+        finally:
+            b.free()
+
+    def beam_states(self, bufs, parents, *, groups: int, k: int, k_src: int | None = None, sync: bool = True, stream=None) -> None:
+        """Device buffers follow their beams (asca_beam_states): `bufs` lists (src, dst or None
+        for in place, outer, bytes) with DevBuf src (outer, groups, k_src, bytes) and dst
+        (outer, groups, k, bytes); parents: (groups*k) ints, a DevBuf of them, or None for a
+        fork."""
+        ks = k if k_src is None else k_src
+        n = len(bufs)
+        for src, dst, outer, nbytes in bufs:
+            for b, w in ((src, ks), (src if dst is None else dst, k)):
+                if b.nbytes < outer * groups * w * nbytes:
+                    raise ValueError(f"a buffer of {b.nbytes} bytes for {outer} x {groups} x {w} x {nbytes}")
+        if isinstance(parents, DevBuf):
+            up, size = parents, parents.nbytes // 4
+        else:
+            up, size = None, groups * k if parents is None else len(parents)
+            if parents is not None:
+                up = DevBuf.from_array(np.asarray(parents, np.int32))
+        try:
+            if size < groups * k:
+                raise ValueError(f"{size} parents for {groups} x {k} slots")
+            at = lambda j: (C.c_void_p * max(n, 1))(*[None if t[j] is None else t[j].ptr for t in bufs])  # noqa: E731
+            num = lambda j: (C.c_uint64 * max(n, 1))(*[t[j] for t in bufs])  # noqa: E731
+            _lib.call("asca_beam_states", at(0), at(1), num(2), num(3), n, _vp(up), groups, ks, k, stream)
+            if sync or (up is not None and up is not parents):
+                _lib.call("asca_stream_sync", stream)
+        finally:
+            if up is not None and up is not parents:
+                up.free()
 
     # -- decode -------------------------------------------------------------
     def new_decode_states(self, n_seq: int, n_heads: int, dh: int) -> DevBuf:

@@ -15,7 +15,8 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from .gpu import DevBuf, GradList, _vp, describe, gpu
+from . import search
+from .gpu import DevBuf, GradList, Teacher, _vp, describe, gpu
 
 _f32 = np.float32
 
@@ -131,6 +132,30 @@ class DeviceModel:
         _lib.call("asca_model_forward_backward", self._h, _vp(ids), _vp(targets), batch, seq, _vp(lb), stream)
         return self._read_loss() if sync else None
 
+    def distill(self, ids, targets, batch: int, teacher: Teacher, alpha: float = 0.5, weights=None, sync: bool = True):
+        """forward_backward with asca_distill's loss: (1 - alpha) of the cross-entropy of the
+        targets (None with alpha = 1) and alpha of the distance to the teacher's largest logits
+        of the same rows, at its temperature; `weights`: a weight a row."""
+        n = len(ids)
+        if batch < 1 or n % batch or n < 1 or (targets is not None and len(targets) != n):
+            raise ValueError("ids/targets must hold batch * seq tokens each")
+        if teacher.rows != n:
+            raise ValueError(f"a teacher of {teacher.rows} rows for {n}")
+        if weights is not None and np.shape(weights) != (n,):
+            raise ValueError(f"weights has shape {np.shape(weights)}, expected {(n,)}")
+        di = self._ids("ids", ids)
+        dt = None if targets is None else self._ids("tgt", targets)
+        dw = None
+        if weights is not None:
+            w = np.ascontiguousarray(weights, dtype=_f32)
+            dw = self._bufs.get("weights")
+            if dw is None or dw.nbytes < w.nbytes:
+                dw = self._bufs["weights"] = DevBuf(w.nbytes)
+            dw.upload(w)
+        _lib.call("asca_model_distill", self._h, _vp(di), _vp(dt), _vp(teacher.values), _vp(teacher.ids), _vp(teacher.lse),
+                  teacher.k, _vp(dw), teacher.temperature, alpha, batch, n // batch, _vp(self._loss_buf()), None)
+        return self._read_loss() if sync else None
+
     def clip_grads(self, max_norm: float, sync: bool = True, stream=None):
         """Scale every gradient by min(1, max_norm / (norm + 1e-6)), norm the 2-norm
         over all of them (asca_grads_clip), between forward_backward and adamw:
@@ -174,16 +199,44 @@ class DeviceModel:
         n = len(ids)
         if states.nbytes < 4 * n * self.decode_state_floats():
             raise ValueError("states buffer too small for %d sequences" % n)
-        di = self._ids("dec_ids", ids)
-        lb = self._bufs.get("decode_logits")
-        if lb is None or lb.nbytes < 4 * n * self.vocab:
-            lb = DevBuf(4 * n * self.vocab)
-            self._bufs["decode_logits"] = lb
-        _lib.call("asca_model_decode_step", self._h, _vp(di), n, _vp(states), _vp(lb), None)
+        lb = self._step_dev(self._ids("dec_ids", ids), n, states)
         if not sync:
             return None
         _lib.call("asca_sync")
         return lb.to_host((n, self.vocab))
+
+    def _step_dev(self, ids: DevBuf, n: int, states: DevBuf) -> DevBuf:
+        """The device logits of one step on device ids (uint32)."""
+        lb = self._bufs.get("decode_logits")
+        if lb is None or lb.nbytes < 4 * n * self.vocab:
+            lb = DevBuf(4 * n * self.vocab)
+            self._bufs["decode_logits"] = lb
+        _lib.call("asca_model_decode_step", self._h, _vp(ids), n, _vp(states), _vp(lb), None)
+        return lb
+
+    def _state_bufs(self, states: DevBuf, n: int) -> list:
+        """The decode states' layout, (L, n) states of a layer each."""
+        if states.nbytes < 4 * n * self.decode_state_floats():
+            raise ValueError("states buffer too small for %d sequences" % n)
+        return [(states, self.n_layers, 4 * self.decode_state_floats() // self.n_layers)]
+
+    def beam_search(self, ids, beams: int, steps: int, eos: int | None = None):
+        """The `beams` best continuations, up to `steps` tokens, of n prompts of one length,
+        ids (n, T): (tokens, scores) of search.beam_search."""
+        ids = np.atleast_2d(np.asarray(ids))
+        n, T = ids.shape
+        if n == 0 or T == 0:
+            raise ValueError(f"ids of shape {ids.shape} have no row to go on from")
+        search.check(n, beams, steps, eos, self.vocab)
+        one, many = self.new_decode_state(n), self.new_decode_state(n * beams)
+        try:
+            for t in range(T):
+                self.step(ids[:, t], one, sync=False)
+            logits = self._bufs["decode_logits"]
+            return search.beam_search(self, logits, one, many, n, beams, steps, eos)
+        finally:
+            one.free()
+            many.free()
 
     def _read_loss(self) -> float:
         _lib.call("asca_sync")

@@ -11,7 +11,9 @@ The embedding stays as it is set: no gradient of it is formed (unlike DeviceMode
 
 It trains (forward_backward, clip, adamw), reads prompts of different lengths
 (prompt) and decodes one row for many sequences on their states (step), like
-DeviceModel does for the delta block.
+DeviceModel does for the delta block.  It learns from a teacher's largest logits and
+leaves its own for a student (forward_backward, teacher), and searches over beams
+(beam_search).
 """
 from __future__ import annotations
 
@@ -19,8 +21,8 @@ import ctypes as C
 
 import numpy as np
 
-from . import _lib
-from .gpu import F32, DevBuf, GradList, _vp, describe, gpu
+from . import _lib, search
+from .gpu import F32, DevBuf, GradList, Teacher, _vp, describe, gpu
 
 _f32 = np.float32
 EPS = 1e-6
@@ -133,12 +135,13 @@ class SsmModel:
     def _forward(self, ids, batch: int, keep: bool, states=None, lens=None, one: bool = False) -> C.c_void_p:
         """Normalised rows after the last layer.  `keep`: layer by layer, for the
         backward; `states`: (conv, scan) states that the rows go on from and leave
-        (`one`: a single row each, updated in place)."""
-        rows, d, N, W, R, X = len(ids), self.d, self.N, self.W, self.R, self.X
+        (`one`: a single row each, updated in place; ids may be on the device then)."""
+        rows, d, N, W, R, X = batch if isinstance(ids, DevBuf) else len(ids), self.d, self.N, self.W, self.R, self.X
         T = rows // batch
         tag = (lambda k, i: f"{k}.{i}") if keep else (lambda k, i: f"{k}.{i % 2}")
         x, nrm = self._rows(tag("x", 0), rows, d), self._rows(tag("n", 0), rows, d)
-        _lib.call("asca_gather_rows", self._p("embed"), self._up("ids", ids, np.int32), rows, d, x, None)
+        _lib.call("asca_gather_rows", self._p("embed"), _vp(ids) if isinstance(ids, DevBuf) else self._up("ids", ids, np.int32),
+                  rows, d, x, None)
         _lib.call("asca_block_norm_fwd", x, d, None, 0, None, 0, None, None, self._p("w_pre.0"), None, 0, nrm, d, rows, d, EPS, F32, None)
         for i in range(self.L):
             uz, c, y = self._rows(tag("uz", i), rows, 2 * d), self._rows(tag("c", i), rows, d), self._rows(tag("y", i), rows, d)
@@ -183,16 +186,30 @@ class SsmModel:
         return logits
 
     # -- training -------------------------------------------------------------------
-    def forward_backward(self, ids, targets, batch: int) -> float:
-        """Mean cross-entropy of batch sequences (rows b*T ..), its gradients in grads()."""
+    def forward_backward(self, ids, targets, batch: int, teacher: Teacher | None = None, alpha: float = 0.5,
+                         weights=None) -> float:
+        """Mean cross-entropy of batch sequences (rows b*T ..), its gradients in grads().  With
+        a teacher's largest logits of the same rows the mean of asca_distill's loss, alpha of
+        the teacher (targets may be None with alpha = 1), `weights` a weight a row."""
         rows, d, V, N, W, R, X, L = len(ids), self.d, self.vocab, self.N, self.W, self.R, self.X, self.L
-        if batch < 1 or rows < 1 or rows % batch or np.shape(ids) != (rows,) or np.shape(targets) != (rows,):
+        if batch < 1 or rows < 1 or rows % batch or np.shape(ids) != (rows,) or (
+                np.shape(targets) != (rows,) and not (targets is None and teacher is not None and alpha == 1.0)):
             raise ValueError("ids/targets must hold batch * seq tokens each")
+        if teacher is not None and teacher.rows != rows:
+            raise ValueError(f"a teacher of {teacher.rows} rows for {rows}")
+        if weights is not None and (teacher is None or np.shape(weights) != (rows,)):
+            raise ValueError(f"weights of shape {np.shape(weights)}, expected {(rows,)} and a teacher")
         T = rows // batch
         nrm = self._forward(self._ids(ids), batch, True)
         logits = self._head(nrm, rows)
         dlog, losses = self._rows("dlog", rows, V), self._rows("losses", rows, 1)
-        _lib.call("asca_cross_entropy", logits, self._up("tgt", targets, np.uint32), rows, V, dlog, losses, None)
+        tgt = None if targets is None else self._up("tgt", targets, np.uint32)
+        if teacher is None:
+            _lib.call("asca_cross_entropy", logits, tgt, rows, V, dlog, losses, None)
+        else:
+            _lib.call("asca_distill", logits, V, _vp(teacher.values), _vp(teacher.ids), _vp(teacher.lse), teacher.k, tgt,
+                      None if weights is None else self._up("weights", weights, _f32), teacher.temperature, alpha, 1.0 / rows, losses,
+                      dlog, V, rows, V, F32, None)
         dn, dr, do, duz = (self._rows(k, rows, c) for k, c in (("dn", d), ("dr", d), ("do", d), ("duz", 2 * d)))
         dy, dc, ddt, drbc = (self._rows(k, rows, c) for k, c in (("dy", d), ("dc", d), ("ddt", d), ("drbc", X)))
         self._gemm(1, 0, d, V, rows, nrm, d, dlog, V, self._g("head"), V)
@@ -235,6 +252,18 @@ class SsmModel:
         off = self._at["head"]   # all but the embedding, which comes first
         at = lambda k: C.c_void_p(self._flat[k].ptr + 4 * off)  # noqa: E731
         _lib.call("asca_adamw", at("params"), at("grads"), at("m"), at("v"), self.n_floats - off, s[0], beta1, beta2, s[1], s[2], None)
+
+    def teacher(self, ids, batch: int, k: int, temperature: float = 1.0, rest: bool = True) -> Teacher:
+        """The k largest logits of each row of batch sequences on the device, and with `rest`
+        the whole sum's logarithm, for a student's forward_backward."""
+        rows = len(ids)
+        if batch < 1 or rows < 1 or rows % batch or np.shape(ids) != (rows,):
+            raise ValueError("ids must hold batch * seq tokens")
+        logits = self._head(self._forward(self._ids(ids), batch, False), rows)
+        t = Teacher(DevBuf(rows * k * 4), DevBuf(rows * k * 4), DevBuf(rows * 4) if rest else None, rows, k, temperature)
+        _lib.call("asca_top_logits", logits, self.vocab, rows, self.vocab, k, t.temperature, _vp(t.values), _vp(t.ids), _vp(t.lse),
+                  F32, None)
+        return t
 
     # -- serving ----------------------------------------------------------------------
     def new_state(self, n_seq: int) -> tuple[DevBuf, DevBuf]:
@@ -289,6 +318,30 @@ class SsmModel:
         self._head(nrm, len(ids))
         _lib.call("asca_sync")
         return self._bufs["logits"].to_host((len(ids), self.vocab))
+
+    def _step_dev(self, ids: DevBuf, n: int, states) -> DevBuf:
+        """The device logits of one step on device ids."""
+        self._head(self._forward(ids, n, False, self._states(states, n), one=True), n)
+        return self._bufs["logits"]
+
+    def _state_bufs(self, states, n: int) -> list:
+        """The states' layout, (L, n) states of a layer each."""
+        self._states(states, n)
+        return [(b, self.L, k * self.d * 4) for b, k in zip(states, (self.W - 1, self.N), strict=True) if k]
+
+    def beam_search(self, ids, beams: int, steps: int, lens=None, eos: int | None = None):
+        """The `beams` best continuations, up to `steps` tokens, of n prompts, ids (n, T) of
+        which sequence b has lens[b]: (tokens, scores) of search.beam_search."""
+        ids = np.atleast_2d(np.asarray(ids))
+        n = len(ids)
+        search.check(n, beams, steps, eos, self.vocab)
+        one, many = self.new_state(n), self.new_state(n * beams)
+        try:
+            self.prompt(ids, one, lens)
+            return search.beam_search(self, self._bufs["logits"], one, many, n, beams, steps, eos)
+        finally:
+            for b in (*one, *many):
+                b.free()
 
     def close(self) -> None:
         self._clip.close()

@@ -478,6 +478,12 @@ ASCA_API int asca_model_adamw_step_count(const asca_model* model, uint32_t* step
  * afterwards (or a synchronisation of it) sees every gradient. */
 ASCA_API int asca_model_forward_backward(asca_model* model, const uint32_t* ids, const uint32_t* targets,
                                          int batch, int seq, float* loss, void* stream);
+/* asca_model_forward_backward with asca_distill's loss in the place of the mean
+ * cross-entropy: *loss and the gradients are of the losses' mean over the batch*seq rows
+ * (its arguments as there, device pointers over those rows).  No reference counterpart. */
+ASCA_API int asca_model_distill(asca_model* model, const uint32_t* ids, const uint32_t* targets, const float* tval,
+                                const int32_t* tids, const float* tlse, int K, const float* weights, float temperature,
+                                float alpha, int batch, int seq, float* loss, void* stream);
 /* The optimiser step over every tensor (model.rs:797-802 / AdamW::update). */
 ASCA_API int asca_model_adamw(asca_model* model, void* stream);
 /* forward_backward followed by asca_model_adamw: one training step.  The
@@ -616,6 +622,74 @@ ASCA_API int asca_grads_norm(void* grads, float* out, void* stream);
  * into out[1], and dst = c src.  A norm that is not finite gives c = 0 (an
  * infinite one) or NaN, and what c src then is: the caller sees it in out. */
 ASCA_API int asca_grads_clip(void* grads, float max_norm, float* out, void* stream);
+
+/* ------------------------------------------------ behind the logits -- */
+
+/* The operators that work on a model's logits beside asca_cross_entropy: their
+ * largest, distillation from a teacher's, and a beam search's steps.  The reference
+ * has no counterpart.
+ *   - Logits are (rows, V) f32 or bf16 (`dtype`) with a row stride `ld` >= V in
+ *     elements, at any address that is a multiple of an element.
+ *   - All arithmetic is f32 or more; results are deterministic.
+ *   - What a call needs for itself comes from the scratch that the library keeps
+ *     for each stream (see asca_delta_ws_bytes). */
+
+/* The K (1..64) largest logits of each row, descending, of equal ones the lower id
+ * first: values and ids (rows, K), and lse (rows, or NULL) = log sum exp(z / temperature).
+ * NaN and -inf are not listed: a row with fewer others ends in entries of value -inf and
+ * id -1.  A NaN or +inf in a row makes its lse infinite or NaN. */
+ASCA_API int asca_top_logits(const void* logits, long ld, long rows, int V, int K, float temperature, float* values,
+                             int32_t* ids, float* lse, int dtype, void* stream);
+
+/* Distillation from a teacher's largest logits, loss and gradient of T rows.
+ *   tval, tids (T, K) : the teacher's logits and their ids, K 1..64; an id outside
+ *     0 .. V-1 is no entry, entries of one id are one with the sum of their p
+ *   tlse (T) : the teacher's log sum exp(logits / temperature) over all its ids:
+ *     p_k = exp(tval_k / temperature - tlse), and what they leave of 1, p_r, is one
+ *     class more, met by the student's sum q_r over the ids that are not listed (left
+ *     out where that is zero because every other logit is -inf).  NULL: p is the
+ *     softmax of tval / temperature over the row's entries.
+ *   q = softmax(logits / temperature)
+ *   losses_t = w_t ((1 - alpha) CE_t + alpha temperature^2 (sum p log(p / q) + p_r log(p_r / q_r)))
+ *   dlogits  = scale * d losses_t / d logits, of `dtype`, rounded once; NULL = not wanted;
+ *     may be the logits (with the same stride)
+ *   targets (T) for CE_t, the cross-entropy of the unscaled logits (no CE_t for a target
+ *     >= V); may be NULL where alpha = 1.  tval and tids may be NULL where alpha = 0.
+ *   weights (T), NULL = ones: w_t, also the gradient that comes back to losses_t.  A row of
+ *     weight zero is not read; its loss and gradient are zero.
+ * alpha is 0..1, V at most 2^20.  A row without entries has no part of weight alpha. */
+ASCA_API int asca_distill(const void* logits, long ld, const float* tval, const int32_t* tids, const float* tlse, int K,
+                          const uint32_t* targets, const float* weights, float temperature, float alpha, float scale,
+                          float* losses, void* dlogits, long lddl, long T, int V, int dtype, void* stream);
+
+/* One choice of a beam search: for each of `groups` searches the K (1..32) best of the
+ * candidates scores_b + logits_bi - log sum exp(logits_b) of its beams b and tokens i, of
+ * equal ones the lowest b V + i first (compared in 64 bits).
+ *   logits (groups*K, V); scores (groups*K): a beam whose score, or whose logits' sum, is
+ *     not finite has no candidates, and a logit of -inf or NaN is none
+ *   eos >= 0 with ended, new_ended (groups*K): an ended beam's only candidate is itself
+ *     (token eos, its score; its logits are not read), and a beam that takes eos is ended.
+ *     eos < 0: both NULL
+ *   new_scores, new_ended, tokens, parents (groups*K), parents in 0 .. K-1 within the
+ *     group.  `stay` = 0: best first.  Else a beam's best child keeps the beam's slot and
+ *     the others take what is left in their order, so that few states move.
+ *   A slot without a candidate has the score -inf, itself as its parent and token eos (0
+ *     without one).
+ * new_scores may be scores and new_ended ended; tokens are ids for the next step. */
+ASCA_API int asca_beam_step(const void* logits, long ld, const float* scores, const int32_t* ended, int eos, int stay,
+                            float* new_scores, int32_t* new_ended, uint32_t* tokens, int32_t* parents, int groups, int K,
+                            int V, int dtype, void* stream);
+
+/* What the beams of `groups` searches carry follows them to their slots, for `count` (up to
+ * 8) buffers at once: buffer i is (outer[i], groups, k_src, bytes[i] bytes) and becomes
+ * (outer[i], groups, k_dst, bytes[i]) with slot j the source's slot parents[group*k_dst + j]
+ * (device; NULL = slot 0 of each group: a fork of one sequence to k_dst beams).  A parent
+ * outside 0 .. k_src-1 leaves its slot as it is.
+ *   dst NULL, or dst[i] NULL or src[i]: in place (k_src = k_dst); only slots that change
+ *   are touched.  Other destinations must not overlap any source.
+ * src, dst, outer and bytes are host arrays, read before the call returns; 1 to 32 beams. */
+ASCA_API int asca_beam_states(void** src, void** dst, const uint64_t* outer, const uint64_t* bytes, int count,
+                              const int32_t* parents, int groups, int k_src, int k_dst, void* stream);
 
 #ifdef __cplusplus
 }
