@@ -21,6 +21,54 @@ ASCA_DEV float key_value(uint64_t k) {
 }
 ASCA_DEV unsigned key_place(uint64_t k) { return ~(unsigned)k; }
 
+// ------------------------------------------------------ lanes of a wave
+
+// The larger or the smaller of x and what lane ^ M holds, M a power of two
+template <int M>
+ASCA_DEV float lane_pick(float x, bool larger) {
+    float a = x, b;
+    if constexpr (M == 1) b = dpp<DPP_QUAD_XOR1>(x);
+    if constexpr (M == 2) b = dpp<DPP_QUAD_XOR2>(x);
+    if constexpr (M == 4) b = dpp<DPP_HALF_MIRROR>(dpp<0x1B>(x));   // ^3 (quad_perm [3,2,1,0]), then ^7
+    if constexpr (M == 8) b = dpp<DPP_ROW_ROR8>(x);
+    if constexpr (M == 16 || M == 32) {   // the swap leaves the pair in both lanes, in either order
+        const unsigned u = __float_as_uint(x);
+        auto r = M == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false)
+                         : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+    }
+    const float hi = fmaxf(a, b), lo = fminf(a, b);
+    return larger ? hi : lo;
+}
+
+ASCA_DEV float wave_max(float x) {
+    x = lane_pick<1>(x, true), x = lane_pick<2>(x, true), x = lane_pick<4>(x, true);
+    x = lane_pick<8>(x, true), x = lane_pick<16>(x, true);
+    return lane_pick<32>(x, true);
+}
+
+// The steps of a bitonic network of runs of N lanes: `down` lanes' runs fall, the others' rise
+template <int N>
+ASCA_DEV float lane_merge(float x, bool down) {
+    const int l = threadIdx.x;
+    if constexpr (N >= 64) x = lane_pick<32>(x, !(l & 32) == down);
+    if constexpr (N >= 32) x = lane_pick<16>(x, !(l & 16) == down);
+    if constexpr (N >= 16) x = lane_pick<8>(x, !(l & 8) == down);
+    if constexpr (N >= 8) x = lane_pick<4>(x, !(l & 4) == down);
+    if constexpr (N >= 4) x = lane_pick<2>(x, !(l & 2) == down);
+    return lane_pick<1>(x, !(l & 1) == down);
+}
+// The wave's values, the largest in lane 0
+ASCA_DEV float lane_sort(float x) {
+    const int l = threadIdx.x;
+    x = lane_merge<2>(x, !(l & 2));
+    x = lane_merge<4>(x, !(l & 4));
+    x = lane_merge<8>(x, !(l & 8));
+    x = lane_merge<16>(x, !(l & 16));
+    x = lane_merge<32>(x, !(l & 32));
+    return lane_merge<64>(x, true);
+}
+
 template <typename T>
 ASCA_DEV T wave_max_t(T x) {
 #pragma unroll
@@ -59,6 +107,55 @@ ASCA_DEV T block_sum_t(T x, T* lds) {
 #pragma unroll
     for (int w = 1; w < NW; ++w) x += lds[w];
     return x;
+}
+
+// ------------------------------------------------------------ row pieces
+
+// A row's n elements as 16-byte pieces: `head` elements before the first whole piece of the
+// address space, nb pieces of W, fewer than W after them.
+template <typename E>
+struct Pieces {
+    static constexpr int W = 16 / sizeof(E);
+    const E* p;
+    int n, head, nb;
+    ASCA_DEV Pieces(const E* row, int len) : p(row), n(len) {
+        const int off = (int)(reinterpret_cast<uintptr_t>(row) / sizeof(E) % W);
+        head = min(off ? W - off : 0, n);
+        nb = (n - head) / W;
+    }
+    ASCA_DEV uint4 piece(int i) const { return reinterpret_cast<const uint4*>(p + head)[i]; }
+    ASCA_DEV int col(int i) const { return head + i * W; }   // the first column of a piece
+    // the column outside the pieces that thread t of at least 2 W takes, or -1
+    ASCA_DEV int edge(int t) const {
+        if (t < head) return t;
+        const int c = head + nb * W + t - W;
+        return t >= W && c < n ? c : -1;
+    }
+    ASCA_DEV int edge_thread(int c) const { return c < head ? c : c - head - nb * W + W; }
+};
+
+template <typename E>
+ASCA_DEV uint4 piece_of(float v);   // all its values
+template <>
+ASCA_DEV uint4 piece_of<float>(float v) {
+    const unsigned u = __float_as_uint(v);
+    return make_uint4(u, u, u, u);
+}
+template <>
+ASCA_DEV uint4 piece_of<bf16_t>(float v) {   // of a value that bf16 holds
+    const unsigned u = __float_as_uint(v), w = u >> 16 | (u & 0xffff0000u);
+    return make_uint4(w, w, w, w);
+}
+// What is made of a piece after this is made anew: the compiler would keep the 32-bit values
+// of an earlier look at it, in twice its registers (bf16).
+ASCA_DEV void piece_again(uint4& r) { asm("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w)); }
+ASCA_DEV void piece_values(uint4 r, float (&v)[4]) {
+    v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
+}
+ASCA_DEV void piece_values(uint4 r, float (&v)[8]) {
+    const unsigned u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[2 * k] = __uint_as_float(u[k] << 16), v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
 }
 
 }  // namespace asca

@@ -13,64 +13,248 @@ constexpr int TOP_MAX_K = 64;    // listed logits a row
 constexpr int BEAM_MAX_K = 32;   // beams a group
 constexpr int BEAM_BUFS = 8;     // state buffers a call
 
-struct TopArgs {
-    const void* z;
-    long ld, rows;
-    int V, K;
-    float tau;
-    float* values;
-    int32_t* ids;
-    float* lse;
+// ------------------------------------------------------------ selection
+// A team of NW waves finds the K largest of what it holds in registers.  The K-th largest of
+// its lanes' own maxima is at most the K-th largest of all, so what lies below it is none of
+// them; the few values that are left (between K and the K lanes' own) go to LDS and are
+// ranked by counting the larger ones.  Each value is looked at twice, in registers.  Where
+// more are left than LDS has room for (rows of equal values), K rounds take the largest key
+// below the last one.
+
+template <int NW>
+struct TeamLds {
+    static constexpr int CAP = NW == 1 ? 256 : 1024;
+    uint64_t keys[CAP];
+    float lists[NW][64];
+    float sums[NW];
+    uint64_t best[NW];
+    int count;
 };
 
-// m and log sum exp((z - m) / tau) of a row by a block of 256; the logarithm in 64 bits
-template <typename E>
-ASCA_DEV void row_lse(const E* z, int V, float itau, float& m, double& ls, float* lds) {
-    float mx = -INFINITY;
-    for (int c = threadIdx.x; c < V; c += 256) mx = fmaxf(mx, act_load(z + c));
-    m = block_max_t<4>(mx, lds);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f;
-    for (int c = threadIdx.x; c < V; c += 256) s += __builtin_amdgcn_exp2f((act_load(z + c) - ref) * itau * LOG2E);
-    ls = log((double)block_sum_t<4>(s, lds));
-    m = ref;
-}
-
-template <typename E>
-__global__ __launch_bounds__(256) void top_k(TopArgs p) {
-    __shared__ float lds[4];
-    __shared__ uint64_t keys[4];
-    const long row = blockIdx.x;
-    const E* z = static_cast<const E*>(p.z) + row * p.ld;
-    float m;
-    double ls;
-    row_lse(z, p.V, 1.0f / p.tau, m, ls, lds);
-    if (p.lse && threadIdx.x == 0) p.lse[row] = (float)((double)m / (double)p.tau + ls);
-    uint64_t last = ~0ull;
-    for (int k = 0; k < p.K; ++k) {
-        uint64_t best = 0;
-        for (int c = threadIdx.x; c < p.V; c += 256) {
-            const uint64_t key = logit_key(act_load(z + c), c);
-            if (key < last && key > best) best = key;
-        }
-        last = block_max_t<4>(best, keys);
-        if (threadIdx.x == 0) {
-            p.values[row * p.K + k] = last ? key_value(last) : -INFINITY;
-            p.ids[row * p.K + k] = last ? (int)key_place(last) : -1;
-        }
+template <int NW>
+ASCA_DEV void team_sync() {
+    if constexpr (NW == 1) {   // a wave's own LDS accesses, in order
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
     }
 }
 
-struct BeamArgs {
+// The K-th largest of the lanes' x (-inf where fewer are above it); the waves' maxima are
+// lists[w][0] afterwards.  Clears the list of keys and leaves it writable.
+template <int NW>
+ASCA_DEV float team_kth(float x, int K, TeamLds<NW>& l) {
+    const int lane = threadIdx.x & 63, w = NW == 1 ? 0 : threadIdx.x >> 6;
+    x = lane_sort(x);
+    if (lane == 0 && w == 0) l.count = 0;
+    l.lists[w][lane] = x;
+    team_sync<NW>();
+    if constexpr (NW == 4) {
+        // two sorted lists: the larger of one and the other backwards are the largest of both
+        const float ab = lane_merge<64>(fmaxf(l.lists[0][lane], l.lists[1][63 - lane]), true);
+        const float cd = lane_merge<64>(fmaxf(l.lists[2][lane], l.lists[3][63 - lane]), false);
+        x = lane_merge<64>(fmaxf(ab, cd), true);
+    }
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), K - 1));
+}
+
+template <int NW>
+ASCA_DEV void team_push(uint64_t key, TeamLds<NW>& l) {
+    const int at = atomicAdd(&l.count, 1);
+    if (at < TeamLds<NW>::CAP) l.keys[at] = key;
+}
+
+// The K largest keys to out(rank, key), 0 where there are fewer.  each(f) calls f with every
+// key of the thread's, for the rounds.
+template <int NW, typename Each, typename Out>
+ASCA_DEV void team_rank(int K, TeamLds<NW>& l, Each each, Out out) {
+    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+    team_sync<NW>();
+    const int n = l.count;
+    if (n <= TeamLds<NW>::CAP) {
+        for (int i = tid; i < n; i += 64 * NW) {
+            const uint64_t key = l.keys[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += l.keys[j] > key;
+            if (rank < K) out(rank, key);
+        }
+        for (int r = n + tid; r < K; r += 64 * NW) out(r, 0);
+        return;
+    }
+    uint64_t last = ~0ull;
+    for (int k = 0; k < K; ++k) {
+        uint64_t best = 0;
+        each([&](uint64_t key) {
+            if (key < last && key > best) best = key;
+        });
+        best = wave_max_t(best);
+        if constexpr (NW > 1) {
+            team_sync<NW>();
+            if ((threadIdx.x & 63) == 0) l.best[threadIdx.x >> 6] = best;
+            team_sync<NW>();
+            for (int w = 0; w < NW; ++w) best = l.best[w] > best ? l.best[w] : best;
+        }
+        last = best;
+        if (tid == 0) out(k, best);
+    }
+}
+
+struct TopArgs {
     const void* z;
-    long ld;
+    long ld, rows;
+    int V, K, S, slice;   // S slices of `slice` columns a row, each a team's
+    float tau, ct;        // ct = log2(e) / tau
+    float* values;        // with S = 1 and no search
+    int32_t* ids;
+    float* lse;
+    uint64_t* keys;       // else (rows, S, K)
+    float2* sums;         // (rows, S): the largest and the sum of exp((z - it) / tau)
+    const float* scores;  // a search's: rows of beams that have no candidates are not read
+    const int32_t* ended;
+};
+
+ASCA_DEV bool beam_reads(const TopArgs& p, long row) {
+    return !p.scores || (fabsf(p.scores[row]) < INFINITY && !(p.ended && p.ended[row] != 0));
+}
+
+ASCA_DEV void top_write(const TopArgs& p, long row, int rank, uint64_t key) {
+    p.values[row * p.K + rank] = key ? key_value(key) : -INFINITY;
+    p.ids[row * p.K + rank] = key ? (int)key_place(key) : -1;
+}
+
+// A slice of a row in R pieces a thread.  `out` takes (rank, key), `sum` the slice's largest
+// and its sum from one thread.
+template <typename E, int NW, int R, typename Out, typename Sum>
+ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW>& l, Out out, Sum sum) {
+    constexpr int NT = 64 * NW, W = Pieces<E>::W;
+    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const Pieces<E> r(row + c0, n);
+    uint4 raw[R];
+    float cm[R], mx = -INFINITY, ev = -INFINITY;
+    const int ec = r.edge(tid);
+    if (r.nb > 0)
+#pragma unroll
+        for (int j = 0; j < R; ++j) raw[j] = r.piece(min(j * NT + tid, r.nb - 1));
+    if (ec >= 0) ev = act_load(r.p + ec);
+    float v[W];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        if (j * NT + tid >= r.nb) raw[j] = piece_of<E>(-INFINITY);
+        piece_values(raw[j], v);
+        cm[j] = v[0];
+#pragma unroll
+        for (int k = 1; k < W; ++k) cm[j] = fmaxf(cm[j], v[k]);
+        mx = fmaxf(mx, cm[j]);
+    }
+    mx = fmaxf(mx, ev);   // a NaN is none of them
+    const float kth = team_kth<NW>(mx, K, l);
+#pragma unroll
+    for (int j = 0; j < R; ++j) piece_again(raw[j]);
+    float m = l.lists[NW == 1 ? 0 : threadIdx.x >> 6][0];
+    const float ref = m > -INFINITY ? m : 0.0f;
+    float s = __builtin_amdgcn_exp2f((ev - ref) * ct);
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        piece_values(raw[j], v);
+#pragma unroll
+        for (int k = 0; k < W; ++k) s += __builtin_amdgcn_exp2f((v[k] - ref) * ct);
+    }
+    s = wave_sum(s);
+#pragma unroll
+    for (int j = 0; j < R; ++j) piece_again(raw[j]);
+    if (NW > 1 && (threadIdx.x & 63) == 0) l.sums[threadIdx.x >> 6] = s;
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+        if (cm[j] >= kth) {
+            piece_values(raw[j], v);
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+                if (v[k] >= kth && v[k] > -INFINITY) team_push<NW>(logit_key(v[k], c0 + r.col(j * NT + tid) + k), l);
+        }
+    if (ev >= kth && ev > -INFINITY) team_push<NW>(logit_key(ev, c0 + ec), l);
+    auto each = [&](auto f) {
+        for (int c = tid; c < n; c += NT) f(logit_key(act_load(r.p + c), c0 + c));   // rare: from memory
+    };
+    team_rank<NW>(K, l, each, out);
+    if (tid != 0) return;
+    if constexpr (NW > 1) {
+        float top = m = l.lists[0][0];
+        for (int w = 1; w < NW; ++w) m = fmaxf(m, l.lists[w][0]);
+        s = 0.0f;
+        for (int w = 0; w < NW; ++w) {
+            top = l.lists[w][0];
+            s += top > -INFINITY ? l.sums[w] * __builtin_amdgcn_exp2f((top - m) * ct) : l.sums[w];
+        }
+    }
+    sum(m, s);
+}
+
+// Teams of NW waves, four waves a block, a slice each
+template <typename E, int NW, int R>
+__global__ __launch_bounds__(256) void top_slice_k(TopArgs p) {
+    __shared__ TeamLds<NW> lds[4 / NW];
+    const int team = NW == 1 ? threadIdx.x >> 6 : 0;
+    const long unit = (long)blockIdx.x * (4 / NW) + team, row = unit / p.S;
+    if (row >= p.rows || !beam_reads(p, row)) return;   // a whole team's
+    const int c0 = (int)(unit % p.S) * p.slice, n = min(p.slice, p.V - c0);
+    auto out = [&](int rank, uint64_t key) {
+        if (p.values) top_write(p, row, rank, key);
+        else p.keys[unit * p.K + rank] = key;
+    };
+    auto sum = [&](float m, float s) {
+        if (!p.values) p.sums[unit] = make_float2(m, s);
+        else if (p.lse) p.lse[row] = (float)((double)m / (double)p.tau + log((double)s));
+    };
+    top_slice<E, NW, R>(static_cast<const E*>(p.z) + row * p.ld, c0, n, p.K, p.ct, lds[team], out, sum);
+}
+
+// log sum exp of a row from its slices, by a wave: in every lane, in 64 bits
+ASCA_DEV double slices_lse(const float2* sums, int S, double tau) {
+    const int lane = threadIdx.x & 63;
+    double m = -INFINITY, s = 0.0;
+    for (int i = lane; i < S; i += 64) m = fmax(m, (double)sums[i].x);
+    m = wave_max_t(m);
+    for (int i = lane; i < S; i += 64)   // of nothing but -inf: a sum of zero, or NaN
+        s += sums[i].y * (sums[i].x > -INFINITY ? exp(((double)sums[i].x - m) / tau) : 1.0);
+    return m / tau + log(wave_sum_t(s));
+}
+
+// The K largest of a row's S K keys, one block a row
+__global__ __launch_bounds__(256) void top_merge_k(TopArgs p) {
+    __shared__ TeamLds<4> l;
+    const long row = blockIdx.x;
+    const uint64_t* keys = p.keys + row * p.S * p.K;
+    const int n = p.S * p.K;
+    float mx = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += 256)
+        if (keys[i]) mx = fmaxf(mx, key_value(keys[i]));
+    const float kth = team_kth<4>(mx, p.K, l);
+    auto each = [&](auto f) {
+        for (int i = threadIdx.x; i < n; i += 256) f(keys[i]);
+    };
+    each([&](uint64_t key) {
+        if (key && key_value(key) >= kth) team_push<4>(key, l);
+    });
+    team_rank<4>(p.K, l, each, [&](int rank, uint64_t key) { top_write(p, row, rank, key); });
+    if (p.lse && threadIdx.x < 64) {
+        const double s = slices_lse(p.sums + row * p.S, p.S, p.tau);
+        if (threadIdx.x == 0) p.lse[row] = (float)s;
+    }
+}
+
+// ------------------------------------------------------------- beam search
+
+struct BeamArgs {
     const float* scores;
     const int32_t* ended;
     float* new_scores;
     int32_t* new_ended;
     uint32_t* tokens;
     int32_t* parents;
-    int K, V, eos, stay;
+    int K, V, S, eos, stay;
+    const uint64_t* keys;   // (groups K, S, K)
+    const float2* sums;     // (groups K, S)
 };
 
 struct BeamPick {
@@ -91,7 +275,7 @@ ASCA_DEV int beam_slot(int parent, int K, bool stay) {
     unsigned taken = 0;
     for (int j = 0; j < K; ++j)
         if (firsts >> j & 1) taken |= 1u << __builtin_amdgcn_readlane(parent, j);
-    const uint64_t rest = ~firsts & ((K < 64 ? 1ull << K : 0) - 1);
+    const uint64_t rest = ~firsts & ((1ull << K) - 1);
     int want = __popcll(rest & ((1ull << lane) - 1)), slot = parent;
     if (!first)
         for (int j = 0; j < K; ++j)
@@ -99,7 +283,7 @@ ASCA_DEV int beam_slot(int parent, int K, bool stay) {
     return slot;
 }
 
-// A group's picks, best first, in the first K lanes of the first wave, to its slots
+// A group's picks, best first, in the first K lanes of a wave, to its slots
 ASCA_DEV void beam_write(const BeamArgs& p, long group, const BeamPick& pick) {
     const int lane = threadIdx.x & 63;
     const int slot = beam_slot(pick.parent, p.K, p.stay);
@@ -115,62 +299,93 @@ ASCA_DEV void beam_write(const BeamArgs& p, long group, const BeamPick& pick) {
     if (p.new_ended) p.new_ended[at] = end;
 }
 
-// Whether a beam's candidates count: its score and its logits' sum are finite
-ASCA_DEV bool beam_finite(double x) { return fabs(x) < INFINITY; }
+constexpr int BEAM_CAP = 1024;   // candidates that are ranked in LDS
 
-template <typename E>
-__global__ __launch_bounds__(256) void beam_step_k(BeamArgs p) {
-    __shared__ float lds[4];
-    __shared__ double base[BEAM_MAX_K], best[4];
-    __shared__ uint64_t places[4], chosen[BEAM_MAX_K];
-    __shared__ double values[BEAM_MAX_K];
+struct BeamLds {
+    double base[BEAM_MAX_K];     // what a beam's logits are added to (-inf: it has no candidates)
+    int ended[BEAM_MAX_K];
+    float lists[4][64];
+    double score[BEAM_CAP];
+    uint64_t place[BEAM_CAP];
+    double best[4];
+    uint64_t best_place[4];
+    BeamPick picks[BEAM_MAX_K];
+    int count;
+};
+
+ASCA_DEV bool beam_better(double a, uint64_t pa, double b, uint64_t pb) { return a > b || (a == b && pa < pb); }
+
+// The K best of a group's candidates, a block a group.  As a row's selection, with the scores
+// in 64 bits; the threshold compares them rounded to 32, which keeps their order.
+__global__ __launch_bounds__(256) void beam_merge_k(BeamArgs p) {
+    __shared__ BeamLds l;
     const long group = blockIdx.x;
-    const E* z = static_cast<const E*>(p.z) + group * p.K * p.ld;
-    for (int b = 0; b < p.K; ++b) {
-        const double s = p.scores[group * p.K + b];
-        float m;
-        double ls = 0.0, x = -INFINITY;
-        const bool end = p.ended && p.ended[group * p.K + b] != 0;
-        if (!end) row_lse(z + b * p.ld, p.V, 1.0f, m, ls, lds);
-        if (end) x = s;
-        else x = s - ((double)m + ls);
-        if (threadIdx.x == 0) base[b] = beam_finite(s) && beam_finite(x) ? x : (double)-INFINITY;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, K = p.K, per = p.S * K;
+    for (int b = w; b < K; b += 4) {
+        const long row = group * K + b;
+        const double s = p.scores[row];
+        const bool end = p.ended && p.ended[row] != 0, fin = fabs(s) < INFINITY;
+        double x = s;
+        if (fin && !end) x = s - slices_lse(p.sums + row * p.S, p.S, 1.0);
+        if (lane == 0) l.base[b] = fin && fabs(x) < INFINITY ? x : (double)-INFINITY, l.ended[b] = end;
     }
+    if (threadIdx.x < K) l.picks[threadIdx.x] = BeamPick{-INFINITY, -1, 0};
+    if (threadIdx.x == 0) l.count = 0;
     __syncthreads();
-    double last = INFINITY;
-    uint64_t lastp = 0;
-    for (int k = 0; k < p.K; ++k) {
-        double v = -INFINITY;
-        uint64_t vp = ~0ull;
-        auto offer = [&](double x, uint64_t at) {
-            if (!(x < last || (x == last && at > lastp))) return;
-            if (x > v || (x == v && at < vp)) v = x, vp = at;
-        };
-        for (int b = 0; b < p.K; ++b) {
-            if (base[b] == -INFINITY) continue;
-            if (p.ended && p.ended[group * p.K + b] != 0) {
-                if (threadIdx.x == 0) offer(base[b], (uint64_t)b * p.V + p.eos);
+    auto each = [&](auto f) {
+        for (int i = threadIdx.x; i < K * per; i += 256) {
+            const int b = i / per;
+            if (l.base[b] == -INFINITY) continue;
+            if (l.ended[b]) {
+                if (i == b * per) f(l.base[b], (uint64_t)b * p.V + p.eos);
                 continue;
             }
-            for (int c = threadIdx.x; c < p.V; c += 256) {
-                const float t = act_load(z + b * p.ld + c);
-                if (t > -INFINITY) offer(base[b] + t, (uint64_t)b * p.V + c);
-            }
+            const uint64_t key = p.keys[group * K * per + i];
+            if (key) f(l.base[b] + (double)key_value(key), (uint64_t)b * p.V + key_place(key));
         }
-        const double top = block_max_t<4>(v, best);
-        const uint64_t place = ~block_max_t<4>(v == top ? ~vp : (uint64_t)0, places);
-        if (threadIdx.x == 0) values[k] = top, chosen[k] = place;
-        last = top, lastp = place;
+    };
+    float mx = -INFINITY;
+    each([&](double x, uint64_t) { mx = fmaxf(mx, (float)x); });
+    l.lists[w][lane] = lane_sort(mx);
+    __syncthreads();
+    const float ab = lane_merge<64>(fmaxf(l.lists[0][lane], l.lists[1][63 - lane]), true);
+    const float cd = lane_merge<64>(fmaxf(l.lists[2][lane], l.lists[3][63 - lane]), false);
+    const float kth = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_merge<64>(fmaxf(ab, cd), true)), K - 1));
+    each([&](double x, uint64_t at) {
+        if ((float)x < kth) return;
+        const int i = atomicAdd(&l.count, 1);
+        if (i < BEAM_CAP) l.score[i] = x, l.place[i] = at;
+    });
+    __syncthreads();
+    const int n = l.count;
+    auto pick = [&](int rank, double x, uint64_t at) { l.picks[rank] = BeamPick{x, (int)(at / p.V), (unsigned)(at % p.V)}; };
+    if (n <= BEAM_CAP) {
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const double x = l.score[i];
+            const uint64_t at = l.place[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += beam_better(l.score[j], l.place[j], x, at);
+            if (rank < K) pick(rank, x, at);
+        }
+    } else {
+        double last = INFINITY;
+        uint64_t lastp = 0;
+        for (int k = 0; k < K; ++k) {
+            double v = -INFINITY;
+            uint64_t vp = ~0ull;
+            each([&](double x, uint64_t at) {
+                if (beam_better(last, lastp, x, at) && beam_better(x, at, v, vp)) v = x, vp = at;
+            });
+            const double top = block_max_t<4>(v, l.best);
+            const uint64_t place = ~block_max_t<4>(v == top ? ~vp : (uint64_t)0, l.best_place);
+            if (top == -INFINITY) break;
+            if (threadIdx.x == 0) pick(k, top, place);
+            last = top, lastp = place;
+        }
     }
     __syncthreads();
     if (threadIdx.x >= 64) return;
-    BeamPick pick{-INFINITY, -1, 0};
-    if (threadIdx.x < p.K && values[threadIdx.x] > -INFINITY) {
-        pick.score = values[threadIdx.x];
-        pick.parent = (int)(chosen[threadIdx.x] / p.V);
-        pick.token = (unsigned)(chosen[threadIdx.x] % p.V);
-    }
-    beam_write(p, group, pick);
+    beam_write(p, group, lane < K ? l.picks[lane] : BeamPick{-INFINITY, -1, 0});
 }
 
 struct StatesArgs {
@@ -225,6 +440,51 @@ static int rows_check(const char* fn, long rows, int V, long ld, const void* z, 
     return ASCA_OK;
 }
 
+// Slices of the rows and the launch over them; with a.scores, or where a row has more than one,
+// their keys and sums go to scratch (and a.values is cleared).
+//   Rows of up to 64 x 8 pieces are a wave's where there are enough of them for four waves a
+//   CU; else slices are a block's, as many as give about four blocks a CU, between one piece
+//   a thread (shorter ones cost more in the merge than they spread) and eight (32 registers).
+template <typename E>
+static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const char* fn) {
+    constexpr int W = 16 / sizeof(E);
+    const long want = 4l * std::max(cu_count(), 1);
+    const bool wave = a.V <= 64 * 8 * W && (a.rows >= want || a.V <= 64 * W);
+    if (wave) {
+        a.S = 1;
+        a.slice = a.V;
+    } else {
+        const long least = (a.V + 256l * 8 * W - 1) / (256l * 8 * W), most = (a.V + 256l * W - 1) / (256l * W);
+        const long s = std::max(least, std::min(most, (want + a.rows - 1) / a.rows));
+        a.slice = (int)(((a.V + s - 1) / s + W - 1) / W * W);
+        a.S = (a.V + a.slice - 1) / a.slice;
+    }
+    a.ct = (float)(1.4426950408889634 / (double)a.tau);
+    const long units = a.rows * a.S, blocks = wave ? (units + 3) / 4 : units;
+    if (!grid_fits(blocks, 256) || !grid_fits(a.rows, 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows (%ld)", fn, a.rows);
+    if (a.S > 1 || a.scores) {
+        int rc = scratch.get(((size_t)units * a.K + units) * 2, st);
+        if (rc) return rc;
+        a.keys = reinterpret_cast<uint64_t*>(scratch.ws.p);
+        a.sums = reinterpret_cast<float2*>(a.keys + units * a.K);
+        a.values = nullptr;
+    }
+    int rc = pre_launch("top_slice");
+    if (rc) return rc;
+    const dim3 grid((unsigned)blocks), block(256);
+    const int per = (a.slice / W + (wave ? 63 : 255)) / (wave ? 64 : 256);   // pieces a thread
+    auto go = [&](auto nw) {
+        constexpr int NW = decltype(nw)::value;
+        if (per <= 1) hipLaunchKernelGGL((top_slice_k<E, NW, 1>), grid, block, 0, st, a);
+        else if (per <= 2) hipLaunchKernelGGL((top_slice_k<E, NW, 2>), grid, block, 0, st, a);
+        else if (per <= 4) hipLaunchKernelGGL((top_slice_k<E, NW, 4>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((top_slice_k<E, NW, 8>), grid, block, 0, st, a);
+    };
+    if (wave) go(std::integral_constant<int, 1>());
+    else go(std::integral_constant<int, 4>());
+    return post_launch("top_slice");
+}
+
 extern "C" {
 
 int asca_top_logits(const void* logits, long ld, long rows, int V, int K, float temperature, float* values,
@@ -236,15 +496,21 @@ int asca_top_logits(const void* logits, long ld, long rows, int V, int K, float 
     if (!(temperature > 0.0f) || !(temperature < INFINITY))
         return fail(ASCA_ERR_INVALID, "%s: temperature %g", fn, (double)temperature);
     if (rows > 0 && (!logits || !values || !ids)) return fail(ASCA_ERR_INVALID, "null pointer in %s", fn);
-    if (!grid_fits(rows, 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows (%ld)", fn, rows);
+    if (!grid_fits(rows, 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows (%ld)", fn, rows);   // a merge's blocks
+    TopArgs a{};
+    a.z = logits, a.ld = ld, a.rows = rows, a.V = V, a.K = K, a.tau = temperature;
+    a.values = values, a.ids = ids, a.lse = lse;
     return act_dispatch(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
         if (rows == 0) return (int)ASCA_OK;
-        int r = pre_launch("top_logits");
-        if (r) return r;
-        const TopArgs a{logits, ld, rows, V, K, temperature, values, ids, lse};
-        hipLaunchKernelGGL(top_k<E>, dim3((unsigned)rows), dim3(256), 0, as_stream(stream), a);
-        return post_launch("top_logits");
+        const hipStream_t st = as_stream(stream);
+        StreamScratch scratch;
+        int r = top_slices<E>(a, scratch, st, fn);
+        if (r || a.S == 1) return r;
+        a.values = values;
+        if ((r = pre_launch("top_merge"))) return r;
+        hipLaunchKernelGGL(top_merge_k, dim3((unsigned)rows), dim3(256), 0, st, a);
+        return post_launch("top_merge");
     });
 }
 
@@ -261,15 +527,19 @@ int asca_beam_step(const void* logits, long ld, const float* scores, const int32
         if (groups > 0) return fail(ASCA_ERR_INVALID, "%s: eos, ended and new_ended go together", fn);
     if (groups > 0 && (!logits || !scores || !new_scores || !tokens || !parents))
         return fail(ASCA_ERR_INVALID, "null pointer in %s", fn);
-    if (!grid_fits(groups, 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many groups (%d)", fn, groups);
+    TopArgs a{};
+    a.z = logits, a.ld = ld, a.rows = (long)groups * K, a.V = V, a.K = K, a.tau = 1.0f;
+    a.scores = scores, a.ended = ended;
     return act_dispatch(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
         if (groups == 0) return (int)ASCA_OK;
-        int r = pre_launch("beam_step");
-        if (r) return r;
-        const BeamArgs a{logits, ld, scores, ended, new_scores, new_ended, tokens, parents, K, V, eos < 0 ? -1 : eos, stay};
-        hipLaunchKernelGGL(beam_step_k<E>, dim3((unsigned)groups), dim3(256), 0, as_stream(stream), a);
-        return post_launch("beam_step");
+        const hipStream_t st = as_stream(stream);
+        StreamScratch scratch;
+        int r = top_slices<E>(a, scratch, st, fn);
+        if (r || (r = pre_launch("beam_merge"))) return r;
+        const BeamArgs b{scores, ended, new_scores, new_ended, tokens, parents, K, V, a.S, eos < 0 ? -1 : eos, stay, a.keys, a.sums};
+        hipLaunchKernelGGL(beam_merge_k, dim3((unsigned)groups), dim3(256), 0, st, b);
+        return post_launch("beam_merge");
     });
 }
 
