@@ -391,41 +391,60 @@ __global__ __launch_bounds__(256) void beam_merge_k(BeamArgs p) {
 struct StatesArgs {
     const char* src[BEAM_BUFS];
     char* dst[BEAM_BUFS];
-    unsigned long outer[BEAM_BUFS], bytes[BEAM_BUFS];
-    unsigned long first[BEAM_BUFS + 1];   // blocks before each buffer's
+    unsigned long bytes[BEAM_BUFS];
+    unsigned first[BEAM_BUFS], chunks[BEAM_BUFS];   // blocks before each buffer's; blocks a state
     const int32_t* parents;
     int count, groups, ks, kd;
 };
 
-// A block takes 256 words of the states of one group in one outer row.  A thread reads its
-// words of all the slots that change before it writes any, so that a buffer may be its own
-// destination; no other thread touches them.
-template <typename W>
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// Words a thread moves for each of up to KM slots: 64 registers of 16-byte words (128 with KM = 32).
+// Two for KM = 4 were as fast where states move and twice as slow where none does (19 us of empty
+// blocks for 128 x 4 x 1 MB); a loop over several runs a block cost 7% where they do.
+template <int KM>
+constexpr int st_u() { return KM <= 4 ? 4 : KM <= 8 ? 2 : 1; }
+
+// A block takes 256 U words of the states of one group in one outer row.  A thread reads its
+// words of the slots that change before it writes any, so that a buffer may be its own
+// destination; no other thread touches them.  What several slots take from one parent comes
+// from memory once, then from a cache.
+template <typename W, int KM>
 __global__ __launch_bounds__(256) void beam_states_k(StatesArgs p) {
+    constexpr int U = st_u<KM>();
     int i = 0;
     while (i + 1 < p.count && blockIdx.x >= p.first[i + 1]) ++i;
-    const unsigned long words = p.bytes[i] / sizeof(W), per = (words + 255) / 256;
-    unsigned long b = blockIdx.x - p.first[i];
-    const unsigned long w = b % per * 256 + threadIdx.x;
-    b /= per;
-    const long group = b % p.groups, outer = b / p.groups;
-    if (w >= words) return;
-    const W* src = reinterpret_cast<const W*>(p.src[i]) + (outer * p.groups + group) * p.ks * words + w;
-    W* dst = reinterpret_cast<W*>(p.dst[i]) + (outer * p.groups + group) * p.kd * words + w;
-    W v[BEAM_MAX_K];
-    auto from = [&](int j) {
-        const int q = p.parents ? p.parents[group * p.kd + j] : 0;
-        return q < 0 || q >= p.ks || (src == dst && q == j) ? -1 : q;
-    };
+    const unsigned b = blockIdx.x - p.first[i], unit = b / p.chunks[i], group = unit % p.groups;
+    const unsigned long words = p.bytes[i] / sizeof(W), at = (unsigned long)(b % p.chunks[i]) * (256 * U) + threadIdx.x;
+    const W* src = reinterpret_cast<const W*>(p.src[i]) + (unsigned long)unit * p.ks * words;
+    W* dst = reinterpret_cast<W*>(p.dst[i]) + (unsigned long)unit * p.kd * words;
+    int from[KM];   // the slot that is read, -1 where nothing changes
 #pragma unroll
-    for (int j = 0; j < BEAM_MAX_K; ++j)
-        if (j < p.kd) {
-            const int q = from(j);
-            if (q >= 0) v[j] = src[q * words];
-        }
+    for (int j = 0; j < KM; ++j) {
+        const int q = j < p.kd ? p.parents ? p.parents[(long)group * p.kd + j] : 0 : -1;
+        from[j] = q < 0 || q >= p.ks || (src == dst && q == j) ? -1 : q;
+    }
+    W v[KM][U];
 #pragma unroll
-    for (int j = 0; j < BEAM_MAX_K; ++j)
-        if (j < p.kd && from(j) >= 0) dst[j * words] = v[j];
+    for (int j = 0; j < KM; ++j)
+        if (from[j] >= 0)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (at + u * 256 < words) v[j][u] = src[from[j] * words + at + u * 256];
+#pragma unroll
+    for (int j = 0; j < KM; ++j)
+        if (from[j] >= 0)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (at + u * 256 < words) dst[j * words + at + u * 256] = v[j][u];
+}
+
+template <typename W>
+static void beam_states_launch(const StatesArgs& a, dim3 grid, hipStream_t st) {
+    if (a.kd <= 4) hipLaunchKernelGGL((beam_states_k<W, 4>), grid, dim3(256), 0, st, a);
+    else if (a.kd <= 8) hipLaunchKernelGGL((beam_states_k<W, 8>), grid, dim3(256), 0, st, a);
+    else if (a.kd <= 16) hipLaunchKernelGGL((beam_states_k<W, 16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((beam_states_k<W, 32>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace asca
@@ -556,6 +575,7 @@ int asca_beam_states(void** src, void** dst, const uint64_t* outer, const uint64
     a.groups = groups;
     a.ks = k_src;
     a.kd = k_dst;
+    uint64_t rows[BEAM_BUFS];
     unsigned word = 16;
     for (int i = 0; i < count; ++i) {
         if (outer[i] > (uint64_t)1 << 40 || bytes[i] > (uint64_t)1 << 40)
@@ -577,26 +597,28 @@ int asca_beam_states(void** src, void** dst, const uint64_t* outer, const uint64
         const int n = a.count++;
         a.src[n] = static_cast<const char*>(src[i]);
         a.dst[n] = static_cast<char*>(d);
-        a.outer[n] = outer[i];
         a.bytes[n] = bytes[i];
+        rows[n] = outer[i];
     }
     if (a.count == 0) return ASCA_OK;
-    __uint128_t blocks = 0;
+    const uint64_t step = 256ull * word * (k_dst <= 4 ? st_u<4>() : k_dst <= 8 ? st_u<8>() : st_u<32>());
+    uint64_t blocks = 0;
     for (int i = 0; i < a.count; ++i) {
-        a.first[i] = (unsigned long)blocks;
-        blocks += (__uint128_t)((a.bytes[i] / word + 255) / 256) * a.outer[i] * groups;
-        if (blocks >= (1ul << 24)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too much to move in one call", fn);
+        const uint64_t chunks = (a.bytes[i] + step - 1) / step;
+        const __uint128_t n = (__uint128_t)chunks * rows[i] * groups + blocks;
+        if (n >= (uint64_t)1 << 40 || !grid_fits((long)n, 256))
+            return fail(ASCA_ERR_UNSUPPORTED, "%s: too much to move in one call", fn);
+        a.first[i] = (unsigned)blocks;
+        a.chunks[i] = (unsigned)chunks;
+        blocks = (uint64_t)n;
     }
     int rc = pre_launch("beam_states");
     if (rc) return rc;
     const dim3 grid((unsigned)blocks);
     const hipStream_t st = as_stream(stream);
-    if (word == 16)
-        hipLaunchKernelGGL(beam_states_k<uint4>, grid, dim3(256), 0, st, a);
-    else if (word == 4)
-        hipLaunchKernelGGL(beam_states_k<uint32_t>, grid, dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL(beam_states_k<uint8_t>, grid, dim3(256), 0, st, a);
+    if (word == 16) beam_states_launch<u32x4>(a, grid, st);
+    else if (word == 4) beam_states_launch<uint32_t>(a, grid, st);
+    else beam_states_launch<uint8_t>(a, grid, st);
     return post_launch("beam_states");
 }
 
