@@ -7,6 +7,8 @@
 //   dz_i / scale = w [(1 - a) (softmax(z)_i - [i = target]) + a tau (q_i - p_i)] for listed i, for
 //   the others q_i (1 - p_r / q_r) in the place of q_i - p_i (without tlse q_i)
 // Entries of one id are one entry with the sum of their p.
+#include <algorithm>
+
 #include "logits.h"
 #include "ops.h"
 
@@ -27,130 +29,468 @@ struct DistillArgs {
     void* dz;
     long lddz, T;
     int V, K;
-    float tau, alpha, scale;
+    float tau, ct, alpha, scale;   // ct = log2(e) / tau
 };
 
-// The lists' entries of a row, one a lane of every wave
+// An entry of a row's list, one a lane
 struct Entry {
-    int id;        // below 0: none
-    float z;       // the student's logit there
-    double lp;     // log p (-inf: p = 0)
+    int id;       // below 0: none
+    float z;      // the student's logit there
+    double lp;    // log p
     float p;
 };
 
-ASCA_DEV double wave_sum_d(double x) { return wave_sum_t(x); }
+// exp(x) of a double, to f32's precision: the argument's rounding is put back
+ASCA_DEV float exp_d(double x) {
+    const double y = x * 1.4426950408889634;
+    const float h = (float)y;
+    return h > -INFINITY ? __builtin_amdgcn_exp2f(h) * (1.0f + (float)(y - h) * 0.693147181f) : h == -INFINITY ? 0.0f : h;
+}
+// log(x) to 2^-24 (not relative to a large result): that of the exponent in 64 bits
+ASCA_DEV double log_d(float x) {
+    float m = __builtin_amdgcn_frexp_mantf(x);   // 0.5 to 1
+    int e = __builtin_amdgcn_frexp_expf(x);
+    if (m < 0.70710678f) m *= 2.0f, --e;
+    return ((double)e + (double)__builtin_amdgcn_logf(m)) * LN2;
+}
 
+// p of a row's entries (id and the teacher's logit in lp), in a wave; `twice`: some id may
+// be there more than once.  The first of one id's entries has their sum, the others are none.
+ASCA_DEV void entry_probs(const DistillArgs& p, long row, bool twice, Entry& en, float& total, float& rest) {
+    const int lane = threadIdx.x & 63;
+    const double itau = 1.0 / (double)p.tau;
+    const bool on = en.id >= 0;
+    if (p.tlse) {
+        en.lp = en.lp * itau - (double)p.tlse[row];
+        en.p = on ? exp_d(en.lp) : 0.0f;
+    } else {
+        const float v = on ? (float)en.lp : -INFINITY, m = wave_max(v);   // a NaN is not the largest
+        if (m == -INFINITY) {
+            en.lp = -INFINITY;   // no entry, or none above -inf
+            en.p = on && v != v ? v : 0.0f;
+        } else {
+            en.lp = (en.lp - (double)m) * itau;
+            const float e = on ? exp_d(en.lp) : 0.0f, s = wave_sum(e);
+            en.lp -= log_d(s);
+            en.p = e / s;
+        }
+    }
+    if (twice)
+        for (int j = 0; j < p.K; ++j) {
+            const int id = __builtin_amdgcn_readlane(en.id, j);
+            const uint64_t same = __ballot(en.id == id);
+            if (id < 0 || (same & (same - 1)) == 0) continue;
+            const float sum = wave_sum(en.id == id ? en.p : 0.0f);
+            if (lane == j) en.p = sum, en.lp = log_d(sum);
+            else if (en.id == id) en.id = -1, en.p = 0.0f;
+        }
+    total = wave_sum(en.p);
+    rest = p.tlse ? fmaxf(0.0f, 1.0f - total) : 0.0f;
+}
+
+// The sums over the columns outside the list: the largest of them and their exponentials'
+// sums from it, at the temperature and at 1
+struct Outside {
+    float m, st, s1;
+};
+ASCA_DEV Outside outside_join(Outside a, Outside b, float ct, bool two) {
+    const float m = fmaxf(a.m, b.m), ref = m > -INFINITY ? m : 0.0f;   // sums of nothing are 0, or NaN
+    auto at = [&](float x, float s, float c) { return x > -INFINITY ? s * __builtin_amdgcn_exp2f((x - ref) * c) : s; };
+    return {m, at(a.m, a.st, ct) + at(b.m, b.st, ct), two ? at(a.m, a.s1, LOG2E) + at(b.m, b.s1, LOG2E) : 0.0f};
+}
+
+// What a row's loss and gradient are made of
+struct Coefs {
+    float mr;          // the others' exponentials are measured from it, the entries' from mx
+    float As, Bt;      // dz of the others: As exp((z - mr) / tau) + Bt exp(z - mr)
+    float Qs, Bs;      // of an entry: Qs exp((z - mx) / tau) + Bs exp(z - mx) - gs p
+    float gs, gh, mx;  // gh is taken off at the target
+};
+
+// From the others' sums and the entries, in a wave; the loss where it is wanted.
+// Where the temperatures are one, or only one counts, `two` is false and one sum serves both.
+template <bool TWO>
+ASCA_DEV Coefs distill_coefs(const DistillArgs& p, float w, const Entry& en, float total, float rest, Outside o, bool has_tg, float zt,
+                             bool want, float& loss) {
+    const bool on = en.id >= 0;
+    const float mx = fmaxf(o.m, wave_max(on ? en.z : -INFINITY));   // of the row
+    Coefs c;
+    c.mx = mx;
+    c.mr = o.m > -INFINITY ? o.m : mx;
+    const float ft = __builtin_amdgcn_exp2f((c.mr - mx) * p.ct), f1 = TWO ? __builtin_amdgcn_exp2f((c.mr - mx) * LOG2E) : ft;
+    const float et = on ? __builtin_amdgcn_exp2f((en.z - mx) * p.ct) : 0.0f;
+    const float at = o.st * ft + wave_sum(et);
+    float a1 = at;
+    if (TWO) a1 = o.s1 * f1 + wave_sum(on ? __builtin_amdgcn_exp2f((en.z - mx) * LOG2E) : 0.0f);
+    const bool tail = rest > 0.0f && o.st > 0.0f;
+    if (want) {
+        const double itau = 1.0 / (double)p.tau, lse = (double)mx * itau + log_d(at);
+        float kl = wave_sum(on && en.p != 0.0f ? (float)((double)en.p * (en.lp - ((double)en.z * itau - lse))) : 0.0f);
+        double l = 0.0;
+        if (p.alpha > 0.0f) {
+            l = kl;
+            if (tail) l += (double)rest * (log_d(rest) - (log_d(o.st) + (double)c.mr * itau - lse));
+            l *= (double)p.alpha * p.tau * p.tau;
+        }
+        if (has_tg) l += (1.0 - (double)p.alpha) * ((double)mx + log_d(a1) - (double)zt);
+        loss = (float)(l * (double)w);
+    }
+    c.gs = p.scale * w * p.alpha * p.tau;
+    c.gh = has_tg ? p.scale * w * (1.0f - p.alpha) : 0.0f;
+    // the sum of p that the gradient meets: a rest that the student cannot give is left out
+    const float mass = tail ? 1.0f : total;
+    c.Qs = c.gs * mass / at;
+    c.As = c.gs * (mass * ft / at - (tail ? rest / o.st : 0.0f));
+    c.Bs = c.gh / a1;
+    c.Bt = c.gh * f1 / a1;
+    if (!TWO) c.As += c.Bt, c.Qs += c.Bs;
+    return c;
+}
+
+template <bool TWO>
+ASCA_DEV float grad_other(const Coefs& c, float ct, float z) {
+    const float x = z - c.mr;
+    const float g = c.As * __builtin_amdgcn_exp2f(x * ct);
+    return TWO ? g + c.Bt * __builtin_amdgcn_exp2f(x * LOG2E) : g;
+}
+template <bool TWO>
+ASCA_DEV float grad_entry(const Coefs& c, float ct, float z, float prob, bool target) {
+    const float x = z - c.mx;
+    const float g = c.Qs * __builtin_amdgcn_exp2f(x * ct) + (TWO ? c.Bs * __builtin_amdgcn_exp2f(x * LOG2E) : 0.0f);
+    return g - c.gs * prob - (target ? c.gh : 0.0f);
+}
+
+template <int NW, int WORDS>
+struct DistillLds {
+    unsigned bits[WORDS];   // a bit for every column of a piece: it is listed
+    unsigned edge;          // and of those outside the pieces, by thread
+    Outside part[NW];
+    float z[64], p[64];     // the entries
+    int id[64];
+    float total, rest, zt;  // zt: the student's logit at the target
+};
+
+template <int NW>
+ASCA_DEV void distill_sync() {
+    if constexpr (NW == 1) {   // a wave's own LDS accesses, in order
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        lds_barrier();         // the row's loads stay in flight
+    }
+}
+
+// V values of a piece to the same place in another row of the same alignment
+ASCA_DEV void piece_store(float* d, const float (&v)[4]) { act_store_n<4>(d, v); }
+ASCA_DEV void piece_store(bf16_t* d, const float (&v)[8]) {
+    unsigned u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        bf16_t b[2];
+        act_store(b, v[2 * k]), act_store(b + 1, v[2 * k + 1]);
+        u[k] = b[0] | (unsigned)b[1] << 16;
+    }
+    *reinterpret_cast<uint4*>(d) = make_uint4(u[0], u[1], u[2], u[3]);
+}
 template <typename E>
-__global__ __launch_bounds__(256) void distill_k(DistillArgs p) {
-    extern __shared__ unsigned bits[];   // a bit for every column: it is listed
-    __shared__ float lds[4];
+ASCA_DEV void row_piece_store(E* d, bool whole, const float (&v)[16 / sizeof(E)]) {
+    if (whole) {
+        piece_store(d, v);
+    } else {   // the gradient's rows lie otherwise
+#pragma unroll
+        for (int k = 0; k < 16 / (int)sizeof(E); ++k) act_store(d + k, v[k]);
+    }
+}
+
+// Rows in the registers of a team of NW waves, R pieces a thread: a row is read once and its
+// gradient written once.  The list's columns are taken out by a bitmap in LDS, so that the
+// others' sum is formed without them (a difference of sums would lose it where the student is
+// sure of the list); the list's own terms are added from one wave's lanes.
+template <typename E, int NW, int R, bool TWO>
+__global__ __launch_bounds__(NW == 16 ? 1024 : 256) void distill_rows_k(DistillArgs p) {
+    constexpr int NT = 64 * NW, W = Pieces<E>::W, WORDS = NT * R * W / 32, TEAMS = NW == 1 ? 4 : 1;
+    __shared__ DistillLds<NW, WORDS> lds[TEAMS];
+    const int team = NW == 1 ? threadIdx.x >> 6 : 0, tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6;
+    const long row = (long)blockIdx.x * TEAMS + team;
+    if (row >= p.T) return;
+    DistillLds<NW, WORDS>& l = lds[team];
+    const E* z = static_cast<const E*>(p.z) + row * p.ld;
+    E* dz = p.dz ? static_cast<E*>(p.dz) + row * p.lddz : nullptr;
+    const float w = p.weights ? p.weights[row] : 1.0f;
+    if (w == 0.0f) {
+        if (tid == 0) p.losses[row] = 0.0f;
+        if (dz)
+            for (int c = tid; c < p.V; c += NT) act_store(dz + c, 0.0f);
+        return;
+    }
+    const bool lists = wave == 0 && lane < p.K;
+    Entry en{-1, 0.0f, 0.0, 0.0f};
+    float tv = 0.0f;
+    if (lists) en.id = p.tids[row * p.K + lane], tv = p.tval[row * p.K + lane];
+    const unsigned tg = p.alpha < 1.0f ? p.targets[row] : ~0u;
+    const Pieces<E> r(z, p.V);
+    uint4 raw[R];
+    if (r.nb > 0)
+#pragma unroll
+        for (int j = 0; j < R; ++j) raw[j] = r.piece(min(j * NT + tid, r.nb - 1));
+    const int ec = r.edge(tid);
+    float ev = -INFINITY;
+    if (ec >= 0) ev = act_load(z + ec);
+    const bool has_tg = tg < (unsigned)p.V;
+#pragma unroll
+    for (int i = tid; i < WORDS; i += NT) l.bits[i] = 0;
+    if (tid == 0) l.edge = 0;
+    distill_sync<NW>();
+    if (wave == 0) {
+        bool twice = false;
+        const float zt = has_tg ? act_load(z + tg) : 0.0f;
+        if (en.id >= p.V) en.id = -1;
+        en.lp = tv;
+        if (en.id >= 0) {
+            en.z = act_load(z + en.id);
+            const int rel = en.id - r.head;
+            const bool in = rel >= 0 && rel < r.nb * W;
+            const unsigned bit = 1u << (in ? rel & 31 : r.edge_thread(en.id));
+            twice = (atomicOr(in ? &l.bits[rel >> 5] : &l.edge, bit) & bit) != 0;
+        }
+        float total, rest;
+        entry_probs(p, row, __ballot(twice) != 0, en, total, rest);
+        l.id[lane] = en.id, l.z[lane] = en.z, l.p[lane] = en.p;
+        if (lane == 0) l.total = total, l.rest = rest, l.zt = zt;
+    }
+    distill_sync<NW>();
+    // the list out of the row, and the others' largest and sums, a wave's own first
+    float v[W];
+    Outside o{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const int i = j * NT + tid;
+        const unsigned bits = l.bits[i * W / 32] >> (i * W % 32) & ((1u << W) - 1);
+        if (i >= r.nb) raw[j] = piece_of<E>(-INFINITY);
+        if (__ballot(bits != 0)) piece_mask(raw[j], bits, E());
+        piece_again(raw[j]);
+        piece_values(raw[j], v);
+#pragma unroll
+        for (int k = 0; k < W; ++k) o.m = fmaxf(o.m, v[k]);
+        if (R >= 8) __builtin_amdgcn_sched_barrier(0);   // one piece's values in registers at a time
+    }
+    if (l.edge >> (tid & 31) & 1 && tid < 2 * W) ev = -INFINITY;
+    o.m = wave_max(fmaxf(o.m, ev));
+    const float ref = o.m > -INFINITY ? o.m : 0.0f;
+    o.st = __builtin_amdgcn_exp2f((ev - ref) * p.ct);
+    if (TWO) o.s1 = __builtin_amdgcn_exp2f((ev - ref) * LOG2E);
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        piece_again(raw[j]);
+        piece_values(raw[j], v);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            o.st += __builtin_amdgcn_exp2f((v[k] - ref) * p.ct);
+            if (TWO) o.s1 += __builtin_amdgcn_exp2f((v[k] - ref) * LOG2E);
+        }
+        if (R >= 8) __builtin_amdgcn_sched_barrier(0);
+    }
+    o.st = wave_sum(o.st);
+    if (TWO) o.s1 = wave_sum(o.s1);
+    if constexpr (NW > 1) {
+        if (lane == 0) l.part[wave] = o;
+        lds_barrier();
+        o = l.part[0];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) o = outside_join(o, l.part[k], p.ct, TWO);
+        if (wave != 0) en.id = l.id[lane], en.z = l.z[lane], en.p = l.p[lane];
+    }
+    float loss = 0.0f;
+    const float zt = l.zt;
+    const Coefs c = distill_coefs<TWO>(p, w, en, l.total, l.rest, o, has_tg, zt, wave == 0, loss);
+    if (tid == 0) p.losses[row] = loss;
+    if (!dz) return;
+    const bool whole = (reinterpret_cast<uintptr_t>(dz) - reinterpret_cast<uintptr_t>(z)) % 16 == 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const int i = j * NT + tid;
+        piece_again(raw[j]);
+        piece_values(raw[j], v);
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[k] = grad_other<TWO>(c, p.ct, v[k]);
+        if (i < r.nb) row_piece_store<E>(dz + r.col(i), whole, v);
+        if (R >= 8) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (ec >= 0) act_store(dz + ec, grad_other<TWO>(c, p.ct, ev));
+    // the list's columns and the target's, over what was written there just now: by the wave that
+    // wrote it, whose stores to an address stay in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    auto mine = [&](int col) {
+        const int rel = col - r.head;
+        return NW == 1 || (rel >= 0 && rel < r.nb * W ? rel / W % NT / 64 : 0) == wave;
+    };
+    if (en.id >= 0 && mine(en.id)) act_store(dz + en.id, grad_entry<TWO>(c, p.ct, en.z, en.p, (unsigned)en.id == tg));
+    const bool tg_listed = __ballot(has_tg && en.id == (int)tg) != 0;
+    if (lane == 0 && has_tg && !tg_listed && mine(tg)) act_store(dz + tg, grad_other<TWO>(c, p.ct, zt) - c.gh);
+}
+
+// Rows that no team's registers hold: read twice, by 1024 threads, the second time mostly from
+// a cache (256 rows of 131072 f32 are half of the last-level one's)
+template <typename E, bool TWO>
+__global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
+    constexpr int NW = 16, NT = 1024, W = Pieces<E>::W, U = 4;
+    extern __shared__ unsigned bits[];
+    __shared__ DistillLds<NW, 1> l;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const long row = blockIdx.x;
     const E* z = static_cast<const E*>(p.z) + row * p.ld;
     E* dz = p.dz ? static_cast<E*>(p.dz) + row * p.lddz : nullptr;
-    const int V = p.V, lane = threadIdx.x & 63;
     const float w = p.weights ? p.weights[row] : 1.0f;
     if (w == 0.0f) {
-        if (threadIdx.x == 0) p.losses[row] = 0.0f;
+        if (tid == 0) p.losses[row] = 0.0f;
         if (dz)
-            for (int c = threadIdx.x; c < V; c += 256) act_store(dz + c, 0.0f);
+            for (int c = tid; c < p.V; c += NT) act_store(dz + c, 0.0f);
         return;
     }
-    for (int i = threadIdx.x; i < (V + 31) / 32; i += 256) bits[i] = 0;
-    __syncthreads();
-    const bool soft = p.alpha > 0.0f, hard = p.alpha < 1.0f;
-    const unsigned tg = hard ? p.targets[row] : ~0u;
-    const bool has_tg = tg < (unsigned)V;
-    const float zt = has_tg ? act_load(z + tg) : 0.0f;
-    // entries
-    Entry en{-1, 0.0f, -INFINITY, 0.0f};
-    if (soft && lane < p.K) en.id = p.tids[row * p.K + lane];
-    if (en.id >= V) en.id = -1;
-    const double itau = 1.0 / (double)p.tau;
-    if (en.id >= 0) {
-        en.z = act_load(z + en.id);
-        en.lp = (double)p.tval[row * p.K + lane] * itau;
-        atomicOr(&bits[en.id >> 5], 1u << (en.id & 31));
-    }
-    if (p.tlse) {
-        en.lp -= soft ? (double)p.tlse[row] : 0.0;
-    } else {
-        const double m = wave_max_t(en.id >= 0 ? en.lp : (double)-INFINITY);
-        if (m == -INFINITY) {
-            en.lp = -INFINITY;   // no entry, or none above -inf
-        } else {
-            en.lp -= m;
-            en.lp -= log(wave_sum_d(en.id >= 0 ? exp(en.lp) : 0.0));
+    Entry en{-1, 0.0f, 0.0, 0.0f};
+    float tv = 0.0f;
+    if (wave == 0 && lane < p.K) en.id = p.tids[row * p.K + lane], tv = p.tval[row * p.K + lane];
+    const unsigned tg = p.alpha < 1.0f ? p.targets[row] : ~0u;
+    const bool has_tg = tg < (unsigned)p.V;
+    const Pieces<E> r(z, p.V);
+    const int words = (r.nb * W + 31) / 32;
+    for (int i = tid; i < words; i += NT) bits[i] = 0;
+    if (tid == 0) l.edge = 0;
+    const int ec = r.edge(tid);
+    float ev = -INFINITY;
+    if (ec >= 0) ev = act_load(z + ec);
+    lds_barrier();
+    if (wave == 0) {
+        bool twice = false;
+        const float zt = has_tg ? act_load(z + tg) : 0.0f;
+        if (en.id >= p.V) en.id = -1;
+        en.lp = tv;
+        if (en.id >= 0) {
+            en.z = act_load(z + en.id);
+            const int rel = en.id - r.head;
+            const bool in = rel >= 0 && rel < r.nb * W;
+            const unsigned bit = 1u << (in ? rel & 31 : r.edge_thread(en.id));
+            twice = (atomicOr(in ? &bits[rel >> 5] : &l.edge, bit) & bit) != 0;
         }
+        float total, rest;
+        entry_probs(p, row, __ballot(twice) != 0, en, total, rest);
+        l.id[lane] = en.id, l.z[lane] = en.z, l.p[lane] = en.p;
+        if (lane == 0) l.total = total, l.rest = rest, l.zt = zt;
     }
-    double pd = en.id >= 0 ? exp(en.lp) : 0.0;
-    const double total = wave_sum_d(pd);
-    // entries of one id: the first has their sum, the others are none
-    for (int j = 0; j < p.K && soft; ++j) {
-        const int id = __builtin_amdgcn_readlane(en.id, j);
-        if (id < 0) continue;
-        const uint64_t same = __ballot(en.id == id);
-        if ((same & (same - 1)) == 0) continue;
-        const double sum = wave_sum_d(en.id == id ? pd : 0.0);
-        if (lane == j) pd = sum, en.lp = log(sum);
-        else if (en.id == id) en.id = -1, pd = 0.0;
+    lds_barrier();
+    if (tid < 2 * W && l.edge >> tid & 1) ev = -INFINITY;
+    Outside o{ev, 0.0f, 0.0f};
+    {
+        const float ref = ev > -INFINITY ? ev : 0.0f;
+        o.st = __builtin_amdgcn_exp2f((ev - ref) * p.ct);   // 1, 0 or NaN
+        o.s1 = o.st;
     }
-    en.p = (float)pd;
-    const bool rest = p.tlse != nullptr && soft;
-    const float pr = rest ? (float)fmax(0.0, 1.0 - total) : 0.0f;
-    __syncthreads();
-    // the columns outside the list: their largest, and their sums at both temperatures
-    const float ct = (float)(itau * 1.4426950408889634), c1 = LOG2E;
-    auto listed = [&](int c) { return bits[c >> 5] >> (c & 31) & 1; };
-    float m = -INFINITY, mx = en.id >= 0 ? en.z : -INFINITY;
-    for (int c = threadIdx.x; c < V; c += 256)
-        if (!listed(c)) m = fmaxf(m, act_load(z + c));
-    m = block_max_t<4>(m, lds);
-    mx = fmaxf(m, wave_max_t(mx));
-    const float mr = m > -INFINITY ? m : mx;   // what the others are measured from
-    float st = 0.0f, s1 = 0.0f;
-    for (int c = threadIdx.x; c < V; c += 256)
-        if (!listed(c)) {
-            const float v = act_load(z + c);
-            st += __builtin_amdgcn_exp2f((v - mr) * ct);
-            s1 += __builtin_amdgcn_exp2f((v - mr) * c1);
+    for (int i0 = tid; i0 < r.nb; i0 += U * NT) {
+        uint4 raw[U];
+        Outside n{-INFINITY, 0.0f, 0.0f};
+        float v[W];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = r.piece(min(i0 + u * NT, r.nb - 1));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * NT;
+            if (i >= r.nb) raw[u] = piece_of<E>(-INFINITY);
+            else piece_mask(raw[u], bits[i * W / 32] >> (i * W % 32) & ((1u << W) - 1), E());
+            piece_values(raw[u], v);
+#pragma unroll
+            for (int k = 0; k < W; ++k) n.m = fmaxf(n.m, v[k]);
         }
-    st = block_sum_t<4>(st, lds);
-    s1 = block_sum_t<4>(s1, lds);
-    const float et = en.id >= 0 ? __builtin_amdgcn_exp2f((en.z - mx) * ct) : 0.0f;
-    const float e1 = en.id >= 0 ? __builtin_amdgcn_exp2f((en.z - mx) * c1) : 0.0f;
-    const float ft = __builtin_amdgcn_exp2f((mr - mx) * ct), f1 = __builtin_amdgcn_exp2f((mr - mx) * c1);
-    const float at = st * ft + wave_sum(et), a1 = s1 * f1 + wave_sum(e1);   // of all columns, from mx
-    const bool tail = pr > 0.0f && st > 0.0f;
-    // loss
-    if (threadIdx.x < 64) {
-        const double lse = (double)mx * itau + log((double)at);
-        double kl = en.id >= 0 && en.p > 0.0f ? pd * (en.lp - ((double)en.z * itau - lse)) : 0.0;
-        kl = wave_sum_d(kl);
-        if (tail) kl += (double)pr * (log((double)pr) - (log((double)st) + (double)mr * itau - lse));
-        double loss = soft ? (double)p.alpha * p.tau * p.tau * kl : 0.0;
-        if (has_tg) loss += (1.0 - (double)p.alpha) * ((double)mx + log((double)a1) - (double)zt);
-        if (threadIdx.x == 0) p.losses[row] = (float)(loss * w);
+        const float ref = n.m > -INFINITY ? n.m : 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            piece_values(raw[u], v);
+#pragma unroll
+            for (int k = 0; k < W; ++k) {
+                n.st += __builtin_amdgcn_exp2f((v[k] - ref) * p.ct);
+                if (TWO) n.s1 += __builtin_amdgcn_exp2f((v[k] - ref) * LOG2E);
+            }
+        }
+        o = outside_join(o, n, p.ct, TWO);
     }
+    {
+        const float m = wave_max(o.m);
+        const Outside n = outside_join(o, {m, 0.0f, 0.0f}, p.ct, TWO);
+        o = {m, wave_sum(n.st), TWO ? wave_sum(n.s1) : 0.0f};
+    }
+    if (lane == 0) l.part[wave] = o;
+    lds_barrier();
+    o = l.part[0];
+    for (int k = 1; k < NW; ++k) o = outside_join(o, l.part[k], p.ct, TWO);
+    if (wave != 0) en.id = l.id[lane], en.z = l.z[lane], en.p = l.p[lane];
+    float loss = 0.0f;
+    const float zt = l.zt;
+    const Coefs c = distill_coefs<TWO>(p, w, en, l.total, l.rest, o, has_tg, zt, wave == 0, loss);
+    if (tid == 0) p.losses[row] = loss;
     if (!dz) return;
-    const float gs = p.scale * w * p.alpha * p.tau, gh = has_tg ? p.scale * w * (1.0f - p.alpha) : 0.0f;
-    // the sum of p that the gradient meets: a rest that the student cannot give is left out
-    const float mass = tail ? 1.0f : (float)total;
-    const float Qs = gs * mass / at, As = gs * (mass * ft / at - (tail ? pr / st : 0.0f));
-    const float Bt = gh * f1 / a1, Bs = gh / a1;
-    __syncthreads();   // every wave has read what it needs of the row: dz may be z
-    for (int c = threadIdx.x; c < V; c += 256) {
-        if (listed(c) || (has_tg && (unsigned)c == tg)) continue;
-        const float v = act_load(z + c) - mr;
-        float g = As * __builtin_amdgcn_exp2f(v * ct);
-        if (gh != 0.0f) g += Bt * __builtin_amdgcn_exp2f(v * c1);
-        act_store(dz + c, g);
+    const bool whole = (reinterpret_cast<uintptr_t>(dz) - reinterpret_cast<uintptr_t>(z)) % 16 == 0;
+    // (dz may be z: a thread writes the pieces that it reads, and all have read the entries)
+    for (int i0 = tid; i0 < r.nb; i0 += U * NT) {
+        uint4 raw[U];
+        float v[W];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = r.piece(min(i0 + u * NT, r.nb - 1));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * NT;
+            piece_values(raw[u], v);
+#pragma unroll
+            for (int k = 0; k < W; ++k) v[k] = grad_other<TWO>(c, p.ct, v[k]);
+            if (i < r.nb) row_piece_store<E>(dz + r.col(i), whole, v);
+        }
     }
-    if (threadIdx.x < 64 && en.id >= 0)
-        act_store(dz + en.id, Qs * et - gs * en.p + Bs * e1 - ((unsigned)en.id == tg ? gh : 0.0f));
-    if (threadIdx.x == 0 && has_tg && !listed(tg)) {
-        const float v = zt - mr;
-        act_store(dz + tg, As * __builtin_amdgcn_exp2f(v * ct) + Bt * __builtin_amdgcn_exp2f(v * c1) - gh);
+    if (ec >= 0) act_store(dz + ec, grad_other<TWO>(c, p.ct, ev));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // as in distill_rows_k
+    auto mine = [&](int col) {
+        const int rel = col - r.head;
+        return (rel >= 0 && rel < r.nb * W ? rel / W % NT / 64 : 0) == wave;
+    };
+    if (en.id >= 0 && mine(en.id)) act_store(dz + en.id, grad_entry<TWO>(c, p.ct, en.z, en.p, (unsigned)en.id == tg));
+    const bool tg_listed = __ballot(has_tg && en.id == (int)tg) != 0;
+    if (lane == 0 && has_tg && !tg_listed && mine(tg)) act_store(dz + tg, grad_other<TWO>(c, p.ct, zt) - c.gh);
+}
+
+template <typename E, bool TWO>
+static int distill_launch(const DistillArgs& a, hipStream_t st) {
+    constexpr int W = 16 / sizeof(E);
+    const long pieces = (a.V + W - 1) / W;
+    int r;
+    if (pieces > 1024 * 16) {
+        const size_t lds = ((size_t)a.V + 31) / 32 * 4;
+        if ((r = allow_lds(reinterpret_cast<const void*>(&distill_long_k<E, TWO>), lds))) return r;
+        if ((r = pre_launch("distill_long"))) return r;
+        hipLaunchKernelGGL((distill_long_k<E, TWO>), dim3((unsigned)a.T), dim3(1024), lds, st, a);
+        return post_launch("distill_long");
     }
+    if ((r = pre_launch("distill_rows"))) return r;
+    const bool many = a.T >= 4l * std::max(cu_count(), 1);
+    auto go = [&](auto nw, auto rr) {
+        constexpr int NW = decltype(nw)::value, R = decltype(rr)::value;
+        hipLaunchKernelGGL((distill_rows_k<E, NW, R, TWO>), dim3((unsigned)(NW == 1 ? (a.T + 3) / 4 : a.T)), dim3(NW == 16 ? 1024 : 256), 0,
+                           st, a);
+    };
+    std::integral_constant<int, 1> n1;
+    std::integral_constant<int, 2> n2;
+    std::integral_constant<int, 4> n4;
+    std::integral_constant<int, 8> n8;
+    std::integral_constant<int, 16> n16;
+    if (pieces <= 64) go(n1, n1);
+    else if (pieces <= 64 * 2 && many) go(n1, n2);
+    else if (pieces <= 64 * 4 && many) go(n1, n4);
+    else if (pieces <= 64 * 8 && many) go(n1, n8);
+    else if (pieces <= 256) go(n4, n1);
+    else if (pieces <= 256 * 2) go(n4, n2);
+    else if (pieces <= 256 * 4) go(n4, n4);
+    else if (pieces <= 256 * 8) go(n4, n8);
+    else if (pieces <= 1024 * 4) go(n16, n4);
+    else if (pieces <= 1024 * 8) go(n16, n8);
+    else go(n16, n16);
+    return post_launch("distill_rows");
 }
 
 }  // namespace asca
@@ -190,13 +530,13 @@ int asca_distill(const void* logits, long ld, const float* tval, const int32_t* 
     return act_dispatch(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
         if (T == 0) return (int)ASCA_OK;
-        const size_t lds = ((size_t)V + 31) / 32 * 4;
-        int r = allow_lds(reinterpret_cast<const void*>(&distill_k<E>), lds);
-        if (r || (r = pre_launch("distill"))) return r;
+        // one exponential serves both parts where they have one temperature, or one does not count
+        const bool two = alpha > 0.0f && alpha < 1.0f && temperature != 1.0f;
+        const float ct = alpha > 0.0f ? (float)(1.4426950408889634 / (double)temperature) : LOG2E;
         const DistillArgs a{logits, ld, tval, tids, tlse, targets, weights, losses, dlogits, lddl, T, V, alpha > 0.0f ? K : 0,
-                            temperature, alpha, scale};
-        hipLaunchKernelGGL(distill_k<E>, dim3((unsigned)T), dim3(256), lds, as_stream(stream), a);
-        return post_launch("distill");
+                            alpha > 0.0f ? temperature : 1.0f, ct, alpha, scale};
+        const hipStream_t st = as_stream(stream);
+        return two ? distill_launch<E, true>(a, st) : distill_launch<E, false>(a, st);
     });
 }
 

@@ -146,6 +146,18 @@ ASCA_DEV uint4 piece_of<bf16_t>(float v) {   // of a value that bf16 holds
     const unsigned u = __float_as_uint(v), w = u >> 16 | (u & 0xffff0000u);
     return make_uint4(w, w, w, w);
 }
+// -inf in the places of the bits that are set
+ASCA_DEV void piece_mask(uint4& r, unsigned bits4, float) {
+    r.x = bits4 & 1 ? 0xff800000u : r.x, r.y = bits4 & 2 ? 0xff800000u : r.y;
+    r.z = bits4 & 4 ? 0xff800000u : r.z, r.w = bits4 & 8 ? 0xff800000u : r.w;
+}
+ASCA_DEV void piece_mask(uint4& r, unsigned bits8, bf16_t) {
+    auto two = [](unsigned v, unsigned b) {
+        v = b & 1 ? (v & 0xffff0000u) | 0xff80u : v;
+        return b & 2 ? (v & 0xffffu) | 0xff800000u : v;
+    };
+    r.x = two(r.x, bits8), r.y = two(r.y, bits8 >> 2), r.z = two(r.z, bits8 >> 4), r.w = two(r.w, bits8 >> 6);
+}
 // What is made of a piece after this is made anew: the compiler would keep the 32-bit values
 // of an earlier look at it, in twice its registers (bf16).
 ASCA_DEV void piece_again(uint4& r) { asm("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w)); }
