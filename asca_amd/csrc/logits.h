@@ -21,6 +21,20 @@ ASCA_DEV float key_value(uint64_t k) {
 }
 ASCA_DEV unsigned key_place(uint64_t k) { return ~(unsigned)k; }
 
+// exp(x) of a double, to f32's precision: the argument's rounding is put back
+ASCA_DEV float exp_d(double x) {
+    const double y = x * 1.4426950408889634;
+    const float h = (float)y;
+    return h > -INFINITY ? __builtin_amdgcn_exp2f(h) * (1.0f + (float)(y - h) * 0.693147181f) : h == -INFINITY ? 0.0f : h;
+}
+// log(x) to 2^-24 (not relative to a large result): that of the exponent in 64 bits
+ASCA_DEV double log_d(float x) {
+    float m = __builtin_amdgcn_frexp_mantf(x);   // 0.5 to 1
+    int e = __builtin_amdgcn_frexp_expf(x);
+    if (m < 0.70710678f) m *= 2.0f, --e;
+    return ((double)e + (double)__builtin_amdgcn_logf(m)) * LN2;
+}
+
 // ------------------------------------------------------ lanes of a wave
 
 // The larger or the smaller of x and what lane ^ M holds, M a power of two

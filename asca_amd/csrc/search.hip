@@ -15,20 +15,22 @@ constexpr int BEAM_BUFS = 8;     // state buffers a call
 
 // ------------------------------------------------------------ selection
 // A team of NW waves finds the K largest of what it holds in registers.  The K-th largest of
-// its lanes' own maxima is at most the K-th largest of all, so what lies below it is none of
-// them; the few values that are left (between K and the K lanes' own) go to LDS and are
-// ranked by counting the larger ones.  Each value is looked at twice, in registers.  Where
-// more are left than LDS has room for (rows of equal values), K rounds take the largest key
+// its lanes' own maxima (of groups of lanes, in a wide team) is at most the K-th largest of
+// all, so what lies below it is none of them.  The pieces with something above it, some more
+// than K, go to LDS by a ballot for each piece of the wave; a wave looks through its own and
+// keeps what is above, and what all waves kept is ranked by counting the larger ones.  Where
+// more is left than LDS has room for (rows of equal values), K rounds take the largest key
 // below the last one.
 
 template <int NW>
 struct TeamLds {
-    static constexpr int CAP = NW == 1 ? 256 : 1024;
-    uint64_t keys[CAP];
-    float lists[NW][64];
-    float sums[NW];
+    static constexpr int PIECES = NW == 1 ? 128 : 64, KEYS = NW == 1 ? 256 : 128;   // a wave
+    uint4 piece[NW][PIECES];
+    unsigned place[NW][PIECES];   // of the piece's first value
+    uint64_t keys[NW][KEYS];
+    float lists[NW][64], sums[NW], tops[NW];
     uint64_t best[NW];
-    int count;
+    int n[NW];                    // keys; above KEYS: too many
 };
 
 template <int NW>
@@ -40,46 +42,69 @@ ASCA_DEV void team_sync() {
         __syncthreads();
     }
 }
-
-// The K-th largest of the lanes' x (-inf where fewer are above it); the waves' maxima are
-// lists[w][0] afterwards.  Clears the list of keys and leaves it writable.
 template <int NW>
-ASCA_DEV float team_kth(float x, int K, TeamLds<NW>& l) {
-    const int lane = threadIdx.x & 63, w = NW == 1 ? 0 : threadIdx.x >> 6;
-    x = lane_sort(x);
-    if (lane == 0 && w == 0) l.count = 0;
-    l.lists[w][lane] = x;
-    team_sync<NW>();
-    if constexpr (NW == 4) {
-        // two sorted lists: the larger of one and the other backwards are the largest of both
+ASCA_DEV int team_wave() { return NW == 1 ? 0 : threadIdx.x >> 6; }
+
+ASCA_DEV float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
+
+// A value that at least K of the team's x and y reach, near the K-th largest of all that they
+// are maxima of (-inf where fewer are above it).  With G groups some G log(G / (G - K)) values
+// reach it: 18 for K = 16 of 64, 89 for 64 of 128, 74 for 64 of 256.
+template <int NW>
+ASCA_DEV float team_kth(float x, float y, int K, TeamLds<NW>& l) {
+    const int lane = threadIdx.x & 63, w = team_wave<NW>();
+    if constexpr (NW == 1) {
+        if (K <= 16) return lane_value(lane_sort(fmaxf(x, y)), K - 1);
+        x = lane_sort(x);   // the larger of one sorted list and another backwards are the largest of both
+        l.lists[0][lane] = lane_sort(y);
+        team_sync<1>();
+        return lane_value(lane_merge<64>(fmaxf(x, l.lists[0][63 - lane]), true), K - 1);
+    } else {
+        x = fmaxf(x, y);
+        if (K > 16) x = lane_sort(x);
+        l.lists[w][lane] = x;
+        __syncthreads();
+        if (K <= 16) {   // 64 groups of 4 lanes
+            x = fmaxf(fmaxf(l.lists[0][lane], l.lists[1][lane]), fmaxf(l.lists[2][lane], l.lists[3][lane]));
+            return lane_value(lane_sort(x), K - 1);
+        }
         const float ab = lane_merge<64>(fmaxf(l.lists[0][lane], l.lists[1][63 - lane]), true);
         const float cd = lane_merge<64>(fmaxf(l.lists[2][lane], l.lists[3][63 - lane]), false);
-        x = lane_merge<64>(fmaxf(ab, cd), true);
+        return lane_value(lane_merge<64>(fmaxf(ab, cd), true), K - 1);
     }
-    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), K - 1));
 }
 
+// Appends the lanes' keys (0: none) to the wave's; n is the same in all lanes
 template <int NW>
-ASCA_DEV void team_push(uint64_t key, TeamLds<NW>& l) {
-    const int at = atomicAdd(&l.count, 1);
-    if (at < TeamLds<NW>::CAP) l.keys[at] = key;
+ASCA_DEV void wave_push(uint64_t key, int& n, TeamLds<NW>& l) {
+    const uint64_t some = __ballot(key != 0);
+    const int at = n + __builtin_amdgcn_mbcnt_hi((unsigned)(some >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)some, 0));
+    if (key && at < TeamLds<NW>::KEYS) l.keys[team_wave<NW>()][at] = key;
+    n += __popcll(some);
 }
 
-// The K largest keys to out(rank, key), 0 where there are fewer.  each(f) calls f with every
-// key of the thread's, for the rounds.
+// The K largest of the waves' keys, whose numbers n the team has seen, to out(rank, key), 0
+// where there are fewer.  each(f) calls f with every key of the thread's, for the rounds.
 template <int NW, typename Each, typename Out>
 ASCA_DEV void team_rank(int K, TeamLds<NW>& l, Each each, Out out) {
-    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
-    team_sync<NW>();
-    const int n = l.count;
-    if (n <= TeamLds<NW>::CAP) {
-        for (int i = tid; i < n; i += 64 * NW) {
-            const uint64_t key = l.keys[i];
+    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x, w = team_wave<NW>();
+    int all = 0;
+    bool fits = true;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        const int k = l.n[i];
+        all += k;
+        fits &= k <= TeamLds<NW>::KEYS;
+    }
+    if (fits) {
+        for (int i = threadIdx.x & 63; i < l.n[w]; i += 64) {
+            const uint64_t key = l.keys[w][i];
             int rank = 0;
-            for (int j = 0; j < n; ++j) rank += l.keys[j] > key;
+            for (int v = 0; v < NW; ++v)
+                for (int j = 0; j < l.n[v]; ++j) rank += l.keys[v][j] > key;
             if (rank < K) out(rank, key);
         }
-        for (int r = n + tid; r < K; r += 64 * NW) out(r, 0);
+        for (int r = all + tid; r < K; r += 64 * NW) out(r, 0);
         return;
     }
     uint64_t last = ~0ull;
@@ -91,9 +116,9 @@ ASCA_DEV void team_rank(int K, TeamLds<NW>& l, Each each, Out out) {
         best = wave_max_t(best);
         if constexpr (NW > 1) {
             team_sync<NW>();
-            if ((threadIdx.x & 63) == 0) l.best[threadIdx.x >> 6] = best;
+            if ((threadIdx.x & 63) == 0) l.best[w] = best;
             team_sync<NW>();
-            for (int w = 0; w < NW; ++w) best = l.best[w] > best ? l.best[w] : best;
+            for (int i = 0; i < NW; ++i) best = l.best[i] > best ? l.best[i] : best;
         }
         last = best;
         if (tid == 0) out(k, best);
@@ -104,7 +129,8 @@ struct TopArgs {
     const void* z;
     long ld, rows;
     int V, K, S, slice;   // S slices of `slice` columns a row, each a team's
-    float tau, ct;        // ct = log2(e) / tau
+    double itau;          // 1 / tau
+    float ct;             // log2(e) / tau
     float* values;        // with S = 1 and no search
     int32_t* ids;
     float* lse;
@@ -127,119 +153,168 @@ ASCA_DEV void top_write(const TopArgs& p, long row, int rank, uint64_t key) {
 // and its sum from one thread.
 template <typename E, int NW, int R, typename Out, typename Sum>
 ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW>& l, Out out, Sum sum) {
-    constexpr int NT = 64 * NW, W = Pieces<E>::W;
-    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+    constexpr int NT = 64 * NW, W = Pieces<E>::W, PIECES = TeamLds<NW>::PIECES;
+    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x, lane = threadIdx.x & 63, wave = team_wave<NW>();
     const Pieces<E> r(row + c0, n);
     uint4 raw[R];
-    float cm[R], mx = -INFINITY, ev = -INFINITY;
+    float cm[R], ma = -INFINITY, mb = -INFINITY, ev = -INFINITY;   // two groups a lane
     const int ec = r.edge(tid);
-    if (r.nb > 0)
 #pragma unroll
-        for (int j = 0; j < R; ++j) raw[j] = r.piece(min(j * NT + tid, r.nb - 1));
+    for (int j = 0; j < R; ++j)
+        if (j * NT < r.nb) raw[j] = r.piece(min(j * NT + tid, r.nb - 1));
     if (ec >= 0) ev = act_load(r.p + ec);
     float v[W];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
+        cm[j] = -INFINITY;
+        if (j * NT >= r.nb) continue;   // the whole team's
         if (j * NT + tid >= r.nb) raw[j] = piece_of<E>(-INFINITY);
         piece_values(raw[j], v);
-        cm[j] = v[0];
+        float a = v[0], b = v[W / 2];   // a NaN is none of them
 #pragma unroll
-        for (int k = 1; k < W; ++k) cm[j] = fmaxf(cm[j], v[k]);
-        mx = fmaxf(mx, cm[j]);
+        for (int k = 1; k < W / 2; ++k) a = fmaxf(a, v[k]), b = fmaxf(b, v[k + W / 2]);
+        cm[j] = fmaxf(a, b);
+        if (R == 1) ma = a, mb = b;
+        else if (j % 2 == 0) ma = fmaxf(ma, cm[j]);
+        else mb = fmaxf(mb, cm[j]);
     }
-    mx = fmaxf(mx, ev);   // a NaN is none of them
-    const float kth = team_kth<NW>(mx, K, l);
+    ma = fmaxf(ma, ev);
+    // The wave's sum from its own largest.  exp2(v ct - rc) is one step and the exponential; what
+    // rounding ref ct to rc does is the same in every term and taken off at the end.
+    const float m = wave_max(fmaxf(ma, mb)), ref = m > -INFINITY ? m : 0.0f, rc = ref * ct;
+    float s;
+    if (fabsf(rc) < 65536.0f) {
+        s = __builtin_amdgcn_exp2f(fmaf(ev, ct, -rc));
 #pragma unroll
-    for (int j = 0; j < R; ++j) piece_again(raw[j]);
-    float m = l.lists[NW == 1 ? 0 : threadIdx.x >> 6][0];
-    const float ref = m > -INFINITY ? m : 0.0f;
-    float s = __builtin_amdgcn_exp2f((ev - ref) * ct);
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        piece_values(raw[j], v);
-#pragma unroll
-        for (int k = 0; k < W; ++k) s += __builtin_amdgcn_exp2f((v[k] - ref) * ct);
-    }
-    s = wave_sum(s);
-#pragma unroll
-    for (int j = 0; j < R; ++j) piece_again(raw[j]);
-    if (NW > 1 && (threadIdx.x & 63) == 0) l.sums[threadIdx.x >> 6] = s;
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-        if (cm[j] >= kth) {
+        for (int j = 0; j < R; ++j) {
+            if (j * NT >= r.nb) continue;
+            piece_again(raw[j]);
             piece_values(raw[j], v);
 #pragma unroll
-            for (int k = 0; k < W; ++k)
-                if (v[k] >= kth && v[k] > -INFINITY) team_push<NW>(logit_key(v[k], c0 + r.col(j * NT + tid) + k), l);
+            for (int k = 0; k < W; ++k) s += __builtin_amdgcn_exp2f(fmaf(v[k], ct, -rc));
         }
-    if (ev >= kth && ev > -INFINITY) team_push<NW>(logit_key(ev, c0 + ec), l);
-    auto each = [&](auto f) {
-        for (int c = tid; c < n; c += NT) f(logit_key(act_load(r.p + c), c0 + c));   // rare: from memory
-    };
-    team_rank<NW>(K, l, each, out);
-    if (tid != 0) return;
-    if constexpr (NW > 1) {
-        float top = m = l.lists[0][0];
-        for (int w = 1; w < NW; ++w) m = fmaxf(m, l.lists[w][0]);
-        s = 0.0f;
-        for (int w = 0; w < NW; ++w) {
-            top = l.lists[w][0];
-            s += top > -INFINITY ? l.sums[w] * __builtin_amdgcn_exp2f((top - m) * ct) : l.sums[w];
+        s *= __builtin_amdgcn_exp2f(-fmaf(ref, ct, -rc));
+    } else {   // where it would be more than the terms
+        s = __builtin_amdgcn_exp2f((ev - ref) * ct);
+        for (int j = 0; j < R; ++j) {
+            const int i = j * NT + tid;
+            if (i >= r.nb) break;
+            piece_values(r.piece(i), v);
+#pragma unroll
+            for (int k = 0; k < W; ++k) s += __builtin_amdgcn_exp2f((v[k] - ref) * ct);
         }
     }
-    sum(m, s);
+    s = wave_sum(s);
+    const float kth = team_kth<NW>(ma, mb, K, l);
+    // pieces with something to keep, and what it is
+    int np = 0, nk = 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        if (j * NT >= r.nb) continue;
+        const bool some = cm[j] >= kth && cm[j] > -INFINITY;
+        const uint64_t which = __ballot(some);
+        const int at = np + __builtin_amdgcn_mbcnt_hi((unsigned)(which >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)which, 0));
+        if (some && at < PIECES) l.piece[wave][at] = raw[j], l.place[wave][at] = c0 + r.col(j * NT + tid);
+        np += __popcll(which);
+    }
+    wave_push<NW>(ev >= kth ? logit_key(ev, c0 + ec) : 0, nk, l);
+    team_sync<1>();   // the wave's own
+    if (np > PIECES) {
+        nk = TeamLds<NW>::KEYS + 1;
+    } else {
+        const E* in = reinterpret_cast<const E*>(l.piece[wave]);
+        for (int i = lane; i - lane < np * W; i += 64) {
+            const float x = i < np * W ? act_load(in + i) : -INFINITY;
+            wave_push<NW>(x >= kth ? logit_key(x, l.place[wave][i / W] + i % W) : 0, nk, l);
+        }
+    }
+    if (lane == 0) l.n[wave] = nk, l.sums[wave] = s, l.tops[wave] = m;
+    team_sync<NW>();
+    if (tid == 0) {
+        float t = l.tops[0], u = l.sums[0];
+        if constexpr (NW > 1) {
+            for (int w = 1; w < NW; ++w) t = fmaxf(t, l.tops[w]);
+            u = 0.0f;
+            for (int w = 0; w < NW; ++w)   // a wave of nothing but -inf: a sum of zero, or NaN
+                u += l.tops[w] > -INFINITY ? l.sums[w] * __builtin_amdgcn_exp2f((l.tops[w] - t) * ct) : l.sums[w];
+        }
+        sum(t, u);
+    }
+    team_rank<NW>(
+        K, l,
+        [&](auto f) {   // rare: from memory
+            for (int c = tid; c < n; c += NT) f(logit_key(act_load(r.p + c), c0 + c));
+        },
+        out);
 }
 
 // Teams of NW waves, four waves a block, a slice each
 template <typename E, int NW, int R>
 __global__ __launch_bounds__(256) void top_slice_k(TopArgs p) {
-    __shared__ TeamLds<NW> lds[4 / NW];
+    constexpr int TEAMS = 4 / NW;
+    __shared__ TeamLds<NW> lds[TEAMS];
     const int team = NW == 1 ? threadIdx.x >> 6 : 0;
-    const long unit = (long)blockIdx.x * (4 / NW) + team, row = unit / p.S;
+    const long unit = (long)blockIdx.x * TEAMS + team, row = p.S == 1 ? unit : unit / p.S;
     if (row >= p.rows || !beam_reads(p, row)) return;   // a whole team's
-    const int c0 = (int)(unit % p.S) * p.slice, n = min(p.slice, p.V - c0);
+    const int c0 = p.S == 1 ? 0 : (int)(unit % p.S) * p.slice, n = min(p.slice, p.V - c0);
     auto out = [&](int rank, uint64_t key) {
         if (p.values) top_write(p, row, rank, key);
         else p.keys[unit * p.K + rank] = key;
     };
     auto sum = [&](float m, float s) {
         if (!p.values) p.sums[unit] = make_float2(m, s);
-        else if (p.lse) p.lse[row] = (float)((double)m / (double)p.tau + log((double)s));
+        else if (p.lse) p.lse[row] = (float)((double)m * p.itau + log_d(s));
     };
     top_slice<E, NW, R>(static_cast<const E*>(p.z) + row * p.ld, c0, n, p.K, p.ct, lds[team], out, sum);
 }
 
-// log sum exp of a row from its slices, by a wave: in every lane, in 64 bits
-ASCA_DEV double slices_lse(const float2* sums, int S, double tau) {
+// log sum exp of a row from its slices, by a wave: in every lane
+ASCA_DEV double slices_lse(const float2* sums, int S, double itau) {
     const int lane = threadIdx.x & 63;
-    double m = -INFINITY, s = 0.0;
-    for (int i = lane; i < S; i += 64) m = fmax(m, (double)sums[i].x);
-    m = wave_max_t(m);
+    float m = -INFINITY, s = 0.0f;
+    for (int i = lane; i < S; i += 64) m = fmaxf(m, sums[i].x);
+    m = wave_max(m);
     for (int i = lane; i < S; i += 64)   // of nothing but -inf: a sum of zero, or NaN
-        s += sums[i].y * (sums[i].x > -INFINITY ? exp(((double)sums[i].x - m) / tau) : 1.0);
-    return m / tau + log(wave_sum_t(s));
+        s += sums[i].x > -INFINITY ? sums[i].y * exp_d(((double)sums[i].x - (double)m) * itau) : sums[i].y;
+    return (double)m * itau + log_d(wave_sum(s));
 }
 
-// The K largest of a row's S K keys, one block a row
+// The K largest of a row's S K keys, a team of NW waves a row
+template <int NW>
 __global__ __launch_bounds__(256) void top_merge_k(TopArgs p) {
-    __shared__ TeamLds<4> l;
-    const long row = blockIdx.x;
+    constexpr int TEAMS = 4 / NW, NT = 64 * NW;
+    __shared__ TeamLds<NW> lds[TEAMS];
+    TeamLds<NW>& l = lds[NW == 1 ? threadIdx.x >> 6 : 0];
+    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const long row = (long)blockIdx.x * TEAMS + (NW == 1 ? threadIdx.x >> 6 : 0);
+    if (row >= p.rows) return;
     const uint64_t* keys = p.keys + row * p.S * p.K;
     const int n = p.S * p.K;
-    float mx = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += 256)
-        if (keys[i]) mx = fmaxf(mx, key_value(keys[i]));
-    const float kth = team_kth<4>(mx, p.K, l);
-    auto each = [&](auto f) {
-        for (int i = threadIdx.x; i < n; i += 256) f(keys[i]);
-    };
-    each([&](uint64_t key) {
-        if (key && key_value(key) >= kth) team_push<4>(key, l);
-    });
-    team_rank<4>(p.K, l, each, [&](int rank, uint64_t key) { top_write(p, row, rank, key); });
-    if (p.lse && threadIdx.x < 64) {
-        const double s = slices_lse(p.sums + row * p.S, p.S, p.tau);
-        if (threadIdx.x == 0) p.lse[row] = (float)s;
+    auto at = [&](int i) { return keys[i % p.S * p.K + i / p.S]; };   // the slices' largest first, over all lanes
+    float ma = -INFINITY, mb = -INFINITY;
+    for (int i = tid, j = 0; i < n; i += NT, ++j) {
+        const uint64_t key = at(i);
+        const float v = key ? key_value(key) : -INFINITY;
+        if (j & 1) mb = fmaxf(mb, v);
+        else ma = fmaxf(ma, v);
+    }
+    const float kth = team_kth<NW>(ma, mb, p.K, l);
+    int nk = 0;
+    for (int i = tid; i - tid < n; i += NT) {
+        const uint64_t key = i < n ? at(i) : 0;
+        wave_push<NW>(key && key_value(key) >= kth ? key : 0, nk, l);
+    }
+    if ((threadIdx.x & 63) == 0) l.n[team_wave<NW>()] = nk;
+    team_sync<NW>();
+    team_rank<NW>(
+        p.K, l,
+        [&](auto f) {
+            for (int i = tid; i < n; i += NT) f(keys[i]);
+        },
+        [&](int rank, uint64_t key) { top_write(p, row, rank, key); });
+    if (p.lse && tid < 64) {
+        const double s = slices_lse(p.sums + row * p.S, p.S, p.itau);
+        if (tid == 0) p.lse[row] = (float)s;
     }
 }
 
@@ -333,14 +408,14 @@ __global__ __launch_bounds__(256) void beam_merge_k(BeamArgs p) {
     if (threadIdx.x == 0) l.count = 0;
     __syncthreads();
     auto each = [&](auto f) {
-        for (int i = threadIdx.x; i < K * per; i += 256) {
-            const int b = i / per;
+        for (int i = threadIdx.x; i < K * per; i += 256) {   // the slices' largest first, over all lanes
+            const int rank = i / (K * p.S), slice = i % (K * p.S), b = slice / p.S;
             if (l.base[b] == -INFINITY) continue;
             if (l.ended[b]) {
-                if (i == b * per) f(l.base[b], (uint64_t)b * p.V + p.eos);
+                if (rank == 0 && slice == b * p.S) f(l.base[b], (uint64_t)b * p.V + p.eos);
                 continue;
             }
-            const uint64_t key = p.keys[group * K * per + i];
+            const uint64_t key = p.keys[group * K * per + slice * K + rank];
             if (key) f(l.base[b] + (double)key_value(key), (uint64_t)b * p.V + key_place(key));
         }
     };
@@ -464,12 +539,14 @@ static int rows_check(const char* fn, long rows, int V, long ld, const void* z, 
 //   Rows of up to 64 x 8 pieces are a wave's where there are enough of them for four waves a
 //   CU; else slices are a block's, as many as give about four blocks a CU, between one piece
 //   a thread (shorter ones cost more in the merge than they spread) and eight (32 registers).
+//   Whole rows of up to 1024 x 8 pieces in blocks of 16 waves are slower than their slices and
+//   a merge (4096 x 16384 f32, 16 of them: 120 us against 60).
 template <typename E>
 static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const char* fn) {
     constexpr int W = 16 / sizeof(E);
     const long want = 4l * std::max(cu_count(), 1);
-    const bool wave = a.V <= 64 * 8 * W && (a.rows >= want || a.V <= 64 * W);
-    if (wave) {
+    const int nw = a.V <= 64 * 8 * W && (a.rows >= want || a.V <= 64 * W) ? 1 : 4;
+    if (nw == 1) {
         a.S = 1;
         a.slice = a.V;
     } else {
@@ -478,8 +555,8 @@ static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const 
         a.slice = (int)(((a.V + s - 1) / s + W - 1) / W * W);
         a.S = (a.V + a.slice - 1) / a.slice;
     }
-    a.ct = (float)(1.4426950408889634 / (double)a.tau);
-    const long units = a.rows * a.S, blocks = wave ? (units + 3) / 4 : units;
+    a.ct = (float)(1.4426950408889634 * a.itau);
+    const long units = a.rows * a.S, blocks = nw == 1 ? (units + 3) / 4 : units;
     if (!grid_fits(blocks, 256) || !grid_fits(a.rows, 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows (%ld)", fn, a.rows);
     if (a.S > 1 || a.scores) {
         int rc = scratch.get(((size_t)units * a.K + units) * 2, st);
@@ -490,16 +567,17 @@ static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const 
     }
     int rc = pre_launch("top_slice");
     if (rc) return rc;
-    const dim3 grid((unsigned)blocks), block(256);
-    const int per = (a.slice / W + (wave ? 63 : 255)) / (wave ? 64 : 256);   // pieces a thread
-    auto go = [&](auto nw) {
-        constexpr int NW = decltype(nw)::value;
-        if (per <= 1) hipLaunchKernelGGL((top_slice_k<E, NW, 1>), grid, block, 0, st, a);
-        else if (per <= 2) hipLaunchKernelGGL((top_slice_k<E, NW, 2>), grid, block, 0, st, a);
-        else if (per <= 4) hipLaunchKernelGGL((top_slice_k<E, NW, 4>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((top_slice_k<E, NW, 8>), grid, block, 0, st, a);
+    const dim3 grid((unsigned)blocks);
+    const int per = (a.slice / W + 64 * nw - 1) / (64 * nw);   // pieces a thread
+    auto go = [&](auto n) {
+        constexpr int NW = decltype(n)::value;
+        void (*k)(TopArgs) = per <= 1   ? top_slice_k<E, NW, 1>
+                             : per <= 2 ? top_slice_k<E, NW, 2>
+                             : per <= 4 ? top_slice_k<E, NW, 4>
+                                        : top_slice_k<E, NW, 8>;
+        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a);
     };
-    if (wave) go(std::integral_constant<int, 1>());
+    if (nw == 1) go(std::integral_constant<int, 1>());
     else go(std::integral_constant<int, 4>());
     return post_launch("top_slice");
 }
@@ -517,7 +595,7 @@ int asca_top_logits(const void* logits, long ld, long rows, int V, int K, float 
     if (rows > 0 && (!logits || !values || !ids)) return fail(ASCA_ERR_INVALID, "null pointer in %s", fn);
     if (!grid_fits(rows, 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows (%ld)", fn, rows);   // a merge's blocks
     TopArgs a{};
-    a.z = logits, a.ld = ld, a.rows = rows, a.V = V, a.K = K, a.tau = temperature;
+    a.z = logits, a.ld = ld, a.rows = rows, a.V = V, a.K = K, a.itau = 1.0 / (double)temperature;
     a.values = values, a.ids = ids, a.lse = lse;
     return act_dispatch(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
@@ -528,7 +606,9 @@ int asca_top_logits(const void* logits, long ld, long rows, int V, int K, float 
         if (r || a.S == 1) return r;
         a.values = values;
         if ((r = pre_launch("top_merge"))) return r;
-        hipLaunchKernelGGL(top_merge_k, dim3((unsigned)rows), dim3(256), 0, st, a);
+        // a wave a row where it holds few keys
+        if (a.S * K <= 256) hipLaunchKernelGGL(top_merge_k<1>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL(top_merge_k<4>, dim3((unsigned)rows), dim3(256), 0, st, a);
         return post_launch("top_merge");
     });
 }
@@ -547,7 +627,7 @@ int asca_beam_step(const void* logits, long ld, const float* scores, const int32
     if (groups > 0 && (!logits || !scores || !new_scores || !tokens || !parents))
         return fail(ASCA_ERR_INVALID, "null pointer in %s", fn);
     TopArgs a{};
-    a.z = logits, a.ld = ld, a.rows = (long)groups * K, a.V = V, a.K = K, a.tau = 1.0f;
+    a.z = logits, a.ld = ld, a.rows = (long)groups * K, a.V = V, a.K = K, a.itau = 1.0;
     a.scores = scores, a.ended = ended;
     return act_dispatch(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
