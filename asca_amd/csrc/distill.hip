@@ -196,8 +196,8 @@ template <typename E, int NW, int R, bool TWO>
 __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void distill_rows_k(DistillArgs p) {
     constexpr int NT = 64 * NW, W = Pieces<E>::W, WORDS = NT * R * W / 32, TEAMS = NW == 1 ? 4 : 1;
     __shared__ DistillLds<NW, WORDS> lds[TEAMS];
-    const int team = NW == 1 ? threadIdx.x >> 6 : 0, tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6;
+    const int team = NW == 1 ? wave_id() : 0, tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : wave_id();
     const long row = (long)blockIdx.x * TEAMS + team;
     if (row >= p.T) return;
     DistillLds<NW, WORDS>& l = lds[team];
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void distill_rows_k(DistillA
         piece_again(raw[j]);
         piece_values(raw[j], v);
 #pragma unroll
-        for (int k = 0; k < W; ++k) o.m = fmaxf(o.m, v[k]);
+        for (int k = 0; k < W; ++k) o.m = max_or_nan(o.m, v[k]);
         if (R >= 8) __builtin_amdgcn_sched_barrier(0);   // one piece's values in registers at a time
     }
     if (l.edge >> (tid & 31) & 1 && tid < 2 * W) ev = -INFINITY;
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
     constexpr int NW = 16, NT = 1024, W = Pieces<E>::W, U = 4;
     extern __shared__ unsigned bits[];
     __shared__ DistillLds<NW, 1> l;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const long row = blockIdx.x;
     const E* z = static_cast<const E*>(p.z) + row * p.ld;
     E* dz = p.dz ? static_cast<E*>(p.dz) + row * p.lddz : nullptr;
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
             else piece_mask(raw[u], bits[i * W / 32] >> (i * W % 32) & ((1u << W) - 1), E());
             piece_values(raw[u], v);
 #pragma unroll
-            for (int k = 0; k < W; ++k) n.m = fmaxf(n.m, v[k]);
+            for (int k = 0; k < W; ++k) n.m = max_or_nan(n.m, v[k]);
         }
         const float ref = n.m > -INFINITY ? n.m : 0.0f;
 #pragma unroll

@@ -37,51 +37,65 @@ ASCA_DEV double log_d(float x) {
 
 // ------------------------------------------------------ lanes of a wave
 
-// The larger or the smaller of x and what lane ^ M holds, M a power of two
+// The wave's number in its block, in a scalar register with all that follows from it
+ASCA_DEV int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// What lane ^ M holds, M = 1, 2, 4 or 8
 template <int M>
-ASCA_DEV float lane_pick(float x, bool larger) {
-    float a = x, b;
-    if constexpr (M == 1) b = dpp<DPP_QUAD_XOR1>(x);
-    if constexpr (M == 2) b = dpp<DPP_QUAD_XOR2>(x);
-    if constexpr (M == 4) b = dpp<DPP_HALF_MIRROR>(dpp<0x1B>(x));   // ^3 (quad_perm [3,2,1,0]), then ^7
-    if constexpr (M == 8) b = dpp<DPP_ROW_ROR8>(x);
-    if constexpr (M == 16 || M == 32) {   // the swap leaves the pair in both lanes, in either order
+ASCA_DEV float lane_xor(float x) {
+    if constexpr (M == 1) return dpp<DPP_QUAD_XOR1>(x);
+    if constexpr (M == 2) return dpp<DPP_QUAD_XOR2>(x);
+    if constexpr (M == 4) return dpp<DPP_HALF_MIRROR>(dpp<0x1B>(x));   // ^3 (quad_perm [3,2,1,0]), then ^7
+    return dpp<DPP_ROW_ROR8>(x);
+}
+// The larger of x and what lane ^ M holds with c = inf, the smaller with c = -inf: the median
+// with it, one instruction (no NaN; max and min would each first quiet theirs).
+template <int M>
+ASCA_DEV float lane_pick(float x, float c) {
+    if constexpr (M >= 16) {   // the swap leaves the pair in both lanes, in either order
         const unsigned u = __float_as_uint(x);
         auto r = M == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false)
                          : __builtin_amdgcn_permlane32_swap(u, u, false, false);
-        a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+        return __builtin_amdgcn_fmed3f(__uint_as_float(r[0]), __uint_as_float(r[1]), c);
+    } else {
+        return __builtin_amdgcn_fmed3f(x, lane_xor<M>(x), c);
     }
-    const float hi = fmaxf(a, b), lo = fminf(a, b);
-    return larger ? hi : lo;
 }
-
+// The largest of the wave's values; a NaN is none of them
 ASCA_DEV float wave_max(float x) {
-    x = lane_pick<1>(x, true), x = lane_pick<2>(x, true), x = lane_pick<4>(x, true);
-    x = lane_pick<8>(x, true), x = lane_pick<16>(x, true);
-    return lane_pick<32>(x, true);
+    x = lane_pick<1>(x, INFINITY), x = lane_pick<2>(x, INFINITY), x = lane_pick<4>(x, INFINITY);
+    x = lane_pick<8>(x, INFINITY), x = lane_pick<16>(x, INFINITY);
+    return lane_pick<32>(x, INFINITY);
 }
 
-// The steps of a bitonic network of runs of N lanes: `down` lanes' runs fall, the others' rise
+template <int M>
+ASCA_DEV float lane_step(float x) { return lane_pick<M>(x, threadIdx.x & M ? -INFINITY : INFINITY); }
+// The steps of a bitonic network that sort runs of N lanes, the largest first
 template <int N>
-ASCA_DEV float lane_merge(float x, bool down) {
-    const int l = threadIdx.x;
-    if constexpr (N >= 64) x = lane_pick<32>(x, !(l & 32) == down);
-    if constexpr (N >= 32) x = lane_pick<16>(x, !(l & 16) == down);
-    if constexpr (N >= 16) x = lane_pick<8>(x, !(l & 8) == down);
-    if constexpr (N >= 8) x = lane_pick<4>(x, !(l & 4) == down);
-    if constexpr (N >= 4) x = lane_pick<2>(x, !(l & 2) == down);
-    return lane_pick<1>(x, !(l & 1) == down);
+ASCA_DEV float lane_merge(float x) {
+    if constexpr (N >= 64) x = lane_step<32>(x);
+    if constexpr (N >= 32) x = lane_step<16>(x);
+    if constexpr (N >= 16) x = lane_step<8>(x);
+    if constexpr (N >= 8) x = lane_step<4>(x);
+    if constexpr (N >= 4) x = lane_step<2>(x);
+    return lane_step<1>(x);
 }
-// The wave's values, the largest in lane 0
+// x, or -x in the lanes of `bits`
+ASCA_DEV float lane_flip(float x, unsigned bits) { return __uint_as_float(__float_as_uint(x) ^ (bits ? 0x80000000u : 0u)); }
+// The wave's values, the largest in lane 0: every other run of a stage is sorted the other
+// way round, as the largest first of -x
 ASCA_DEV float lane_sort(float x) {
-    const int l = threadIdx.x;
-    x = lane_merge<2>(x, !(l & 2));
-    x = lane_merge<4>(x, !(l & 4));
-    x = lane_merge<8>(x, !(l & 8));
-    x = lane_merge<16>(x, !(l & 16));
-    x = lane_merge<32>(x, !(l & 32));
-    return lane_merge<64>(x, true);
+    const unsigned l = threadIdx.x, d = l ^ l >> 1;   // bit k of d: bits k and k + 1 differ
+    x = lane_merge<2>(lane_flip(x, l & 2));
+    x = lane_merge<4>(lane_flip(x, d & 2));
+    x = lane_merge<8>(lane_flip(x, d & 4));
+    x = lane_merge<16>(lane_flip(x, d & 8));
+    x = lane_merge<32>(lane_flip(x, d & 16));
+    return lane_merge<64>(lane_flip(x, l & 32));
 }
+
+// The larger of two, or NaN where either is
+ASCA_DEV float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 template <typename T>
 ASCA_DEV T wave_max_t(T x) {

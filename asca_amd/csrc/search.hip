@@ -19,15 +19,15 @@ constexpr int BEAM_BUFS = 8;     // state buffers a call
 // all, so what lies below it is none of them.  The pieces with something above it, some more
 // than K, go to LDS by a ballot for each piece of the wave; a wave looks through its own and
 // keeps what is above, and what all waves kept is ranked by counting the larger ones.  Where
-// more is left than LDS has room for (rows of equal values), K rounds take the largest key
-// below the last one.
+// more is left than LDS has room for (rows of equal values), or a NaN is among them, K rounds
+// take the largest key below the last one.
 
 template <int NW>
 struct TeamLds {
     static constexpr int PIECES = NW == 1 ? 128 : 64, KEYS = NW == 1 ? 256 : 128;   // a wave
     uint4 piece[NW][PIECES];
     unsigned place[NW][PIECES];   // of the piece's first value
-    uint64_t keys[NW][KEYS];
+    alignas(16) uint64_t keys[NW][KEYS];
     float lists[NW][64], sums[NW], tops[NW];
     uint64_t best[NW];
     int n[NW];                    // keys; above KEYS: too many
@@ -43,9 +43,17 @@ ASCA_DEV void team_sync() {
     }
 }
 template <int NW>
-ASCA_DEV int team_wave() { return NW == 1 ? 0 : threadIdx.x >> 6; }
+ASCA_DEV int team_wave() { return NW == 1 ? 0 : wave_id(); }
 
 ASCA_DEV float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
+
+// The 64 largest of four sorted lists in LDS, sorted
+ASCA_DEV float four_lists(const float (&l)[4][64]) {
+    const int lane = threadIdx.x & 63;
+    const float ab = lane_merge<64>(fmaxf(l[0][lane], l[1][63 - lane]));
+    const float cd = lane_merge<64>(-fmaxf(l[2][lane], l[3][63 - lane]));   // backwards
+    return lane_merge<64>(fmaxf(ab, -cd));
+}
 
 // A value that at least K of the team's x and y reach, near the K-th largest of all that they
 // are maxima of (-inf where fewer are above it).  With G groups some G log(G / (G - K)) values
@@ -58,7 +66,7 @@ ASCA_DEV float team_kth(float x, float y, int K, TeamLds<NW>& l) {
         x = lane_sort(x);   // the larger of one sorted list and another backwards are the largest of both
         l.lists[0][lane] = lane_sort(y);
         team_sync<1>();
-        return lane_value(lane_merge<64>(fmaxf(x, l.lists[0][63 - lane]), true), K - 1);
+        return lane_value(lane_merge<64>(fmaxf(x, l.lists[0][63 - lane])), K - 1);
     } else {
         x = fmaxf(x, y);
         if (K > 16) x = lane_sort(x);
@@ -68,9 +76,7 @@ ASCA_DEV float team_kth(float x, float y, int K, TeamLds<NW>& l) {
             x = fmaxf(fmaxf(l.lists[0][lane], l.lists[1][lane]), fmaxf(l.lists[2][lane], l.lists[3][lane]));
             return lane_value(lane_sort(x), K - 1);
         }
-        const float ab = lane_merge<64>(fmaxf(l.lists[0][lane], l.lists[1][63 - lane]), true);
-        const float cd = lane_merge<64>(fmaxf(l.lists[2][lane], l.lists[3][63 - lane]), false);
-        return lane_value(lane_merge<64>(fmaxf(ab, cd), true), K - 1);
+        return lane_value(four_lists(l.lists), K - 1);
     }
 }
 
@@ -81,6 +87,33 @@ ASCA_DEV void wave_push(uint64_t key, int& n, TeamLds<NW>& l) {
     const int at = n + __builtin_amdgcn_mbcnt_hi((unsigned)(some >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)some, 0));
     if (key && at < TeamLds<NW>::KEYS) l.keys[team_wave<NW>()][at] = key;
     n += __popcll(some);
+}
+
+// The ranks of the wave's n keys among all waves', R a lane
+template <int NW, int R, typename Out>
+ASCA_DEV void wave_rank(int K, int n, TeamLds<NW>& l, Out out) {
+    const int lane = threadIdx.x & 63, w = team_wave<NW>();
+    uint64_t key[R];
+    int rank[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = lane + 64 * r < n ? l.keys[w][lane + 64 * r] : 0, rank[r] = 0;
+    for (int v = 0; v < NW; ++v)
+        for (int j = 0; j < l.n[v]; j += 2) {   // (an odd number of them ends in a 0)
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&l.keys[v][j]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) rank[r] += (two.x > key[r]) + (two.y > key[r]);
+        }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (lane + 64 * r < n && rank[r] < K) out(rank[r], key[r]);
+}
+
+// The keys' end, for all to see: their number, and one 0 more
+template <int NW>
+ASCA_DEV void wave_end(int n, TeamLds<NW>& l) {
+    if ((threadIdx.x & 63) != 0) return;
+    l.n[team_wave<NW>()] = n;
+    if (n < TeamLds<NW>::KEYS) l.keys[team_wave<NW>()][n] = 0;
 }
 
 // The K largest of the waves' keys, whose numbers n the team has seen, to out(rank, key), 0
@@ -97,13 +130,10 @@ ASCA_DEV void team_rank(int K, TeamLds<NW>& l, Each each, Out out) {
         fits &= k <= TeamLds<NW>::KEYS;
     }
     if (fits) {
-        for (int i = threadIdx.x & 63; i < l.n[w]; i += 64) {
-            const uint64_t key = l.keys[w][i];
-            int rank = 0;
-            for (int v = 0; v < NW; ++v)
-                for (int j = 0; j < l.n[v]; ++j) rank += l.keys[v][j] > key;
-            if (rank < K) out(rank, key);
-        }
+        const int n = l.n[w];
+        if (n <= 64) wave_rank<NW, 1>(K, n, l, out);
+        else if (n <= 128) wave_rank<NW, 2>(K, n, l, out);
+        else if constexpr (TeamLds<NW>::KEYS > 128) wave_rank<NW, TeamLds<NW>::KEYS / 64>(K, n, l, out);
         for (int r = all + tid; r < K; r += 64 * NW) out(r, 0);
         return;
     }
@@ -170,15 +200,16 @@ ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW
         if (j * NT >= r.nb) continue;   // the whole team's
         if (j * NT + tid >= r.nb) raw[j] = piece_of<E>(-INFINITY);
         piece_values(raw[j], v);
-        float a = v[0], b = v[W / 2];   // a NaN is none of them
+        float a = v[0], b = v[W / 2];
 #pragma unroll
-        for (int k = 1; k < W / 2; ++k) a = fmaxf(a, v[k]), b = fmaxf(b, v[k + W / 2]);
-        cm[j] = fmaxf(a, b);
+        for (int k = 1; k < W / 2; ++k) a = max_or_nan(a, v[k]), b = max_or_nan(b, v[k + W / 2]);
+        cm[j] = max_or_nan(a, b);
         if (R == 1) ma = a, mb = b;
-        else if (j % 2 == 0) ma = fmaxf(ma, cm[j]);
-        else mb = fmaxf(mb, cm[j]);
+        else if (j % 2 == 0) ma = max_or_nan(ma, cm[j]);
+        else mb = max_or_nan(mb, cm[j]);
     }
-    ma = fmaxf(ma, ev);
+    ma = max_or_nan(ma, ev);
+    const bool nan = __ballot(ma != ma || mb != mb) != 0;   // (a maximum that leaves it out takes twice as long)
     // The wave's sum from its own largest.  exp2(v ct - rc) is one step and the exponential; what
     // rounding ref ct to rc does is the same in every term and taken off at the end.
     const float m = wave_max(fmaxf(ma, mb)), ref = m > -INFINITY ? m : 0.0f, rc = ref * ct;
@@ -219,7 +250,7 @@ ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW
     }
     wave_push<NW>(ev >= kth ? logit_key(ev, c0 + ec) : 0, nk, l);
     team_sync<1>();   // the wave's own
-    if (np > PIECES) {
+    if (np > PIECES || nan) {
         nk = TeamLds<NW>::KEYS + 1;
     } else {
         const E* in = reinterpret_cast<const E*>(l.piece[wave]);
@@ -228,7 +259,8 @@ ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW
             wave_push<NW>(x >= kth ? logit_key(x, l.place[wave][i / W] + i % W) : 0, nk, l);
         }
     }
-    if (lane == 0) l.n[wave] = nk, l.sums[wave] = s, l.tops[wave] = m;
+    wave_end<NW>(nk, l);
+    if (lane == 0) l.sums[wave] = s, l.tops[wave] = m;
     team_sync<NW>();
     if (tid == 0) {
         float t = l.tops[0], u = l.sums[0];
@@ -253,10 +285,10 @@ template <typename E, int NW, int R>
 __global__ __launch_bounds__(256) void top_slice_k(TopArgs p) {
     constexpr int TEAMS = 4 / NW;
     __shared__ TeamLds<NW> lds[TEAMS];
-    const int team = NW == 1 ? threadIdx.x >> 6 : 0;
-    const long unit = (long)blockIdx.x * TEAMS + team, row = p.S == 1 ? unit : unit / p.S;
+    const int team = NW == 1 ? wave_id() : 0, slice = NW == 1 ? 0 : blockIdx.x % (unsigned)p.S;
+    const long unit = (long)blockIdx.x * TEAMS + team, row = NW == 1 ? unit : blockIdx.x / (unsigned)p.S;   // NW = 1: S = 1
     if (row >= p.rows || !beam_reads(p, row)) return;   // a whole team's
-    const int c0 = p.S == 1 ? 0 : (int)(unit % p.S) * p.slice, n = min(p.slice, p.V - c0);
+    const int c0 = slice * p.slice, n = min(p.slice, p.V - c0);
     auto out = [&](int rank, uint64_t key) {
         if (p.values) top_write(p, row, rank, key);
         else p.keys[unit * p.K + rank] = key;
@@ -284,13 +316,13 @@ template <int NW>
 __global__ __launch_bounds__(256) void top_merge_k(TopArgs p) {
     constexpr int TEAMS = 4 / NW, NT = 64 * NW;
     __shared__ TeamLds<NW> lds[TEAMS];
-    TeamLds<NW>& l = lds[NW == 1 ? threadIdx.x >> 6 : 0];
-    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const long row = (long)blockIdx.x * TEAMS + (NW == 1 ? threadIdx.x >> 6 : 0);
+    const int team = NW == 1 ? wave_id() : 0, tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+    TeamLds<NW>& l = lds[team];
+    const long row = (long)blockIdx.x * TEAMS + team;
     if (row >= p.rows) return;
     const uint64_t* keys = p.keys + row * p.S * p.K;
     const int n = p.S * p.K;
-    auto at = [&](int i) { return keys[i % p.S * p.K + i / p.S]; };   // the slices' largest first, over all lanes
+    auto at = [&](unsigned i) { return keys[i % p.S * p.K + i / (unsigned)p.S]; };   // the slices' largest first, over all lanes
     float ma = -INFINITY, mb = -INFINITY;
     for (int i = tid, j = 0; i < n; i += NT, ++j) {
         const uint64_t key = at(i);
@@ -304,7 +336,7 @@ __global__ __launch_bounds__(256) void top_merge_k(TopArgs p) {
         const uint64_t key = i < n ? at(i) : 0;
         wave_push<NW>(key && key_value(key) >= kth ? key : 0, nk, l);
     }
-    if ((threadIdx.x & 63) == 0) l.n[team_wave<NW>()] = nk;
+    wave_end<NW>(nk, l);
     team_sync<NW>();
     team_rank<NW>(
         p.K, l,
@@ -423,9 +455,7 @@ __global__ __launch_bounds__(256) void beam_merge_k(BeamArgs p) {
     each([&](double x, uint64_t) { mx = fmaxf(mx, (float)x); });
     l.lists[w][lane] = lane_sort(mx);
     __syncthreads();
-    const float ab = lane_merge<64>(fmaxf(l.lists[0][lane], l.lists[1][63 - lane]), true);
-    const float cd = lane_merge<64>(fmaxf(l.lists[2][lane], l.lists[3][63 - lane]), false);
-    const float kth = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_merge<64>(fmaxf(ab, cd), true)), K - 1));
+    const float kth = lane_value(four_lists(l.lists), K - 1);
     each([&](double x, uint64_t at) {
         if ((float)x < kth) return;
         const int i = atomicAdd(&l.count, 1);
