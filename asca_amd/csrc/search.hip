@@ -390,107 +390,156 @@ ASCA_DEV int beam_slot(int parent, int K, bool stay) {
     return slot;
 }
 
-// A group's picks, best first, in the first K lanes of a wave, to its slots
-ASCA_DEV void beam_write(const BeamArgs& p, long group, const BeamPick& pick) {
-    const int lane = threadIdx.x & 63;
-    const int slot = beam_slot(pick.parent, p.K, p.stay);
-    if (lane >= p.K) return;
-    const long at = group * p.K + slot;
-    const bool some = pick.parent >= 0;
-    const bool end = some && p.ended && (p.ended[group * p.K + pick.parent] != 0 || (int)pick.token == p.eos);
-    // every lane has read what the caller's buffers held before any writes: new_ended may be ended
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    p.new_scores[at] = some ? (float)pick.score : -INFINITY;
-    p.tokens[at] = some ? pick.token : p.eos >= 0 ? (unsigned)p.eos : 0u;
-    p.parents[at] = some ? pick.parent : slot;
-    if (p.new_ended) p.new_ended[at] = end;
-}
-
-constexpr int BEAM_CAP = 1024;   // candidates that are ranked in LDS
+constexpr int BEAM_CAP = 512;   // candidates that are ranked in LDS
 
 struct BeamLds {
     double base[BEAM_MAX_K];     // what a beam's logits are added to (-inf: it has no candidates)
     int ended[BEAM_MAX_K];
     float lists[4][64];
     double score[BEAM_CAP];
-    uint64_t place[BEAM_CAP];
-    double best[4];
-    uint64_t best_place[4];
+    unsigned place[BEAM_CAP][2];   // beam, token
+    double best[16];
+    uint64_t best_place[16];
     BeamPick picks[BEAM_MAX_K];
     int count;
 };
 
+// A group's picks, best first, in the first K lanes of a wave, to its slots
+ASCA_DEV void beam_write(const BeamArgs& p, long group, const BeamPick& pick, const int* ended) {
+    const int lane = threadIdx.x & 63;
+    const int slot = beam_slot(pick.parent, p.K, p.stay);
+    if (lane >= p.K) return;
+    const long at = group * p.K + slot;
+    const bool some = pick.parent >= 0;
+    p.new_scores[at] = some ? (float)pick.score : -INFINITY;
+    p.tokens[at] = some ? pick.token : p.eos >= 0 ? (unsigned)p.eos : 0u;
+    p.parents[at] = some ? pick.parent : slot;
+    if (p.new_ended) p.new_ended[at] = some && (ended[pick.parent] != 0 || (int)pick.token == p.eos);
+}
+
 ASCA_DEV bool beam_better(double a, uint64_t pa, double b, uint64_t pb) { return a > b || (a == b && pa < pb); }
 
-// The K best of a group's candidates, a block a group.  As a row's selection, with the scores
-// in 64 bits; the threshold compares them rounded to 32, which keeps their order.
-__global__ __launch_bounds__(256) void beam_merge_k(BeamArgs p) {
-    __shared__ BeamLds l;
-    const long group = blockIdx.x;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, K = p.K, per = p.S * K;
-    for (int b = w; b < K; b += 4) {
-        const long row = group * K + b;
-        const double s = p.scores[row];
-        const bool end = p.ended && p.ended[row] != 0, fin = fabs(s) < INFINITY;
-        double x = s;
-        if (fin && !end) x = s - slices_lse(p.sums + row * p.S, p.S, 1.0);
-        if (lane == 0) l.base[b] = fin && fabs(x) < INFINITY ? x : (double)-INFINITY, l.ended[b] = end;
+// The K best of a group's candidates by the first 256 threads of a block of NW waves.  As a
+// row's selection, with the scores in 64 bits; the threshold compares them rounded to 32, which
+// keeps their order.  keys (K, S, K) and sums (K, S) are the group's own.
+template <int NW, typename Keys, typename Sums>
+ASCA_DEV void beam_merge(const BeamArgs& p, long group, BeamLds& l, Keys keys, Sums sums) {
+    const int tid = threadIdx.x, lane = tid & 63, w = wave_id(), K = p.K, S = p.S, L = K * S;
+    // log sum exp of every beam, by as many lanes as its slices need; all beams' at once
+    int width = 1;
+    while (width < S && width < 64) width *= 2;
+    const bool in = w < 4;
+    for (int b = tid / width; in && b < (K + 256 / width - 1) / (256 / width) * (256 / width); b += 256 / width) {
+        const bool on = b < K;
+        const double s = on ? (double)p.scores[group * K + b] : (double)-INFINITY;
+        const bool end = on && p.ended && p.ended[group * K + b] != 0, fin = fabs(s) < INFINITY;
+        float m = -INFINITY, t = 0.0f;
+        const bool read = fin && !end;
+        for (int i = tid % width; i < S && read; i += width) m = fmaxf(m, sums[b * S + i].x);
+        for (int x = width / 2; x >= 1; x /= 2) m = fmaxf(m, __shfl_xor(m, x, 64));
+        for (int i = tid % width; i < S && read; i += width) {   // of nothing but -inf: a sum of zero, or NaN
+            const float2 v = sums[b * S + i];
+            t += v.x > -INFINITY ? v.y * exp_d((double)v.x - (double)m) : v.y;
+        }
+        for (int x = width / 2; x >= 1; x /= 2) t += __shfl_xor(t, x, 64);
+        const double x = read ? s - ((double)m + log_d(t)) : s;
+        if (on && tid % width == 0) l.base[b] = fin && fabs(x) < INFINITY ? x : (double)-INFINITY, l.ended[b] = end;
     }
-    if (threadIdx.x < K) l.picks[threadIdx.x] = BeamPick{-INFINITY, -1, 0};
-    if (threadIdx.x == 0) l.count = 0;
+    if (tid < K) l.picks[tid] = BeamPick{-INFINITY, -1, 0};
+    if (tid == 0) l.count = 0;
     __syncthreads();
-    auto each = [&](auto f) {
-        for (int i = threadIdx.x; i < K * per; i += 256) {   // the slices' largest first, over all lanes
-            const int rank = i / (K * p.S), slice = i % (K * p.S), b = slice / p.S;
-            if (l.base[b] == -INFINITY) continue;
+    // every candidate: the slices' largest first, over all threads
+    const float is = 1.0f / (float)S;
+    const int dr = 256 / L, ds = 256 % L;
+    auto each = [&](int ranks, auto f) {
+        for (int rank = in ? tid / L : ranks, slice = tid % L; rank < ranks; rank += dr, slice += ds) {
+            if (slice >= L) {
+                slice -= L;
+                if (++rank >= ranks) break;
+            }
+            const int b = (int)(((float)slice + 0.5f) * is);   // slice / S
+            const double base = l.base[b];
+            if (base == -INFINITY) continue;
             if (l.ended[b]) {
-                if (rank == 0 && slice == b * p.S) f(l.base[b], (uint64_t)b * p.V + p.eos);
+                if (rank == 0 && slice == b * S) f(base, b, (unsigned)p.eos);
                 continue;
             }
-            const uint64_t key = p.keys[group * K * per + slice * K + rank];
-            if (key) f(l.base[b] + (double)key_value(key), (uint64_t)b * p.V + key_place(key));
+            const uint64_t key = keys[slice * K + rank];
+            if (key) f(base + (double)key_value(key), b, key_place(key));
         }
     };
+    // the threshold: from each slice's first ones, as many of them as there are lanes
     float mx = -INFINITY;
-    each([&](double x, uint64_t) { mx = fmaxf(mx, (float)x); });
-    l.lists[w][lane] = lane_sort(mx);
+    each(min(K, (255 + L) / L), [&](double x, int, unsigned) { mx = fmaxf(mx, (float)x); });
+    if (in) l.lists[w][lane] = lane_sort(mx);
     __syncthreads();
-    const float kth = lane_value(four_lists(l.lists), K - 1);
-    each([&](double x, uint64_t at) {
+    const float kth = in ? lane_value(four_lists(l.lists), K - 1) : 0.0f;
+    each(K, [&](double x, int b, unsigned token) {
         if ((float)x < kth) return;
         const int i = atomicAdd(&l.count, 1);
-        if (i < BEAM_CAP) l.score[i] = x, l.place[i] = at;
+        if (i < BEAM_CAP) l.score[i] = x, l.place[i][0] = b, l.place[i][1] = token;
     });
     __syncthreads();
     const int n = l.count;
-    auto pick = [&](int rank, double x, uint64_t at) { l.picks[rank] = BeamPick{x, (int)(at / p.V), (unsigned)(at % p.V)}; };
     if (n <= BEAM_CAP) {
-        for (int i = threadIdx.x; i < n; i += 256) {
+        for (int i = tid; i < n; i += 64 * NW) {
             const double x = l.score[i];
-            const uint64_t at = l.place[i];
+            const unsigned b = l.place[i][0], t = l.place[i][1];
             int rank = 0;
-            for (int j = 0; j < n; ++j) rank += beam_better(l.score[j], l.place[j], x, at);
-            if (rank < K) pick(rank, x, at);
+            for (int j = 0; j < n; ++j) {
+                const double y = l.score[j];
+                const unsigned c = l.place[j][0], u = l.place[j][1];
+                rank += y > x || (y == x && (c < b || (c == b && u < t)));
+            }
+            if (rank < K) l.picks[rank] = BeamPick{x, (int)b, t};
         }
-    } else {
+    } else {   // rows of equal values: K rounds, each the best below the last
         double last = INFINITY;
         uint64_t lastp = 0;
         for (int k = 0; k < K; ++k) {
             double v = -INFINITY;
             uint64_t vp = ~0ull;
-            each([&](double x, uint64_t at) {
+            each(K, [&](double x, int b, unsigned token) {
+                const uint64_t at = (uint64_t)b << 32 | token;
                 if (beam_better(last, lastp, x, at) && beam_better(x, at, v, vp)) v = x, vp = at;
             });
-            const double top = block_max_t<4>(v, l.best);
-            const uint64_t place = ~block_max_t<4>(v == top ? ~vp : (uint64_t)0, l.best_place);
+            const double top = block_max_t<NW>(v, l.best);
+            const uint64_t place = ~block_max_t<NW>(v == top ? ~vp : (uint64_t)0, l.best_place);
             if (top == -INFINITY) break;
-            if (threadIdx.x == 0) pick(k, top, place);
+            if (tid == 0) l.picks[k] = BeamPick{top, (int)(place >> 32), (unsigned)place};
             last = top, lastp = place;
         }
     }
     __syncthreads();
-    if (threadIdx.x >= 64) return;
-    beam_write(p, group, lane < K ? l.picks[lane] : BeamPick{-INFINITY, -1, 0});
+    if (w == 0) beam_write(p, group, lane < K ? l.picks[lane] : BeamPick{-INFINITY, -1, 0}, l.ended);
+}
+
+// A block a group
+__global__ __launch_bounds__(256) void beam_merge_k(BeamArgs p) {
+    __shared__ BeamLds l;
+    const long group = blockIdx.x;
+    beam_merge<4>(p, group, l, p.keys + group * p.K * p.S * p.K, p.sums + group * p.K * p.S);
+}
+
+// Rows of R pieces a lane: a block's NW waves select from the group's rows in turn, then it
+// merges them, in one launch
+template <typename E, int R, int NW>
+__global__ __launch_bounds__(64 * NW) void beam_small_k(BeamArgs p, TopArgs t) {
+    __shared__ BeamLds l;
+    __shared__ TeamLds<1> team[NW];
+    __shared__ uint64_t keys[BEAM_MAX_K * BEAM_MAX_K];
+    __shared__ float2 sums[BEAM_MAX_K];
+    const long group = blockIdx.x;
+    const int w = wave_id(), K = p.K;
+    for (int b = w; b < K; b += NW) {
+        const long row = group * K + b;
+        if (!beam_reads(t, row)) continue;
+        top_slice<E, 1, R>(
+            static_cast<const E*>(t.z) + row * t.ld, 0, t.V, K, t.ct, team[w], [&](int rank, uint64_t key) { keys[b * K + rank] = key; },
+            [&](float m, float s) { sums[b] = make_float2(m, s); });
+    }
+    __syncthreads();
+    beam_merge<NW>(p, group, l, keys, sums);
 }
 
 struct StatesArgs {
@@ -663,10 +712,23 @@ int asca_beam_step(const void* logits, long ld, const float* scores, const int32
         using E = std::remove_pointer_t<decltype(e)>;
         if (groups == 0) return (int)ASCA_OK;
         const hipStream_t st = as_stream(stream);
+        BeamArgs b{scores, ended, new_scores, new_ended, tokens, parents, K, V, 1, eos < 0 ? -1 : eos, stay, nullptr, nullptr};
+        int r;
+        const int pieces = (V + 16 / (int)sizeof(E) - 1) / (16 / (int)sizeof(E));
+        if (pieces <= 128) {   // both halves in one launch
+            if ((r = pre_launch("beam_small"))) return r;
+            a.S = 1, a.slice = V, a.ct = LOG2E;
+            // a wave a beam where the blocks are few
+            const int nw = K <= 4 || groups > 2 * cu_count() ? 4 : K <= 8 ? 8 : 16;
+            void (*k)(BeamArgs, TopArgs) = nw == 4   ? pieces <= 64 ? beam_small_k<E, 1, 4> : beam_small_k<E, 2, 4>
+                                           : nw == 8 ? pieces <= 64 ? beam_small_k<E, 1, 8> : beam_small_k<E, 2, 8>
+                                                     : pieces <= 64 ? beam_small_k<E, 1, 16> : beam_small_k<E, 2, 16>;
+            hipLaunchKernelGGL(k, dim3((unsigned)groups), dim3(64 * nw), 0, st, b, a);
+            return post_launch("beam_small");
+        }
         StreamScratch scratch;
-        int r = top_slices<E>(a, scratch, st, fn);
-        if (r || (r = pre_launch("beam_merge"))) return r;
-        const BeamArgs b{scores, ended, new_scores, new_ended, tokens, parents, K, V, a.S, eos < 0 ? -1 : eos, stay, a.keys, a.sums};
+        if ((r = top_slices<E>(a, scratch, st, fn)) || (r = pre_launch("beam_merge"))) return r;
+        b.S = a.S, b.keys = a.keys, b.sums = a.sums;
         hipLaunchKernelGGL(beam_merge_k, dim3((unsigned)groups), dim3(256), 0, st, b);
         return post_launch("beam_merge");
     });
