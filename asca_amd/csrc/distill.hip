@@ -193,7 +193,7 @@ ASCA_DEV void row_piece_store(E* d, bool whole, const float (&v)[16 / sizeof(E)]
 // others' sum is formed without them (a difference of sums would lose it where the student is
 // sure of the list); the list's own terms are added from one wave's lanes.
 template <typename E, int NW, int R, bool TWO>
-__global__ __launch_bounds__(NW == 16 ? 1024 : 256) void distill_rows_k(DistillArgs p) {
+__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void distill_rows_k(DistillArgs p) {
     constexpr int NT = 64 * NW, W = Pieces<E>::W, WORDS = NT * R * W / 32, TEAMS = NW == 1 ? 4 : 1;
     __shared__ DistillLds<NW, WORDS> lds[TEAMS];
     const int team = NW == 1 ? wave_id() : 0, tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -457,7 +457,7 @@ static int distill_launch(const DistillArgs& a, hipStream_t st) {
     const bool many = a.T >= 4l * std::max(cu_count(), 1);
     auto go = [&](auto nw, auto rr) {
         constexpr int NW = decltype(nw)::value, R = decltype(rr)::value;
-        hipLaunchKernelGGL((distill_rows_k<E, NW, R, TWO>), dim3((unsigned)(NW == 1 ? (a.T + 3) / 4 : a.T)), dim3(NW == 16 ? 1024 : 256), 0,
+        hipLaunchKernelGGL((distill_rows_k<E, NW, R, TWO>), dim3((unsigned)(NW == 1 ? (a.T + 3) / 4 : a.T)), dim3(NW == 1 ? 256 : 64 * NW), 0,
                            st, a);
     };
     std::integral_constant<int, 1> n1;
@@ -473,8 +473,8 @@ static int distill_launch(const DistillArgs& a, hipStream_t st) {
     else if (pieces <= 256 * 2) go(n4, n2);
     else if (pieces <= 256 * 4) go(n4, n4);
     else if (pieces <= 256 * 8) go(n4, n8);
-    else if (pieces <= 1024 * 4) go(n16, n4);
-    else if (pieces <= 1024 * 8) go(n16, n8);
+    else if (pieces <= 512 * 8) go(n8, n8);
+    else if (pieces <= 512 * 16) go(n8, n16);
     else go(n16, n16);
     return post_launch("distill_rows");
 }
