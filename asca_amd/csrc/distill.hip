@@ -17,6 +17,8 @@ namespace asca {
 constexpr int DISTILL_MAX_K = 64;          // entries a row: one for each lane of a wave
 constexpr int DISTILL_MAX_V = 1 << 20;     // columns that the bitmap in LDS has bits for
 
+struct Expo;
+struct SplitRow;
 struct DistillArgs {
     const void* z;
     long ld;
@@ -30,105 +32,119 @@ struct DistillArgs {
     long lddz, T;
     int V, K;
     float tau, ct, alpha, scale;   // ct = log2(e) / tau
+    double itau;                   // 1 / tau
+    int S, slice;                  // a split row's slices
+    Expo* parts;                   // (T, S)
+    SplitRow* split;               // (T)
 };
+
+// A sum of exponentials of some of a row's logits, at the temperature and at 1, and the largest
+// of them, from which they are measured (-inf: none, or only -inf; the sums are zero, or NaN)
+struct Expo {
+    float m, st, s1;
+};
+// One exponential serves both where the temperatures are one or only one counts (not TWO).
+template <bool TWO>
+ASCA_DEV Expo expo_join(Expo a, Expo b, float ct) {
+    const float m = fmaxf(a.m, b.m);
+    auto at = [&](float x, float s, float c) { return x > -INFINITY ? s * __builtin_amdgcn_exp2f((x - m) * c) : s; };
+    return {m, at(a.m, a.st, ct) + at(b.m, b.st, ct), TWO ? at(a.m, a.s1, LOG2E) + at(b.m, b.s1, LOG2E) : 0.0f};
+}
 
 // An entry of a row's list, one a lane
 struct Entry {
     int id;       // below 0: none
-    float z;      // the student's logit there
-    double lp;    // log p
-    float p;
+    float z, p;   // the student's logit there, and p
+};
+// What a row's entries are together
+struct List {
+    Expo e;       // of their logits
+    float total;  // sum of p
+    float rest;   // what it leaves of 1, with tlse
+    float part;   // sum of p (log p - (z - ref) / tau), ref = their largest logit (0 where that is -inf)
+    float zt;     // the student's logit at the target
 };
 
-// p of a row's entries (id and the teacher's logit in lp), in a wave; `twice`: some id may
+// 1 / x to 2^-23
+ASCA_DEV float recip(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// A row's list, in a wave: id and z are there, tv is the teacher's logit; `twice`: some id may
 // be there more than once.  The first of one id's entries has their sum, the others are none.
-ASCA_DEV void entry_probs(const DistillArgs& p, long row, bool twice, Entry& en, float& total, float& rest) {
+template <bool TWO>
+ASCA_DEV List list_of(const DistillArgs& p, long row, float tv, bool twice, Entry& en) {
     const int lane = threadIdx.x & 63;
-    const double itau = 1.0 / (double)p.tau;
-    const bool on = en.id >= 0;
+    bool on = en.id >= 0;
+    double lp;   // log p
+    en.p = 0.0f;
     if (p.tlse) {
-        en.lp = en.lp * itau - (double)p.tlse[row];
-        en.p = on ? exp_d(en.lp) : 0.0f;
+        lp = (double)tv * p.itau - (double)p.tlse[row];
+        if (on) en.p = exp_d(lp);
     } else {
-        const float v = on ? (float)en.lp : -INFINITY, m = wave_max(v);   // a NaN is not the largest
-        if (m == -INFINITY) {
-            en.lp = -INFINITY;   // no entry, or none above -inf
-            en.p = on && v != v ? v : 0.0f;
-        } else {
-            en.lp = (en.lp - (double)m) * itau;
-            const float e = on ? exp_d(en.lp) : 0.0f, s = wave_sum(e);
-            en.lp -= log_d(s);
-            en.p = e / s;
-        }
+        const float m = wave_max(on ? tv : -INFINITY), ref = m == -INFINITY ? 0.0f : m;   // no entry, or none above -inf
+        lp = ((double)tv - (double)ref) * p.itau;
+        const float e = on ? exp_d(lp) : 0.0f, s = wave_sum(e);
+        if (m != -INFINITY) en.p = e * recip(s);
+        lp -= log_d(s);
     }
-    if (twice)
+    if (twice) {
         for (int j = 0; j < p.K; ++j) {
             const int id = __builtin_amdgcn_readlane(en.id, j);
             const uint64_t same = __ballot(en.id == id);
             if (id < 0 || (same & (same - 1)) == 0) continue;
             const float sum = wave_sum(en.id == id ? en.p : 0.0f);
-            if (lane == j) en.p = sum, en.lp = log_d(sum);
+            if (lane == j) en.p = sum, lp = log_d(sum);
             else if (en.id == id) en.id = -1, en.p = 0.0f;
         }
-    total = wave_sum(en.p);
-    rest = p.tlse ? fmaxf(0.0f, 1.0f - total) : 0.0f;
+        on = en.id >= 0;
+    }
+    List l;
+    l.e.m = wave_max(on ? en.z : -INFINITY);
+    const float x = en.z - (l.e.m > -INFINITY ? l.e.m : 0.0f);
+    l.e.st = on ? __builtin_amdgcn_exp2f(x * p.ct) : 0.0f;
+    l.e.s1 = TWO && on ? __builtin_amdgcn_exp2f(x * LOG2E) : 0.0f;
+    l.total = en.p;
+    l.part = en.p != 0.0f ? (float)((double)en.p * (lp - (double)x * p.itau)) : 0.0f;
+    wave_sum4(l.e.st, l.e.s1, l.total, l.part);
+    l.rest = p.tlse ? fmaxf(0.0f, 1.0f - l.total) : 0.0f;
+    return l;
 }
 
-// The sums over the columns outside the list: the largest of them and their exponentials'
-// sums from it, at the temperature and at 1
-struct Outside {
-    float m, st, s1;
-};
-ASCA_DEV Outside outside_join(Outside a, Outside b, float ct, bool two) {
-    const float m = fmaxf(a.m, b.m), ref = m > -INFINITY ? m : 0.0f;   // sums of nothing are 0, or NaN
-    auto at = [&](float x, float s, float c) { return x > -INFINITY ? s * __builtin_amdgcn_exp2f((x - ref) * c) : s; };
-    return {m, at(a.m, a.st, ct) + at(b.m, b.st, ct), two ? at(a.m, a.s1, LOG2E) + at(b.m, b.s1, LOG2E) : 0.0f};
-}
-
-// What a row's loss and gradient are made of
+// What a row's gradient is made of: of the others (not listed) As 2^((z - mr) ct) + Bt 2^((z - mr) log2 e),
+// of an entry Qs 2^((z - mx) ct) + Bs 2^((z - mx) log2 e) - gs p; gh is taken off at the target.
 struct Coefs {
-    float mr;          // the others' exponentials are measured from it, the entries' from mx
-    float As, Bt;      // dz of the others: As exp((z - mr) / tau) + Bt exp(z - mr)
-    float Qs, Bs;      // of an entry: Qs exp((z - mx) / tau) + Bs exp(z - mx) - gs p
-    float gs, gh, mx;  // gh is taken off at the target
+    float mr, mx, As, Bt, Qs, Bs, gs, gh;
 };
 
-// From the others' sums and the entries, in a wave; the loss where it is wanted.
-// Where the temperatures are one, or only one counts, `two` is false and one sum serves both.
+// From the sums over the others (o) and the list; the loss where it is wanted
 template <bool TWO>
-ASCA_DEV Coefs distill_coefs(const DistillArgs& p, float w, const Entry& en, float total, float rest, Outside o, bool has_tg, float zt,
-                             bool want, float& loss) {
-    const bool on = en.id >= 0;
-    const float mx = fmaxf(o.m, wave_max(on ? en.z : -INFINITY));   // of the row
+ASCA_DEV Coefs distill_coefs(const DistillArgs& p, float w, Expo o, const List& l, bool has_tg, bool want, float& loss) {
+    const Expo all = expo_join<TWO>(o, l.e, p.ct);
     Coefs c;
-    c.mx = mx;
-    c.mr = o.m > -INFINITY ? o.m : mx;
-    const float ft = __builtin_amdgcn_exp2f((c.mr - mx) * p.ct), f1 = TWO ? __builtin_amdgcn_exp2f((c.mr - mx) * LOG2E) : ft;
-    const float et = on ? __builtin_amdgcn_exp2f((en.z - mx) * p.ct) : 0.0f;
-    const float at = o.st * ft + wave_sum(et);
-    float a1 = at;
-    if (TWO) a1 = o.s1 * f1 + wave_sum(on ? __builtin_amdgcn_exp2f((en.z - mx) * LOG2E) : 0.0f);
-    const bool tail = rest > 0.0f && o.st > 0.0f;
+    c.mx = all.m;
+    c.mr = o.m > -INFINITY ? o.m : c.mx;
+    const float ft = __builtin_amdgcn_exp2f((c.mr - c.mx) * p.ct), f1 = TWO ? __builtin_amdgcn_exp2f((c.mr - c.mx) * LOG2E) : ft;
+    const float a1 = TWO ? all.s1 : all.st;
+    const bool tail = l.rest > 0.0f && o.st > 0.0f;
     if (want) {
-        const double itau = 1.0 / (double)p.tau, lse = (double)mx * itau + log_d(at);
-        float kl = wave_sum(on && en.p != 0.0f ? (float)((double)en.p * (en.lp - ((double)en.z * itau - lse))) : 0.0f);
-        double l = 0.0;
+        const double lt = log_d(all.st), l1 = TWO ? log_d(a1) : lt;
+        double v = 0.0;
         if (p.alpha > 0.0f) {
-            l = kl;
-            if (tail) l += (double)rest * (log_d(rest) - (log_d(o.st) + (double)c.mr * itau - lse));
-            l *= (double)p.alpha * p.tau * p.tau;
+            const float ref = l.e.m > -INFINITY ? l.e.m : 0.0f;
+            if (l.total != 0.0f) v = (double)l.part + (double)l.total * (((double)c.mx - (double)ref) * p.itau + lt);
+            if (tail) v += (double)l.rest * (log_d(l.rest) - log_d(o.st) + ((double)c.mx - (double)c.mr) * p.itau + lt);
+            v *= (double)p.alpha * p.tau * p.tau;
         }
-        if (has_tg) l += (1.0 - (double)p.alpha) * ((double)mx + log_d(a1) - (double)zt);
-        loss = (float)(l * (double)w);
+        if (has_tg) v += (1.0 - (double)p.alpha) * ((double)c.mx + l1 - (double)l.zt);
+        loss = (float)(v * (double)w);
     }
     c.gs = p.scale * w * p.alpha * p.tau;
     c.gh = has_tg ? p.scale * w * (1.0f - p.alpha) : 0.0f;
     // the sum of p that the gradient meets: a rest that the student cannot give is left out
-    const float mass = tail ? 1.0f : total;
-    c.Qs = c.gs * mass / at;
-    c.As = c.gs * (mass * ft / at - (tail ? rest / o.st : 0.0f));
-    c.Bs = c.gh / a1;
-    c.Bt = c.gh * f1 / a1;
+    const float mass = tail ? 1.0f : l.total, qt = mass * recip(all.st), q1 = c.gh * recip(a1);
+    c.Qs = c.gs * qt;
+    c.As = c.gs * (qt * ft - (tail ? l.rest * recip(o.st) : 0.0f));
+    c.Bs = q1;
+    c.Bt = q1 * f1;
     if (!TWO) c.As += c.Bt, c.Qs += c.Bs;
     return c;
 }
@@ -148,12 +164,11 @@ ASCA_DEV float grad_entry(const Coefs& c, float ct, float z, float prob, bool ta
 
 template <int NW, int WORDS>
 struct DistillLds {
-    unsigned bits[WORDS];   // a bit for every column of a piece: it is listed
-    unsigned edge;          // and of those outside the pieces, by thread
-    Outside part[NW];
-    float z[64], p[64];     // the entries
-    int id[64];
-    float total, rest, zt;  // zt: the student's logit at the target
+    unsigned bits[WORDS ? WORDS : 1];   // a bit for every column of a piece: it is listed
+    unsigned edge;                      // and of those outside the pieces, by thread
+    Expo part[NW];
+    Entry en[64];
+    List list;
 };
 
 template <int NW>
@@ -166,7 +181,7 @@ ASCA_DEV void distill_sync() {
     }
 }
 
-// V values of a piece to the same place in another row of the same alignment
+// The values of a piece to the same columns of another row
 ASCA_DEV void piece_store(float* d, const float (&v)[4]) { act_store_n<4>(d, v); }
 ASCA_DEV void piece_store(bf16_t* d, const float (&v)[8]) {
     unsigned u[4];
@@ -188,6 +203,148 @@ ASCA_DEV void row_piece_store(E* d, bool whole, const float (&v)[16 / sizeof(E)]
     }
 }
 
+// Marks a listed column (of the row that r is of) in the bitmap; whether it was marked before
+template <typename E>
+ASCA_DEV bool mark(const Pieces<E>& r, int col, unsigned* bits, unsigned* edge) {
+    const int rel = col - r.head;
+    const bool in = rel >= 0 && rel < r.nb * Pieces<E>::W;
+    const unsigned bit = 1u << (in ? rel & 31 : r.edge_thread(col));
+    return (atomicOr(in ? bits + (rel >> 5) : edge, bit) & bit) != 0;
+}
+// The wave of NW that holds a column
+template <typename E, int NW>
+ASCA_DEV int wave_of(const Pieces<E>& r, int col) {
+    const int rel = col - r.head;
+    return rel >= 0 && rel < r.nb * Pieces<E>::W ? rel / Pieces<E>::W % (64 * NW) / 64 : 0;
+}
+
+// R pieces a thread of a row, or of a slice of one, in the registers of NW waves
+template <typename E, int NW, int R>
+struct RowRegs {
+    static constexpr int NT = 64 * NW, W = Pieces<E>::W;
+    uint4 raw[R ? R : 1];
+    float ev;   // the column outside the pieces that is the thread's
+    int ec;
+
+    ASCA_DEV void load(const Pieces<E>& r, int tid) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) raw[j] = r.piece(min(j * NT + tid, r.nb - 1));   // nb > 0 with R > 0
+        ec = r.edge(tid);
+        ev = -INFINITY;
+        if (ec >= 0) ev = act_load(r.p + ec);
+    }
+    // -inf in the place of what is listed and of what lies past the end; the thread's largest
+    ASCA_DEV float mask(const Pieces<E>& r, int tid, const unsigned* bits, unsigned edge) {
+        float m = -INFINITY, v[W];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const int i = j * NT + tid;
+            const unsigned b = bits[i * W / 32] >> (i * W % 32) & ((1u << W) - 1);
+            if (i >= r.nb) raw[j] = piece_of<E>(-INFINITY);
+            if (__ballot(b != 0)) piece_mask(raw[j], b, E());
+            piece_again(raw[j]);
+            piece_values(raw[j], v);
+#pragma unroll
+            for (int k = 0; k < W; ++k) m = max_or_nan(m, v[k]);
+            if (R >= 8) __builtin_amdgcn_sched_barrier(0);   // one piece's values in registers at a time
+        }
+        if (tid < 32 && edge >> tid & 1) ev = -INFINITY;
+        return max_or_nan(m, ev);
+    }
+    // f of every value, in its place
+    template <typename F>
+    ASCA_DEV void each(F f) {
+        float v[W];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            piece_again(raw[j]);
+            piece_values(raw[j], v);
+#pragma unroll
+            for (int k = 0; k < W; ++k) f(v[k]);
+            if (R >= 8) __builtin_amdgcn_sched_barrier(0);
+        }
+        f(ev);
+    }
+    // The wave's sums, from its largest m.  exp2(v c - rc) is one step and the exponential; what
+    // rounding m c to rc does is the same in every term and taken off at the end.
+    template <bool TWO>
+    ASCA_DEV Expo sums(float m, float ct) {
+        const float ref = m > -INFINITY ? m : 0.0f, rt = ref * ct, r1 = ref * LOG2E;
+        float st = 0.0f, s1 = 0.0f;
+        if (fabsf(rt) < 65536.0f && fabsf(r1) < 65536.0f) {
+            each([&](float v) {
+                st += __builtin_amdgcn_exp2f(fmaf(v, ct, -rt));
+                if (TWO) s1 += __builtin_amdgcn_exp2f(fmaf(v, LOG2E, -r1));
+            });
+            st *= __builtin_amdgcn_exp2f(-fmaf(ref, ct, -rt));
+            if (TWO) s1 *= __builtin_amdgcn_exp2f(-fmaf(ref, LOG2E, -r1));
+        } else {   // where that would be more than the terms
+            each([&](float v) {
+                st += __builtin_amdgcn_exp2f((v - ref) * ct);
+                if (TWO) s1 += __builtin_amdgcn_exp2f((v - ref) * LOG2E);
+            });
+        }
+        float x = 0.0f, y = 0.0f;
+        if (TWO) wave_sum4(st, s1, x, y);
+        else st = wave_sum(st);
+        return {m, st, s1};
+    }
+    template <typename F>
+    ASCA_DEV void store_each(const Pieces<E>& r, int tid, E* d, bool whole, F f) {
+        float v[W];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const int i = j * NT + tid;
+            piece_again(raw[j]);
+            piece_values(raw[j], v);
+#pragma unroll
+            for (int k = 0; k < W; ++k) v[k] = f(v[k]);
+            if (i < r.nb) row_piece_store<E>(d + r.col(i), whole, v);
+            if (R >= 8) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (ec >= 0) act_store(d + ec, f(ev));
+    }
+    // The gradient of everything as if it were not listed
+    template <bool TWO>
+    ASCA_DEV void store(const Pieces<E>& r, int tid, E* d, const Coefs& c, float ct) {
+        const bool whole = (reinterpret_cast<uintptr_t>(d) - reinterpret_cast<uintptr_t>(r.p)) % 16 == 0;
+        const float rt = c.mr * ct, r1 = c.mr * LOG2E;
+        if (fabsf(rt) < 65536.0f && fabsf(r1) < 65536.0f) {   // as in the sums
+            const float A = c.As * __builtin_amdgcn_exp2f(-fmaf(c.mr, ct, -rt));
+            const float B = TWO ? c.Bt * __builtin_amdgcn_exp2f(-fmaf(c.mr, LOG2E, -r1)) : 0.0f;
+            store_each(r, tid, d, whole, [&](float v) {
+                const float g = A * __builtin_amdgcn_exp2f(fmaf(v, ct, -rt));
+                return TWO ? fmaf(B, __builtin_amdgcn_exp2f(fmaf(v, LOG2E, -r1)), g) : g;
+            });
+        } else {
+            store_each(r, tid, d, whole, [&](float v) { return grad_other<TWO>(c, ct, v); });
+        }
+    }
+};
+
+// The list's columns and the target's, over what was written there just now, by the wave that
+// wrote it: its stores to an address stay in order.  r and d are of the row or of the slice from c0.
+template <typename E, int NW, bool TWO>
+ASCA_DEV void store_listed(const DistillArgs& p, const Pieces<E>& r, int c0, int wave, E* d, const Coefs& c, const Entry& en,
+                           unsigned tg, bool has_tg, float zt) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    auto mine = [&](int col) { return col >= 0 && col < r.n && (NW == 1 || wave_of<E, NW>(r, col) == wave); };
+    if (en.id >= 0 && mine(en.id - c0)) act_store(d + en.id - c0, grad_entry<TWO>(c, p.ct, en.z, en.p, (unsigned)en.id == tg));
+    const bool listed = __ballot(has_tg && en.id == (int)tg) != 0;
+    if ((threadIdx.x & 63) == 0 && has_tg && !listed && mine((int)tg - c0))
+        act_store(d + (int)tg - c0, grad_other<TWO>(c, p.ct, zt) - c.gh);
+}
+
+ASCA_DEV unsigned target_of(const DistillArgs& p, long row) { return p.alpha < 1.0f ? p.targets[row] : ~0u; }
+
+// A row without weight is not read
+template <typename E>
+ASCA_DEV void no_weight(const DistillArgs& p, long row, int c0, int n, int tid, int threads) {
+    if (tid == 0 && c0 == 0) p.losses[row] = 0.0f;
+    if (p.dz)
+        for (int c = tid; c < n; c += threads) act_store(static_cast<E*>(p.dz) + row * p.lddz + c0 + c, 0.0f);
+}
+
 // Rows in the registers of a team of NW waves, R pieces a thread: a row is read once and its
 // gradient written once.  The list's columns are taken out by a bitmap in LDS, so that the
 // others' sum is formed without them (a difference of sums would lose it where the student is
@@ -202,118 +359,141 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void distill_rows_k(Distil
     if (row >= p.T) return;
     DistillLds<NW, WORDS>& l = lds[team];
     const E* z = static_cast<const E*>(p.z) + row * p.ld;
-    E* dz = p.dz ? static_cast<E*>(p.dz) + row * p.lddz : nullptr;
     const float w = p.weights ? p.weights[row] : 1.0f;
-    if (w == 0.0f) {
-        if (tid == 0) p.losses[row] = 0.0f;
-        if (dz)
-            for (int c = tid; c < p.V; c += NT) act_store(dz + c, 0.0f);
-        return;
-    }
-    const bool lists = wave == 0 && lane < p.K;
-    Entry en{-1, 0.0f, 0.0, 0.0f};
+    if (w == 0.0f) return no_weight<E>(p, row, 0, p.V, tid, NT);
+    Entry en{-1, 0.0f, 0.0f};
     float tv = 0.0f;
-    if (lists) en.id = p.tids[row * p.K + lane], tv = p.tval[row * p.K + lane];
-    const unsigned tg = p.alpha < 1.0f ? p.targets[row] : ~0u;
-    const Pieces<E> r(z, p.V);
-    uint4 raw[R];
-    if (r.nb > 0)
-#pragma unroll
-        for (int j = 0; j < R; ++j) raw[j] = r.piece(min(j * NT + tid, r.nb - 1));
-    const int ec = r.edge(tid);
-    float ev = -INFINITY;
-    if (ec >= 0) ev = act_load(z + ec);
-    const bool has_tg = tg < (unsigned)p.V;
+    if (wave == 0 && p.K) {
+        const long at = row * p.K + min(lane, p.K - 1);
+        en.id = p.tids[at], tv = p.tval[at];
+    }
+    const Pieces<E> r(z, p.V, R > 0);
+    RowRegs<E, NW, R> x;
+    x.load(r, tid);
 #pragma unroll
     for (int i = tid; i < WORDS; i += NT) l.bits[i] = 0;
     if (tid == 0) l.edge = 0;
     distill_sync<NW>();
+    const unsigned tg = target_of(p, row);
+    const bool has_tg = tg < (unsigned)p.V;
+    List li;
     if (wave == 0) {
-        bool twice = false;
+        if (lane >= p.K || en.id >= p.V) en.id = -1;
         const float zt = has_tg ? act_load(z + tg) : 0.0f;
-        if (en.id >= p.V) en.id = -1;
-        en.lp = tv;
+        bool twice = false;
         if (en.id >= 0) {
             en.z = act_load(z + en.id);
-            const int rel = en.id - r.head;
-            const bool in = rel >= 0 && rel < r.nb * W;
-            const unsigned bit = 1u << (in ? rel & 31 : r.edge_thread(en.id));
-            twice = (atomicOr(in ? &l.bits[rel >> 5] : &l.edge, bit) & bit) != 0;
+            twice = mark<E>(r, en.id, l.bits, &l.edge);
         }
-        float total, rest;
-        entry_probs(p, row, __ballot(twice) != 0, en, total, rest);
-        l.id[lane] = en.id, l.z[lane] = en.z, l.p[lane] = en.p;
-        if (lane == 0) l.total = total, l.rest = rest, l.zt = zt;
+        li = list_of<TWO>(p, row, tv, __ballot(twice) != 0, en);
+        li.zt = zt;
+        if constexpr (NW > 1) {
+            l.en[lane] = en;
+            if (lane == 0) l.list = li;
+        }
     }
     distill_sync<NW>();
-    // the list out of the row, and the others' largest and sums, a wave's own first
-    float v[W];
-    Outside o{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        const int i = j * NT + tid;
-        const unsigned bits = l.bits[i * W / 32] >> (i * W % 32) & ((1u << W) - 1);
-        if (i >= r.nb) raw[j] = piece_of<E>(-INFINITY);
-        if (__ballot(bits != 0)) piece_mask(raw[j], bits, E());
-        piece_again(raw[j]);
-        piece_values(raw[j], v);
-#pragma unroll
-        for (int k = 0; k < W; ++k) o.m = max_or_nan(o.m, v[k]);
-        if (R >= 8) __builtin_amdgcn_sched_barrier(0);   // one piece's values in registers at a time
-    }
-    if (l.edge >> (tid & 31) & 1 && tid < 2 * W) ev = -INFINITY;
-    o.m = wave_max(fmaxf(o.m, ev));
-    const float ref = o.m > -INFINITY ? o.m : 0.0f;
-    o.st = __builtin_amdgcn_exp2f((ev - ref) * p.ct);
-    if (TWO) o.s1 = __builtin_amdgcn_exp2f((ev - ref) * LOG2E);
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        piece_again(raw[j]);
-        piece_values(raw[j], v);
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-            o.st += __builtin_amdgcn_exp2f((v[k] - ref) * p.ct);
-            if (TWO) o.s1 += __builtin_amdgcn_exp2f((v[k] - ref) * LOG2E);
-        }
-        if (R >= 8) __builtin_amdgcn_sched_barrier(0);
-    }
-    o.st = wave_sum(o.st);
-    if (TWO) o.s1 = wave_sum(o.s1);
+    Expo o = x.template sums<TWO>(wave_max(x.mask(r, tid, l.bits, l.edge)), p.ct);
     if constexpr (NW > 1) {
         if (lane == 0) l.part[wave] = o;
         lds_barrier();
         o = l.part[0];
 #pragma unroll
-        for (int k = 1; k < NW; ++k) o = outside_join(o, l.part[k], p.ct, TWO);
-        if (wave != 0) en.id = l.id[lane], en.z = l.z[lane], en.p = l.p[lane];
+        for (int k = 1; k < NW; ++k) o = expo_join<TWO>(o, l.part[k], p.ct);
+        en = l.en[lane], li = l.list;
     }
     float loss = 0.0f;
-    const float zt = l.zt;
-    const Coefs c = distill_coefs<TWO>(p, w, en, l.total, l.rest, o, has_tg, zt, wave == 0, loss);
+    const Coefs c = distill_coefs<TWO>(p, w, o, li, has_tg, wave == 0, loss);
     if (tid == 0) p.losses[row] = loss;
-    if (!dz) return;
-    const bool whole = (reinterpret_cast<uintptr_t>(dz) - reinterpret_cast<uintptr_t>(z)) % 16 == 0;
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        const int i = j * NT + tid;
-        piece_again(raw[j]);
-        piece_values(raw[j], v);
-#pragma unroll
-        for (int k = 0; k < W; ++k) v[k] = grad_other<TWO>(c, p.ct, v[k]);
-        if (i < r.nb) row_piece_store<E>(dz + r.col(i), whole, v);
-        if (R >= 8) __builtin_amdgcn_sched_barrier(0);
+    if (!p.dz) return;
+    E* dz = static_cast<E*>(p.dz) + row * p.lddz;
+    x.template store<TWO>(r, tid, dz, c, p.ct);
+    store_listed<E, NW, TWO>(p, r, 0, wave, dz, c, en, tg, has_tg, li.zt);
+}
+
+// A few long rows: S slices each, a block's of 4 waves.  The first launch leaves the slices'
+// sums, and from the first slice the list; the second forms the gradient.
+struct SplitRow {
+    Entry en[64];
+    List list;
+};
+template <typename E, int R, bool TWO>
+__global__ __launch_bounds__(256) void distill_part_k(DistillArgs p) {
+    constexpr int WORDS = 256 * R * Pieces<E>::W / 32;
+    __shared__ DistillLds<4, WORDS> l;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const int slice = blockIdx.x % (unsigned)p.S, c0 = slice * p.slice, n = min(p.slice, p.V - c0);
+    const long row = blockIdx.x / (unsigned)p.S;
+    const E* z = static_cast<const E*>(p.z) + row * p.ld;
+    if (p.weights && p.weights[row] == 0.0f) return;
+    Entry en{-1, 0.0f, 0.0f};
+    float tv = 0.0f;
+    if (wave == 0 && p.K) {
+        const long at = row * p.K + min(lane, p.K - 1);
+        en.id = p.tids[at], tv = p.tval[at];
     }
-    if (ec >= 0) act_store(dz + ec, grad_other<TWO>(c, p.ct, ev));
-    // the list's columns and the target's, over what was written there just now: by the wave that
-    // wrote it, whose stores to an address stay in order
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    auto mine = [&](int col) {
-        const int rel = col - r.head;
-        return NW == 1 || (rel >= 0 && rel < r.nb * W ? rel / W % NT / 64 : 0) == wave;
-    };
-    if (en.id >= 0 && mine(en.id)) act_store(dz + en.id, grad_entry<TWO>(c, p.ct, en.z, en.p, (unsigned)en.id == tg));
-    const bool tg_listed = __ballot(has_tg && en.id == (int)tg) != 0;
-    if (lane == 0 && has_tg && !tg_listed && mine(tg)) act_store(dz + tg, grad_other<TWO>(c, p.ct, zt) - c.gh);
+    const Pieces<E> r(z + c0, n, true);
+    RowRegs<E, 4, R> x;
+    x.load(r, tid);
+#pragma unroll
+    for (int i = tid; i < WORDS; i += 256) l.bits[i] = 0;
+    if (tid == 0) l.edge = 0;
+    lds_barrier();
+    if (wave == 0) {
+        if (lane >= p.K || en.id >= p.V) en.id = -1;
+        if (en.id >= c0 && en.id - c0 < n) mark<E>(r, en.id - c0, l.bits, &l.edge);
+        if (slice == 0) {
+            const unsigned tg = target_of(p, row);
+            const float zt = tg < (unsigned)p.V ? act_load(z + tg) : 0.0f;
+            if (en.id >= 0) en.z = act_load(z + en.id);
+            bool twice = false;   // (the bitmap is of this slice alone)
+            for (int j = 0; j < p.K; ++j) twice |= j < lane && en.id >= 0 && __builtin_amdgcn_readlane(en.id, j) == en.id;
+            List li = list_of<TWO>(p, row, tv, __ballot(twice) != 0, en);
+            li.zt = zt;
+            p.split[row].en[lane] = en;
+            if (lane == 0) p.split[row].list = li;
+        }
+    }
+    lds_barrier();
+    const Expo o = x.template sums<TWO>(wave_max(x.mask(r, tid, l.bits, l.edge)), p.ct);
+    if (lane == 0) l.part[wave] = o;
+    lds_barrier();
+    if (tid == 0) {
+        Expo a = l.part[0];
+        for (int k = 1; k < 4; ++k) a = expo_join<TWO>(a, l.part[k], p.ct);
+        p.parts[blockIdx.x] = a;
+    }
+}
+template <typename E, int R, bool TWO>
+__global__ __launch_bounds__(256) void distill_finish_k(DistillArgs p) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const int slice = blockIdx.x % (unsigned)p.S, c0 = slice * p.slice, n = min(p.slice, p.V - c0);
+    const long row = blockIdx.x / (unsigned)p.S;
+    const E* z = static_cast<const E*>(p.z) + row * p.ld + c0;
+    const float w = p.weights ? p.weights[row] : 1.0f;
+    if (w == 0.0f) return no_weight<E>(p, row, c0, n, tid, 256);
+    const Pieces<E> r(z, n, true);
+    RowRegs<E, 4, R> x;
+    if (p.dz) x.load(r, tid);
+    const Entry en = p.split[row].en[lane];
+    const List li = p.split[row].list;
+    const unsigned tg = target_of(p, row);
+    const bool has_tg = tg < (unsigned)p.V;
+    // S <= 64: a slice a lane, joined in the same order by every wave
+    Expo o{-INFINITY, 0.0f, 0.0f};
+    if (lane < p.S) o = p.parts[row * p.S + lane];
+    const float m = wave_max(o.m);
+    o = expo_join<TWO>(o, {m, 0.0f, 0.0f}, p.ct);
+    float u = 0.0f, v = 0.0f;
+    wave_sum4(o.st, o.s1, u, v);
+    o.m = m;
+    float loss = 0.0f;
+    const Coefs c = distill_coefs<TWO>(p, w, o, li, has_tg, slice == 0 && wave == 0, loss);
+    if (tid == 0 && slice == 0) p.losses[row] = loss;
+    if (!p.dz) return;
+    E* dz = static_cast<E*>(p.dz) + row * p.lddz + c0;
+    x.template store<TWO>(r, tid, dz, c, p.ct);
+    store_listed<E, 4, TWO>(p, r, c0, wave, dz, c, en, tg, has_tg, li.zt);
 }
 
 // Rows that no team's registers hold: read twice, by 1024 threads, the second time mostly from
@@ -322,24 +502,19 @@ template <typename E, bool TWO>
 __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
     constexpr int NW = 16, NT = 1024, W = Pieces<E>::W, U = 4;
     extern __shared__ unsigned bits[];
-    __shared__ DistillLds<NW, 1> l;
+    __shared__ DistillLds<NW, 0> l;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const long row = blockIdx.x;
     const E* z = static_cast<const E*>(p.z) + row * p.ld;
-    E* dz = p.dz ? static_cast<E*>(p.dz) + row * p.lddz : nullptr;
     const float w = p.weights ? p.weights[row] : 1.0f;
-    if (w == 0.0f) {
-        if (tid == 0) p.losses[row] = 0.0f;
-        if (dz)
-            for (int c = tid; c < p.V; c += NT) act_store(dz + c, 0.0f);
-        return;
-    }
-    Entry en{-1, 0.0f, 0.0, 0.0f};
+    if (w == 0.0f) return no_weight<E>(p, row, 0, p.V, tid, NT);
+    Entry en{-1, 0.0f, 0.0f};
     float tv = 0.0f;
-    if (wave == 0 && lane < p.K) en.id = p.tids[row * p.K + lane], tv = p.tval[row * p.K + lane];
-    const unsigned tg = p.alpha < 1.0f ? p.targets[row] : ~0u;
-    const bool has_tg = tg < (unsigned)p.V;
-    const Pieces<E> r(z, p.V);
+    if (wave == 0 && p.K) {
+        const long at = row * p.K + min(lane, p.K - 1);
+        en.id = p.tids[at], tv = p.tval[at];
+    }
+    const Pieces<E> r(z, p.V, true);
     const int words = (r.nb * W + 31) / 32;
     for (int i = tid; i < words; i += NT) bits[i] = 0;
     if (tid == 0) l.edge = 0;
@@ -347,34 +522,28 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
     float ev = -INFINITY;
     if (ec >= 0) ev = act_load(z + ec);
     lds_barrier();
+    const unsigned tg = target_of(p, row);
+    const bool has_tg = tg < (unsigned)p.V;
     if (wave == 0) {
-        bool twice = false;
+        if (lane >= p.K || en.id >= p.V) en.id = -1;
         const float zt = has_tg ? act_load(z + tg) : 0.0f;
-        if (en.id >= p.V) en.id = -1;
-        en.lp = tv;
+        bool twice = false;
         if (en.id >= 0) {
             en.z = act_load(z + en.id);
-            const int rel = en.id - r.head;
-            const bool in = rel >= 0 && rel < r.nb * W;
-            const unsigned bit = 1u << (in ? rel & 31 : r.edge_thread(en.id));
-            twice = (atomicOr(in ? &bits[rel >> 5] : &l.edge, bit) & bit) != 0;
+            twice = mark<E>(r, en.id, bits, &l.edge);
         }
-        float total, rest;
-        entry_probs(p, row, __ballot(twice) != 0, en, total, rest);
-        l.id[lane] = en.id, l.z[lane] = en.z, l.p[lane] = en.p;
-        if (lane == 0) l.total = total, l.rest = rest, l.zt = zt;
+        List li = list_of<TWO>(p, row, tv, __ballot(twice) != 0, en);
+        li.zt = zt;
+        l.en[lane] = en;
+        if (lane == 0) l.list = li;
     }
     lds_barrier();
-    if (tid < 2 * W && l.edge >> tid & 1) ev = -INFINITY;
-    Outside o{ev, 0.0f, 0.0f};
-    {
-        const float ref = ev > -INFINITY ? ev : 0.0f;
-        o.st = __builtin_amdgcn_exp2f((ev - ref) * p.ct);   // 1, 0 or NaN
-        o.s1 = o.st;
-    }
+    if (tid < 32 && l.edge >> tid & 1) ev = -INFINITY;
+    const float e = __builtin_amdgcn_exp2f(ev - (ev > -INFINITY ? ev : 0.0f));   // 1, 0 or NaN
+    Expo o{ev, e, e};
     for (int i0 = tid; i0 < r.nb; i0 += U * NT) {
         uint4 raw[U];
-        Outside n{-INFINITY, 0.0f, 0.0f};
+        Expo n{-INFINITY, 0.0f, 0.0f};
         float v[W];
 #pragma unroll
         for (int u = 0; u < U; ++u) raw[u] = r.piece(min(i0 + u * NT, r.nb - 1));
@@ -397,23 +566,26 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
                 if (TWO) n.s1 += __builtin_amdgcn_exp2f((v[k] - ref) * LOG2E);
             }
         }
-        o = outside_join(o, n, p.ct, TWO);
+        o = expo_join<TWO>(o, n, p.ct);
     }
     {
         const float m = wave_max(o.m);
-        const Outside n = outside_join(o, {m, 0.0f, 0.0f}, p.ct, TWO);
-        o = {m, wave_sum(n.st), TWO ? wave_sum(n.s1) : 0.0f};
+        o = expo_join<TWO>(o, {m, 0.0f, 0.0f}, p.ct);
+        float x = 0.0f, y = 0.0f;
+        wave_sum4(o.st, o.s1, x, y);
+        o.m = m;
     }
     if (lane == 0) l.part[wave] = o;
     lds_barrier();
     o = l.part[0];
-    for (int k = 1; k < NW; ++k) o = outside_join(o, l.part[k], p.ct, TWO);
-    if (wave != 0) en.id = l.id[lane], en.z = l.z[lane], en.p = l.p[lane];
+    for (int k = 1; k < NW; ++k) o = expo_join<TWO>(o, l.part[k], p.ct);
+    en = l.en[lane];
+    const List li = l.list;
     float loss = 0.0f;
-    const float zt = l.zt;
-    const Coefs c = distill_coefs<TWO>(p, w, en, l.total, l.rest, o, has_tg, zt, wave == 0, loss);
+    const Coefs c = distill_coefs<TWO>(p, w, o, li, has_tg, wave == 0, loss);
     if (tid == 0) p.losses[row] = loss;
-    if (!dz) return;
+    if (!p.dz) return;
+    E* dz = static_cast<E*>(p.dz) + row * p.lddz;
     const bool whole = (reinterpret_cast<uintptr_t>(dz) - reinterpret_cast<uintptr_t>(z)) % 16 == 0;
     // (dz may be z: a thread writes the pieces that it reads, and all have read the entries)
     for (int i0 = tid; i0 < r.nb; i0 += U * NT) {
@@ -431,21 +603,45 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
         }
     }
     if (ec >= 0) act_store(dz + ec, grad_other<TWO>(c, p.ct, ev));
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // as in distill_rows_k
-    auto mine = [&](int col) {
-        const int rel = col - r.head;
-        return (rel >= 0 && rel < r.nb * W ? rel / W % NT / 64 : 0) == wave;
-    };
-    if (en.id >= 0 && mine(en.id)) act_store(dz + en.id, grad_entry<TWO>(c, p.ct, en.z, en.p, (unsigned)en.id == tg));
-    const bool tg_listed = __ballot(has_tg && en.id == (int)tg) != 0;
-    if (lane == 0 && has_tg && !tg_listed && mine(tg)) act_store(dz + tg, grad_other<TWO>(c, p.ct, zt) - c.gh);
+    store_listed<E, NW, TWO>(p, r, 0, wave, dz, c, en, tg, has_tg, li.zt);
 }
 
 template <typename E, bool TWO>
-static int distill_launch(const DistillArgs& a, hipStream_t st) {
+static int distill_launch(DistillArgs a, hipStream_t st) {
     constexpr int W = 16 / sizeof(E);
-    const long pieces = (a.V + W - 1) / W;
+    const long pieces = (a.V + W - 1) / W, cus = std::max(cu_count(), 1);
     int r;
+    // Rows that are fewer than the CUs and long: slices of 256 x 4 pieces at the most, of about
+    // the whole device, at most 64 a row
+    if (a.T * 2 <= cus && pieces > 1024) {
+        const long most = std::min(64l, (pieces + 255) / 256), least = std::min(most, (pieces + 256 * 8 - 1) / (256 * 8));
+        const long s = std::max(least, std::min(most, 2 * cus / a.T));
+        a.slice = (int)((pieces + s - 1) / s * W);
+        a.S = (a.V + a.slice - 1) / a.slice;
+        if (a.V - (a.S - 1) * a.slice < 2 * W) --a.S, a.slice += 2 * W;   // no slice without a whole piece
+        const int per = (a.slice / W + 255) / 256;
+        if (per <= 8) {
+            StreamScratch scratch;
+            const size_t parts = ((size_t)a.T * a.S * sizeof(Expo) + 15) / 16 * 16;
+            if ((r = scratch.get((parts + (size_t)a.T * sizeof(SplitRow)) / 4, st))) return r;
+            a.parts = reinterpret_cast<Expo*>(scratch.ws.p);
+            a.split = reinterpret_cast<SplitRow*>(reinterpret_cast<char*>(scratch.ws.p) + parts);
+            const dim3 grid((unsigned)(a.T * a.S)), block(256);
+            void (*part)(DistillArgs) = per <= 1   ? distill_part_k<E, 1, TWO>
+                                        : per <= 2 ? distill_part_k<E, 2, TWO>
+                                        : per <= 4 ? distill_part_k<E, 4, TWO>
+                                                   : distill_part_k<E, 8, TWO>;
+            void (*finish)(DistillArgs) = per <= 1   ? distill_finish_k<E, 1, TWO>
+                                          : per <= 2 ? distill_finish_k<E, 2, TWO>
+                                          : per <= 4 ? distill_finish_k<E, 4, TWO>
+                                                     : distill_finish_k<E, 8, TWO>;
+            if ((r = pre_launch("distill_part"))) return r;
+            hipLaunchKernelGGL(part, grid, block, 0, st, a);
+            if ((r = post_launch("distill_part")) || (r = pre_launch("distill_finish"))) return r;
+            hipLaunchKernelGGL(finish, grid, block, 0, st, a);
+            return post_launch("distill_finish");
+        }
+    }
     if (pieces > 1024 * 16) {
         const size_t lds = ((size_t)a.V + 31) / 32 * 4;
         if ((r = allow_lds(reinterpret_cast<const void*>(&distill_long_k<E, TWO>), lds))) return r;
@@ -454,18 +650,20 @@ static int distill_launch(const DistillArgs& a, hipStream_t st) {
         return post_launch("distill_long");
     }
     if ((r = pre_launch("distill_rows"))) return r;
-    const bool many = a.T >= 4l * std::max(cu_count(), 1);
+    const bool many = a.T >= 4 * cus;
     auto go = [&](auto nw, auto rr) {
         constexpr int NW = decltype(nw)::value, R = decltype(rr)::value;
-        hipLaunchKernelGGL((distill_rows_k<E, NW, R, TWO>), dim3((unsigned)(NW == 1 ? (a.T + 3) / 4 : a.T)), dim3(NW == 1 ? 256 : 64 * NW), 0,
-                           st, a);
+        hipLaunchKernelGGL((distill_rows_k<E, NW, R, TWO>), dim3((unsigned)(NW == 1 ? (a.T + 3) / 4 : a.T)),
+                           dim3(NW == 1 ? 256 : 64 * NW), 0, st, a);
     };
+    std::integral_constant<int, 0> n0;
     std::integral_constant<int, 1> n1;
     std::integral_constant<int, 2> n2;
     std::integral_constant<int, 4> n4;
     std::integral_constant<int, 8> n8;
     std::integral_constant<int, 16> n16;
-    if (pieces <= 64) go(n1, n1);
+    if (a.V < 2 * W) go(n1, n0);   // maybe no whole piece
+    else if (pieces <= 64) go(n1, n1);
     else if (pieces <= 64 * 2 && many) go(n1, n2);
     else if (pieces <= 64 * 4 && many) go(n1, n4);
     else if (pieces <= 64 * 8 && many) go(n1, n8);
@@ -520,7 +718,8 @@ int asca_distill(const void* logits, long ld, const float* tval, const int32_t* 
         const bool two = alpha > 0.0f && alpha < 1.0f && temperature != 1.0f;
         const float ct = alpha > 0.0f ? (float)(1.4426950408889634 / (double)temperature) : LOG2E;
         const DistillArgs a{logits, ld, tval, tids, tlse, targets, weights, losses, dlogits, lddl, T, V, alpha > 0.0f ? K : 0,
-                            alpha > 0.0f ? temperature : 1.0f, ct, alpha, scale};
+                            alpha > 0.0f ? temperature : 1.0f, ct, alpha, scale, alpha > 0.0f ? 1.0 / (double)temperature : 1.0, 1, V,
+                            nullptr, nullptr};
         const hipStream_t st = as_stream(stream);
         return two ? distill_launch<E, true>(a, st) : distill_launch<E, false>(a, st);
     });

@@ -61,11 +61,28 @@ ASCA_DEV float lane_pick(float x, float c) {
         return __builtin_amdgcn_fmed3f(x, lane_xor<M>(x), c);
     }
 }
-// The largest of the wave's values; a NaN is none of them
+// The larger of two, or NaN where either is (one instruction for three of them; a maximum that
+// leaves a NaN out quiets each operand first)
+ASCA_DEV float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// The largest of the wave's values, NaN where one is
 ASCA_DEV float wave_max(float x) {
-    x = lane_pick<1>(x, INFINITY), x = lane_pick<2>(x, INFINITY), x = lane_pick<4>(x, INFINITY);
-    x = lane_pick<8>(x, INFINITY), x = lane_pick<16>(x, INFINITY);
-    return lane_pick<32>(x, INFINITY);
+    x = max_or_nan(x, lane_xor<1>(x));
+    x = max_or_nan(x, lane_xor<2>(x));
+    x = max_or_nan(x, dpp<DPP_HALF_MIRROR>(x));   // four lanes hold the same
+    x = max_or_nan(x, dpp<DPP_ROW_MIRROR>(x));
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = max_or_nan(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max_or_nan(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+ASCA_DEV float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
+
+// The sums of four values over the wave together: a third of the steps that they take apart
+ASCA_DEV void wave_sum4(float& a, float& b, float& c, float& d) {
+    const float x = group_sum<16>(tsum16(tsum32(a, b), tsum32(c, d)));
+    a = lane_value(x, 0), c = lane_value(x, 16), b = lane_value(x, 32), d = lane_value(x, 48);
 }
 
 template <int M>
@@ -93,9 +110,6 @@ ASCA_DEV float lane_sort(float x) {
     x = lane_merge<32>(lane_flip(x, d & 16));
     return lane_merge<64>(lane_flip(x, l & 32));
 }
-
-// The larger of two, or NaN where either is
-ASCA_DEV float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 template <typename T>
 ASCA_DEV T wave_max_t(T x) {
@@ -146,14 +160,16 @@ struct Pieces {
     static constexpr int W = 16 / sizeof(E);
     const E* p;
     int n, head, nb;
-    ASCA_DEV Pieces(const E* row, int len) : p(row), n(len) {
+    // (without pieces all of up to 2 W - 1 elements are at the edges)
+    ASCA_DEV Pieces(const E* row, int len, bool pieces = true) : p(row), n(len) {
         const int off = (int)(reinterpret_cast<uintptr_t>(row) / sizeof(E) % W);
         head = min(off ? W - off : 0, n);
-        nb = (n - head) / W;
+        nb = pieces ? (n - head) / W : 0;
     }
     ASCA_DEV uint4 piece(int i) const { return reinterpret_cast<const uint4*>(p + head)[i]; }
     ASCA_DEV int col(int i) const { return head + i * W; }   // the first column of a piece
-    // the column outside the pieces that thread t of at least 2 W takes, or -1
+    // the column outside the pieces that thread t takes, or -1: one of the first 2 W, of the first 32
+    // without pieces
     ASCA_DEV int edge(int t) const {
         if (t < head) return t;
         const int c = head + nb * W + t - W;

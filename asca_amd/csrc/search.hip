@@ -45,8 +45,6 @@ ASCA_DEV void team_sync() {
 template <int NW>
 ASCA_DEV int team_wave() { return NW == 1 ? 0 : wave_id(); }
 
-ASCA_DEV float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
-
 // The 64 largest of four sorted lists in LDS, sorted
 ASCA_DEV float four_lists(const float (&l)[4][64]) {
     const int lane = threadIdx.x & 63;
