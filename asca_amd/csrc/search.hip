@@ -31,6 +31,7 @@ struct TeamLds {
     float lists[NW][64], sums[NW], tops[NW];
     uint64_t best[NW];
     int n[NW];                    // keys; above KEYS: too many
+    int rank[NW == 1 ? 1 : NW * KEYS];
 };
 
 template <int NW>
@@ -87,28 +88,46 @@ ASCA_DEV void wave_push(uint64_t key, int& n, TeamLds<NW>& l) {
     n += __popcll(some);
 }
 
-// The ranks of the wave's n keys among all waves', R a lane
+// How many of the wave's own keys are larger than each of the team's n, R of these a lane;
+// a wide team's waves add theirs up
 template <int NW, int R, typename Out>
-ASCA_DEV void wave_rank(int K, int n, TeamLds<NW>& l, Out out) {
+ASCA_DEV void team_count(int K, int n, TeamLds<NW>& l, Out out) {
     const int lane = threadIdx.x & 63, w = team_wave<NW>();
     uint64_t key[R];
     int rank[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) key[r] = lane + 64 * r < n ? l.keys[w][lane + 64 * r] : 0, rank[r] = 0;
-    for (int v = 0; v < NW; ++v)
-        for (int j = 0; j < l.n[v]; j += 2) {   // (an odd number of them ends in a 0)
-            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&l.keys[v][j]);
+    for (int r = 0; r < R; ++r) {
+        int i = lane + 64 * r, v = 0;
+        key[r] = 0, rank[r] = 0;
+        if (i >= n) continue;
 #pragma unroll
-            for (int r = 0; r < R; ++r) rank[r] += (two.x > key[r]) + (two.y > key[r]);
-        }
+        for (int u = 0; u < NW - 1; ++u)   // the i-th of all
+            if (i >= l.n[u] && v == u) i -= l.n[u], ++v;
+        key[r] = l.keys[v][i];
+    }
+    for (int j = 0; j < l.n[w]; j += 2) {   // (an odd number of them ends in a 0)
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&l.keys[w][j]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) rank[r] += (two.x > key[r]) + (two.y > key[r]);
+    }
+    if constexpr (NW > 1) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (lane + 64 * r < n) atomicAdd(&l.rank[lane + 64 * r], rank[r]);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; ++r) rank[r] = l.rank[lane + 64 * r];
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r)
-        if (lane + 64 * r < n && rank[r] < K) out(rank[r], key[r]);
+        if (r % NW == w && lane + 64 * r < n && rank[r] < K) out(rank[r], key[r]);
 }
 
 // The keys' end, for all to see: their number, and one 0 more
 template <int NW>
 ASCA_DEV void wave_end(int n, TeamLds<NW>& l) {
+    if constexpr (NW > 1)
+        for (int i = threadIdx.x; i < NW * TeamLds<NW>::KEYS; i += 64 * NW) l.rank[i] = 0;
     if ((threadIdx.x & 63) != 0) return;
     l.n[team_wave<NW>()] = n;
     if (n < TeamLds<NW>::KEYS) l.keys[team_wave<NW>()][n] = 0;
@@ -128,10 +147,10 @@ ASCA_DEV void team_rank(int K, TeamLds<NW>& l, Each each, Out out) {
         fits &= k <= TeamLds<NW>::KEYS;
     }
     if (fits) {
-        const int n = l.n[w];
-        if (n <= 64) wave_rank<NW, 1>(K, n, l, out);
-        else if (n <= 128) wave_rank<NW, 2>(K, n, l, out);
-        else if constexpr (TeamLds<NW>::KEYS > 128) wave_rank<NW, TeamLds<NW>::KEYS / 64>(K, n, l, out);
+        if (all <= 64) team_count<NW, 1>(K, all, l, out);
+        else if (all <= 128) team_count<NW, 2>(K, all, l, out);
+        else if (all <= 256) team_count<NW, 4>(K, all, l, out);
+        else if constexpr (NW > 1) team_count<NW, 8>(K, all, l, out);
         for (int r = all + tid; r < K; r += 64 * NW) out(r, 0);
         return;
     }
@@ -618,6 +637,7 @@ static int rows_check(const char* fn, long rows, int V, long ld, const void* z, 
 //   a thread (shorter ones cost more in the merge than they spread) and eight (32 registers).
 //   Whole rows of up to 1024 x 8 pieces in blocks of 16 waves are slower than their slices and
 //   a merge (4096 x 16384 f32, 16 of them: 120 us against 60).
+constexpr int TOP_R = 16;   // pieces a thread at most
 template <typename E>
 static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const char* fn) {
     constexpr int W = 16 / sizeof(E);
@@ -627,7 +647,7 @@ static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const 
         a.S = 1;
         a.slice = a.V;
     } else {
-        const long least = (a.V + 256l * 8 * W - 1) / (256l * 8 * W), most = (a.V + 256l * W - 1) / (256l * W);
+        const long least = (a.V + 256l * TOP_R * W - 1) / (256l * TOP_R * W), most = (a.V + 256l * W - 1) / (256l * W);
         const long s = std::max(least, std::min(most, (want + a.rows - 1) / a.rows));
         a.slice = (int)(((a.V + s - 1) / s + W - 1) / W * W);
         a.S = (a.V + a.slice - 1) / a.slice;
@@ -651,7 +671,8 @@ static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const 
         void (*k)(TopArgs) = per <= 1   ? top_slice_k<E, NW, 1>
                              : per <= 2 ? top_slice_k<E, NW, 2>
                              : per <= 4 ? top_slice_k<E, NW, 4>
-                                        : top_slice_k<E, NW, 8>;
+                             : per <= 8 ? top_slice_k<E, NW, 8>
+                                        : top_slice_k<E, NW, 16>;
         hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a);
     };
     if (nw == 1) go(std::integral_constant<int, 1>());
