@@ -242,10 +242,10 @@ struct RowRegs {
         for (int j = 0; j < R; ++j) {
             const int i = j * NT + tid;
             const unsigned b = bits[i * W / 32] >> (i * W % 32) & ((1u << W) - 1);
-            if (i >= r.nb) raw[j] = piece_of<E>(-INFINITY);
+            if (i >= r.nb) raw[j] = piece_none<E>();
             if (__ballot(b != 0)) piece_mask(raw[j], b, E());
             piece_again(raw[j]);
-            piece_values(raw[j], v);
+            piece_values(raw[j], v, E());
 #pragma unroll
             for (int k = 0; k < W; ++k) m = max_or_nan(m, v[k]);
             if (R >= 8) __builtin_amdgcn_sched_barrier(0);   // one piece's values in registers at a time
@@ -260,7 +260,7 @@ struct RowRegs {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             piece_again(raw[j]);
-            piece_values(raw[j], v);
+            piece_values(raw[j], v, E());
 #pragma unroll
             for (int k = 0; k < W; ++k) f(v[k]);
             if (R >= 8) __builtin_amdgcn_sched_barrier(0);
@@ -298,7 +298,7 @@ struct RowRegs {
         for (int j = 0; j < R; ++j) {
             const int i = j * NT + tid;
             piece_again(raw[j]);
-            piece_values(raw[j], v);
+            piece_values(raw[j], v, E());
 #pragma unroll
             for (int k = 0; k < W; ++k) v[k] = f(v[k]);
             if (i < r.nb) row_piece_store<E>(d + r.col(i), whole, v);
@@ -552,16 +552,16 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * NT;
-            if (i >= r.nb) raw[u] = piece_of<E>(-INFINITY);
+            if (i >= r.nb) raw[u] = piece_none<E>();
             else piece_mask(raw[u], bits[i * W / 32] >> (i * W % 32) & ((1u << W) - 1), E());
-            piece_values(raw[u], v);
+            piece_values(raw[u], v, E());
 #pragma unroll
             for (int k = 0; k < W; ++k) n.m = max_or_nan(n.m, v[k]);
         }
         const float ref = n.m > -INFINITY ? n.m : 0.0f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            piece_values(raw[u], v);
+            piece_values(raw[u], v, E());
 #pragma unroll
             for (int k = 0; k < W; ++k) {
                 n.st += __builtin_amdgcn_exp2f((v[k] - ref) * p.ct);
@@ -599,7 +599,7 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * NT;
-            piece_values(raw[u], v);
+            piece_values(raw[u], v, E());
 #pragma unroll
             for (int k = 0; k < W; ++k) v[k] = grad_other<TWO>(c, p.ct, v[k]);
             if (i < r.nb) row_piece_store<E>(dz + r.col(i), whole, v);

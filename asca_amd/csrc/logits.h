@@ -153,11 +153,20 @@ ASCA_DEV T block_sum_t(T x, T* lds) {
 
 // ------------------------------------------------------------ row pieces
 
-// A row's n elements as 16-byte pieces: `head` elements before the first whole piece of the
-// address space, nb pieces of W, fewer than W after them.
-template <typename E>
+// A row's n elements as pieces of B bytes (16 or 8): `head` elements before the first whole
+// piece of the address space, nb pieces of W, fewer than W after them.
+template <int B>
+struct PieceRaw {
+    typedef uint4 type;
+};
+template <>
+struct PieceRaw<8> {
+    typedef uint2 type;
+};
+template <typename E, int B = 16>
 struct Pieces {
-    static constexpr int W = 16 / sizeof(E);
+    static constexpr int W = B / sizeof(E);
+    typedef typename PieceRaw<B>::type Raw;
     const E* p;
     int n, head, nb;
     // (without pieces all of up to 2 W - 1 elements are at the edges)
@@ -166,7 +175,7 @@ struct Pieces {
         head = min(off ? W - off : 0, n);
         nb = pieces ? (n - head) / W : 0;
     }
-    ASCA_DEV uint4 piece(int i) const { return reinterpret_cast<const uint4*>(p + head)[i]; }
+    ASCA_DEV Raw piece(int i) const { return reinterpret_cast<const Raw*>(p + head)[i]; }
     ASCA_DEV int col(int i) const { return head + i * W; }   // the first column of a piece
     // the column outside the pieces that thread t takes, or -1: one of the first 2 W, of the first 32
     // without pieces
@@ -178,17 +187,12 @@ struct Pieces {
     ASCA_DEV int edge_thread(int c) const { return c < head ? c : c - head - nb * W + W; }
 };
 
-template <typename E>
-ASCA_DEV uint4 piece_of(float v);   // all its values
-template <>
-ASCA_DEV uint4 piece_of<float>(float v) {
-    const unsigned u = __float_as_uint(v);
-    return make_uint4(u, u, u, u);
-}
-template <>
-ASCA_DEV uint4 piece_of<bf16_t>(float v) {   // of a value that bf16 holds
-    const unsigned u = __float_as_uint(v), w = u >> 16 | (u & 0xffff0000u);
-    return make_uint4(w, w, w, w);
+// A piece that is nothing but -inf
+template <typename E, int B = 16>
+ASCA_DEV typename PieceRaw<B>::type piece_none() {
+    const unsigned w = sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
+    if constexpr (B == 16) return make_uint4(w, w, w, w);
+    else return make_uint2(w, w);
 }
 // -inf in the places of the bits that are set
 ASCA_DEV void piece_mask(uint4& r, unsigned bits4, float) {
@@ -202,16 +206,19 @@ ASCA_DEV void piece_mask(uint4& r, unsigned bits8, bf16_t) {
     };
     r.x = two(r.x, bits8), r.y = two(r.y, bits8 >> 2), r.z = two(r.z, bits8 >> 4), r.w = two(r.w, bits8 >> 6);
 }
+// The values of a piece
+ASCA_DEV void piece_values(uint4 r, float (&v)[4], float) {
+    v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
+}
+ASCA_DEV void piece_values(uint2 r, float (&v)[2], float) { v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y); }
+ASCA_DEV void piece_values(uint2 r, float (&v)[4], bf16_t) { act_values(r, v); }
+ASCA_DEV void piece_values(uint4 r, float (&v)[8], bf16_t) {
+    act_values(make_uint2(r.x, r.y), v);
+    act_values(make_uint2(r.z, r.w), v + 4);
+}
 // What is made of a piece after this is made anew: the compiler would keep the 32-bit values
 // of an earlier look at it, in twice its registers (bf16).
 ASCA_DEV void piece_again(uint4& r) { asm("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w)); }
-ASCA_DEV void piece_values(uint4 r, float (&v)[4]) {
-    v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
-}
-ASCA_DEV void piece_values(uint4 r, float (&v)[8]) {
-    const unsigned u[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[2 * k] = __uint_as_float(u[k] << 16), v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-}
+ASCA_DEV void piece_again(uint2& r) { asm("" : "+v"(r.x), "+v"(r.y)); }
 
 }  // namespace asca

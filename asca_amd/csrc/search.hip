@@ -196,14 +196,15 @@ ASCA_DEV void top_write(const TopArgs& p, long row, int rank, uint64_t key) {
     p.ids[row * p.K + rank] = key ? (int)key_place(key) : -1;
 }
 
-// A slice of a row in R pieces a thread.  `out` takes (rank, key), `sum` the slice's largest
+// A slice of a row in R pieces of B bytes a thread.  `out` takes (rank, key), `sum` the slice's largest
 // and its sum from one thread.
-template <typename E, int NW, int R, typename Out, typename Sum>
+template <typename E, int NW, int R, int B, typename Out, typename Sum>
 ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW>& l, Out out, Sum sum) {
-    constexpr int NT = 64 * NW, W = Pieces<E>::W, PIECES = TeamLds<NW>::PIECES;
+    constexpr int NT = 64 * NW, W = Pieces<E, B>::W, PIECES = TeamLds<NW>::PIECES;
+    typedef typename Pieces<E, B>::Raw Raw;
     const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x, lane = threadIdx.x & 63, wave = team_wave<NW>();
-    const Pieces<E> r(row + c0, n);
-    uint4 raw[R];
+    const Pieces<E, B> r(row + c0, n);
+    Raw raw[R];
     float cm[R], ma = -INFINITY, mb = -INFINITY, ev = -INFINITY;   // two groups a lane
     const int ec = r.edge(tid);
 #pragma unroll
@@ -215,8 +216,8 @@ ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW
     for (int j = 0; j < R; ++j) {
         cm[j] = -INFINITY;
         if (j * NT >= r.nb) continue;   // the whole team's
-        if (j * NT + tid >= r.nb) raw[j] = piece_of<E>(-INFINITY);
-        piece_values(raw[j], v);
+        if (j * NT + tid >= r.nb) raw[j] = piece_none<E, B>();
+        piece_values(raw[j], v, E());
         float a = v[0], b = v[W / 2];
 #pragma unroll
         for (int k = 1; k < W / 2; ++k) a = max_or_nan(a, v[k]), b = max_or_nan(b, v[k + W / 2]);
@@ -237,7 +238,7 @@ ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW
         for (int j = 0; j < R; ++j) {
             if (j * NT >= r.nb) continue;
             piece_again(raw[j]);
-            piece_values(raw[j], v);
+            piece_values(raw[j], v, E());
 #pragma unroll
             for (int k = 0; k < W; ++k) s += __builtin_amdgcn_exp2f(fmaf(v[k], ct, -rc));
         }
@@ -247,7 +248,7 @@ ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW
         for (int j = 0; j < R; ++j) {
             const int i = j * NT + tid;
             if (i >= r.nb) break;
-            piece_values(r.piece(i), v);
+            piece_values(r.piece(i), v, E());
 #pragma unroll
             for (int k = 0; k < W; ++k) s += __builtin_amdgcn_exp2f((v[k] - ref) * ct);
         }
@@ -262,7 +263,7 @@ ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW
         const bool some = cm[j] >= kth && cm[j] > -INFINITY;
         const uint64_t which = __ballot(some);
         const int at = np + __builtin_amdgcn_mbcnt_hi((unsigned)(which >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)which, 0));
-        if (some && at < PIECES) l.piece[wave][at] = raw[j], l.place[wave][at] = c0 + r.col(j * NT + tid);
+        if (some && at < PIECES) reinterpret_cast<Raw*>(l.piece[wave])[at] = raw[j], l.place[wave][at] = c0 + r.col(j * NT + tid);
         np += __popcll(which);
     }
     wave_push<NW>(ev >= kth ? logit_key(ev, c0 + ec) : 0, nk, l);
@@ -298,7 +299,7 @@ ASCA_DEV void top_slice(const E* row, int c0, int n, int K, float ct, TeamLds<NW
 }
 
 // Teams of NW waves, four waves a block, a slice each
-template <typename E, int NW, int R>
+template <typename E, int NW, int R, int B>
 __global__ __launch_bounds__(256) void top_slice_k(TopArgs p) {
     constexpr int TEAMS = 4 / NW;
     __shared__ TeamLds<NW> lds[TEAMS];
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(256) void top_slice_k(TopArgs p) {
         if (!p.values) p.sums[unit] = make_float2(m, s);
         else if (p.lse) p.lse[row] = (float)((double)m * p.itau + log_d(s));
     };
-    top_slice<E, NW, R>(static_cast<const E*>(p.z) + row * p.ld, c0, n, p.K, p.ct, lds[team], out, sum);
+    top_slice<E, NW, R, B>(static_cast<const E*>(p.z) + row * p.ld, c0, n, p.K, p.ct, lds[team], out, sum);
 }
 
 // log sum exp of a row from its slices, by a wave: in every lane
@@ -538,9 +539,9 @@ __global__ __launch_bounds__(256) void beam_merge_k(BeamArgs p) {
     beam_merge<4>(p, group, l, p.keys + group * p.K * p.S * p.K, p.sums + group * p.K * p.S);
 }
 
-// Rows of R pieces a lane: a block's NW waves select from the group's rows in turn, then it
+// Rows of R pieces of B bytes a lane: a block's NW waves select from the group's rows in turn, then it
 // merges them, in one launch
-template <typename E, int R, int NW>
+template <typename E, int R, int B, int NW>
 __global__ __launch_bounds__(64 * NW) void beam_small_k(BeamArgs p, TopArgs t) {
     __shared__ BeamLds l;
     __shared__ TeamLds<1> team[NW];
@@ -551,7 +552,7 @@ __global__ __launch_bounds__(64 * NW) void beam_small_k(BeamArgs p, TopArgs t) {
     for (int b = w; b < K; b += NW) {
         const long row = group * K + b;
         if (!beam_reads(t, row)) continue;
-        top_slice<E, 1, R>(
+        top_slice<E, 1, R, B>(
             static_cast<const E*>(t.z) + row * t.ld, 0, t.V, K, t.ct, team[w], [&](int rank, uint64_t key) { keys[b * K + rank] = key; },
             [&](float m, float s) { sums[b] = make_float2(m, s); });
     }
@@ -666,17 +667,23 @@ static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const 
     if (rc) return rc;
     const dim3 grid((unsigned)blocks);
     const int per = (a.slice / W + 64 * nw - 1) / (64 * nw);   // pieces a thread
-    auto go = [&](auto n) {
-        constexpr int NW = decltype(n)::value;
-        void (*k)(TopArgs) = per <= 1   ? top_slice_k<E, NW, 1>
-                             : per <= 2 ? top_slice_k<E, NW, 2>
-                             : per <= 4 ? top_slice_k<E, NW, 4>
-                             : per <= 8 ? top_slice_k<E, NW, 8>
-                                        : top_slice_k<E, NW, 16>;
-        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a);
-    };
-    if (nw == 1) go(std::integral_constant<int, 1>());
-    else go(std::integral_constant<int, 4>());
+    void (*k)(TopArgs);
+    if (nw == 1) {
+        // pieces of 8 bytes where 32 lanes hold the row in pieces of 16: 64 of 256 bf16 logits are
+        // ranked from 89 of them then, else from all (16384 rows 63 -> 25 us)
+        k = a.V <= 32 * W ? top_slice_k<E, 1, 1, 8>
+            : per <= 1    ? top_slice_k<E, 1, 1, 16>
+            : per <= 2    ? top_slice_k<E, 1, 2, 16>
+            : per <= 4    ? top_slice_k<E, 1, 4, 16>
+                          : top_slice_k<E, 1, 8, 16>;
+    } else {
+        k = per <= 1   ? top_slice_k<E, 4, 1, 16>
+            : per <= 2 ? top_slice_k<E, 4, 2, 16>
+            : per <= 4 ? top_slice_k<E, 4, 4, 16>
+            : per <= 8 ? top_slice_k<E, 4, 8, 16>
+                       : top_slice_k<E, 4, 16, 16>;
+    }
+    hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a);
     return post_launch("top_slice");
 }
 
@@ -739,9 +746,13 @@ int asca_beam_step(const void* logits, long ld, const float* scores, const int32
             a.S = 1, a.slice = V, a.ct = LOG2E;
             // a wave a beam where the blocks are few
             const int nw = K <= 4 || groups > 2 * cu_count() ? 4 : K <= 8 ? 8 : 16;
-            void (*k)(BeamArgs, TopArgs) = nw == 4   ? pieces <= 64 ? beam_small_k<E, 1, 4> : beam_small_k<E, 2, 4>
-                                           : nw == 8 ? pieces <= 64 ? beam_small_k<E, 1, 8> : beam_small_k<E, 2, 8>
-                                                     : pieces <= 64 ? beam_small_k<E, 1, 16> : beam_small_k<E, 2, 16>;
+            auto of = [&](auto w) {
+                constexpr int NW = decltype(w)::value;
+                return pieces <= 32 ? beam_small_k<E, 1, 8, NW> : pieces <= 64 ? beam_small_k<E, 1, 16, NW> : beam_small_k<E, 2, 16, NW>;
+            };
+            void (*k)(BeamArgs, TopArgs) = nw == 4   ? of(std::integral_constant<int, 4>())
+                                           : nw == 8 ? of(std::integral_constant<int, 8>())
+                                                     : of(std::integral_constant<int, 16>());
             hipLaunchKernelGGL(k, dim3((unsigned)groups), dim3(64 * nw), 0, st, b, a);
             return post_launch("beam_small");
         }
