@@ -70,7 +70,7 @@ ASCA_DEV float recip(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // A row's list, in a wave: id and z are there, tv is the teacher's logit; `twice`: some id may
 // be there more than once.  The first of one id's entries has their sum, the others are none.
-template <bool TWO>
+template <bool TWO, bool EXACT>
 ASCA_DEV List list_of(const DistillArgs& p, long row, float tv, bool twice, Entry& en) {
     const int lane = threadIdx.x & 63;
     bool on = en.id >= 0;
@@ -84,7 +84,7 @@ ASCA_DEV List list_of(const DistillArgs& p, long row, float tv, bool twice, Entr
         lp = ((double)tv - (double)ref) * p.itau;
         const float e = on ? exp_d(lp) : 0.0f, s = wave_sum(e);
         if (m != -INFINITY) en.p = e * recip(s);
-        lp -= log_d(s);
+        lp -= log_of<EXACT>(s);
     }
     if (twice) {
         for (int j = 0; j < p.K; ++j) {
@@ -92,7 +92,7 @@ ASCA_DEV List list_of(const DistillArgs& p, long row, float tv, bool twice, Entr
             const uint64_t same = __ballot(en.id == id);
             if (id < 0 || (same & (same - 1)) == 0) continue;
             const float sum = wave_sum(en.id == id ? en.p : 0.0f);
-            if (lane == j) en.p = sum, lp = log_d(sum);
+            if (lane == j) en.p = sum, lp = log_of<EXACT>(sum);
             else if (en.id == id) en.id = -1, en.p = 0.0f;
         }
         on = en.id >= 0;
@@ -115,38 +115,69 @@ struct Coefs {
     float mr, mx, As, Bt, Qs, Bs, gs, gh;
 };
 
-// From the sums over the others (o) and the list; the loss where it is wanted
+// The whole row's sums from the others' (o) and the list's, measured from mx, and the share of
+// either in them
+struct Whole {
+    float mx, mr, ft, f1, at, a1;   // ft, f1: from mr to mx at both temperatures
+    float qr, gap;                  // q_r, and q_r - p_r
+    bool tail;                      // there is a rest that the student can give
+};
 template <bool TWO>
-ASCA_DEV Coefs distill_coefs(const DistillArgs& p, float w, Expo o, const List& l, bool has_tg, bool want, float& loss) {
-    const Expo all = expo_join<TWO>(o, l.e, p.ct);
+ASCA_DEV Whole whole_of(const DistillArgs& p, Expo o, const List& l) {
+    Whole h;
+    h.mx = fmaxf(o.m, l.e.m);
+    h.mr = o.m > -INFINITY ? o.m : h.mx;
+    auto from = [&](float m, float x) { return m > -INFINITY ? __builtin_amdgcn_exp2f((m - h.mx) * x) : 1.0f; };
+    const float fl = from(l.e.m, p.ct);
+    h.ft = from(h.mr, p.ct);
+    h.a1 = h.at = o.st * h.ft + l.e.st * fl;
+    h.f1 = h.ft;
+    if (TWO) h.f1 = from(h.mr, LOG2E), h.a1 = o.s1 * h.f1 + l.e.s1 * from(l.e.m, LOG2E);
+    h.tail = l.rest > 0.0f && o.st > 0.0f;
+    // q_r - p_r as the lists' difference where they are the smaller part: it cancels where student
+    // and teacher are near
+    h.qr = o.st * h.ft / h.at;
+    h.gap = l.total < 0.5f ? l.total - l.e.st * fl / h.at : h.qr - l.rest;
+    return h;
+}
+template <bool TWO>
+ASCA_DEV Coefs distill_coefs(const DistillArgs& p, float w, Expo o, const List& l, bool has_tg) {
+    const Whole h = whole_of<TWO>(p, o, l);
     Coefs c;
-    c.mx = all.m;
-    c.mr = o.m > -INFINITY ? o.m : c.mx;
-    const float ft = __builtin_amdgcn_exp2f((c.mr - c.mx) * p.ct), f1 = TWO ? __builtin_amdgcn_exp2f((c.mr - c.mx) * LOG2E) : ft;
-    const float a1 = TWO ? all.s1 : all.st;
-    const bool tail = l.rest > 0.0f && o.st > 0.0f;
-    if (want) {
-        const double lt = log_d(all.st), l1 = TWO ? log_d(a1) : lt;
-        double v = 0.0;
-        if (p.alpha > 0.0f) {
-            const float ref = l.e.m > -INFINITY ? l.e.m : 0.0f;
-            if (l.total != 0.0f) v = (double)l.part + (double)l.total * (((double)c.mx - (double)ref) * p.itau + lt);
-            if (tail) v += (double)l.rest * (log_d(l.rest) - log_d(o.st) + ((double)c.mx - (double)c.mr) * p.itau + lt);
-            v *= (double)p.alpha * p.tau * p.tau;
-        }
-        if (has_tg) v += (1.0 - (double)p.alpha) * ((double)c.mx + l1 - (double)l.zt);
-        loss = (float)(v * (double)w);
-    }
+    c.mx = h.mx, c.mr = h.mr;
     c.gs = p.scale * w * p.alpha * p.tau;
     c.gh = has_tg ? p.scale * w * (1.0f - p.alpha) : 0.0f;
     // the sum of p that the gradient meets: a rest that the student cannot give is left out
-    const float mass = tail ? 1.0f : l.total, qt = mass * recip(all.st), q1 = c.gh * recip(a1);
+    const float qt = (h.tail ? 1.0f : l.total) * recip(h.at), q1 = c.gh * recip(h.a1);
     c.Qs = c.gs * qt;
-    c.As = c.gs * (qt * ft - (tail ? l.rest * recip(o.st) : 0.0f));
+    c.As = c.gs * (h.tail ? h.gap * recip(o.st) : qt * h.ft);
     c.Bs = q1;
-    c.Bt = q1 * f1;
+    c.Bt = q1 * h.f1;
     if (!TWO) c.As += c.Bt, c.Qs += c.Bs;
     return c;
+}
+// The loss, after the gradient: its doubles would stand beside the row's registers (4096 x 50000
+// bf16 204 -> 288 us).  EXACT takes the logarithms to 1e-10: tau^2 times the roundings of log_d are
+// as much as the loss's own where student and teacher are near; it costs rows of a wave each a
+// tenth of their time.
+template <bool TWO, bool EXACT>
+ASCA_DEV float distill_loss(const DistillArgs& p, float w, Expo o, const List& l, bool has_tg) {
+    const Whole h = whole_of<TWO>(p, o, l);
+    const double lt = log_of<EXACT>(h.at), l1 = TWO ? log_of<EXACT>(h.a1) : lt;
+    double v = 0.0;
+    if (p.alpha > 0.0f) {
+        const float ref = l.e.m > -INFINITY ? l.e.m : 0.0f;
+        if (l.total != 0.0f) v = (double)l.part + (double)l.total * (((double)h.mx - (double)ref) * p.itau + lt);
+        if (h.tail) {   // + p_r log(p_r / q_r)
+            double r;
+            if (EXACT && fabsf(h.gap) < 0.3f * h.qr) r = artanh2(-(double)h.gap, 2.0 * (double)h.qr - (double)h.gap);
+            else r = log_of<EXACT>(l.rest) - log_of<EXACT>(o.st) + ((double)h.mx - (double)h.mr) * p.itau + lt;
+            v += (double)l.rest * r;
+        }
+        v *= (double)p.alpha * p.tau * p.tau;
+    }
+    if (has_tg) v += (1.0 - (double)p.alpha) * ((double)h.mx + l1 - (double)l.zt);
+    return (float)(v * (double)w);
 }
 
 template <bool TWO>
@@ -387,7 +418,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void distill_rows_k(Distil
             en.z = act_load(z + en.id);
             twice = mark<E>(r, en.id, l.bits, &l.edge);
         }
-        li = list_of<TWO>(p, row, tv, __ballot(twice) != 0, en);
+        li = list_of<TWO, (NW > 1)>(p, row, tv, __ballot(twice) != 0, en);
         li.zt = zt;
         if constexpr (NW > 1) {
             l.en[lane] = en;
@@ -404,13 +435,15 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void distill_rows_k(Distil
         for (int k = 1; k < NW; ++k) o = expo_join<TWO>(o, l.part[k], p.ct);
         en = l.en[lane], li = l.list;
     }
-    float loss = 0.0f;
-    const Coefs c = distill_coefs<TWO>(p, w, o, li, has_tg, wave == 0, loss);
+    if (p.dz) {
+        const Coefs c = distill_coefs<TWO>(p, w, o, li, has_tg);
+        E* dz = static_cast<E*>(p.dz) + row * p.lddz;
+        x.template store<TWO>(r, tid, dz, c, p.ct);
+        store_listed<E, NW, TWO>(p, r, 0, wave, dz, c, en, tg, has_tg, li.zt);
+    }
+    if (wave != 0) return;
+    const float loss = distill_loss<TWO, (NW > 1)>(p, w, o, li, has_tg);
     if (tid == 0) p.losses[row] = loss;
-    if (!p.dz) return;
-    E* dz = static_cast<E*>(p.dz) + row * p.lddz;
-    x.template store<TWO>(r, tid, dz, c, p.ct);
-    store_listed<E, NW, TWO>(p, r, 0, wave, dz, c, en, tg, has_tg, li.zt);
 }
 
 // A few long rows: S slices each, a block's of 4 waves.  The first launch leaves the slices'
@@ -450,7 +483,7 @@ __global__ __launch_bounds__(256) void distill_part_k(DistillArgs p) {
             if (en.id >= 0) en.z = act_load(z + en.id);
             bool twice = false;   // (the bitmap is of this slice alone)
             for (int j = 0; j < p.K; ++j) twice |= j < lane && en.id >= 0 && __builtin_amdgcn_readlane(en.id, j) == en.id;
-            List li = list_of<TWO>(p, row, tv, __ballot(twice) != 0, en);
+            List li = list_of<TWO, true>(p, row, tv, __ballot(twice) != 0, en);
             li.zt = zt;
             p.split[row].en[lane] = en;
             if (lane == 0) p.split[row].list = li;
@@ -489,13 +522,15 @@ __global__ __launch_bounds__(256) void distill_finish_k(DistillArgs p) {
     float u = 0.0f, v = 0.0f;
     wave_sum4(o.st, o.s1, u, v);
     o.m = m;
-    float loss = 0.0f;
-    const Coefs c = distill_coefs<TWO>(p, w, o, li, has_tg, slice == 0 && wave == 0, loss);
-    if (tid == 0 && slice == 0) p.losses[row] = loss;
-    if (!p.dz) return;
-    E* dz = static_cast<E*>(p.dz) + row * p.lddz + c0;
-    x.template store<TWO>(r, tid, dz, c, p.ct);
-    store_listed<E, 4, TWO>(p, r, c0, wave, dz, c, en, tg, has_tg, li.zt);
+    if (p.dz) {
+        const Coefs c = distill_coefs<TWO>(p, w, o, li, has_tg);
+        E* dz = static_cast<E*>(p.dz) + row * p.lddz + c0;
+        x.template store<TWO>(r, tid, dz, c, p.ct);
+        store_listed<E, 4, TWO>(p, r, c0, wave, dz, c, en, tg, has_tg, li.zt);
+    }
+    if (wave != 0 || slice != 0) return;
+    const float loss = distill_loss<TWO, true>(p, w, o, li, has_tg);
+    if (tid == 0) p.losses[row] = loss;
 }
 
 // Rows that no team's registers hold: read twice, by 1024 threads, the second time mostly from
@@ -534,7 +569,7 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
             en.z = act_load(z + en.id);
             twice = mark<E>(r, en.id, bits, &l.edge);
         }
-        List li = list_of<TWO>(p, row, tv, __ballot(twice) != 0, en);
+        List li = list_of<TWO, true>(p, row, tv, __ballot(twice) != 0, en);
         li.zt = zt;
         l.en[lane] = en;
         if (lane == 0) l.list = li;
@@ -583,10 +618,12 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
     for (int k = 1; k < NW; ++k) o = expo_join<TWO>(o, l.part[k], p.ct);
     en = l.en[lane];
     const List li = l.list;
-    float loss = 0.0f;
-    const Coefs c = distill_coefs<TWO>(p, w, o, li, has_tg, wave == 0, loss);
-    if (tid == 0) p.losses[row] = loss;
+    if (wave == 0) {
+        const float loss = distill_loss<TWO, true>(p, w, o, li, has_tg);
+        if (tid == 0) p.losses[row] = loss;
+    }
     if (!p.dz) return;
+    const Coefs c = distill_coefs<TWO>(p, w, o, li, has_tg);
     E* dz = static_cast<E*>(p.dz) + row * p.lddz;
     const bool whole = (reinterpret_cast<uintptr_t>(dz) - reinterpret_cast<uintptr_t>(z)) % 16 == 0;
     // (dz may be z: a thread writes the pieces that it reads, and all have read the entries)

@@ -27,12 +27,35 @@ ASCA_DEV float exp_d(double x) {
     const float h = (float)y;
     return h > -INFINITY ? __builtin_amdgcn_exp2f(h) * (1.0f + (float)(y - h) * 0.693147181f) : h == -INFINITY ? 0.0f : h;
 }
-// log(x) to 2^-24 (not relative to a large result): that of the exponent in 64 bits
+// log(x): to 2^-24 (not relative to a large result), or to 1e-10, where small differences of
+// logarithms or scores next to each other count
 ASCA_DEV double log_d(float x) {
     float m = __builtin_amdgcn_frexp_mantf(x);   // 0.5 to 1
     int e = __builtin_amdgcn_frexp_expf(x);
     if (m < 0.70710678f) m *= 2.0f, --e;
     return ((double)e + (double)__builtin_amdgcn_logf(m)) * LN2;
+}
+// 2 artanh(a / b), |a / b| < 0.172: its odd powers up to the 11th
+ASCA_DEV double artanh2(double a, double b) {
+    double r = __builtin_amdgcn_rcp(b);
+    r = fma(fma(-b, r, 1.0), r, r);
+    const double t = a * r, q = t * t;
+    double v = 2.0 / 11;
+    v = fma(v, q, 2.0 / 9), v = fma(v, q, 2.0 / 7), v = fma(v, q, 2.0 / 5), v = fma(v, q, 2.0 / 3), v = fma(v, q, 2.0);
+    return v * t;
+}
+ASCA_DEV double log_exact(float x) {
+    float m = __builtin_amdgcn_frexp_mantf(x);
+    int e = __builtin_amdgcn_frexp_expf(x);
+    if (m < 0.70710678f) m *= 2.0f, --e;
+    const double l = artanh2((double)m - 1.0, (double)m + 1.0);   // log m
+    return x > 0.0f && x < INFINITY ? fma((double)e, LN2, l) : (double)__builtin_amdgcn_logf(x);
+}
+// log of one or the other kind
+template <bool EXACT>
+ASCA_DEV double log_of(float x) {
+    if constexpr (EXACT) return log_exact(x);
+    return log_d(x);
 }
 
 // ------------------------------------------------------ lanes of a wave

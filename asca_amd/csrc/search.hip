@@ -460,7 +460,7 @@ ASCA_DEV void beam_merge(const BeamArgs& p, long group, BeamLds& l, Keys keys, S
             t += v.x > -INFINITY ? v.y * exp_d((double)v.x - (double)m) : v.y;
         }
         for (int x = width / 2; x >= 1; x /= 2) t += __shfl_xor(t, x, 64);
-        const double x = read ? s - ((double)m + log_d(t)) : s;
+        const double x = read ? s - ((double)m + log_exact(t)) : s;
         if (on && tid % width == 0) l.base[b] = fin && fabs(x) < INFINITY ? x : (double)-INFINITY, l.ended[b] = end;
     }
     if (tid < K) l.picks[tid] = BeamPick{-INFINITY, -1, 0};
