@@ -647,8 +647,9 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
 }
 
 template <typename E, bool TWO>
-static int distill_launch(DistillArgs a, hipStream_t st) {
+static int distill_launch(DistillArgs a, hipStream_t st, const char* fn) {
     constexpr int W = 16 / sizeof(E);
+    if (!grid_fits(a.T, 1024)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows (%ld)", fn, a.T);
     const long pieces = (a.V + W - 1) / W, cus = std::max(cu_count(), 1);
     int r;
     // Rows that are fewer than the CUs and long: slices of 256 x 4 pieces at the most, of about
@@ -761,7 +762,7 @@ int asca_distill(const void* logits, long ld, const float* tval, const int32_t* 
                             alpha > 0.0f ? temperature : 1.0f, ct, alpha, scale, alpha > 0.0f ? 1.0 / (double)temperature : 1.0, 1, V,
                             nullptr, nullptr};
         const hipStream_t st = as_stream(stream);
-        return two ? distill_launch<E, true>(a, st) : distill_launch<E, false>(a, st);
+        return two ? distill_launch<E, true>(a, st, fn) : distill_launch<E, false>(a, st, fn);
     });
 }
 

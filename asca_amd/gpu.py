@@ -262,6 +262,12 @@ def from_bf16(x: np.ndarray) -> np.ndarray:
     return (np.ascontiguousarray(x, dtype=np.uint16).astype(np.uint32) << 16).view(_f32)
 
 
+def _entry_ids(ids) -> np.ndarray:
+    """Ids of a teacher's entries as int32; what no id can be is no entry."""
+    a = np.asarray(ids)
+    return np.where((a < 0) | (a > 0x7fffffff), -1, a).astype(np.int32)
+
+
 F32, BF16 = 0, 1   # ASCA_F32, ASCA_BF16: element types of activation rows
 
 
@@ -386,7 +392,7 @@ class Teacher:
         if values.ndim != 2 or ids.shape != values.shape or (lse is not None and np.shape(lse) != values.shape[:1]):
             raise ValueError(f"values {values.shape}, ids {ids.shape}, lse {np.shape(lse)}")
         rows, k = values.shape
-        return cls(DevBuf.from_host(values), DevBuf.from_array(ids.astype(np.int32)),
+        return cls(DevBuf.from_host(values), DevBuf.from_array(_entry_ids(ids)),
                    None if lse is None else DevBuf.from_host(np.asarray(lse, _f32)), rows, k, temperature)
 
     def to_host(self):
@@ -1066,7 +1072,7 @@ class Gpu:
             bl = b.up(logits)
             dl, ls = b.new(logits.nbytes) if grad else None, b.new(T * 4)
             _lib.call("asca_distill", _vp(bl), V, _vp(b.up(tval, "tval", (T, K))),
-                      _vp(None if tids is None else b.up(np.asarray(tids, np.int32))), _vp(b.up(tlse, "tlse", (T,))), K,
+                      _vp(None if tids is None else b.up(_entry_ids(tids))), _vp(b.up(tlse, "tlse", (T,))), K,
                       _vp(None if targets is None else b.up(np.asarray(targets, np.uint32))), _vp(b.up(weights, "weights", (T,))),
                       temperature, alpha, scale, _vp(ls), _vp(dl), V, T, V, ty, None)
             _lib.call("asca_sync")

@@ -131,6 +131,39 @@ def test_top_of_strided_rows(g, rows, V, K, pad, off, bf16):
     m.get()
 
 
+# as many rows as fill the device: a wave's rows of each number of pieces, whole rows and slices of a block
+MANY = [(1100, 100, 64), (1030, 256, 31), (1030, 300, 16), (1100, 700, 64), (1030, 1900, 20), (1025, 3900, 33), (1040, 9000, 64),
+        (1050, 20011, 5), (1030, 33001, 17)]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,V,K", MANY)
+def test_top_of_many_rows(g, rows, V, K, bf16):
+    from asca_amd import _lib, gpu
+
+    print(f"[top] rows={rows} V={V} K={K} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(rows + V)
+    z, val = to_dev(rng.standard_normal((rows, V)), bf16)
+    m = Strided(z, 1, 1)
+    v, i, s = gpu.DevBuf(rows * K * 4), gpu.DevBuf(rows * K * 4), gpu.DevBuf(rows * 4)
+    _lib.call("asca_top_logits", m.ptr, m.ld, rows, V, K, 0.7, _p(v), _p(i), _p(s), int(bf16), None)
+    _lib.call("asca_sync")
+    check_top((v.to_host((rows, K)), i.to_host((rows, K), np.int32), s.to_host((rows,))), val, K, 0.7)
+
+
+@pytest.mark.parametrize("V", [90, 1000, 30000])
+def test_top_of_large_logits(g, V):
+    """Logits whose scaled size is past what one step of the exponent's argument keeps."""
+    rng = np.random.default_rng(V)
+    z = (rng.standard_normal((4, V)) + np.array([[1e5], [-1e5], [3e6], [-1e30]])).astype(np.float32)
+    for tau in (1.0, 0.01):
+        v, i, s = g.top_logits(z, 7, tau)
+        rv, ri, rs = lo.top(z, 7, tau)
+        np.testing.assert_array_equal(i, ri)
+        np.testing.assert_array_equal(v, rv)
+        assert (np.abs(s - rs) <= U * np.abs(rs) + delta(z[:1], tau)).all()
+
+
 def orders(V):
     """Rows in which the largest lie where a selection by parts goes wrong."""
     up_ = np.arange(V) / 64.0
@@ -238,6 +271,53 @@ def test_distill_of_strided_rows(g, T, V, K, pad, off, gpad, goff, inplace, bf16
     check_distill((ls.to_host((T,)), out.get()), val, tv, ids, bf16, tlse=tl, targets=tg, temperature=2.0, alpha=0.5)
     if not inplace:
         np.testing.assert_array_equal(m.get(), z)
+
+
+# rows that are not few for their length, in each number of waves and pieces
+ROWS = [(1030, 5, 3), (1030, 130, 9), (1030, 300, 16), (1030, 700, 33), (1030, 1500, 5), (1030, 3500, 64), (40, 1003, 20), (40, 3001, 7),
+        (40, 5003, 64), (40, 9001, 11), (40, 17001, 30), (36, 30001, 64), (130, 40001, 5), (130, 70003, 64), (129, 140001, 3)]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("T,V,K", ROWS)
+def test_distill_of_many_rows(g, T, V, K, inplace, bf16):
+    from asca_amd import _lib, gpu
+
+    print(f"[distill] T={T} V={V} K={K} bf16={bf16} inplace={inplace}", flush=True)
+    rng = np.random.default_rng(T + V)
+    z, val = to_dev(rng.standard_normal((T, V)) * 2, bf16)
+    ids = rng.integers(-1, V, (T, K)).astype(np.int32)   # some twice
+    tv = (rng.standard_normal((T, K)) + 3).astype(np.float32)
+    tl = np.array([lo.lse(r.astype(np.float64) / 2) for r in tv], np.float32) + 0.3
+    tg, w = rng.integers(0, V + 2, T), np.where(np.arange(T) % 5 == 2, 0, rng.uniform(0.5, 2, T)).astype(np.float32)
+    m = Strided(z, 1, 1)
+    out = m if inplace else Strided(z, 1, 1, fill=0)
+    ls, bt, bi, bl, btg, bw = gpu.DevBuf(T * 4), up(tv), up(ids), up(tl), up(tg, np.uint32), up(w)
+    rest = not inplace
+    _lib.call("asca_distill", m.ptr, m.ld, _p(bt), _p(bi), _p(bl if rest else None), K, _p(btg), _p(bw), 2.0, 0.5, 1.0, _p(ls), out.ptr,
+              out.ld, T, V, int(bf16), None)
+    _lib.call("asca_sync")
+    check_distill((ls.to_host((T,)), out.get()), val, tv, ids, bf16, tlse=tl if rest else None, targets=tg, weights=w, temperature=2.0,
+                  alpha=0.5)
+
+
+@pytest.mark.parametrize("T,V", [(3, 60), (3, 900), (40, 9001), (2, 40000), (130, 70003)])
+def test_distill_of_large_logits(g, T, V):
+    """Logits whose scaled size is past what one step of the exponent's argument keeps: the same
+    losses and gradients as without what all of a row have in common."""
+    rng = np.random.default_rng(V)
+    z = np.round(rng.standard_normal((T, V)) * 64) / 64
+    ids = np.stack([rng.permutation(V)[:6] for _ in range(T)]).astype(np.int32)
+    tv = rng.standard_normal((T, 6)).astype(np.float32)
+    tl = np.array([lo.lse(r.astype(np.float64) / 2) for r in tv], np.float32) + 0.2
+    kw = dict(tlse=tl, targets=ids[:, 1], temperature=2.0, alpha=0.5)
+    for add in (0.0, 1e5, -1e5, 2.0 ** 17):   # exact sums in f32
+        x = (z + add).astype(np.float32)
+        got = g.distill(x, tv, ids, **kw)
+        L, dz, (tl_, tg_) = lo.distill(z, tv, ids, **kw)
+        d = delta(z)
+        assert (np.abs(got[0] - L) <= U * np.abs(L) + d * tl_).all() and (np.abs(got[1] - dz) <= U * np.abs(dz) + d * tg_ + 1e-37).all()
 
 
 @pytest.mark.parametrize("V", [50, 700, 9000, 40000, 140000])
@@ -407,6 +487,25 @@ def test_beam_first_step(g, stay):
     z, val = logits(rng, 12, 500, False)
     sc = np.where(np.arange(12) % 6 == 0, 0.0, -np.inf).astype(np.float32)
     check_step(g.beam_step(z, sc, k=6, stay=stay), val, sc, 6, stay=stay)
+
+
+@pytest.mark.parametrize("V", [30000, 70000])
+def test_beam_first_step_of_many_beams(g, V):
+    """A single beam of 32 counts, whose slices' first keys are fewer than the beams."""
+    rng = np.random.default_rng(V)
+    z, val = to_dev(rng.standard_normal((64, V)), False)
+    sc = np.where(np.arange(64) % 32 == 5, -1.0, -np.inf).astype(np.float32)
+    for stay in (False, True):
+        check_step(g.beam_step(z, sc, k=32, stay=stay), val, sc, 32, stay=stay)
+
+
+@pytest.mark.parametrize("G,K,V", [(600, 9, 256), (300, 4, 2100), (300, 16, 700), (260, 4, 9001)])
+def test_beam_step_of_many_groups(g, G, K, V):
+    rng = np.random.default_rng(G)
+    z, val = to_dev(rng.standard_normal((G * K, V)) * 2, True)
+    sc = (-5 - 3 * rng.random(G * K)).astype(np.float32)
+    end = (rng.random(G * K) < 0.2).astype(np.int32)
+    check_step(g.beam_step(z, sc, k=K, ended=end, eos=3, stay=True), val, sc, K, end, 3, True)
 
 
 @pytest.mark.parametrize("V", [3, 50, 3000, 70000])
@@ -604,6 +703,41 @@ def test_on_two_streams_at_once(g):
             np.testing.assert_array_equal(a, w[k], err_msg=k)
     for s in sts:
         _lib.call("asca_stream_destroy", s)
+
+
+def test_from_several_host_threads(g):
+    import threading
+
+    from asca_amd import _lib
+
+    sets = [_decode_calls(g, np.random.default_rng(50 + s), G=2 + s, V=3001 + 9000 * s) for s in range(4)]
+    want = []
+    for run, get, *_ in sets:
+        run(None)
+        _lib.call("asca_sync")
+        want.append(get())
+    errs = []
+
+    def work(i):
+        try:
+            s = C.c_void_p()
+            _lib.call("asca_stream_create", C.byref(s))
+            for _ in range(30):
+                sets[i][0](s)
+            _lib.call("asca_stream_sync", s)
+            _lib.call("asca_stream_destroy", s)
+        except BaseException as e:  # noqa: BLE001 (reported below)
+            errs.append(repr(e))
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join(60)
+    assert not errs and not any(t.is_alive() for t in ts)
+    for (run, get, *_), w in zip(sets, want):
+        for k, a in get().items():
+            np.testing.assert_array_equal(a, w[k], err_msg=k)
 
 
 def test_captured_calls_replay_the_eager_results(g):

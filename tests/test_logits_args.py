@@ -83,6 +83,25 @@ def test_beam_states(bad, want):
     assert states(**bad) == want and _lib.load().asca_last_error()
 
 
+def test_more_blocks_than_a_launch_takes():
+    """Rows that memory could hold, in blocks of more threads than 256."""
+    assert distill(T=9 << 20, V=8200, ld=8200, lddl=8200, ty=1) == UNSUPPORTED
+    assert top(rows=9 << 20, V=40000, ld=40000) == UNSUPPORTED
+
+
+def test_right_calls_get_as_far_as_the_device():
+    lib = _lib.load()
+    n = C.c_int(0)
+    if lib.asca_device_count(C.byref(n)) == 0 and n.value > 0:
+        pytest.skip("a GPU is present; this checks the no-device path")
+    assert top() == top(V=70000, ld=70000) == distill() == distill(V=70000, ld=70000, lddl=70000) == 4
+    assert step() == step(V=70000, ld=70000) == states() == states(dst=0x9000000, ks=1) == 4
+
+
+def test_ids_that_are_none():
+    np.testing.assert_array_equal(gpu._entry_ids([[3, -1, 1 << 31, (1 << 32) + 2, 0x7fffffff]]), [[3, -1, -1, -1, 0x7fffffff]])
+
+
 def test_pointers_may_be_null_where_nothing_is_there():
     lib = _lib.load()
     assert lib.asca_beam_states(None, None, None, None, 0, None, 3, 1, 4, None) == 0
