@@ -571,11 +571,14 @@ struct StatesArgs {
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-// Words a thread moves for each of up to KM slots: 64 registers of 16-byte words (128 with KM = 32).
-// Two for KM = 4 were as fast where states move and twice as slow where none does (19 us of empty
-// blocks for 128 x 4 x 1 MB); a loop over several runs a block cost 7% where they do.
-template <int KM>
-constexpr int st_u() { return KM <= 4 ? 4 : KM <= 8 ? 2 : 1; }
+// Words a thread moves for each of up to KM slots: 64 registers (128 with KM = 32 and 16 bytes a
+// word).  Half of them for KM = 4 were as fast where states move and twice as slow where none does
+// (19 us of empty blocks for 128 x 4 x 1 MB); a loop over several runs a block cost 7% where they do.
+template <typename W, int KM>
+constexpr int st_u() {
+    constexpr int u = 64 * 4 / (KM * (sizeof(W) < 4 ? 4 : (int)sizeof(W)));
+    return u < 1 ? 1 : u > 8 ? 8 : u;
+}
 
 // A block takes 256 U words of the states of one group in one outer row.  A thread reads its
 // words of the slots that change before it writes any, so that a buffer may be its own
@@ -583,7 +586,7 @@ constexpr int st_u() { return KM <= 4 ? 4 : KM <= 8 ? 2 : 1; }
 // from memory once, then from a cache.
 template <typename W, int KM>
 __global__ __launch_bounds__(256) void beam_states_k(StatesArgs p) {
-    constexpr int U = st_u<KM>();
+    constexpr int U = st_u<W, KM>();
     int i = 0;
     while (i + 1 < p.count && blockIdx.x >= p.first[i + 1]) ++i;
     const unsigned b = blockIdx.x - p.first[i], unit = b / p.chunks[i], group = unit % p.groups;
@@ -741,14 +744,21 @@ int asca_beam_step(const void* logits, long ld, const float* scores, const int32
         BeamArgs b{scores, ended, new_scores, new_ended, tokens, parents, K, V, 1, eos < 0 ? -1 : eos, stay, nullptr, nullptr};
         int r;
         const int pieces = (V + 16 / (int)sizeof(E) - 1) / (16 / (int)sizeof(E));
-        if (pieces <= 128) {   // both halves in one launch
+        // Both halves in one launch where a lane holds a few pieces of a row (1 x 4 x 256: 7 us against 8.2,
+        // 1000 x 16 x 256 19.5 against 22), or some where its block has a wave for every beam (2 x 4 x 2000
+        // f32 8.5 against 9.7, 512 x 4 x 2000 9.7 against 11.9, but 300 x 16 x 2000 29 against 20).
+        if (pieces <= 128 || (pieces <= 512 && (K <= 4 || groups <= cu_count()))) {
             if ((r = pre_launch("beam_small"))) return r;
             a.S = 1, a.slice = V, a.ct = LOG2E;
             // a wave a beam where the blocks are few
             const int nw = K <= 4 || groups > 2 * cu_count() ? 4 : K <= 8 ? 8 : 16;
             auto of = [&](auto w) {
                 constexpr int NW = decltype(w)::value;
-                return pieces <= 32 ? beam_small_k<E, 1, 8, NW> : pieces <= 64 ? beam_small_k<E, 1, 16, NW> : beam_small_k<E, 2, 16, NW>;
+                return pieces <= 32    ? beam_small_k<E, 1, 8, NW>
+                       : pieces <= 64  ? beam_small_k<E, 1, 16, NW>
+                       : pieces <= 128 ? beam_small_k<E, 2, 16, NW>
+                       : pieces <= 256 ? beam_small_k<E, 4, 16, NW>
+                                       : beam_small_k<E, 8, 16, NW>;
             };
             void (*k)(BeamArgs, TopArgs) = nw == 4   ? of(std::integral_constant<int, 4>())
                                            : nw == 8 ? of(std::integral_constant<int, 8>())
@@ -803,7 +813,11 @@ int asca_beam_states(void** src, void** dst, const uint64_t* outer, const uint64
         rows[n] = outer[i];
     }
     if (a.count == 0) return ASCA_OK;
-    const uint64_t step = 256ull * word * (k_dst <= 4 ? st_u<4>() : k_dst <= 8 ? st_u<8>() : st_u<32>());
+    auto steps = [&](auto w) {
+        using W = decltype(w);
+        return k_dst <= 4 ? st_u<W, 4>() : k_dst <= 8 ? st_u<W, 8>() : k_dst <= 16 ? st_u<W, 16>() : st_u<W, 32>();
+    };
+    const uint64_t step = 256ull * word * (word == 16 ? steps(u32x4()) : word == 4 ? steps(uint32_t()) : steps(uint8_t()));
     uint64_t blocks = 0;
     for (int i = 0; i < a.count; ++i) {
         const uint64_t chunks = (a.bytes[i] + step - 1) / step;
