@@ -143,14 +143,7 @@ ASCA_DEV T wave_max_t(T x) {
     }
     return x;
 }
-template <typename T>
-ASCA_DEV T wave_sum_t(T x) {
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) x += __shfl_xor(x, s, 64);
-    return x;
-}
-
-// The largest (the sum) over a block of 64 NW threads, in every thread; `lds` holds NW values.
+// The largest over a block of 64 NW threads, in every thread; `lds` holds NW values.
 template <int NW, typename T>
 ASCA_DEV T block_max_t(T x, T* lds) {
     x = wave_max_t(x);
@@ -160,17 +153,6 @@ ASCA_DEV T block_max_t(T x, T* lds) {
     x = lds[0];
 #pragma unroll
     for (int w = 1; w < NW; ++w) x = lds[w] > x ? lds[w] : x;
-    return x;
-}
-template <int NW, typename T>
-ASCA_DEV T block_sum_t(T x, T* lds) {
-    x = wave_sum_t(x);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = lds[0];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) x += lds[w];
     return x;
 }
 

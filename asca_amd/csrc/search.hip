@@ -329,8 +329,9 @@ ASCA_DEV double slices_lse(const float2* sums, int S, double itau) {
     return (double)m * itau + log_d(wave_sum(s));
 }
 
-// The K largest of a row's S K keys, a team of NW waves a row
-template <int NW>
+// The K largest of a row's S K keys by a team of NW waves, with R keys a thread in registers (R = 0:
+// read twice)
+template <int NW, int R>
 __global__ __launch_bounds__(256) void top_merge_k(TopArgs p) {
     constexpr int TEAMS = 4 / NW, NT = 64 * NW;
     __shared__ TeamLds<NW> lds[TEAMS];
@@ -340,27 +341,36 @@ __global__ __launch_bounds__(256) void top_merge_k(TopArgs p) {
     if (row >= p.rows) return;
     const uint64_t* keys = p.keys + row * p.S * p.K;
     const int n = p.S * p.K;
-    auto at = [&](unsigned i) { return keys[i % p.S * p.K + i / (unsigned)p.S]; };   // the slices' largest first, over all lanes
+    const float is = 1.0f / (float)p.S;
+    auto at = [&](int i) -> uint64_t {   // the slices' largest first, over all lanes
+        if (i >= n) return 0;
+        const int rank = R ? (int)(((float)i + 0.5f) * is) : (int)((unsigned)i / (unsigned)p.S);   // (exact for few)
+        return keys[(i - rank * p.S) * p.K + rank];
+    };
+    uint64_t mine[R ? R : 1];
+#pragma unroll
+    for (int j = 0; j < R; ++j) mine[j] = at(tid + j * NT);
+    auto each = [&](auto f) {   // every key of the team's, and for all of its threads together
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) f(mine[j], j);
+        } else {
+            for (int i = tid, j = 0; i - tid < n; i += NT, ++j) f(at(i), j);
+        }
+    };
     float ma = -INFINITY, mb = -INFINITY;
-    for (int i = tid, j = 0; i < n; i += NT, ++j) {
-        const uint64_t key = at(i);
+    each([&](uint64_t key, int j) {
         const float v = key ? key_value(key) : -INFINITY;
         if (j & 1) mb = fmaxf(mb, v);
         else ma = fmaxf(ma, v);
-    }
+    });
     const float kth = team_kth<NW>(ma, mb, p.K, l);
     int nk = 0;
-    for (int i = tid; i - tid < n; i += NT) {
-        const uint64_t key = i < n ? at(i) : 0;
-        wave_push<NW>(key && key_value(key) >= kth ? key : 0, nk, l);
-    }
+    each([&](uint64_t key, int) { wave_push<NW>(key && key_value(key) >= kth ? key : 0, nk, l); });
     wave_end<NW>(nk, l);
     team_sync<NW>();
     team_rank<NW>(
-        p.K, l,
-        [&](auto f) {
-            for (int i = tid; i < n; i += NT) f(keys[i]);
-        },
+        p.K, l, [&](auto f) { each([&](uint64_t key, int) { f(key); }); },
         [&](int rank, uint64_t key) { top_write(p, row, rank, key); });
     if (p.lse && tid < 64) {
         const double s = slices_lse(p.sums + row * p.S, p.S, p.itau);
@@ -715,8 +725,12 @@ int asca_top_logits(const void* logits, long ld, long rows, int V, int K, float 
         a.values = values;
         if ((r = pre_launch("top_merge"))) return r;
         // a wave a row where it holds few keys
-        if (a.S * K <= 256) hipLaunchKernelGGL(top_merge_k<1>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(top_merge_k<4>, dim3((unsigned)rows), dim3(256), 0, st, a);
+        const int n = a.S * K;
+        if (n <= 256) {
+            hipLaunchKernelGGL((n <= 128 ? top_merge_k<1, 2> : top_merge_k<1, 4>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+        } else {
+            hipLaunchKernelGGL((n <= 1024 ? top_merge_k<4, 4> : top_merge_k<4, 0>), dim3((unsigned)rows), dim3(256), 0, st, a);
+        }
         return post_launch("top_merge");
     });
 }
