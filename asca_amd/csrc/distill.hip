@@ -726,7 +726,7 @@ int asca::distill_check(const char* fn, const DistillTeacher& t, const uint32_t*
     if (T < 0 || V <= 0) return fail(ASCA_ERR_INVALID, "%s: bad shape %ld x %d", fn, T, V);
     if (V > DISTILL_MAX_V) return fail(ASCA_ERR_UNSUPPORTED, "%s: V=%d (up to %d)", fn, V, DISTILL_MAX_V);
     if (!(t.alpha >= 0.0f && t.alpha <= 1.0f)) return fail(ASCA_ERR_INVALID, "%s: alpha=%g (0 to 1)", fn, (double)t.alpha);
-    if (!(t.temperature > 0.0f) || !(t.temperature < INFINITY))
+    if (!logits_temperature(t.temperature))
         return fail(ASCA_ERR_INVALID, "%s: temperature %g", fn, (double)t.temperature);
     if (t.alpha > 0.0f && (t.K < 1 || t.K > DISTILL_MAX_K))
         return fail(ASCA_ERR_UNSUPPORTED, "%s: K=%d (1 to %d)", fn, t.K, DISTILL_MAX_K);

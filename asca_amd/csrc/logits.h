@@ -7,6 +7,9 @@ namespace asca {
 constexpr float LOG2E = 1.44269504f;
 constexpr double LN2 = 0.693147180559945309;
 
+// Temperatures that entry points take: log2(e) / tau, and logits times it, are finite
+inline bool logits_temperature(float tau) { return tau >= 1e-30f && tau < INFINITY; }
+
 // A key that orders values descending by value, then ascending by place: the larger of two
 // keys is the larger value, or the lower place of equal ones (0 and -0 are equal).  Values
 // that are never listed (NaN, -inf) have the key 0.

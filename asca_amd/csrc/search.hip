@@ -708,7 +708,7 @@ int asca_top_logits(const void* logits, long ld, long rows, int V, int K, float 
     int rc = rows_check(fn, rows, V, ld, logits, dtype);
     if (rc) return rc;
     if (K < 1 || K > TOP_MAX_K) return fail(ASCA_ERR_UNSUPPORTED, "%s: K=%d (1 to %d)", fn, K, TOP_MAX_K);
-    if (!(temperature > 0.0f) || !(temperature < INFINITY))
+    if (!logits_temperature(temperature))
         return fail(ASCA_ERR_INVALID, "%s: temperature %g", fn, (double)temperature);
     if (rows > 0 && (!logits || !values || !ids)) return fail(ASCA_ERR_INVALID, "null pointer in %s", fn);
     if (!grid_fits(rows, 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows (%ld)", fn, rows);   // a merge's blocks
@@ -748,6 +748,7 @@ int asca_beam_step(const void* logits, long ld, const float* scores, const int32
         if (groups > 0) return fail(ASCA_ERR_INVALID, "%s: eos, ended and new_ended go together", fn);
     if (groups > 0 && (!logits || !scores || !new_scores || !tokens || !parents))
         return fail(ASCA_ERR_INVALID, "null pointer in %s", fn);
+    if (!grid_fits(groups, 256)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many groups (%d)", fn, groups);
     TopArgs a{};
     a.z = logits, a.ld = ld, a.rows = (long)groups * K, a.V = V, a.K = K, a.itau = 1.0;
     a.scores = scores, a.ended = ended;
@@ -802,6 +803,7 @@ int asca_beam_states(void** src, void** dst, const uint64_t* outer, const uint64
     a.ks = k_src;
     a.kd = k_dst;
     uint64_t rows[BEAM_BUFS];
+    int which[BEAM_BUFS];
     unsigned word = 16;
     for (int i = 0; i < count; ++i) {
         if (outer[i] > (uint64_t)1 << 40 || bytes[i] > (uint64_t)1 << 40)
@@ -812,12 +814,6 @@ int asca_beam_states(void** src, void** dst, const uint64_t* outer, const uint64
         if (!src[i]) return fail(ASCA_ERR_INVALID, "%s: buffer %d is NULL", fn, i);
         if (d == src[i] && k_src != k_dst)
             return fail(ASCA_ERR_INVALID, "%s: buffer %d goes from %d to %d beams in place", fn, i, k_src, k_dst);
-        if (d != src[i]) {
-            const auto s0 = reinterpret_cast<uintptr_t>(src[i]), d0 = reinterpret_cast<uintptr_t>(d);
-            const __uint128_t n = (__uint128_t)outer[i] * bytes[i] * groups;
-            if (s0 < d0 + n * k_dst && d0 < s0 + n * k_src)
-                return fail(ASCA_ERR_INVALID, "%s: buffer %d overlaps its destination", fn, i);
-        }
         const auto mix = reinterpret_cast<uintptr_t>(src[i]) | reinterpret_cast<uintptr_t>(d) | (uintptr_t)bytes[i];
         while (mix % word) word = word == 16 ? 4 : 1;
         const int n = a.count++;
@@ -825,7 +821,18 @@ int asca_beam_states(void** src, void** dst, const uint64_t* outer, const uint64
         a.dst[n] = static_cast<char*>(d);
         a.bytes[n] = bytes[i];
         rows[n] = outer[i];
+        which[n] = i;
     }
+    // what is written is no other's, and its own source whole or not at all
+    auto overlap = [&](const char* x, int i, int kx, const char* y, int j, int ky) {
+        const auto x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
+        return x0 < y0 + (__uint128_t)rows[j] * a.bytes[j] * groups * ky && y0 < x0 + (__uint128_t)rows[i] * a.bytes[i] * groups * kx;
+    };
+    for (int i = 0; i < a.count; ++i)
+        for (int j = 0; j < a.count; ++j)
+            if ((a.dst[i] != a.src[j] || i != j) && (overlap(a.dst[i], i, k_dst, a.src[j], j, k_src) ||
+                                                     (i != j && overlap(a.dst[i], i, k_dst, a.dst[j], j, k_dst))))
+                return fail(ASCA_ERR_INVALID, "%s: the destination of buffer %d overlaps buffer %d", fn, which[i], which[j]);
     if (a.count == 0) return ASCA_OK;
     auto steps = [&](auto w) {
         using W = decltype(w);

@@ -632,7 +632,8 @@ ASCA_API int asca_grads_clip(void* grads, float max_norm, float* out, void* stre
  *     elements, at any address that is a multiple of an element.
  *   - All arithmetic is f32 or more; results are deterministic.
  *   - What a call needs for itself comes from the scratch that the library keeps
- *     for each stream (see asca_delta_ws_bytes). */
+ *     for each stream (see asca_delta_ws_bytes).
+ *   - A temperature is 1e-30 or more and finite. */
 
 /* The K (1..64) largest logits of each row, descending, of equal ones the lower id
  * first: values and ids (rows, K), and lse (rows, or NULL) = log sum exp(z / temperature).
@@ -686,7 +687,8 @@ ASCA_API int asca_beam_step(const void* logits, long ld, const float* scores, co
  * (device; NULL = slot 0 of each group: a fork of one sequence to k_dst beams).  A parent
  * outside 0 .. k_src-1 leaves its slot as it is.
  *   dst NULL, or dst[i] NULL or src[i]: in place (k_src = k_dst); only slots that change
- *   are touched.  Other destinations must not overlap any source.
+ *   are touched.  No other destination overlaps a source, and no two destinations each
+ *   other (refused).
  * src, dst, outer and bytes are host arrays, read before the call returns; 1 to 32 beams. */
 ASCA_API int asca_beam_states(void** src, void** dst, const uint64_t* outer, const uint64_t* bytes, int count,
                               const int32_t* parents, int groups, int k_src, int k_dst, void* stream);

@@ -89,6 +89,45 @@ def test_more_blocks_than_a_launch_takes():
     assert top(rows=9 << 20, V=40000, ld=40000) == UNSUPPORTED
 
 
+def test_more_groups_than_a_launch_takes():
+    assert step(groups=1 << 24, K=1, V=1, ld=1) == step(groups=1 << 24, K=1, V=9000, ld=9000) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("tau", [1e-31, 1e-42])
+def test_a_temperature_without_a_finite_inverse(tau):
+    assert top(tau=tau) == distill(tau=tau) == INVALID
+
+
+def pairs(src, dst, k_src=4, outer=2, nbytes=64):
+    n = len(src)
+    arr = lambda t, a: (t * n)(*a)  # noqa: E731
+    return code("asca_beam_states", arr(C.c_void_p, src), arr(C.c_void_p, dst), arr(C.c_uint64, [outer] * n),
+                arr(C.c_uint64, [nbytes] * n), n, P, 3, k_src, 4, None)
+
+
+SIZE = 2 * 3 * 4 * 64   # bytes of a buffer of four beams
+
+
+@pytest.mark.parametrize("src,dst", [
+    ([0x10000, 0x10000], [None, None]),                       # the same buffer twice, in place
+    ([0x10000, 0x10000 + SIZE - 1], [None, None]),
+    ([0x10000, 0x20000], [0x30000, 0x30000]),                 # one destination for two
+    ([0x10000, 0x20000], [0x30000, 0x30000 + SIZE - 16]),
+    ([0x10000, 0x20000], [0x20000, 0x30000]),                 # a destination that is another's source
+    ([0x10000, 0x20000], [None, 0x10000]),
+    ([0x10000, 0x20000], [0x20000 + SIZE - 1, None])])
+def test_beam_states_that_share_memory(src, dst):
+    assert pairs(src, dst) == INVALID and _lib.load().asca_last_error()
+
+
+def test_beam_states_of_one_source():
+    """Two destinations may take from one source, and lie side by side."""
+    n = C.c_int(0)
+    if _lib.load().asca_device_count(C.byref(n)) == 0 and n.value > 0:
+        pytest.skip("a GPU is present; this checks the no-device path")
+    assert pairs([0x10000, 0x10000], [0x30000, 0x30000 + SIZE]) == pairs([0x10000, 0x10000 + SIZE], [None, None]) == 4
+
+
 def test_right_calls_get_as_far_as_the_device():
     lib = _lib.load()
     n = C.c_int(0)
