@@ -654,7 +654,7 @@ static int distill_launch(DistillArgs a, hipStream_t st, const char* fn) {
     int r;
     // Rows that are fewer than the CUs and long: slices of 256 x 4 pieces at the most, of about
     // the whole device, at most 64 a row
-    if (pieces > 1024 && (a.T * 8 <= cus || (a.T * 2 <= cus && pieces > 1024 * 8))) {
+    if (pieces > 1024 * 4 && a.T * (pieces > 1024 * 8 ? 2 : 16) <= cus) {
         const long most = std::min(64l, (pieces + 255) / 256), least = std::min(most, (pieces + 256 * 8 - 1) / (256 * 8));
         const long s = std::max(least, std::min(most, 2 * cus / a.T));
         a.slice = (int)((pieces + s - 1) / s * W);

@@ -646,23 +646,26 @@ static int rows_check(const char* fn, long rows, int V, long ld, const void* z, 
 
 // Slices of the rows and the launch over them; with a.scores, or where a row has more than one,
 // their keys and sums go to scratch (and a.values is cleared).
-//   Rows of up to 64 x 8 pieces are a wave's where there are enough of them for four waves a
-//   CU; else slices are a block's, as many as give about four blocks a CU, between one piece
-//   a thread (shorter ones cost more in the merge than they spread) and eight (32 registers).
-//   Whole rows of up to 1024 x 8 pieces in blocks of 16 waves are slower than their slices and
-//   a merge (4096 x 16384 f32, 16 of them: 120 us against 60).
+//   A wave's rows of up to 64 x 4 pieces, or 64 x 8 where there are enough of them for four waves
+//   a CU (2048 x 2000 f32, 16 of them, 6.1 us against 8.1 in blocks; 512 rows 5.5 against 4.7).
+//   Else a block's, whole up to 256 x 16 pieces: the second launch costs a few rows 3 us, more than
+//   their slices' spread gains (64 x 16384 f32 7.1 us against 8.5 in two slices and more; 1 x 4096
+//   4.1), and many rows pay for the merge.  Longer ones, and a search's, which are merged in any
+//   case (1 x 4 x 32768 bf16 9.9 us, 13.4 with whole rows), in as many slices as give two blocks a CU
+//   (64 x 32768 f32 9.0 us, 9.7 with four; 256 rows 12.1 and 11.6).  Whole rows in blocks of 16
+//   waves were slower than these (4096 x 16384 f32 120 us against 44).
 constexpr int TOP_R = 16;   // pieces a thread at most
 template <typename E>
 static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const char* fn) {
     constexpr int W = 16 / sizeof(E);
-    const long want = 4l * std::max(cu_count(), 1);
-    const int nw = a.V <= 64 * 8 * W && (a.rows >= want || a.V <= 64 * W) ? 1 : 4;
-    if (nw == 1) {
+    const long cus = std::max(cu_count(), 1);
+    const int nw = a.V <= 64 * 4 * W || (a.V <= 64 * 8 * W && a.rows >= 4 * cus) ? 1 : 4;
+    if (nw == 1 || (!a.scores && a.V <= 256 * TOP_R * W)) {
         a.S = 1;
         a.slice = a.V;
     } else {
         const long least = (a.V + 256l * TOP_R * W - 1) / (256l * TOP_R * W), most = (a.V + 256l * W - 1) / (256l * W);
-        const long s = std::max(least, std::min(most, (want + a.rows - 1) / a.rows));
+        const long s = std::max(least, std::min(most, (2 * cus + a.rows - 1) / a.rows));
         a.slice = (int)(((a.V + s - 1) / s + W - 1) / W * W);
         a.S = (a.V + a.slice - 1) / a.slice;
     }
