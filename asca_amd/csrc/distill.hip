@@ -7,6 +7,14 @@
 //   dz_i / scale = w [(1 - a) (softmax(z)_i - [i = target]) + a tau (q_i - p_i)] for listed i, for
 //   the others q_i (1 - p_r / q_r) in the place of q_i - p_i (without tlse q_i)
 // Entries of one id are one entry with the sum of their p.
+//
+// A row has to be read once and its gradient written once: as fast as a copy (5.1 TB/s) where the
+// rows are long and many.  The exponentials bound it else: two a value (the sum and the gradient),
+// four where two temperatures count, each with one step of its own.  Time of a call, one
+// temperature | two, 64 entries a row:
+//   16384 x 256 (16 entries) f32 14 us;   4096 x 8192 f32 45 | 46 us, bf16 30 | 40
+//   4096 x 32768 f32 200 | 202 (5.3 TB/s), bf16 104 (5.2) | 128;   4096 x 50000 bf16 164 | 206
+//   2048 x 131072 f32 559 (read twice), bf16 259 | 321;   8 x 131072 in two launches 10
 #include <algorithm>
 
 #include "logits.h"
@@ -55,13 +63,14 @@ ASCA_DEV Expo expo_join(Expo a, Expo b, float ct) {
 struct Entry {
     int id;       // below 0: none
     float z, p;   // the student's logit there, and p
+    double lp;    // log p, without tlse log(p norm)
 };
 // What a row's entries are together
 struct List {
     Expo e;       // of their logits
     float total;  // sum of p
     float rest;   // what it leaves of 1, with tlse
-    float part;   // sum of p (log p - (z - ref) / tau), ref = their largest logit (0 where that is -inf)
+    float norm;   // without: the sum that made it 1
     float zt;     // the student's logit at the target
 };
 
@@ -70,21 +79,21 @@ ASCA_DEV float recip(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // A row's list, in a wave: id and z are there, tv is the teacher's logit; `twice`: some id may
 // be there more than once.  The first of one id's entries has their sum, the others are none.
-template <bool TWO, bool EXACT>
+template <bool TWO>
 ASCA_DEV List list_of(const DistillArgs& p, long row, float tv, bool twice, Entry& en) {
     const int lane = threadIdx.x & 63;
     bool on = en.id >= 0;
-    double lp;   // log p
-    en.p = 0.0f;
+    List l;
+    en.p = 0.0f, l.norm = 1.0f;
     if (p.tlse) {
-        lp = (double)tv * p.itau - (double)p.tlse[row];
-        if (on) en.p = exp_d(lp);
+        en.lp = (double)tv * p.itau - (double)p.tlse[row];
+        if (on) en.p = exp_d(en.lp);
     } else {
         const float m = wave_max(on ? tv : -INFINITY), ref = m == -INFINITY ? 0.0f : m;   // no entry, or none above -inf
-        lp = ((double)tv - (double)ref) * p.itau;
-        const float e = on ? exp_d(lp) : 0.0f, s = wave_sum(e);
-        if (m != -INFINITY) en.p = e * recip(s);
-        lp -= log_of<EXACT>(s);
+        en.lp = ((double)tv - (double)ref) * p.itau;
+        const float e = on ? exp_d(en.lp) : 0.0f, s = wave_sum(e), r = recip(s);
+        if (m != -INFINITY) en.p = e * fmaf(fmaf(-s, r, 1.0f), r, r);
+        l.norm = s;
     }
     if (twice) {
         for (int j = 0; j < p.K; ++j) {
@@ -92,19 +101,18 @@ ASCA_DEV List list_of(const DistillArgs& p, long row, float tv, bool twice, Entr
             const uint64_t same = __ballot(en.id == id);
             if (id < 0 || (same & (same - 1)) == 0) continue;
             const float sum = wave_sum(en.id == id ? en.p : 0.0f);
-            if (lane == j) en.p = sum, lp = log_of<EXACT>(sum);
+            if (lane == j) en.p = sum, en.lp = log_exact(sum) + log_exact(l.norm);
             else if (en.id == id) en.id = -1, en.p = 0.0f;
         }
         on = en.id >= 0;
     }
-    List l;
     l.e.m = wave_max(on ? en.z : -INFINITY);
     const float x = en.z - (l.e.m > -INFINITY ? l.e.m : 0.0f);
     l.e.st = on ? __builtin_amdgcn_exp2f(x * p.ct) : 0.0f;
     l.e.s1 = TWO && on ? __builtin_amdgcn_exp2f(x * LOG2E) : 0.0f;
     l.total = en.p;
-    l.part = en.p != 0.0f ? (float)((double)en.p * (lp - (double)x * p.itau)) : 0.0f;
-    wave_sum4(l.e.st, l.e.s1, l.total, l.part);
+    float none = 0.0f;
+    wave_sum4(l.e.st, l.e.s1, l.total, none);
     l.rest = p.tlse ? fmaxf(0.0f, 1.0f - l.total) : 0.0f;
     return l;
 }
@@ -156,22 +164,28 @@ ASCA_DEV Coefs distill_coefs(const DistillArgs& p, float w, Expo o, const List& 
     if (!TWO) c.As += c.Bt, c.Qs += c.Bs;
     return c;
 }
-// The loss, after the gradient: its doubles would stand beside the row's registers (4096 x 50000
-// bf16 204 -> 288 us).  EXACT takes the logarithms to 1e-10: tau^2 times the roundings of log_d are
-// as much as the loss's own where student and teacher are near; it costs rows of a wave each a
-// tenth of their time.
-template <bool TWO, bool EXACT>
-ASCA_DEV float distill_loss(const DistillArgs& p, float w, Expo o, const List& l, bool has_tg) {
+// The loss, by the wave that has the entries, after the gradient: its doubles would stand beside the
+// row's registers (4096 x 50000 bf16 204 -> 288 us).  An entry's p (log p - log q) is formed before the
+// sum, as the parts of either are much larger than their difference, and the logarithms are taken to
+// 1e-10, as tau^2 comes to them: four of them at once in as many lanes.
+template <bool TWO>
+ASCA_DEV float distill_loss(const DistillArgs& p, float w, Expo o, const List& l, const Entry& en, bool has_tg) {
     const Whole h = whole_of<TWO>(p, o, l);
-    const double lt = log_of<EXACT>(h.at), l1 = TWO ? log_of<EXACT>(h.a1) : lt;
+    const int lane = threadIdx.x & 63;
+    // p_r near q_r: log(p_r / q_r) from their difference
+    const bool near = h.tail && fabsf(h.gap) < 0.3f * h.qr;
+    const double logs = log_exact(lane == 0 ? h.at : lane == 1 ? h.a1 : lane == 2 ? l.rest : p.tlse ? o.st : l.norm, near && lane == 2,
+                                  -(double)h.gap, 2.0 * (double)h.qr - (double)h.gap);
+    const double lt = lane_value(logs, 0), l1 = TWO ? lane_value(logs, 1) : lt;
     double v = 0.0;
     if (p.alpha > 0.0f) {
         const float ref = l.e.m > -INFINITY ? l.e.m : 0.0f;
-        if (l.total != 0.0f) v = (double)l.part + (double)l.total * (((double)h.mx - (double)ref) * p.itau + lt);
+        // log sum exp((z - ref) / tau), less log norm
+        const double base = ((double)h.mx - (double)ref) * p.itau + lt - (p.tlse ? 0.0 : lane_value(logs, 3));
+        v = wave_sum(en.p != 0.0f ? (float)((double)en.p * (en.lp - ((double)en.z - (double)ref) * p.itau + base)) : 0.0f);
         if (h.tail) {   // + p_r log(p_r / q_r)
-            double r;
-            if (EXACT && fabsf(h.gap) < 0.3f * h.qr) r = artanh2(-(double)h.gap, 2.0 * (double)h.qr - (double)h.gap);
-            else r = log_of<EXACT>(l.rest) - log_of<EXACT>(o.st) + ((double)h.mx - (double)h.mr) * p.itau + lt;
+            double r = lane_value(logs, 2);
+            if (!near) r += ((double)h.mx - (double)h.mr) * p.itau + lt - lane_value(logs, 3);
             v += (double)l.rest * r;
         }
         v *= (double)p.alpha * p.tau * p.tau;
@@ -394,7 +408,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void distill_rows_k(Distil
     const E* z = static_cast<const E*>(p.z) + row * p.ld;
     const float w = p.weights ? p.weights[row] : 1.0f;
     if (w == 0.0f) return no_weight<E>(p, row, 0, p.V, tid, NT);
-    Entry en{-1, 0.0f, 0.0f};
+    Entry en{-1, 0.0f, 0.0f, 0.0};
     float tv = 0.0f;
     if (wave == 0 && p.K) {
         const long at = row * p.K + min(lane, p.K - 1);
@@ -418,7 +432,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void distill_rows_k(Distil
             en.z = act_load(z + en.id);
             twice = mark<E>(r, en.id, l.bits, &l.edge);
         }
-        li = list_of<TWO, (NW > 1)>(p, row, tv, __ballot(twice) != 0, en);
+        li = list_of<TWO>(p, row, tv, __ballot(twice) != 0, en);
         li.zt = zt;
         if constexpr (NW > 1) {
             l.en[lane] = en;
@@ -442,12 +456,13 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void distill_rows_k(Distil
         store_listed<E, NW, TWO>(p, r, 0, wave, dz, c, en, tg, has_tg, li.zt);
     }
     if (wave != 0) return;
-    const float loss = distill_loss<TWO, (NW > 1)>(p, w, o, li, has_tg);
+    const float loss = distill_loss<TWO>(p, w, o, li, en, has_tg);
     if (tid == 0) p.losses[row] = loss;
 }
 
 // A few long rows: S slices each, a block's of 4 waves.  The first launch leaves the slices'
-// sums, and from the first slice the list; the second forms the gradient.
+// sums, and from the first slice the list; the second forms the gradient.  Both wait for memory and
+// the launch (8 x 131072 bf16: 5.5 and 3.9 us, where 4 MB take 1).
 struct SplitRow {
     Entry en[64];
     List list;
@@ -461,7 +476,7 @@ __global__ __launch_bounds__(256) void distill_part_k(DistillArgs p) {
     const long row = blockIdx.x / (unsigned)p.S;
     const E* z = static_cast<const E*>(p.z) + row * p.ld;
     if (p.weights && p.weights[row] == 0.0f) return;
-    Entry en{-1, 0.0f, 0.0f};
+    Entry en{-1, 0.0f, 0.0f, 0.0};
     float tv = 0.0f;
     if (wave == 0 && p.K) {
         const long at = row * p.K + min(lane, p.K - 1);
@@ -483,7 +498,7 @@ __global__ __launch_bounds__(256) void distill_part_k(DistillArgs p) {
             if (en.id >= 0) en.z = act_load(z + en.id);
             bool twice = false;   // (the bitmap is of this slice alone)
             for (int j = 0; j < p.K; ++j) twice |= j < lane && en.id >= 0 && __builtin_amdgcn_readlane(en.id, j) == en.id;
-            List li = list_of<TWO, true>(p, row, tv, __ballot(twice) != 0, en);
+            List li = list_of<TWO>(p, row, tv, __ballot(twice) != 0, en);
             li.zt = zt;
             p.split[row].en[lane] = en;
             if (lane == 0) p.split[row].list = li;
@@ -529,12 +544,13 @@ __global__ __launch_bounds__(256) void distill_finish_k(DistillArgs p) {
         store_listed<E, 4, TWO>(p, r, c0, wave, dz, c, en, tg, has_tg, li.zt);
     }
     if (wave != 0 || slice != 0) return;
-    const float loss = distill_loss<TWO, true>(p, w, o, li, has_tg);
+    const float loss = distill_loss<TWO>(p, w, o, li, en, has_tg);
     if (tid == 0) p.losses[row] = loss;
 }
 
 // Rows that no team's registers hold: read twice, by 1024 threads, the second time mostly from
-// a cache (256 rows of 131072 f32 are half of the last-level one's)
+// a cache (256 rows of 131072 f32 are half of the last-level one's).  2048 of these 559 us, 3.8 TB/s
+// of the two passes that it cannot do without; as two launches over batches of 64 MB 726 us.
 template <typename E, bool TWO>
 __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
     constexpr int NW = 16, NT = 1024, W = Pieces<E>::W, U = 4;
@@ -545,7 +561,7 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
     const E* z = static_cast<const E*>(p.z) + row * p.ld;
     const float w = p.weights ? p.weights[row] : 1.0f;
     if (w == 0.0f) return no_weight<E>(p, row, 0, p.V, tid, NT);
-    Entry en{-1, 0.0f, 0.0f};
+    Entry en{-1, 0.0f, 0.0f, 0.0};
     float tv = 0.0f;
     if (wave == 0 && p.K) {
         const long at = row * p.K + min(lane, p.K - 1);
@@ -569,7 +585,7 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
             en.z = act_load(z + en.id);
             twice = mark<E>(r, en.id, bits, &l.edge);
         }
-        List li = list_of<TWO, true>(p, row, tv, __ballot(twice) != 0, en);
+        List li = list_of<TWO>(p, row, tv, __ballot(twice) != 0, en);
         li.zt = zt;
         l.en[lane] = en;
         if (lane == 0) l.list = li;
@@ -619,7 +635,7 @@ __global__ __launch_bounds__(1024) void distill_long_k(DistillArgs p) {
     en = l.en[lane];
     const List li = l.list;
     if (wave == 0) {
-        const float loss = distill_loss<TWO, true>(p, w, o, li, has_tg);
+        const float loss = distill_loss<TWO>(p, w, o, li, en, has_tg);
         if (tid == 0) p.losses[row] = loss;
     }
     if (!p.dz) return;
@@ -652,8 +668,10 @@ static int distill_launch(DistillArgs a, hipStream_t st, const char* fn) {
     if (!grid_fits(a.T, 1024)) return fail(ASCA_ERR_UNSUPPORTED, "%s: too many rows (%ld)", fn, a.T);
     const long pieces = (a.V + W - 1) / W, cus = std::max(cu_count(), 1);
     int r;
-    // Rows that are fewer than the CUs and long: slices of 256 x 4 pieces at the most, of about
-    // the whole device, at most 64 a row
+    // Long rows that leave CUs idle: slices of up to 256 x 8 pieces, at most 64 a row.  Up to 8192
+    // pieces the second launch costs what the spread gains but for the fewest rows (16 x 32768 f32
+    // 9.7 us against 10.6, 32 rows 10.8 and 10.6); longer ones gain up to half of the CUs (8 x 131072
+    // f32 10.3 us against 33, 128 rows 37 against 41, 192 rows 51 and 53).
     if (pieces > 1024 * 4 && a.T * (pieces > 1024 * 8 ? 2 : 16) <= cus) {
         const long most = std::min(64l, (pieces + 255) / 256), least = std::min(most, (pieces + 256 * 8 - 1) / (256 * 8));
         const long s = std::max(least, std::min(most, 2 * cus / a.T));
@@ -683,7 +701,7 @@ static int distill_launch(DistillArgs a, hipStream_t st, const char* fn) {
             return post_launch("distill_finish");
         }
     }
-    if (pieces > 1024 * 16) {
+    if (pieces > 1024 * 16) {   // more than 16 pieces a thread, 64 registers, in the largest block
         const size_t lds = ((size_t)a.V + 31) / 32 * 4;
         if ((r = allow_lds(reinterpret_cast<const void*>(&distill_long_k<E, TWO>), lds))) return r;
         if ((r = pre_launch("distill_long"))) return r;
@@ -691,6 +709,9 @@ static int distill_launch(DistillArgs a, hipStream_t st, const char* fn) {
         return post_launch("distill_long");
     }
     if ((r = pre_launch("distill_rows"))) return r;
+    // A wave a row, up to 8 pieces a lane, where there are four rows a CU (2048 x 1000 f32 6.6 us, 9.5
+    // in blocks of four waves; 256 rows 4.9 and 5.1), else the fewest waves that hold a row in 64
+    // registers each: 1000 x 32001 f32 54 us in 8 waves, 78 in 16.
     const bool many = a.T >= 4 * cus;
     auto go = [&](auto nw, auto rr) {
         constexpr int NW = decltype(nw)::value, R = decltype(rr)::value;

@@ -47,18 +47,12 @@ ASCA_DEV double artanh2(double a, double b) {
     v = fma(v, q, 2.0 / 9), v = fma(v, q, 2.0 / 7), v = fma(v, q, 2.0 / 5), v = fma(v, q, 2.0 / 3), v = fma(v, q, 2.0);
     return v * t;
 }
-ASCA_DEV double log_exact(float x) {
+ASCA_DEV double log_exact(float x, bool near = false, double a = 0.0, double b = 1.0) {   // near: 2 artanh(a / b)
     float m = __builtin_amdgcn_frexp_mantf(x);
     int e = __builtin_amdgcn_frexp_expf(x);
     if (m < 0.70710678f) m *= 2.0f, --e;
-    const double l = artanh2((double)m - 1.0, (double)m + 1.0);   // log m
-    return x > 0.0f && x < INFINITY ? fma((double)e, LN2, l) : (double)__builtin_amdgcn_logf(x);
-}
-// log of one or the other kind
-template <bool EXACT>
-ASCA_DEV double log_of(float x) {
-    if constexpr (EXACT) return log_exact(x);
-    return log_d(x);
+    const double l = artanh2(near ? a : (double)m - 1.0, near ? b : (double)m + 1.0);   // log m
+    return near ? l : x > 0.0f && x < INFINITY ? fma((double)e, LN2, l) : (double)__builtin_amdgcn_logf(x);
 }
 
 // ------------------------------------------------------ lanes of a wave
@@ -103,6 +97,11 @@ ASCA_DEV float wave_max(float x) {
     return max_or_nan(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+ASCA_DEV double lane_value(double x, int lane) {
+    const uint64_t u = __double_as_longlong(x);
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)u, lane), hi = __builtin_amdgcn_readlane((unsigned)(u >> 32), lane);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
 ASCA_DEV float lane_value(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
 
 // The sums of four values over the wave together: a third of the steps that they take apart
