@@ -653,7 +653,8 @@ ASCA_API int asca_top_logits(const void* logits, long ld, long rows, int V, int 
  *   q = softmax(logits / temperature)
  *   losses_t = w_t ((1 - alpha) CE_t + alpha temperature^2 (sum p log(p / q) + p_r log(p_r / q_r)))
  *   dlogits  = scale * d losses_t / d logits, of `dtype`, rounded once; NULL = not wanted;
- *     may be the logits (with the same stride)
+ *     may be the logits (with the same stride); other rows that share memory with theirs
+ *     are refused
  *   targets (T) for CE_t, the cross-entropy of the unscaled logits (no CE_t for a target
  *     >= V); may be NULL where alpha = 1.  tval and tids may be NULL where alpha = 0.
  *   weights (T), NULL = ones: w_t, also the gradient that comes back to losses_t.  A row of

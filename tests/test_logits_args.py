@@ -98,6 +98,22 @@ def test_a_temperature_without_a_finite_inverse(tau):
     assert top(tau=tau) == distill(tau=tau) == INVALID
 
 
+@pytest.mark.parametrize("bad", [
+    dict(dz=C.c_void_p(0x1004)), dict(dz=C.c_void_p(0x1000 - 4)), dict(dz=C.c_void_p(0x1000 + 40)), dict(dz=C.c_void_p(0x1000 + 76)),
+    dict(dz=C.c_void_p(0x1000 + 36), ld=20, lddl=20), dict(dz=C.c_void_p(0x1000 + 44), ld=20, lddl=20),
+    dict(dz=C.c_void_p(0x1000 + 40), ld=10, lddl=20)])
+def test_gradients_that_share_memory_with_the_logits(bad):
+    assert distill(**bad) == INVALID and _lib.load().asca_last_error()
+
+
+def test_gradients_beside_the_logits():
+    n = C.c_int(0)
+    if _lib.load().asca_device_count(C.byref(n)) == 0 and n.value > 0:
+        pytest.skip("a GPU is present; this checks the no-device path")
+    assert distill(dz=C.c_void_p(0x1000 + 80)) == distill(dz=C.c_void_p(0x1000 + 40), ld=20, lddl=20) == 4
+    assert distill(dz=C.c_void_p(0x1000 - 80)) == distill() == 4
+
+
 def pairs(src, dst, k_src=4, outer=2, nbytes=64):
     n = len(src)
     arr = lambda t, a: (t * n)(*a)  # noqa: E731
