@@ -12,7 +12,7 @@
 // rows are long and many.  The exponentials bound it else: two a value (the sum and the gradient),
 // four where two temperatures count, each with one step of its own.  Time of a call, one
 // temperature | two, 64 entries a row:
-//   16384 x 256 (16 entries) f32 15.5 | 17 us;   4096 x 8192 f32 45 | 46 us, bf16 30 | 40
+//   16384 x 256 (16 entries) f32 15 | 16.4 us, 12.5 | 13 of them the lists';   4096 x 8192 f32 45 | 46 us, bf16 30 | 40
 //   4096 x 32768 f32 200 | 202 (5.3 TB/s), bf16 104 (5.2) | 128;   4096 x 50000 bf16 164 | 206
 //   2048 x 131072 f32 559 (read twice), bf16 259 | 321;   8 x 131072 in two launches 10
 #include <algorithm>
@@ -269,7 +269,11 @@ ASCA_DEV int wave_of(const Pieces<E>& r, int col) {
 template <typename E, int NW, int R>
 struct RowRegs {
     static constexpr int NT = 64 * NW, W = Pieces<E>::W;
+    // the sums' exponentials stay for the gradient where there are registers for them without fewer
+    // waves a SIMD (two temperatures, 16384 x 256 f32 17.1 -> 16.4 us, bf16 19.9 -> 18.4)
+    static constexpr bool KEEP = NW == 1 && R * W <= 8;
     uint4 raw[R ? R : 1];
+    float kt[KEEP ? R * W + 1 : 1], k1[KEEP ? R * W + 1 : 1];
     float ev;   // the column outside the pieces that is the thread's
     int ec;
 
@@ -300,7 +304,7 @@ struct RowRegs {
         if (tid < 32 && edge >> tid & 1) ev = -INFINITY;
         return max_or_nan(m, ev);
     }
-    // f of every value, in its place
+    // f of every value and its number
     template <typename F>
     ASCA_DEV void each(F f) {
         float v[W];
@@ -309,10 +313,10 @@ struct RowRegs {
             piece_again(raw[j]);
             piece_values(raw[j], v, E());
 #pragma unroll
-            for (int k = 0; k < W; ++k) f(v[k]);
+            for (int k = 0; k < W; ++k) f(v[k], j * W + k);
             if (R >= 8) __builtin_amdgcn_sched_barrier(0);
         }
-        f(ev);
+        f(ev, R * W);
     }
     // The wave's sums, from its largest m.  exp2(v c - rc) is one step and the exponential; what
     // rounding m c to rc does is the same in every term and taken off at the end.
@@ -320,17 +324,20 @@ struct RowRegs {
     ASCA_DEV Expo sums(float m, float ct) {
         const float ref = m > -INFINITY ? m : 0.0f, rt = ref * ct, r1 = ref * LOG2E;
         float st = 0.0f, s1 = 0.0f;
+        auto add = [&](float a, float b, int i) {
+            st += a;
+            if (TWO) s1 += b;
+            if constexpr (KEEP) kt[i] = a, k1[i] = b;
+        };
         if (fabsf(rt) < 65536.0f && fabsf(r1) < 65536.0f) {
-            each([&](float v) {
-                st += __builtin_amdgcn_exp2f(fmaf(v, ct, -rt));
-                if (TWO) s1 += __builtin_amdgcn_exp2f(fmaf(v, LOG2E, -r1));
+            each([&](float v, int i) {
+                add(__builtin_amdgcn_exp2f(fmaf(v, ct, -rt)), TWO ? __builtin_amdgcn_exp2f(fmaf(v, LOG2E, -r1)) : 0.0f, i);
             });
             st *= __builtin_amdgcn_exp2f(-fmaf(ref, ct, -rt));
             if (TWO) s1 *= __builtin_amdgcn_exp2f(-fmaf(ref, LOG2E, -r1));
         } else {   // where that would be more than the terms
-            each([&](float v) {
-                st += __builtin_amdgcn_exp2f((v - ref) * ct);
-                if (TWO) s1 += __builtin_amdgcn_exp2f((v - ref) * LOG2E);
+            each([&](float v, int i) {
+                add(__builtin_amdgcn_exp2f((v - ref) * ct), TWO ? __builtin_amdgcn_exp2f((v - ref) * LOG2E) : 0.0f, i);
             });
         }
         float x = 0.0f, y = 0.0f;
@@ -347,11 +354,11 @@ struct RowRegs {
             piece_again(raw[j]);
             piece_values(raw[j], v, E());
 #pragma unroll
-            for (int k = 0; k < W; ++k) v[k] = f(v[k]);
+            for (int k = 0; k < W; ++k) v[k] = f(v[k], j * W + k);
             if (i < r.nb) row_piece_store<E>(d + r.col(i), whole, v);
             if (R >= 8) __builtin_amdgcn_sched_barrier(0);
         }
-        if (ec >= 0) act_store(d + ec, f(ev));
+        if (ec >= 0) act_store(d + ec, f(ev, R * W));
     }
     // The gradient of everything as if it were not listed
     template <bool TWO>
@@ -361,12 +368,12 @@ struct RowRegs {
         if (fabsf(rt) < 65536.0f && fabsf(r1) < 65536.0f) {   // as in the sums
             const float A = c.As * __builtin_amdgcn_exp2f(-fmaf(c.mr, ct, -rt));
             const float B = TWO ? c.Bt * __builtin_amdgcn_exp2f(-fmaf(c.mr, LOG2E, -r1)) : 0.0f;
-            store_each(r, tid, d, whole, [&](float v) {
-                const float g = A * __builtin_amdgcn_exp2f(fmaf(v, ct, -rt));
-                return TWO ? fmaf(B, __builtin_amdgcn_exp2f(fmaf(v, LOG2E, -r1)), g) : g;
+            store_each(r, tid, d, whole, [&](float v, int i) {
+                const float g = A * (KEEP ? kt[KEEP ? i : 0] : __builtin_amdgcn_exp2f(fmaf(v, ct, -rt)));
+                return TWO ? fmaf(B, KEEP ? k1[KEEP ? i : 0] : __builtin_amdgcn_exp2f(fmaf(v, LOG2E, -r1)), g) : g;
             });
         } else {
-            store_each(r, tid, d, whole, [&](float v) { return grad_other<TWO>(c, ct, v); });
+            store_each(r, tid, d, whole, [&](float v, int) { return grad_other<TWO>(c, ct, v); });
         }
     }
 };
