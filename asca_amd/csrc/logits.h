@@ -161,7 +161,9 @@ ASCA_DEV T block_max_t(T x, T* lds) {
 // ------------------------------------------------------------ row pieces
 
 // A row's n elements as pieces of B bytes (16 or 8): `head` elements before the first whole
-// piece of the address space, nb pieces of W, fewer than W after them.
+// piece of the address space, nb pieces of W, fewer than W after them.  `fixed`: the pieces begin
+// at the row's first element, at any address of one, so that which thread has what, and with it
+// the rounding of a sum over the row, is the same wherever the row lies.
 template <int B>
 struct PieceRaw {
     typedef uint4 type;
@@ -177,12 +179,16 @@ struct Pieces {
     const E* p;
     int n, head, nb;
     // (without pieces all of up to 2 W - 1 elements are at the edges)
-    ASCA_DEV Pieces(const E* row, int len, bool pieces = true) : p(row), n(len) {
-        const int off = (int)(reinterpret_cast<uintptr_t>(row) / sizeof(E) % W);
+    ASCA_DEV Pieces(const E* row, int len, bool pieces = true, bool fixed = false) : p(row), n(len) {
+        const int off = fixed ? 0 : (int)(reinterpret_cast<uintptr_t>(row) / sizeof(E) % W);
         head = min(off ? W - off : 0, n);
         nb = pieces ? (n - head) / W : 0;
     }
-    ASCA_DEV Raw piece(int i) const { return reinterpret_cast<const Raw*>(p + head)[i]; }
+    ASCA_DEV Raw piece(int i) const {
+        Raw r;
+        __builtin_memcpy(&r, p + head + (long)i * W, B);   // one load, at any address of an element
+        return r;
+    }
     ASCA_DEV int col(int i) const { return head + i * W; }   // the first column of a piece
     // the column outside the pieces that thread t takes, or -1: one of the first 2 W, of the first 32
     // without pieces

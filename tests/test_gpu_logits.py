@@ -521,6 +521,23 @@ def test_beam_ties_go_to_the_lowest_place(g, V, stay):
         check_step(g.beam_step(z, sc, k=K, stay=stay), z.astype(np.float64), sc, K, stay=stay)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("pad,off", [(0, 0), (4, 0), (0, 3)])
+@pytest.mark.parametrize("G,K,V", [(9, 3, 37), (9, 4, 257), (3, 16, 257), (9, 4, 2001), (2, 5, 9001), (2, 3, 50001), (300, 4, 2501)])
+def test_beams_of_the_same_logits_tie(g, G, K, V, pad, off, bf16):
+    """A group's beams have one row's logits and one score, at addresses that differ by elements:
+    each token ties over the beams, and the ties go to the lowest one."""
+    from asca_amd import _lib, gpu
+
+    z, val = to_dev(np.repeat(np.random.default_rng(G + V + off).standard_normal((G, V)) * 2, K, 0), bf16)
+    n, sc = G * K, np.repeat(-np.random.default_rng(V).random(G), K).astype(np.float32)
+    m, bs, out, tok, par = Strided(z, pad, off), up(sc), gpu.DevBuf(n * 4), gpu.DevBuf(n * 4), gpu.DevBuf(n * 4)
+    for stay in (False, True):
+        _lib.call("asca_beam_step", m.ptr, m.ld, _p(bs), None, -1, int(stay), _p(out), None, _p(tok), _p(par), G, K, V, int(bf16), None)
+        _lib.call("asca_sync")
+        check_step((out.to_host((n,)), tok.to_host((n,), np.uint32), par.to_host((n,), np.int32)), val, sc, K, stay=stay)
+
+
 @pytest.mark.parametrize("V", [9, 300, 40000])
 @pytest.mark.parametrize("stay", [False, True])
 def test_beam_masks_leave_few_or_no_candidates(g, V, stay):
