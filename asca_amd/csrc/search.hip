@@ -18,6 +18,7 @@ namespace asca {
 constexpr int TOP_MAX_K = 64;    // listed logits a row
 constexpr int BEAM_MAX_K = 32;   // beams a group
 constexpr int BEAM_BUFS = 8;     // state buffers a call
+constexpr int ROW_MAX_V = 1 << 30;   // columns: ends of slices and of pieces past them are ints
 
 // ------------------------------------------------------------ selection
 // A team of NW waves finds the K largest of what it holds in registers.  The K-th largest of
@@ -649,6 +650,7 @@ using namespace asca;
 
 static int rows_check(const char* fn, long rows, int V, long ld, const void* z, int dtype) {
     if (rows < 0 || V <= 0) return fail(ASCA_ERR_INVALID, "%s: bad shape %ld x %d", fn, rows, V);
+    if (V > ROW_MAX_V) return fail(ASCA_ERR_UNSUPPORTED, "%s: V=%d (up to %d)", fn, V, ROW_MAX_V);
     if (ld < V) return fail(ASCA_ERR_INVALID, "%s: row stride %ld below %d columns", fn, ld, V);
     if (reinterpret_cast<uintptr_t>(z) % (dtype == ASCA_F32 ? 4 : 2))
         return fail(ASCA_ERR_INVALID, "%s: logits at an address that is no multiple of an element", fn);

@@ -629,7 +629,8 @@ ASCA_API int asca_grads_clip(void* grads, float max_norm, float* out, void* stre
  * largest, distillation from a teacher's, and a beam search's steps.  The reference
  * has no counterpart.
  *   - Logits are (rows, V) f32 or bf16 (`dtype`) with a row stride `ld` >= V in
- *     elements, at any address that is a multiple of an element.
+ *     elements, at any address that is a multiple of an element; V is at most 2^30
+ *     (asca_distill: 2^20).
  *   - All arithmetic is f32 or more; results are deterministic.
  *   - What a call needs for itself comes from the scratch that the library keeps
  *     for each stream (see asca_delta_ws_bytes).

@@ -93,6 +93,14 @@ def test_more_groups_than_a_launch_takes():
     assert step(groups=1 << 24, K=1, V=1, ld=1) == step(groups=1 << 24, K=1, V=9000, ld=9000) == UNSUPPORTED
 
 
+@pytest.mark.parametrize("ty", [0, 1])
+@pytest.mark.parametrize("V", [(1 << 30) + 1, 0x7fffffff - 4, 0x7fffffff])
+def test_vocabularies_past_the_end_of_a_row(V, ty):
+    """Columns of a row are counted in 32 bits, and its slices' ends past the last of them."""
+    assert top(rows=1, V=V, ld=1 << 31, ty=ty) == UNSUPPORTED
+    assert step(groups=1, K=1, V=V, ld=1 << 31, ty=ty) == UNSUPPORTED
+
+
 @pytest.mark.parametrize("tau", [1e-31, 1e-42])
 def test_a_temperature_without_a_finite_inverse(tau):
     assert top(tau=tau) == distill(tau=tau) == INVALID
