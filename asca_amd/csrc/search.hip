@@ -1,7 +1,8 @@
 // The largest logits of rows, and a beam search's steps over them: the choice among a
 // group's beams and tokens, and the states' move to their beams' new slots.
 //   top    the K largest of a row, ties to the lower id; lse = log sum exp(z / tau)
-//   step   the K best of s_b + z_bi - lse_b over b and i, ties to the lower b V + i
+//   step   the K best of s_b + z_bi - lse_b over b and i, ties to the lower b, in one b to the larger
+//          z, then to the lower i
 //   states slot <- state of parent[slot], in place or into other buffers
 //
 // top and step have to read the logits once (a copy's rate is 5.1 TB/s) and rank what may be
@@ -434,9 +435,10 @@ struct BeamLds {
     int ended[BEAM_MAX_K];
     float lists[4][64];
     double score[BEAM_CAP];
-    unsigned place[BEAM_CAP][2];   // beam, token
+    uint64_t key[BEAM_CAP];      // a beam's tokens in their order, by logit and id
+    int beam[BEAM_CAP];
     double best[16];
-    uint64_t best_place[16];
+    uint64_t best_key[16];
     BeamPick picks[BEAM_MAX_K];
     int count;
 };
@@ -454,7 +456,11 @@ ASCA_DEV void beam_write(const BeamArgs& p, long group, const BeamPick& pick, co
     if (p.new_ended) p.new_ended[at] = some && (ended[pick.parent] != 0 || (int)pick.token == p.eos);
 }
 
-ASCA_DEV bool beam_better(double a, uint64_t pa, double b, uint64_t pb) { return a > b || (a == b && pa < pb); }
+// Whether candidate x of beam b comes before y of beam c.  In one beam the keys' order is that of
+// the scores before they are rounded, which may make them equal.
+ASCA_DEV bool beam_before(double x, int b, uint64_t key, double y, int c, uint64_t other) {
+    return x > y || (x == y && (b < c || (b == c && key > other)));
+}
 
 // The K best of a group's candidates by the first 256 threads of a block of NW waves.  As a
 // row's selection, with the scores in 64 bits; the threshold compares them rounded to 32, which
@@ -500,53 +506,52 @@ ASCA_DEV void beam_merge(const BeamArgs& p, long group, BeamLds& l, Keys keys, S
             const double base = l.base[b];
             if (base == -INFINITY) continue;
             if (l.ended[b]) {
-                if (rank == 0 && slice == b * S) f(base, b, (unsigned)p.eos);
+                if (rank == 0 && slice == b * S) f(base, b, (uint64_t)~(unsigned)p.eos);
                 continue;
             }
             const uint64_t key = keys[slice * K + rank];
-            if (key) f(base + (double)key_value(key), b, key_place(key));
+            if (key) f(base + (double)key_value(key), b, key);
         }
     };
     // the threshold: from each slice's first ones, as many of them as there are lanes
     float mx = -INFINITY;
-    each(min(K, (255 + L) / L), [&](double x, int, unsigned) { mx = fmaxf(mx, (float)x); });
+    each(min(K, (255 + L) / L), [&](double x, int, uint64_t) { mx = fmaxf(mx, (float)x); });
     if (in) l.lists[w][lane] = lane_sort(mx);
     __syncthreads();
     const float kth = in ? lane_value(four_lists(l.lists), K - 1) : 0.0f;
-    each(K, [&](double x, int b, unsigned token) {
+    each(K, [&](double x, int b, uint64_t key) {
         if ((float)x < kth) return;
         const int i = atomicAdd(&l.count, 1);
-        if (i < BEAM_CAP) l.score[i] = x, l.place[i][0] = b, l.place[i][1] = token;
+        if (i < BEAM_CAP) l.score[i] = x, l.key[i] = key, l.beam[i] = b;
     });
     __syncthreads();
     const int n = l.count;
     if (n <= BEAM_CAP) {
         for (int i = tid; i < n; i += 64 * NW) {
             const double x = l.score[i];
-            const unsigned b = l.place[i][0], t = l.place[i][1];
+            const uint64_t key = l.key[i];
+            const int b = l.beam[i];
             int rank = 0;
-            for (int j = 0; j < n; ++j) {
-                const double y = l.score[j];
-                const unsigned c = l.place[j][0], u = l.place[j][1];
-                rank += y > x || (y == x && (c < b || (c == b && u < t)));
-            }
-            if (rank < K) l.picks[rank] = BeamPick{x, (int)b, t};
+            for (int j = 0; j < n; ++j) rank += beam_before(l.score[j], l.beam[j], l.key[j], x, b, key);
+            if (rank < K) l.picks[rank] = BeamPick{x, b, key_place(key)};
         }
     } else {   // rows of equal values: K rounds, each the best below the last
         double last = INFINITY;
-        uint64_t lastp = 0;
+        int lastb = 0;
+        uint64_t lastk = 0;
         for (int k = 0; k < K; ++k) {
             double v = -INFINITY;
-            uint64_t vp = ~0ull;
-            each(K, [&](double x, int b, unsigned token) {
-                const uint64_t at = (uint64_t)b << 32 | token;
-                if (beam_better(last, lastp, x, at) && beam_better(x, at, v, vp)) v = x, vp = at;
+            int vb = BEAM_MAX_K;
+            uint64_t vk = 0;
+            each(K, [&](double x, int b, uint64_t key) {
+                if (beam_before(last, lastb, lastk, x, b, key) && beam_before(x, b, key, v, vb, vk)) v = x, vb = b, vk = key;
             });
             const double top = block_max_t<NW>(v, l.best);
-            const uint64_t place = ~block_max_t<NW>(v == top ? ~vp : (uint64_t)0, l.best_place);
             if (top == -INFINITY) break;
-            if (tid == 0) l.picks[k] = BeamPick{top, (int)(place >> 32), (unsigned)place};
-            last = top, lastp = place;
+            const int b = -(int)block_max_t<NW>(v == top ? -(double)vb : -(double)BEAM_MAX_K, l.best);
+            const uint64_t key = block_max_t<NW>(v == top && vb == b ? vk : (uint64_t)0, l.best_key);
+            if (tid == 0) l.picks[k] = BeamPick{top, b, key_place(key)};
+            last = top, lastb = b, lastk = key;
         }
     }
     __syncthreads();

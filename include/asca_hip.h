@@ -667,10 +667,10 @@ ASCA_API int asca_distill(const void* logits, long ld, const float* tval, const 
 
 /* One choice of a beam search: for each of `groups` searches the K (1..32) best of the
  * candidates scores_b + logits_bi - log sum exp(logits_b) of its beams b and tokens i, of
- * equal ones the lowest b V + i first.  They are compared in 64 bits; a log sum is of
- * exponentials and sums in 32, so that candidates of two beams that are nearer than its
- * rounding (about 1e-6 of 1) may come in either order.  Rows of the same logits have the
- * same log sum, wherever they lie.
+ * equal ones the lowest b first, of one beam the larger logit, then the lower i.  They are
+ * compared in 64 bits; a log sum is of exponentials and sums in 32, so that candidates of two
+ * beams that are nearer than its rounding (about 1e-6) may come in either order.  Rows of the
+ * same logits have the same log sum, wherever they lie.
  *   logits (groups*K, V); scores (groups*K): a beam whose score, or whose logits' sum, is
  *     not finite has no candidates, and a logit of -inf or NaN is none
  *   eos >= 0 with ended, new_ended (groups*K): an ended beam's only candidate is itself

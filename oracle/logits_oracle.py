@@ -86,28 +86,29 @@ def distill(logits, tval=None, tids=None, tlse=None, targets=None, weights=None,
 
 
 def beam_step(logits, scores, K, ended=None, eos=-1, stay=False):
-    """(scores, tokens, parents, ended or None) of groups of K beams."""
+    """(scores, tokens, parents, ended or None) of groups of K beams.  Candidates of one score
+    come by their beams, and of one beam by their logits, then by their ids."""
     z, s = np.asarray(logits, f8), np.asarray(scores, f8)
     n, V = z.shape
     ns, tok, par = np.full(n, -np.inf), np.full(n, max(eos, 0), np.uint32), np.zeros(n, np.int32)
     end = np.zeros(n, np.int32)
     for g in range(n // K):
-        cand = []   # (-score, place)
+        cand = []   # (-score, beam, -logit, id)
         for b in range(K):
             r = g * K + b
             if not np.isfinite(s[r]):
                 continue
             if ended is not None and ended[r]:
-                cand.append((-s[r], b * V + eos))
+                cand.append((-s[r], b, 0.0, eos))
                 continue
             norm = lse(z[r]) if not np.isnan(z[r]).any() else np.nan
             if not np.isfinite(norm):
                 continue
             x = s[r] + (z[r] - norm)
-            keep = np.argsort(-x, kind="stable")[:K]   # no more of one beam can be chosen
-            cand += [(-x[c], b * V + int(c)) for c in keep if z[r, c] > -np.inf]
+            keep = np.argsort(-z[r], kind="stable")[:K]   # no more of one beam can be chosen
+            cand += [(-x[c], b, -z[r, c], int(c)) for c in keep if z[r, c] > -np.inf]
         cand = sorted(cand)[:K]
-        picks = [(-c, at // V, at % V) for c, at in cand] + [None] * (K - len(cand))
+        picks = [(-x, b, c) for x, b, _, c in cand] + [None] * (K - len(cand))
         slots, left = {}, list(range(K))
         if stay:
             for r, c in enumerate(picks):

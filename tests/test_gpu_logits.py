@@ -538,6 +538,28 @@ def test_beams_of_the_same_logits_tie(g, G, K, V, pad, off, bf16):
         check_step((out.to_host((n,)), tok.to_host((n,), np.uint32), par.to_host((n,), np.int32)), val, sc, K, stay=stay)
 
 
+@pytest.mark.parametrize("V", [40, 300, 3000, 40000])
+@pytest.mark.parametrize("stay", [False, True])
+def test_beam_logits_below_a_score_s_rounding(g, V, stay):
+    """Logits too small to change a beam's sum in 64 bits: its tokens come in the logits' order
+    whatever the number of beams, after an equal beam's before them."""
+    tiny = np.float32(1e-20)
+    first = None
+    for K in (32, 8, 3, 1):
+        z = np.zeros((K, V), np.float32)
+        z[:, 1::2] = -1.0
+        order = np.random.default_rng(V).permutation(np.arange(0, V, 2))[:12]
+        z[:, order] = tiny * np.arange(12, 0, -1, dtype=np.float32)   # the largest first
+        sc = np.where(np.arange(K) < 2, -1.0, -np.inf).astype(np.float32)
+        got = g.beam_step(z, sc, k=K)
+        picks = list(zip(got[2].tolist(), got[1].tolist()))
+        want = [(b, int(t)) for b in range(2) for t in [*order, *np.setdiff1d(np.arange(0, V, 2), order)]][:K]
+        assert picks == want
+        first = first or picks
+        assert picks == first[:K]
+        check_step(g.beam_step(z, sc, k=K, stay=stay), z.astype(np.float64), sc, K, stay=stay)
+
+
 @pytest.mark.parametrize("V", [9, 300, 40000])
 @pytest.mark.parametrize("stay", [False, True])
 def test_beam_masks_leave_few_or_no_candidates(g, V, stay):
