@@ -189,6 +189,50 @@ def test_a_search_in_which_every_beam_ends(g):
     m.close()
 
 
+def test_a_search_stops_where_every_beam_has_ended(g, monkeypatch):
+    """eos is the likeliest token of every row (channel 0, which every embedding has most of, gives it
+    alone): all beams end, each counted step after that is left out, and tokens and scores are the
+    host's and those of a longer search."""
+    m, p = model()
+    p = {k: a.copy() for k, a in p.items()}
+    p["embed"][:, 0] = 8.0
+    p["head"][0] = 0.0
+    p["head"][0, 3] = 0.7
+    m.set_params(p)
+    rng = np.random.default_rng(6)
+    n, beams, steps = 4, 3, 30
+    ids = rng.integers(0, 17, (n, 5))
+    calls = []
+    step_dev = m._step_dev
+    monkeypatch.setattr(m, "_step_dev", lambda *a: calls.append(1) or step_dev(*a))
+    got, sc = m.beam_search(ids, beams, steps, eos=3)
+    hist = [[list(s) for s in ids for _ in range(beams)]]
+
+    def pick(rows):
+        hist[0] = [list(hist[0][r]) for r in rows]
+
+    def step(tok):
+        for s, x in zip(hist[0], tok):
+            s.append(int(x))
+        return np.stack([oracle_logits(m, p, np.array(s), 1)[-1] for s in hist[0]])
+
+    first = np.stack([oracle_logits(m, p, np.array(s), 1)[-1] for s in ids])
+    assert (first.argmax(1) == 3).all()
+    want, ws = host_search(step, first, beams, steps, 3, pick)
+    assert all(r[-1] == 3 and 3 not in r[:-1] for rows in want for r in rows)
+    ended = max(len(r) for rows in want for r in rows)     # steps after which all have
+    assert 1 < ended <= 16
+    assert len(calls) == (7 if ended <= 8 else 15)         # looked at every 8 steps
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert list(x) == y
+    assert np.abs(sc - ws).max() <= 1e-4 * np.abs(ws).max()
+    more, msc = m.beam_search(ids, beams, 2 * steps, eos=3)
+    np.testing.assert_array_equal(sc, msc)
+    assert all(list(x) == list(y) for a, b in zip(got, more) for x, y in zip(a, b))
+    m.close()
+
+
 def test_the_example_runs(g):
     sys.path.insert(0, str(ROOT))
     try:
