@@ -164,6 +164,17 @@ def test_top_of_large_logits(g, V):
         assert (np.abs(s - rs) <= U * np.abs(rs) + delta(z[:1], tau)).all()
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,V,K", [(1, 1 << 20, 64), (2, (1 << 21) + 3, 17)])
+def test_top_of_the_longest_rows(g, rows, V, K, bf16):
+    """A thread adds at most 16 pieces of 8, a lane then a few slices' sums: 136 terms."""
+    z, val = logits(np.random.default_rng(V), rows, V, bf16)
+    got = g.top_logits(z, K)
+    check_top(got, val, K)
+    rs = lo.top(val, K)[2]
+    assert (np.abs(got[2] - rs) <= U * np.abs(rs) + U * (136 + 48 + 4 * np.log(V) + 4 * np.ptp(val))).all()
+
+
 def orders(V):
     """Rows in which the largest lie where a selection by parts goes wrong."""
     up_ = np.arange(V) / 64.0
@@ -249,6 +260,27 @@ def test_distill(g, T, V, K, bf16):
     L2, none = g.distill(z, tv, ids, grad=False, **kw)
     assert none is None
     np.testing.assert_array_equal(L, L2)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("T,V", [(1, 1 << 20), (2, 600001), (2, (1 << 20) - 3), (3, 524293)])
+def test_distill_of_the_longest_rows(g, T, V, bf16):
+    """The largest bitmap, and rows of more slices than a split has; entries and targets in the last
+    columns.  A thread adds up to 4 pieces of 8, then up to 64 such sums one after another: 96 terms."""
+    print(f"[distill] T={T} V={V} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(V)
+    z, val = logits(rng, T, V, bf16)
+    K = 7
+    tv, ids, tl = teacher(rng, val, K, 2.0)
+    ids[:, 0], ids[:, 1], ids[:, 2] = V - 1, V - 2, 0
+    tg = np.array([V - 1, V - 3, V - 9])[:T]
+    d = delta(val[:, :64 * 96]) + U * 4 * (np.ptp(val) + np.log(V))
+    for rest, alpha in ((True, 0.5), (False, 1.0)):
+        kw = dict(tlse=tl + np.float32(0.5) if rest else None, targets=tg if alpha < 1 else None, temperature=2.0, alpha=alpha)
+        got = g.distill(z, tv, ids, **kw)
+        L, dz, (sl, sg) = lo.distill(val, tv, ids, **kw)
+        assert (np.abs(got[0] - L) <= U * np.abs(L) + d * sl).all()
+        assert (np.abs(value(got[1]) - dz) <= (2.0 ** -8 if bf16 else U) * np.abs(dz) + d * sg + 1e-37).all()
 
 
 @pytest.mark.parametrize("bf16", [False, True])
