@@ -269,8 +269,10 @@ ASCA_DEV int wave_of(const Pieces<E>& r, int col) {
 template <typename E, int NW, int R>
 struct RowRegs {
     static constexpr int NT = 64 * NW, W = Pieces<E>::W;
-    // the sums' exponentials stay for the gradient where there are registers for them without fewer
-    // waves a SIMD (two temperatures, 16384 x 256 f32 17.1 -> 16.4 us, bf16 19.9 -> 18.4)
+    // The sums' exponentials stay for the gradient in rows of a wave with up to 8 values a lane (two
+    // temperatures, 16384 x 256 f32 16.1 us without and 15.6 with, bf16 18.8 and 17.4; 16384 x 500 bf16
+    // 19.9 and 18.6).  16 values would too (16384 x 1000 f32 27.2 and 24.9, bf16 26.9 and 23.6), but are
+    // not kept; in 4 waves they gain nothing (512 x 4000 f32 6.9 either way, 4096 x 8192 44.6).
     static constexpr bool KEEP = NW == 1 && R * W <= 8;
     uint4 raw[R ? R : 1];
     float kt[KEEP ? R * W + 1 : 1], k1[KEEP ? R * W + 1 : 1];
@@ -680,7 +682,8 @@ static int distill_launch(DistillArgs a, hipStream_t st, const char* fn) {
     // Long rows that leave CUs idle: slices of up to 256 x 8 pieces, at most 64 a row.  Up to 8192
     // pieces the second launch costs what the spread gains but for the fewest rows (16 x 32768 f32
     // 9.7 us against 10.6, 32 rows 10.8 and 10.6); longer ones gain up to half of the CUs (8 x 131072
-    // f32 10.3 us against 33, 128 rows 37 against 41, 192 rows 51 and 53).
+    // f32 10.3 us against 33, 128 rows 37 against 41, 192 rows 51 and 53).  What 64 slices do not hold is
+    // a block's row, read twice (1 x 524288 f32 9.9 us, 1 x 524293 83, 1 x 2^20 180; bf16 rows all fit).
     if (pieces > 1024 * 4 && a.T * (pieces > 1024 * 8 ? 2 : 16) <= cus) {
         const long most = std::min(64l, (pieces + 255) / 256), least = std::min(most, (pieces + 256 * 8 - 1) / (256 * 8));
         const long s = std::max(least, std::min(most, 2 * cus / a.T));

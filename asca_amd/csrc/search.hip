@@ -8,7 +8,7 @@
 // top and step have to read the logits once (a copy's rate is 5.1 TB/s) and rank what may be
 // listed; time of a call, 16 of a row: 4096 x 16384 f32 42 us (6.4 TB/s, part of it from the
 // last-level cache), bf16 26 (5.2); 2048 x 131072 f32 196 (5.5), bf16 102 (5.3); 16384 x 256 f32 10.8
-// us, 1.6 TB/s, where the vector unit is busy for 88% of the time (64 of a row: 25 us); 1 x 256 4.3,
+// us, 1.6 TB/s, where the vector unit is busy for 89% of the time (64 of a row: 25 us); 1 x 256 4.3,
 // 1 x 32768 8 us, the launches.  A step: 1 x 4 x 256 6.9 us, 64 x 4 x 131072 f32 31 (4.3 TB/s).
 #include <algorithm>
 
@@ -27,8 +27,10 @@ constexpr int ROW_MAX_V = 1 << 30;   // columns: ends of slices and of pieces pa
 // all, so what lies below it is none of them.  The pieces with something above it, some more
 // than K, go to LDS by a ballot for each piece of the wave; a wave looks through its own and
 // keeps what is above, and what all waves kept is ranked by counting the larger ones.  Where
-// more is left than LDS has room for (rows of equal values), or a NaN is among them, K rounds
-// take the largest key below the last one.
+// more is left than LDS has room for (rows of equal values, or of a finite mask that leaves
+// fewer than K), or a NaN is among them, K rounds take the largest key below the last one, each a
+// read of the row: 4096 x 50001 bf16, 64 of them, 18 ms, 4096 x 16384 f32, 16 of them, 1.6 ms, 1 x
+// 32768, 8 of them, 25 us; a mask of -inf costs nothing.
 
 template <int NW>
 struct TeamLds {
@@ -64,7 +66,12 @@ ASCA_DEV float four_lists(const float (&l)[4][64]) {
 
 // A value that at least K of the team's x and y reach, near the K-th largest of all that they
 // are maxima of (-inf where fewer are above it).  With G groups some G log(G / (G - K)) values
-// reach it: 18 for K = 16 of 64, 89 for 64 of 128, 74 for 64 of 256.
+// reach it: 18 for K = 16 of 64, 89 for 64 of 128, 74 for 64 of 256.  64 groups up to K = 16, for a
+// second list costs a fifth there (16384 x 256 f32, 16 of them, 10.6 us, 12.7 with two).  They would still
+// be faster at K = 32 of most rows (12.5 and 14.0, but 300 bf16 columns 20.1 and 15.9) and slower from 48
+// on (20.5 and 15.9); a block's rows hardly differ (4096 x 50001 bf16, 32 of them, 85.1 and 86.7).
+// A wave's second group is nearly empty just past 64 pieces: 64 of 16384 x 520 bf16 take 163 us, of 512
+// columns 27, of 640 38; of 260 f32 54, of 256 23.
 template <int NW>
 ASCA_DEV float team_kth(float x, float y, int K, TeamLds<NW>& l) {
     const int lane = threadIdx.x & 63, w = team_wave<NW>();
@@ -610,7 +617,8 @@ constexpr int st_u() {
 // words of the slots that change before it writes any, so that a buffer may be its own
 // destination; no other thread touches them.  What several slots take from one parent comes
 // from memory once, then from a cache.  Bound by memory: 128 x 4 x 1 MB of which half moves 94 us,
-// 5.7 TB/s of reads and writes.
+// 5.7 TB/s of reads and writes.  Words are 16, 4 or 1 bytes, as all buffers' sizes and addresses allow: 50 x 15
+// x 272 KB takes 43 us, with 4 bytes more 40, with 2 bytes more 88.
 template <typename W, int KM>
 __global__ __launch_bounds__(256) void beam_states_k(StatesArgs p) {
     constexpr int U = st_u<W, KM>();
@@ -671,7 +679,7 @@ static int rows_check(const char* fn, long rows, int V, long ld, const void* z, 
 //   4.1), and many rows pay for the merge.  Longer ones, and a search's, which are merged in any
 //   case (1 x 4 x 32768 bf16 9.9 us, 13.4 with whole rows), in as many slices as give two blocks a CU
 //   (64 x 32768 f32 9.0 us, 9.7 with four; 256 rows 12.1 and 11.6).  Whole rows in blocks of 16
-//   waves were slower than these (4096 x 16384 f32 120 us against 44).
+//   waves were slower than these (4096 x 16384 f32 120 us against 44; few rows were not tried).
 constexpr int TOP_R = 16;   // pieces a thread at most
 template <typename E>
 static int top_slices(TopArgs& a, StreamScratch& scratch, hipStream_t st, const char* fn) {
